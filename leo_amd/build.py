@@ -3,7 +3,7 @@
     python -m leo_amd.build            # libleo_hip.so (gfx950) + the CPU oracle
 
 libleo_hip.so holds the HIP kernels, the host runtime and the C-ABI of
-include/leo_hip.h. It is built in-tree (leo_amd/_lib/) so that it travels with
+include/leo_hip.h, include/leo_formats.h and include/leo_decode.h. It is built in-tree (leo_amd/_lib/) so that it travels with
 the repository to the GPU box. Every HIP translation unit is compiled with
 -ffp-contract=off (the kernels must round exactly where Leo's CPU executor
 rounds) and with packed-FP32 instructions disabled.
@@ -49,7 +49,7 @@ def build_library() -> pathlib.Path:
     BUILD.mkdir(exist_ok=True)
     LIB_DIR.mkdir(exist_ok=True)
     objects = []
-    for src in ("leo_kernels.hip", "leo_runtime.hip"):
+    for src in ("leo_kernels.hip", "leo_runtime.hip", "leo_q4.hip", "leo_answer.hip"):
         obj = BUILD / (src + ".o")
         _run([HIPCC, *HIP_FLAGS, "-c", CSRC / src, "-o", obj])
         objects.append(obj)

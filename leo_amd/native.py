@@ -215,7 +215,7 @@ def load(path: Optional[pathlib.Path] = None) -> ctypes.CDLL:
     if not target.exists():
         raise RuntimeError(f"{target} is missing: build it with `python -m leo_amd.build` (no CPU fallback exists)")
     lib = ctypes.CDLL(str(target))
-    for name, (restype, argtypes) in {**SIGNATURES, **FORMAT_SIGNATURES}.items():
+    for name, (restype, argtypes) in {**SIGNATURES, **FORMAT_SIGNATURES, **DECODE_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.restype = restype
         fn.argtypes = argtypes
@@ -268,6 +268,53 @@ FORMAT_SIGNATURES = {
     "leo_dataset_entry": (_I32, [_P, _U64, _P]),
     "leo_dataset_story": (_I32, [_P, _U64, _P, _U64, _P]),
     "leo_dataset_pack": (_I32, [_P, _U64, _U64, _P, _U64, _P]),
+}
+
+
+# Every symbol include/leo_decode.h declares, with its argument structs.
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+_I64 = ctypes.c_int64
+
+
+class LeoQ4Shape(ctypes.Structure):
+    _fields_ = [("outputs", _U64), ("inputs", _U64), ("group", _U32), ("scale_type", _I32), ("has_zeros", _U32),
+                ("pad0", _U32)]
+
+
+class LeoQ4Source(ctypes.Structure):
+    _fields_ = [("shape", LeoQ4Shape), ("codes", _P), ("codes_stride", _I64), ("scales", _P), ("scales_stride", _I64),
+                ("zeros", _P), ("zeros_stride", _I64), ("layout", _P), ("layout_bytes", _U64)]
+
+
+class LeoQ4Product(ctypes.Structure):
+    _fields_ = [("shape", LeoQ4Shape), ("layout", _P), ("layout_bytes", _U64), ("rows", _U64), ("x", _P),
+                ("x_stride", _I64), ("bias", _P), ("y", _P), ("y_stride", _I64), ("x_type", _I32), ("y_type", _I32),
+                ("workspace", _P), ("workspace_bytes", _U64)]
+
+
+class LeoLogitControl(ctypes.Structure):
+    _fields_ = [("rows", _U64), ("symbols", _U64), ("logits", _P), ("logits_stride", _I64), ("out", _P),
+                ("out_stride", _I64), ("type", _I32), ("pad0", _U32), ("history", _P), ("history_offsets", _P),
+                ("history_count", _U64), ("repetition", _P), ("presence", _P), ("frequency", _P), ("bias_ids", _P),
+                ("bias_values", _P), ("bias_offsets", _P), ("bias_count", _U64), ("masks", _P), ("masks_stride", _I64),
+                ("mask_count", _U64), ("mask_rows", _P)]
+
+
+class LeoSample(ctypes.Structure):
+    _fields_ = [("rows", _U64), ("symbols", _U64), ("logits", _P), ("logits_stride", _I64), ("type", _I32),
+                ("pad0", _U32), ("noise", _P), ("noise_stride", _I64), ("temperature", _P), ("top_k", _P),
+                ("top_p", _P), ("min_p", _P), ("out_symbols", _P), ("out_logprobs", _P), ("workspace", _P),
+                ("workspace_bytes", _U64)]
+
+
+DECODE_SIGNATURES = {
+    "leo_q4_layout_bytes": (_I32, [_P, _P]),
+    "leo_q4_layout": (_I32, [_P, _P]),
+    "leo_q4_workspace_bytes": (_I32, [_P, _U64, _P]),
+    "leo_q4_matvec": (_I32, [_P, _P]),
+    "leo_control_logits": (_I32, [_P, _P]),
+    "leo_sample_workspace_bytes": (_I32, [_U64, _U64, _P]),
+    "leo_sample": (_I32, [_P, _P]),
 }
 
 
