@@ -60,9 +60,10 @@ int32_t leo_q4_layout(const LeoQ4Source* source, void* stream);
 
 /* y[m, n] = bias[n] + sum over k of x[m, k] * w[n, k] for `rows` rows of x.
  * Sums are held in 32 bits and rounded once to y_type; bias (float) may be
- * NULL. `workspace`: at least leo_q4_workspace_bytes() bytes, 256-byte aligned,
- * used by one stream at a time, all zero before its first use; calls leave the
- * part that has to be zero zeroed. */
+ * NULL. `workspace`: at least leo_q4_workspace_bytes() bytes (none where that is
+ * 0), 256-byte aligned, used by one stream at a time. Its first 64 KiB are zero
+ * before its first use, and every call leaves them so; several operators may
+ * share one. */
 typedef struct LeoQ4Product {
     LeoQ4Shape shape;
     const void* layout;
@@ -78,7 +79,7 @@ typedef struct LeoQ4Product {
     void* workspace;
     uint64_t workspace_bytes;
 } LeoQ4Product;
-int32_t leo_q4_workspace_bytes(const LeoQ4Shape* shape, uint64_t rows, uint64_t* bytes);
+int32_t leo_q4_workspace_bytes(const LeoQ4Shape* shape, uint64_t rows, int32_t x_type, uint64_t* bytes);
 int32_t leo_q4_matvec(const LeoQ4Product* product, void* stream);
 
 /* Control of logits [rows, symbols], in this order for each logit z of symbol v

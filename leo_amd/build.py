@@ -15,6 +15,7 @@ import pathlib
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 ROOT = pathlib.Path(__file__).resolve().parents[1]
 CSRC = ROOT / "leo_amd" / "csrc"
@@ -48,15 +49,15 @@ def _run(cmd):
 def build_library() -> pathlib.Path:
     BUILD.mkdir(exist_ok=True)
     LIB_DIR.mkdir(exist_ok=True)
-    objects = []
+    commands, objects = [], []
     for src in ("leo_kernels.hip", "leo_runtime.hip", "leo_q4.hip", "leo_answer.hip"):
-        obj = BUILD / (src + ".o")
-        _run([HIPCC, *HIP_FLAGS, "-c", CSRC / src, "-o", obj])
-        objects.append(obj)
+        objects.append(BUILD / (src + ".o"))
+        commands.append([HIPCC, *HIP_FLAGS, "-c", CSRC / src, "-o", objects[-1]])
     for src in ("host_model.cpp", "formats.cpp"):
-        obj = BUILD / (pathlib.Path(src).stem + ".o")
-        _run([os.environ.get("CXX", "g++"), *CXX_FLAGS, "-c", CSRC / src, "-o", obj])
-        objects.append(obj)
+        objects.append(BUILD / (pathlib.Path(src).stem + ".o"))
+        commands.append([os.environ.get("CXX", "g++"), *CXX_FLAGS, "-c", CSRC / src, "-o", objects[-1]])
+    with ThreadPoolExecutor(max_workers=len(commands)) as pool:   # one compiler process each
+        list(pool.map(_run, commands))
     tmp = LIB.with_suffix(".so.tmp")
     _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-pthread", *objects, "-o", tmp])
     os.replace(tmp, LIB)

@@ -130,15 +130,15 @@ class Q4Weight:
             zeros_stride=0 if zeros is None else zeros.stride(0), layout=self.layout.data_ptr(),
             layout_bytes=size.value)
         _call("leo_q4_layout", source, self.device)
-        self._workspace_bytes: Dict[int, int] = {}
+        self._workspace_bytes: Dict[Tuple[int, int], int] = {}
 
-    def workspace_bytes(self, rows: int) -> int:
-        """Bytes of workspace that a product with `rows` rows needs."""
-        found = self._workspace_bytes.get(rows)
+    def workspace_bytes(self, rows: int, x_type: int) -> int:
+        """Bytes of workspace that a product with `rows` rows of x needs."""
+        found = self._workspace_bytes.get((rows, x_type))
         if found is None:
             lib, size = native.load(), ctypes.c_uint64()
-            native.check(lib, lib.leo_q4_workspace_bytes(ctypes.byref(self.shape), rows, ctypes.byref(size)))
-            found = self._workspace_bytes[rows] = size.value
+            native.check(lib, lib.leo_q4_workspace_bytes(ctypes.byref(self.shape), rows, x_type, ctypes.byref(size)))
+            found = self._workspace_bytes[rows, x_type] = size.value
         return found
 
     @classmethod
@@ -180,7 +180,7 @@ def q4_matvec(x: torch.Tensor, weight: Q4Weight, bias: Optional[torch.Tensor] = 
         shape=weight.shape, layout=weight.layout.data_ptr(), layout_bytes=weight.layout.numel(), rows=rows,
         x=x.data_ptr(), x_stride=x.stride(0), bias=_vector("bias", bias, torch.float32, weight.device, weight.outputs),
         y=out.data_ptr(), y_stride=out.stride(0), x_type=_TYPES[x.dtype], y_type=_TYPES[out.dtype])
-    _call("leo_q4_matvec", args, weight.device, weight.workspace_bytes(rows))
+    _call("leo_q4_matvec", args, weight.device, weight.workspace_bytes(rows, args.x_type))
     return out
 
 

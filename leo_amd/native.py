@@ -310,7 +310,7 @@ class LeoSample(ctypes.Structure):
 DECODE_SIGNATURES = {
     "leo_q4_layout_bytes": (_I32, [_P, _P]),
     "leo_q4_layout": (_I32, [_P, _P]),
-    "leo_q4_workspace_bytes": (_I32, [_P, _U64, _P]),
+    "leo_q4_workspace_bytes": (_I32, [_P, _U64, _I32, _P]),
     "leo_q4_matvec": (_I32, [_P, _P]),
     "leo_control_logits": (_I32, [_P, _P]),
     "leo_sample_workspace_bytes": (_I32, [_U64, _U64, _P]),

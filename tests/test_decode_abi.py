@@ -54,7 +54,7 @@ def test_null_arguments_are_refused():
         assert "null" in _refused(name, None, None)
     size = ctypes.c_uint64()
     _refused("leo_q4_layout_bytes", None, ctypes.byref(size))
-    _refused("leo_q4_workspace_bytes", None, 1, ctypes.byref(size))
+    _refused("leo_q4_workspace_bytes", None, 1, native.TYPE_F32, ctypes.byref(size))
     _refused("leo_sample_workspace_bytes", 1, 1, None)
 
 
