@@ -49,9 +49,9 @@ inline void require(bool ok, const char* what) {
 // Launches through the returned status, not the thread's last error, which an
 // earlier call of the program may have left.
 template <class... Args>
-void launch(void (*kernel)(Args...), dim3 grid, dim3 block, hipStream_t stream, Args... args) {
+void launch(void (*kernel)(Args...), dim3 grid, dim3 block, uint32_t lds, hipStream_t stream, Args... args) {
     void* list[] = {&args...};
-    const hipError_t status = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, list, 0, stream);
+    const hipError_t status = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, list, lds, stream);
     if (status != hipSuccess)
         throw Error(LEO_ERR_DEVICE, std::string("kernel launch: ") + hipGetErrorString(status));
 }

@@ -253,7 +253,7 @@ int32_t leo_control_logits(const LeoLogitControl* control, void* stream) {
         const auto kernel = c.type == LEO_TYPE_F32   ? leo_control_rows<F32>
                             : c.type == LEO_TYPE_F16 ? leo_control_rows<F16>
                                                      : leo_control_rows<BF16>;
-        launch(kernel, grid, dim3(256), static_cast<hipStream_t>(stream), c);
+        launch(kernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), c);
     });
 }
 
@@ -279,7 +279,7 @@ int32_t leo_sample(const LeoSample* sample, void* stream) {
         const auto kernel = s.type == LEO_TYPE_F32   ? leo_sample_rows<F32>
                             : s.type == LEO_TYPE_F16 ? leo_sample_rows<F16>
                                                      : leo_sample_rows<BF16>;
-        launch(kernel, dim3(static_cast<uint32_t>(s.rows)), dim3(kSampleThreads), static_cast<hipStream_t>(stream), s);
+        launch(kernel, dim3(static_cast<uint32_t>(s.rows)), dim3(kSampleThreads), 0, static_cast<hipStream_t>(stream), s);
     });
 }
 

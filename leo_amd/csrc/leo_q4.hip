@@ -129,6 +129,7 @@ struct TileArgs {
     uint32_t scale_bf16;
     uint32_t rows, inputs, outputs, tiles, blocks;
     uint32_t slices, slice_blocks;
+    uint32_t row_bits, stage_blocks;  // of leo_q4_few: its rows rounded up to a power of two, blocks of x in LDS at a time
     uint32_t* counters;
     float* partials;
 };
@@ -239,224 +240,402 @@ __device__ __forceinline__ half8 weights_of(uint32_t word, half2 minus, half2 mi
     return u.v;
 }
 
-template <int kGroups, bool kZero, bool kWide, int kTiles>
-struct WeightStage {
+// The scales and zeros of one tile's block as bits, and its codes.
+template <int kGroups, bool kZero, bool kWide>
+struct WeightBlock {
     static constexpr int kScaleWords = kWide ? kGroups : (kGroups + 1) / 2;
-    uint4v code[kTiles];
-    uint32_t scale[kTiles][kScaleWords];
-    uint32_t zero[kTiles];
+    uint4v code;
+    uint32_t scale[kScaleWords];
+    uint32_t zero;
+
+    __device__ __forceinline__ void load(const TileArgs& a, uint64_t at, uint32_t lane) {
+        const uint32_t column = lane % kTile;
+        code = reinterpret_cast<const uint4v*>(a.codes)[at * 64 + lane];
+        const uint64_t group = (at * kTile + column) * kGroups;
+        if constexpr (!kWide && kGroups == 1) {
+            scale[0] = reinterpret_cast<const uint16_t*>(a.scales)[group];
+        } else {
+            __builtin_memcpy(scale, __builtin_assume_aligned(a.scales + group * (kWide ? 4 : 2), sizeof(scale)),
+                             sizeof(scale));
+        }
+        if constexpr (kZero) {
+            if constexpr (kGroups == 4) zero = reinterpret_cast<const uint16_t*>(a.zeros)[at * kTile + column];
+            else zero = reinterpret_cast<const uint8_t*>(a.zeros)[at * kTile + column];
+        }
+    }
+    __device__ __forceinline__ float scale_of(int g, bool bf16) const {
+        if constexpr (kWide) {
+            return __uint_as_float(scale[g]);
+        } else {
+            const uint32_t bits = scale[g / 2] >> (16 * (g % 2)) & 0xffffu;
+            return bf16 ? __uint_as_float(bits << 16)
+                        : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+        }
+    }
+    // The 8 weights of a lane in matrix instruction j of the block.
+    __device__ __forceinline__ half8 weights(int j) const {
+        half2 minus = {static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)};
+        half2 minus_high = {static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
+        if constexpr (kZero) {
+            // -(1024 + z) and -(64 + z) are the bits 0xe400 | z and 0xd400 | z << 4
+            const uint32_t z = zero >> (j * kGroups / 4 * 4) & 15u, both = z | z << 16;
+            minus = __builtin_bit_cast(half2, both | 0xe400e400u);
+            minus_high = __builtin_bit_cast(half2, both << 4 | 0xd400d400u);
+        }
+        return weights_of(code[j], minus, minus_high);
+    }
 };
 
-// One workgroup: kTiles tiles of 16 outputs, 16 kRows rows of x and one slice of
-// the inputs, whose blocks its waves take in turn.
-template <class X, int kGroups, bool kZero, bool kWide, int kRows, int kTiles>
-__global__ __launch_bounds__(kRows == 1 ? 512 : 256) void leo_q4_tiles(TileArgs a) {
-    constexpr bool kScaled = !__is_same(X, F16);  // x goes to half precision by a power of two a row and block
-    constexpr int kParts = __is_same(X, F32) ? 2 : 1;
-    constexpr int kRegs = kTiles * kRows * 4;
-    constexpr int kWaves = kRows == 1 ? 8 : 4;
-    using Stage = WeightStage<kGroups, kZero, kWide, kTiles>;
-    __shared__ float joined[kWaves][kRegs][64];
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64;
-    const uint32_t column = lane % 16, quad = lane / 16;
-    const uint32_t tile0 = blockIdx.x * kTiles, row0 = blockIdx.z * kRows * 16;
-    const uint32_t begin = blockIdx.y * a.slice_blocks, end = min(begin + a.slice_blocks, a.blocks);
+// A lane's share of 16 rows (or rows times blocks) and 128 inputs of x on its
+// way to LDS: inputs 32 j + 8 (lane / 16) + 0..7.
+template <class X>
+struct XBlock {
+    static constexpr bool kScaled = !__is_same(X, F16);  // x goes to half precision by a power of two a row and block
+    static constexpr int kParts = __is_same(X, F32) ? 2 : 1;
+    Eight<X> v[4];
 
-    int64_t row_at[kRows];
+    __device__ __forceinline__ void load(const TileArgs& a, uint32_t row, uint32_t block, uint32_t quad) {
+        const int64_t at = min(row, a.rows - 1) * a.x_stride + static_cast<int64_t>(block) * kBlock + quad * 8;
+        const uint32_t inside = a.inputs - block * kBlock;
+        if (inside >= kBlock) {
 #pragma unroll
-    for (int m = 0; m < kRows; ++m) row_at[m] = min(row0 + m * 16 + column, a.rows - 1) * a.x_stride + quad * 8;
-    uint64_t tile_at[kTiles];
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) tile_at[t] = static_cast<uint64_t>(min(tile0 + t, a.tiles - 1)) * a.blocks;
-
-    const auto load_weights = [&](uint32_t block, Stage& s) {
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-            const uint64_t at = tile_at[t] + block;
-            s.code[t] = reinterpret_cast<const uint4v*>(a.codes)[at * 64 + lane];
-            const uint64_t group = (at * kTile + column) * kGroups;
-            if constexpr (!kWide && kGroups == 1) {
-                s.scale[t][0] = reinterpret_cast<const uint16_t*>(a.scales)[group];
-            } else {
-                __builtin_memcpy(s.scale[t], __builtin_assume_aligned(a.scales + group * (kWide ? 4 : 2), sizeof(s.scale[t])),
-                                 sizeof(s.scale[t]));
-            }
-            if constexpr (kZero) {
-                if constexpr (kGroups == 4) s.zero[t] = reinterpret_cast<const uint16_t*>(a.zeros)[at * kTile + column];
-                else s.zero[t] = reinterpret_cast<const uint8_t*>(a.zeros)[at * kTile + column];
-            }
-        }
-    };
-    const auto load_x = [&](uint32_t block, Eight<X> (&v)[kRows][4]) {
-        if ((block + 1) * kBlock <= a.inputs) {
-#pragma unroll
-            for (int m = 0; m < kRows; ++m)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[m][j] = load_eight<X>(a.x, row_at[m] + block * kBlock + 32 * j);
+            for (int j = 0; j < 4; ++j) v[j] = load_eight<X>(a.x, at + 32 * j);
         } else {
 #pragma unroll
-            for (int m = 0; m < kRows; ++m)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    v[m][j] = load_some<X>(a.x, row_at[m] + block * kBlock + 32 * j,
-                                           static_cast<int32_t>(a.inputs - block * kBlock) - 32 * j - 8 * static_cast<int32_t>(quad));
+            for (int j = 0; j < 4; ++j)
+                v[j] = load_some<X>(a.x, at + 32 * j, static_cast<int32_t>(inside) - 32 * j - 8 * static_cast<int32_t>(quad));
         }
-    };
-
-    float4v sum[kTiles][kRows] = {};
-    Stage now, next;
-    Eight<X> x_now[kRows][4], x_next[kRows][4];
-    uint32_t block = begin + wave;
-    if (block < end) {
-        load_weights(block, now);
-        load_x(block, x_now);
     }
-    for (; block < end; block += waves) {
-        if (block + waves < end) {
-            load_weights(block + waves, next);
-            load_x(block + waves, x_next);
+    // Writes part p of instruction j to at(p, j); returns the factor that takes
+    // sums over the block back to x's values. Lanes of one row take part together.
+    template <class At>
+    __device__ __forceinline__ float store(At&& at) const {
+        if constexpr (kScaled) {
+            // the largest value of the row's block goes to 2^14 .. 2^15, below half precision's end
+            const uint32_t e = top_exponent<X>(v);
+            const float factor = __uint_as_float((268u - e) << 23);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                half8 h[kParts];
+                halves<X, kParts>(v[j], factor, h);
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) *at(p, j) = h[p];
+            }
+            return __uint_as_float((e - 14u) << 23);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *at(0, j) = __builtin_bit_cast(half8, v[j].w[0]);
+            return 1.0f;
         }
-        half8 part[kRows][4][kParts];
-        float4v back[kRows];
+    }
+};
+
+// Up to 16 rows: one workgroup takes a tile of 16 outputs and a slice of the
+// inputs, its eight waves the slice's blocks in turn. x goes through LDS once a
+// workgroup, in the order in which matrix instructions take it; with few rows
+// the lanes of a staging wave cover several blocks, so that no lane converts a
+// row that is not there.
+constexpr uint32_t kFewWaves = 8, kAhead = 4;
+
+template <class X, int kGroups, bool kZero, bool kWide>
+__global__ __launch_bounds__(kFewWaves * 64) void leo_q4_few(TileArgs a) {
+    constexpr bool kScaled = XBlock<X>::kScaled;
+    constexpr int kParts = XBlock<X>::kParts;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const uint32_t column = lane % 16, quad = lane / 16;
+    const uint32_t tile = blockIdx.x, bits = a.row_bits;
+    const uint32_t begin = blockIdx.y * a.slice_blocks, end = min(begin + a.slice_blocks, a.blocks);
+    const uint32_t back_rows = max(1u << bits, 4u);
+    half8* parts = reinterpret_cast<half8*>(lds);
+    float* back = reinterpret_cast<float*>(lds + a.stage_blocks * (kParts * 16u << bits) * sizeof(half8));
+    const auto part_at = [&](uint32_t block, uint32_t part, uint32_t j, uint32_t q) {
+        return (((block * kParts + part) * 4 + j) * 4 + q) << bits;
+    };
+    const uint64_t tile_at = static_cast<uint64_t>(tile) * a.blocks;
+    float4v sum = {};
+    for (uint32_t from = begin; from < end; from += a.stage_blocks) {
+        const uint32_t to = min(from + a.stage_blocks, end);
+        WeightBlock<kGroups, kZero, kWide> ring[kAhead];
 #pragma unroll
-        for (int m = 0; m < kRows; ++m) {
-            if constexpr (kScaled) {
-                // the largest value of the block goes to 2^14 .. 2^15, below half precision's end
-                const uint32_t e = top_exponent<X>(x_now[m]);
-                const float factor = __uint_as_float((268u - e) << 23), inverse = __uint_as_float((e - 14u) << 23);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) back[m][i] = __shfl(inverse, static_cast<int>(quad * 4 + i));
-#pragma unroll
-                for (int j = 0; j < 4; ++j) halves<X, kParts>(x_now[m][j], factor, part[m][j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) part[m][j][0] = __builtin_bit_cast(half8, x_now[m][j].w[0]);
+        for (uint32_t u = 0; u < kAhead; ++u)
+            if (from + wave + u * kFewWaves < to) ring[u].load(a, tile_at + from + wave + u * kFewWaves, lane);
+        if (from != begin) __syncthreads();
+        const uint32_t row = column & ((1u << bits) - 1), ahead = column >> bits, step = 16u >> bits;
+        for (uint32_t first = from + wave * step; first < to; first += kFewWaves * step) {
+            const uint32_t block = first + ahead, in_stage = block - from;
+            if (block < to) {
+                XBlock<X> x;
+                x.load(a, row, block, quad);
+                const float factor = x.store([&](uint32_t p, uint32_t j) { return parts + part_at(in_stage, p, j, quad) + row; });
+                if (kScaled && quad == 0) back[in_stage * back_rows + row] = factor;
             }
         }
+        __syncthreads();
+        const uint32_t read_row = min(column, (1u << bits) - 1);
+        for (uint32_t first = from + wave; first < to; first += kAhead * kFewWaves) {
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-            float4v whole[kRows] = {};
+            for (uint32_t u = 0; u < kAhead; ++u) {
+                const uint32_t block = first + u * kFewWaves;
+                if (block < to) {
+                    const uint32_t in_stage = block - from;
+                    float4v whole = {};
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
-                half2 minus = {static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)};
-                half2 minus_high = {static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
-                if constexpr (kZero) {
-                    // -(1024 + z) and -(64 + z) are the bits 0xe400 | z and 0xd400 | z << 4
-                    const uint32_t z = now.zero[t] >> (4 * g) & 15u, both = z | z << 16;
-                    minus = __builtin_bit_cast(half2, both | 0xe400e400u);
-                    minus_high = __builtin_bit_cast(half2, both << 4 | 0xd400d400u);
+                    for (int g = 0; g < kGroups; ++g) {
+                        float4v d = {};
+#pragma unroll
+                        for (int j = g * 4 / kGroups; j < (g + 1) * 4 / kGroups; ++j) {
+                            const half8 w = ring[u].weights(j);
+#pragma unroll
+                            for (int p = 0; p < kParts; ++p)
+                                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(parts[part_at(in_stage, p, j, quad) + read_row], w, d, 0, 0, 0);
+                        }
+                        const float scale = ring[u].scale_of(g, a.scale_bf16);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if constexpr (kScaled) whole[i] = __builtin_fmaf(scale, d[i], whole[i]);
+                            else sum[i] = __builtin_fmaf(scale, d[i], sum[i]);
+                        }
+                    }
+                    if constexpr (kScaled) {
+                        const float4v f = *reinterpret_cast<const float4v*>(back + in_stage * back_rows + 4 * min(quad, back_rows / 4 - 1));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(f[i], whole[i], sum[i]);
+                    }
+                    if (block + kAhead * kFewWaves < to) ring[u].load(a, tile_at + block + kAhead * kFewWaves, lane);
                 }
-                float4v d[kRows] = {};
+            }
+        }
+    }
+
+    // register i of a lane is output 16 tile + column and row 4 quad + i
+    float4v* joined = reinterpret_cast<float4v*>(lds);
+    const uint32_t output = tile * kTile + column;
+    const auto join = [&](float4v v) {  // of all waves, in the first one
+        __syncthreads();
+        joined[wave * 64 + lane] = v;
+        __syncthreads();
+        if (wave == 0) {
 #pragma unroll
-                for (int j = g * 4 / kGroups; j < (g + 1) * 4 / kGroups; ++j) {
-                    const half8 w = weights_of(now.code[t][j], minus, minus_high);
+            for (uint32_t w = 1; w < kFewWaves; ++w) v += joined[w * 64 + lane];
+        }
+        return v;
+    };
+    const auto store = [&](float4v v) {
+        if (wave != 0 || output >= a.outputs) return;
+        const float bias = a.bias ? a.bias[output] : 0.0f;
 #pragma unroll
-                    for (int m = 0; m < kRows; ++m)
+        for (uint32_t i = 0; i < 4; ++i)
+            if (quad * 4 + i < a.rows) store_any(a.y, (quad * 4 + i) * a.y_stride + output, v[i] + bias, a.y_type);
+    };
+    sum = join(sum);
+    if (a.slices == 1) {
+        store(sum);
+        return;
+    }
+    // every slice's sums go to memory; the workgroup that comes last adds them, in the slices' order
+    float* mine = a.partials + static_cast<uint64_t>(tile) * a.slices * 256;
+    if (wave == 0) {
 #pragma unroll
-                        for (int s = 0; s < kParts; ++s)
-                            d[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(part[m][j][s], w, d[m], 0, 0, 0);
-                }
-                float scale;
-                if constexpr (kWide) {
-                    scale = __uint_as_float(now.scale[t][g]);
-                } else {
-                    const uint32_t bits = now.scale[t][g / 2] >> (16 * (g % 2)) & 0xffffu;
-                    scale = a.scale_bf16 ? __uint_as_float(bits << 16)
-                                         : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
-                }
+        for (uint32_t i = 0; i < 4; ++i)
+            if (quad * 4 + i < a.rows) hand_over(mine + blockIdx.y * 256 + i * 64 + lane, sum[i]);
+    }
+    if (!last_to_arrive(a.counters + tile, a.slices)) return;
+    float4v total = {};
+    for (uint32_t s = wave; s < a.slices; s += kFewWaves * 4) {
+        float v[4][4];
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u)  // in flight together; what lies beyond is not added
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i)
+                v[u][i] = take_over(mine + min(s + u * kFewWaves, a.slices - 1) * 256 + i * 64 + lane);
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u)
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) total[i] += s + u * kFewWaves < a.slices ? v[u][i] : 0.0f;
+    }
+    store(join(total));
+}
+
+// More rows: one workgroup takes 16 kRows rows, eight tiles of outputs (two a
+// wave) and a slice of the inputs, block by block: x through two buffers in LDS
+// that its four waves share, codes straight to registers.
+constexpr uint32_t kManyWaves = 4, kManyTiles = 2;
+
+template <class X, int kGroups, bool kZero, bool kWide, int kRows>
+__global__ __launch_bounds__(kManyWaves * 64, 2) void leo_q4_many(TileArgs a) {
+    constexpr bool kScaled = XBlock<X>::kScaled;
+    constexpr int kParts = XBlock<X>::kParts;
+    constexpr int kRegs = kManyTiles * kRows * 4;
+    __shared__ half8 parts[2][kParts][4][kRows][64];
+    __shared__ __attribute__((aligned(16))) float back[2][kRows * 16];
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const uint32_t column = lane % 16, quad = lane / 16;
+    const uint32_t tile0 = (blockIdx.x * kManyWaves + wave) * kManyTiles, row0 = blockIdx.z * kRows * 16;
+    const uint32_t begin = blockIdx.y * a.slice_blocks, end = min(begin + a.slice_blocks, a.blocks);
+    const bool staging = wave < kRows;
+    uint64_t tile_at[kManyTiles];
+#pragma unroll
+    for (uint32_t t = 0; t < kManyTiles; ++t) tile_at[t] = static_cast<uint64_t>(min(tile0 + t, a.tiles - 1)) * a.blocks;
+
+    const auto stage = [&](const XBlock<X>& x, uint32_t buffer) {
+        const float factor = x.store([&](uint32_t p, uint32_t j) { return &parts[buffer][p][j][wave][lane]; });
+        if (kScaled && quad == 0) back[buffer][wave * 16 + column] = factor;
+    };
+    float4v sum[kManyTiles][kRows] = {};
+    WeightBlock<kGroups, kZero, kWide> now[kManyTiles], next[kManyTiles];
+    XBlock<X> x;
+#pragma unroll
+    for (uint32_t t = 0; t < kManyTiles; ++t) now[t].load(a, tile_at[t] + begin, lane);
+    if (staging) {
+        x.load(a, row0 + wave * 16 + column, begin, quad);
+        stage(x, 0);
+    }
+    __syncthreads();
+    for (uint32_t block = begin; block < end; ++block) {
+        const uint32_t buffer = (block - begin) % 2;
+        if (block + 1 < end) {
+#pragma unroll
+            for (uint32_t t = 0; t < kManyTiles; ++t) next[t].load(a, tile_at[t] + block + 1, lane);
+            if (staging) x.load(a, row0 + wave * 16 + column, block + 1, quad);
+        }
+        float4v whole[kManyTiles][kRows] = {};
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            float4v d[kManyTiles][kRows] = {};
+#pragma unroll
+            for (int j = g * 4 / kGroups; j < (g + 1) * 4 / kGroups; ++j) {
+                half8 w[kManyTiles];
+#pragma unroll
+                for (uint32_t t = 0; t < kManyTiles; ++t) w[t] = now[t].weights(j);
+#pragma unroll
+                for (int m = 0; m < kRows; ++m)
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p) {
+                        const half8 v = parts[buffer][p][j][m][lane];
+#pragma unroll
+                        for (uint32_t t = 0; t < kManyTiles; ++t)
+                            d[t][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[t], d[t][m], 0, 0, 0);
+                    }
+            }
+#pragma unroll
+            for (uint32_t t = 0; t < kManyTiles; ++t) {
+                const float scale = now[t].scale_of(g, a.scale_bf16);
 #pragma unroll
                 for (int m = 0; m < kRows; ++m)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        if constexpr (kScaled) whole[m][i] = __builtin_fmaf(scale, d[m][i], whole[m][i]);
-                        else sum[t][m][i] = __builtin_fmaf(scale, d[m][i], sum[t][m][i]);
+                        if constexpr (kScaled) whole[t][m][i] = __builtin_fmaf(scale, d[t][m][i], whole[t][m][i]);
+                        else sum[t][m][i] = __builtin_fmaf(scale, d[t][m][i], sum[t][m][i]);
                     }
             }
-            if constexpr (kScaled) {
+        }
+        if constexpr (kScaled) {
 #pragma unroll
-                for (int m = 0; m < kRows; ++m)
+            for (int m = 0; m < kRows; ++m) {
+                const float4v f = *reinterpret_cast<const float4v*>(&back[buffer][m * 16 + quad * 4]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[t][m][i] = __builtin_fmaf(back[m][i], whole[m][i], sum[t][m][i]);
+                for (uint32_t t = 0; t < kManyTiles; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[t][m][i] = __builtin_fmaf(f[i], whole[t][m][i], sum[t][m][i]);
             }
         }
-        now = next;
+        if (block + 1 < end && staging) stage(x, 1 - buffer);
+        __syncthreads();
 #pragma unroll
-        for (int m = 0; m < kRows; ++m)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x_now[m][j] = x_next[m][j];
+        for (uint32_t t = 0; t < kManyTiles; ++t) now[t] = next[t];
     }
 
-    // a register of a lane is the sum of output 16 tile + column and row 16 m + 4 quad + i
-    const auto row_of = [&](uint32_t reg, uint32_t of) { return row0 + reg / 4 % kRows * 16 + of / 16 * 4 + reg % 4; };
-    const auto each = [&](auto&& f) {
-        __syncthreads();
-        for (uint32_t at = threadIdx.x; at < kRegs * 64; at += blockDim.x) {
-            const uint32_t reg = at / 64, of = at % 64, row = row_of(reg, of);
-            const uint32_t output = (tile0 + reg / (4 * kRows)) * kTile + of % 16;
-            if (row >= a.rows || output >= a.outputs) continue;
-            float v = joined[0][reg][of];
-            for (uint32_t w = 1; w < waves; ++w) v += joined[w][reg][of];
-            f(at, row, output, v);
+    // register r = (t, m, i) of a lane is output 16 (tile0 + t) + column and row 16 m + 4 quad + i
+    const auto store = [&](float4v (&v)[kManyTiles][kRows]) {
+#pragma unroll
+        for (uint32_t t = 0; t < kManyTiles; ++t) {
+            const uint32_t output = (tile0 + t) * kTile + column;
+            if (output >= a.outputs) continue;
+            const float bias = a.bias ? a.bias[output] : 0.0f;
+#pragma unroll
+            for (uint32_t m = 0; m < kRows; ++m)
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t row = row0 + m * 16 + quad * 4 + i;
+                    if (row < a.rows) store_any(a.y, row * a.y_stride + output, v[t][m][i] + bias, a.y_type);
+                }
         }
     };
-    const auto store = [&](uint32_t, uint32_t row, uint32_t output, float v) {
-        store_any(a.y, row * a.y_stride + output, v + (a.bias ? a.bias[output] : 0.0f), a.y_type);
-    };
-#pragma unroll
-    for (int r = 0; r < kRegs; ++r) joined[wave][r][lane] = sum[r / (4 * kRows)][r / 4 % kRows][r % 4];
     if (a.slices == 1) {
-        each(store);
+        store(sum);
         return;
     }
-    // every slice's sums go to memory; the workgroup that comes last adds them, in the slices' order
-    const uint64_t group = blockIdx.z * gridDim.x + blockIdx.x;
-    float* mine = a.partials + group * a.slices * (kRegs * 64);
-    each([&](uint32_t at, uint32_t, uint32_t, float v) { hand_over(mine + blockIdx.y * (kRegs * 64) + at, v); });
+    // as in leo_q4_few
+    constexpr uint32_t kShare = kRegs * kManyWaves * 64;
+    const uint64_t group = static_cast<uint64_t>(blockIdx.z) * gridDim.x + blockIdx.x;
+    float* mine = a.partials + group * a.slices * kShare + wave * (kRegs * 64) + lane;
+#pragma unroll
+    for (uint32_t r = 0; r < kRegs; ++r)
+        hand_over(mine + blockIdx.y * kShare + r * 64, sum[r / (4 * kRows)][r / 4 % kRows][r % 4]);
     if (!last_to_arrive(a.counters + group, a.slices)) return;
-    float total[kRegs] = {};
-    for (uint32_t s = wave; s < a.slices; s += waves)
+    float4v total[kManyTiles][kRows] = {};
+    for (uint32_t s = 0; s < a.slices; ++s) {
+        float v[kRegs];
 #pragma unroll
-        for (int r = 0; r < kRegs; ++r)
-            if (row_of(r, lane) < a.rows && (tile0 + r / (4 * kRows)) * kTile + column < a.outputs)
-                total[r] += take_over(mine + s * (kRegs * 64) + r * 64 + lane);
+        for (uint32_t r = 0; r < kRegs; ++r) v[r] = take_over(mine + s * kShare + r * 64);
 #pragma unroll
-    for (int r = 0; r < kRegs; ++r) joined[wave][r][lane] = total[r];
-    each(store);
+        for (uint32_t r = 0; r < kRegs; ++r) total[r / (4 * kRows)][r / 4 % kRows][r % 4] += v[r];
+    }
+    store(total);
 }
 
+constexpr uint32_t kStageBytes = 32 << 10, kFewGroups = 1024, kManyGroups = 512;
+
 struct Plan {
-    uint32_t rows, tiles, waves;  // rows (of 16) and tiles of a workgroup, waves that share its blocks
+    bool few;         // leo_q4_few, else leo_q4_many
+    uint32_t rows;    // of 16, of one workgroup
     uint32_t groups, slabs, slices, slice_blocks;
+    uint32_t row_bits, stage_blocks, lds;
     uint64_t workspace;
 };
 
 Plan plan_of(const LeoQ4Shape& s, uint64_t rows, int32_t x_type) {
     const Q4Layout l = layout_of(s);
-    Plan p;
-    p.rows = rows <= 16 ? 1 : x_type == LEO_TYPE_F32 ? 2 : 4;
-    p.slabs = static_cast<uint32_t>((rows + 16 * p.rows - 1) / (16 * p.rows));
-    const uint64_t work = l.tiles * l.blocks * p.slabs;
-    p.tiles = p.rows > 1 ? 2 : work < 4096 ? 1 : 4;
-    p.groups = static_cast<uint32_t>((l.tiles + p.tiles - 1) / p.tiles);
-    const uint32_t most = p.rows == 1 ? 8 : 4;
-    p.waves = static_cast<uint32_t>(l.blocks < most ? l.blocks : most);
-    const uint64_t wanted = p.rows == 1 ? 512 : 768;
-    uint64_t slices = (wanted + p.groups * p.slabs - 1) / (static_cast<uint64_t>(p.groups) * p.slabs);
-    slices = std::min<uint64_t>(slices, std::max<uint64_t>(1, l.blocks / (2 * p.waves)));
-    if (static_cast<uint64_t>(p.groups) * p.slabs > kCounters) slices = 1;
-    p.slice_blocks = static_cast<uint32_t>((l.blocks + slices - 1) / slices);
-    p.slices = static_cast<uint32_t>((l.blocks + p.slice_blocks - 1) / p.slice_blocks);
-    p.workspace = p.slices == 1 ? 0 : kCounterBytes + static_cast<uint64_t>(p.groups) * p.slabs * p.slices * p.tiles * p.rows * 1024;
+    const uint32_t blocks = static_cast<uint32_t>(l.blocks);
+    const auto over = [](uint64_t n, uint64_t d) { return static_cast<uint32_t>((n + d - 1) / d); };
+    Plan p{};
+    p.few = rows <= 16;
+    uint32_t share;  // floats that a workgroup hands over
+    if (p.few) {
+        const uint32_t parts = x_type == LEO_TYPE_F32 ? 2 : 1;
+        p.rows = 1;
+        p.slabs = 1;
+        p.groups = static_cast<uint32_t>(l.tiles);
+        while ((1u << p.row_bits) < rows) ++p.row_bits;
+        const uint32_t block_bytes = (parts * 256 << p.row_bits) + 4 * std::max(1u << p.row_bits, 4u);
+        const uint32_t most = std::max(kFewWaves, (kStageBytes / block_bytes) / kFewWaves * kFewWaves);
+        p.slices = std::min(over(kFewGroups, p.groups), std::max(1u, blocks / (kFewWaves * 2)));
+        p.slice_blocks = over(blocks, p.slices);
+        p.stage_blocks = std::min(p.slice_blocks, most);
+        p.lds = std::max(p.stage_blocks * block_bytes, kFewWaves * 64 * 16);
+        share = 256;
+    } else {
+        p.rows = rows <= 32 || x_type == LEO_TYPE_F32 ? 2 : 4;
+        p.slabs = over(rows, 16 * p.rows);
+        p.groups = over(l.tiles, kManyWaves * kManyTiles);
+        p.slices = std::min(over(kManyGroups, static_cast<uint64_t>(p.groups) * p.slabs), std::max(1u, blocks / 4));
+        share = kManyWaves * kManyTiles * p.rows * 256;
+    }
+    if (static_cast<uint64_t>(p.groups) * p.slabs > kCounters) p.slices = 1;
+    p.slice_blocks = over(blocks, p.slices);
+    p.slices = over(blocks, p.slice_blocks);
+    p.workspace = p.slices == 1 ? 0 : kCounterBytes + 4ull * share * p.groups * p.slabs * p.slices;
     return p;
 }
 
 template <class X, int kGroups, bool kZero, bool kWide>
 void launch_tiles(const Plan& p, const TileArgs& a, hipStream_t stream) {
-    const dim3 grid(p.groups, p.slices, p.slabs), block(p.waves * 64);
-    if (p.rows == 1 && p.tiles == 1) launch(leo_q4_tiles<X, kGroups, kZero, kWide, 1, 1>, grid, block, stream, a);
-    else if (p.rows == 1) launch(leo_q4_tiles<X, kGroups, kZero, kWide, 1, 4>, grid, block, stream, a);
-    else if constexpr (__is_same(X, F32)) launch(leo_q4_tiles<X, kGroups, kZero, kWide, 2, 2>, grid, block, stream, a);
-    else launch(leo_q4_tiles<X, kGroups, kZero, kWide, 4, 2>, grid, block, stream, a);
+    const dim3 grid(p.groups, p.slices, p.slabs);
+    if (p.few) return launch(leo_q4_few<X, kGroups, kZero, kWide>, grid, dim3(kFewWaves * 64), p.lds, stream, a);
+    if constexpr (!__is_same(X, F32))
+        if (p.rows == 4) return launch(leo_q4_many<X, kGroups, kZero, kWide, 4>, grid, dim3(kManyWaves * 64), 0, stream, a);
+    launch(leo_q4_many<X, kGroups, kZero, kWide, 2>, grid, dim3(kManyWaves * 64), 0, stream, a);
 }
 
 template <class X, int kGroups>
@@ -507,7 +686,7 @@ int32_t leo_q4_layout(const LeoQ4Source* source, void* stream) {
         const uint64_t count = a.l.tiles * a.l.blocks;
         const uint32_t wide = static_cast<uint32_t>(count < 65536 ? count : 65536);
         launch(leo_q4_lay_out, dim3(wide, static_cast<uint32_t>((count + wide - 1) / wide)), dim3(64),
-               static_cast<hipStream_t>(stream), a);
+               0, static_cast<hipStream_t>(stream), a);
     });
 }
 
@@ -558,6 +737,8 @@ int32_t leo_q4_matvec(const LeoQ4Product* product, void* stream) {
         a.blocks = static_cast<uint32_t>(l.blocks);
         a.slices = plan.slices;
         a.slice_blocks = plan.slice_blocks;
+        a.row_bits = plan.row_bits;
+        a.stage_blocks = plan.stage_blocks;
         a.counters = static_cast<uint32_t*>(p.workspace);
         a.partials = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + (plan.workspace ? kCounterBytes : 0));
         const auto at = static_cast<hipStream_t>(stream);
