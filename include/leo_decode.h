@@ -61,9 +61,8 @@ int32_t leo_q4_layout(const LeoQ4Source* source, void* stream);
 /* y[m, n] = bias[n] + sum over k of x[m, k] * w[n, k] for `rows` rows of x.
  * Sums are held in 32 bits and rounded once to y_type; bias (float) may be
  * NULL. `workspace`: at least leo_q4_workspace_bytes() bytes (none where that is
- * 0), 256-byte aligned, used by one stream at a time. Its first 64 KiB are zero
- * before its first use, and every call leaves them so; several operators may
- * share one. */
+ * 0), 256-byte aligned, whatever they hold; free again when the call's work is
+ * done. */
 typedef struct LeoQ4Product {
     LeoQ4Shape shape;
     const void* layout;

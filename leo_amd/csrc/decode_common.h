@@ -56,34 +56,6 @@ void launch(void (*kernel)(Args...), dim3 grid, dim3 block, uint32_t lds, hipStr
         throw Error(LEO_ERR_DEVICE, std::string("kernel launch: ") + hipGetErrorString(status));
 }
 
-// Workspaces begin with counters that are zero between calls.
-constexpr uint64_t kCounterBytes = 64 << 10, kCounters = kCounterBytes / 4;
-
-// Values that workgroups of one launch hand each other go past the caches of
-// one XCD: stores and loads of agent scope, and the writer waits for its stores
-// before it says so.
-__device__ __forceinline__ void hand_over(float* p, float v) {
-    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float take_over(const float* p) {
-    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-// Whether this workgroup is the last of `count` to arrive, after every wave's
-// handed-over values are in memory. The last one leaves the counter at zero.
-__device__ __forceinline__ bool last_to_arrive(uint32_t* counter, uint32_t count) {
-    __shared__ uint32_t last;
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == count - 1;
-        if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    return last;
-}
-
 }  // namespace leo
 
 #endif

@@ -130,8 +130,7 @@ struct TileArgs {
     uint32_t rows, inputs, outputs, tiles, blocks;
     uint32_t slices, slice_blocks;
     uint32_t row_bits, stage_blocks;  // of leo_q4_few: its rows rounded up to a power of two, blocks of x in LDS at a time
-    uint32_t* counters;
-    float* partials;
+    float* partials;  // [slice][row][16 tiles], where there are several slices
 };
 
 // Eight neighbouring inputs of a row, as the type has them in memory.
@@ -330,12 +329,12 @@ struct XBlock {
     }
 };
 
-// Up to 16 rows: one workgroup takes a tile of 16 outputs and a slice of the
-// inputs, its eight waves the slice's blocks in turn. x goes through LDS once a
-// workgroup, in the order in which matrix instructions take it; with few rows
-// the lanes of a staging wave cover several blocks, so that no lane converts a
+// Few rows: one workgroup takes kFewTiles tiles of 16 outputs and a slice of
+// the inputs, its eight waves the slice's blocks in turn. x goes through LDS
+// once a workgroup, in the order in which matrix instructions take it; the 16
+// row lanes of a staging wave cover several blocks, so that no lane converts a
 // row that is not there.
-constexpr uint32_t kFewWaves = 8, kAhead = 4;
+constexpr uint32_t kFewWaves = 8, kAhead = 2, kFewTiles = 2;
 
 template <class X, int kGroups, bool kZero, bool kWide>
 __global__ __launch_bounds__(kFewWaves * 64) void leo_q4_few(TileArgs a) {
@@ -344,7 +343,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void leo_q4_few(TileArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const uint32_t column = lane % 16, quad = lane / 16;
-    const uint32_t tile = blockIdx.x, bits = a.row_bits;
+    const uint32_t bits = a.row_bits;
     const uint32_t begin = blockIdx.y * a.slice_blocks, end = min(begin + a.slice_blocks, a.blocks);
     const uint32_t back_rows = max(1u << bits, 4u);
     half8* parts = reinterpret_cast<half8*>(lds);
@@ -352,14 +351,19 @@ __global__ __launch_bounds__(kFewWaves * 64) void leo_q4_few(TileArgs a) {
     const auto part_at = [&](uint32_t block, uint32_t part, uint32_t j, uint32_t q) {
         return (((block * kParts + part) * 4 + j) * 4 + q) << bits;
     };
-    const uint64_t tile_at = static_cast<uint64_t>(tile) * a.blocks;
-    float4v sum = {};
+    uint64_t tile_at[kFewTiles];
+#pragma unroll
+    for (uint32_t t = 0; t < kFewTiles; ++t)
+        tile_at[t] = static_cast<uint64_t>(min(blockIdx.x * kFewTiles + t, a.tiles - 1)) * a.blocks;
+    float4v sum[kFewTiles] = {};
     for (uint32_t from = begin; from < end; from += a.stage_blocks) {
         const uint32_t to = min(from + a.stage_blocks, end);
-        WeightBlock<kGroups, kZero, kWide> ring[kAhead];
+        WeightBlock<kGroups, kZero, kWide> ring[kAhead][kFewTiles];
 #pragma unroll
         for (uint32_t u = 0; u < kAhead; ++u)
-            if (from + wave + u * kFewWaves < to) ring[u].load(a, tile_at + from + wave + u * kFewWaves, lane);
+            if (from + wave + u * kFewWaves < to)
+#pragma unroll
+                for (uint32_t t = 0; t < kFewTiles; ++t) ring[u][t].load(a, tile_at[t] + from + wave + u * kFewWaves, lane);
         if (from != begin) __syncthreads();
         const uint32_t row = column & ((1u << bits) - 1), ahead = column >> bits, step = 16u >> bits;
         for (uint32_t first = from + wave * step; first < to; first += kFewWaves * step) {
@@ -379,213 +383,226 @@ __global__ __launch_bounds__(kFewWaves * 64) void leo_q4_few(TileArgs a) {
                 const uint32_t block = first + u * kFewWaves;
                 if (block < to) {
                     const uint32_t in_stage = block - from;
-                    float4v whole = {};
+                    float4v whole[kFewTiles] = {};
 #pragma unroll
                     for (int g = 0; g < kGroups; ++g) {
-                        float4v d = {};
+                        float4v d[kFewTiles] = {};
 #pragma unroll
                         for (int j = g * 4 / kGroups; j < (g + 1) * 4 / kGroups; ++j) {
-                            const half8 w = ring[u].weights(j);
+                            half8 w[kFewTiles];
 #pragma unroll
-                            for (int p = 0; p < kParts; ++p)
-                                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(parts[part_at(in_stage, p, j, quad) + read_row], w, d, 0, 0, 0);
+                            for (uint32_t t = 0; t < kFewTiles; ++t) w[t] = ring[u][t].weights(j);
+#pragma unroll
+                            for (int p = 0; p < kParts; ++p) {
+                                const half8 v = parts[part_at(in_stage, p, j, quad) + read_row];
+#pragma unroll
+                                for (uint32_t t = 0; t < kFewTiles; ++t)
+                                    d[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[t], d[t], 0, 0, 0);
+                            }
                         }
-                        const float scale = ring[u].scale_of(g, a.scale_bf16);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if constexpr (kScaled) whole[i] = __builtin_fmaf(scale, d[i], whole[i]);
-                            else sum[i] = __builtin_fmaf(scale, d[i], sum[i]);
+                        for (uint32_t t = 0; t < kFewTiles; ++t) {
+                            const float scale = ring[u][t].scale_of(g, a.scale_bf16);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if constexpr (kScaled) whole[t][i] = __builtin_fmaf(scale, d[t][i], whole[t][i]);
+                                else sum[t][i] = __builtin_fmaf(scale, d[t][i], sum[t][i]);
+                            }
                         }
                     }
                     if constexpr (kScaled) {
                         const float4v f = *reinterpret_cast<const float4v*>(back + in_stage * back_rows + 4 * min(quad, back_rows / 4 - 1));
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(f[i], whole[i], sum[i]);
+                        for (uint32_t t = 0; t < kFewTiles; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) sum[t][i] = __builtin_fmaf(f[i], whole[t][i], sum[t][i]);
                     }
-                    if (block + kAhead * kFewWaves < to) ring[u].load(a, tile_at + block + kAhead * kFewWaves, lane);
+                    if (block + kAhead * kFewWaves < to)
+#pragma unroll
+                        for (uint32_t t = 0; t < kFewTiles; ++t)
+                            ring[u][t].load(a, tile_at[t] + block + kAhead * kFewWaves, lane);
                 }
             }
         }
     }
 
-    // register i of a lane is output 16 tile + column and row 4 quad + i
+    // register i of a lane is output 16 tile + column and row 4 quad + i; wave t ends up with tile t's sums
     float4v* joined = reinterpret_cast<float4v*>(lds);
-    const uint32_t output = tile * kTile + column;
-    const auto join = [&](float4v v) {  // of all waves, in the first one
-        __syncthreads();
-        joined[wave * 64 + lane] = v;
-        __syncthreads();
-        if (wave == 0) {
+    const uint32_t tile = blockIdx.x * kFewTiles + wave, output = tile * kTile + column;
+    const bool mine = wave < kFewTiles && output < a.outputs;
+    __syncthreads();
 #pragma unroll
-            for (uint32_t w = 1; w < kFewWaves; ++w) v += joined[w * 64 + lane];
-        }
-        return v;
-    };
-    const auto store = [&](float4v v) {
-        if (wave != 0 || output >= a.outputs) return;
-        const float bias = a.bias ? a.bias[output] : 0.0f;
+    for (uint32_t t = 0; t < kFewTiles; ++t) joined[(t * kFewWaves + wave) * 64 + lane] = sum[t];
+    __syncthreads();
+    if (!mine) return;
+    float4v v = {};
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i)
-            if (quad * 4 + i < a.rows) store_any(a.y, (quad * 4 + i) * a.y_stride + output, v[i] + bias, a.y_type);
-    };
-    sum = join(sum);
-    if (a.slices == 1) {
-        store(sum);
-        return;
+    for (uint32_t w = 0; w < kFewWaves; ++w) v += joined[(wave * kFewWaves + w) * 64 + lane];
+    const float bias = a.bias && a.slices == 1 ? a.bias[output] : 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t row = quad * 4 + i;
+        if (row >= a.rows) continue;
+        if (a.slices == 1) store_any(a.y, row * a.y_stride + output, v[i] + bias, a.y_type);
+        else a.partials[(static_cast<uint64_t>(blockIdx.y) * a.rows + row) * (a.tiles * kTile) + output] = v[i];
     }
-    // every slice's sums go to memory; the workgroup that comes last adds them, in the slices' order
-    float* mine = a.partials + static_cast<uint64_t>(tile) * a.slices * 256;
-    if (wave == 0) {
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i)
-            if (quad * 4 + i < a.rows) hand_over(mine + blockIdx.y * 256 + i * 64 + lane, sum[i]);
-    }
-    if (!last_to_arrive(a.counters + tile, a.slices)) return;
-    float4v total = {};
-    for (uint32_t s = wave; s < a.slices; s += kFewWaves * 4) {
-        float v[4][4];
-#pragma unroll
-        for (uint32_t u = 0; u < 4; ++u)  // in flight together; what lies beyond is not added
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i)
-                v[u][i] = take_over(mine + min(s + u * kFewWaves, a.slices - 1) * 256 + i * 64 + lane);
-#pragma unroll
-        for (uint32_t u = 0; u < 4; ++u)
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) total[i] += s + u * kFewWaves < a.slices ? v[u][i] : 0.0f;
-    }
-    store(join(total));
 }
 
 // More rows: one workgroup takes 16 kRows rows, eight tiles of outputs (two a
-// wave) and a slice of the inputs, block by block: x through two buffers in LDS
-// that its four waves share, codes straight to registers.
+// wave) and a slice of the inputs. x goes through two buffers in LDS that the
+// four waves share, each wave bringing 16 rows of one block a step, so a step is
+// 4 / kRows blocks; codes go straight to registers.
 constexpr uint32_t kManyWaves = 4, kManyTiles = 2;
 
 template <class X, int kGroups, bool kZero, bool kWide, int kRows>
 __global__ __launch_bounds__(kManyWaves * 64, 2) void leo_q4_many(TileArgs a) {
     constexpr bool kScaled = XBlock<X>::kScaled;
     constexpr int kParts = XBlock<X>::kParts;
-    constexpr int kRegs = kManyTiles * kRows * 4;
-    __shared__ half8 parts[2][kParts][4][kRows][64];
-    __shared__ __attribute__((aligned(16))) float back[2][kRows * 16];
+    constexpr uint32_t kStep = kManyWaves / kRows;
+    __shared__ half8 parts[2][kStep][kRows][kParts][4][64];
+    __shared__ __attribute__((aligned(16))) float back[2][kStep][kRows * 16];
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const uint32_t column = lane % 16, quad = lane / 16;
     const uint32_t tile0 = (blockIdx.x * kManyWaves + wave) * kManyTiles, row0 = blockIdx.z * kRows * 16;
     const uint32_t begin = blockIdx.y * a.slice_blocks, end = min(begin + a.slice_blocks, a.blocks);
-    const bool staging = wave < kRows;
+    const uint32_t my_block = wave / kRows, my_rows = wave % kRows;  // of a step
     uint64_t tile_at[kManyTiles];
 #pragma unroll
     for (uint32_t t = 0; t < kManyTiles; ++t) tile_at[t] = static_cast<uint64_t>(min(tile0 + t, a.tiles - 1)) * a.blocks;
 
+    // blocks beyond the slice's last are read as that one; they are not multiplied
     const auto stage = [&](const XBlock<X>& x, uint32_t buffer) {
-        const float factor = x.store([&](uint32_t p, uint32_t j) { return &parts[buffer][p][j][wave][lane]; });
-        if (kScaled && quad == 0) back[buffer][wave * 16 + column] = factor;
+        const float factor = x.store([&](uint32_t p, uint32_t j) { return &parts[buffer][my_block][my_rows][p][j][lane]; });
+        if (kScaled && quad == 0) back[buffer][my_block][my_rows * 16 + column] = factor;
+    };
+    const auto load_x = [&](XBlock<X>& x, uint32_t block) {
+        x.load(a, row0 + my_rows * 16 + column, min(block + my_block, end - 1), quad);
     };
     float4v sum[kManyTiles][kRows] = {};
-    WeightBlock<kGroups, kZero, kWide> now[kManyTiles], next[kManyTiles];
+    WeightBlock<kGroups, kZero, kWide> now[kStep][kManyTiles], next[kStep][kManyTiles];
+    const auto load_weights = [&](WeightBlock<kGroups, kZero, kWide> (&w)[kStep][kManyTiles], uint32_t block) {
+#pragma unroll
+        for (uint32_t b = 0; b < kStep; ++b)
+#pragma unroll
+            for (uint32_t t = 0; t < kManyTiles; ++t) w[b][t].load(a, tile_at[t] + min(block + b, end - 1), lane);
+    };
     XBlock<X> x;
-#pragma unroll
-    for (uint32_t t = 0; t < kManyTiles; ++t) now[t].load(a, tile_at[t] + begin, lane);
-    if (staging) {
-        x.load(a, row0 + wave * 16 + column, begin, quad);
-        stage(x, 0);
-    }
+    load_weights(now, begin);
+    load_x(x, begin);
+    stage(x, 0);
     __syncthreads();
-    for (uint32_t block = begin; block < end; ++block) {
-        const uint32_t buffer = (block - begin) % 2;
-        if (block + 1 < end) {
-#pragma unroll
-            for (uint32_t t = 0; t < kManyTiles; ++t) next[t].load(a, tile_at[t] + block + 1, lane);
-            if (staging) x.load(a, row0 + wave * 16 + column, block + 1, quad);
+    uint32_t buffer = 0;
+    for (uint32_t block = begin; block < end; block += kStep, buffer = 1 - buffer) {
+        const bool more = block + kStep < end;
+        if (more) {
+            load_weights(next, block + kStep);
+            load_x(x, block + kStep);
         }
-        float4v whole[kManyTiles][kRows] = {};
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-            float4v d[kManyTiles][kRows] = {};
+        for (uint32_t b = 0; b < kStep; ++b) {
+            if (block + b >= end) break;
+            float4v whole[kManyTiles][kRows] = {};
 #pragma unroll
-            for (int j = g * 4 / kGroups; j < (g + 1) * 4 / kGroups; ++j) {
-                half8 w[kManyTiles];
+            for (int g = 0; g < kGroups; ++g) {
+                float4v d[kManyTiles][kRows] = {};
 #pragma unroll
-                for (uint32_t t = 0; t < kManyTiles; ++t) w[t] = now[t].weights(j);
+                for (int j = g * 4 / kGroups; j < (g + 1) * 4 / kGroups; ++j) {
+                    half8 w[kManyTiles];
 #pragma unroll
-                for (int m = 0; m < kRows; ++m)
+                    for (uint32_t t = 0; t < kManyTiles; ++t) w[t] = now[b][t].weights(j);
 #pragma unroll
-                    for (int p = 0; p < kParts; ++p) {
-                        const half8 v = parts[buffer][p][j][m][lane];
+                    for (int m = 0; m < kRows; ++m)
 #pragma unroll
-                        for (uint32_t t = 0; t < kManyTiles; ++t)
-                            d[t][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[t], d[t][m], 0, 0, 0);
-                    }
+                        for (int p = 0; p < kParts; ++p) {
+                            const half8 v = parts[buffer][b][m][p][j][lane];
+#pragma unroll
+                            for (uint32_t t = 0; t < kManyTiles; ++t)
+                                d[t][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[t], d[t][m], 0, 0, 0);
+                        }
+                }
+#pragma unroll
+                for (uint32_t t = 0; t < kManyTiles; ++t) {
+                    const float scale = now[b][t].scale_of(g, a.scale_bf16);
+#pragma unroll
+                    for (int m = 0; m < kRows; ++m)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if constexpr (kScaled) whole[t][m][i] = __builtin_fmaf(scale, d[t][m][i], whole[t][m][i]);
+                            else sum[t][m][i] = __builtin_fmaf(scale, d[t][m][i], sum[t][m][i]);
+                        }
+                }
             }
+            if constexpr (kScaled) {
 #pragma unroll
-            for (uint32_t t = 0; t < kManyTiles; ++t) {
-                const float scale = now[t].scale_of(g, a.scale_bf16);
+                for (int m = 0; m < kRows; ++m) {
+                    const float4v f = *reinterpret_cast<const float4v*>(&back[buffer][b][m * 16 + quad * 4]);
 #pragma unroll
-                for (int m = 0; m < kRows; ++m)
+                    for (uint32_t t = 0; t < kManyTiles; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (kScaled) whole[t][m][i] = __builtin_fmaf(scale, d[t][m][i], whole[t][m][i]);
-                        else sum[t][m][i] = __builtin_fmaf(scale, d[t][m][i], sum[t][m][i]);
-                    }
+                        for (int i = 0; i < 4; ++i) sum[t][m][i] = __builtin_fmaf(f[i], whole[t][m][i], sum[t][m][i]);
+                }
             }
         }
-        if constexpr (kScaled) {
-#pragma unroll
-            for (int m = 0; m < kRows; ++m) {
-                const float4v f = *reinterpret_cast<const float4v*>(&back[buffer][m * 16 + quad * 4]);
-#pragma unroll
-                for (uint32_t t = 0; t < kManyTiles; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[t][m][i] = __builtin_fmaf(f[i], whole[t][m][i], sum[t][m][i]);
-            }
-        }
-        if (block + 1 < end && staging) stage(x, 1 - buffer);
+        if (more) stage(x, 1 - buffer);
         __syncthreads();
 #pragma unroll
-        for (uint32_t t = 0; t < kManyTiles; ++t) now[t] = next[t];
+        for (uint32_t b = 0; b < kStep; ++b)
+#pragma unroll
+            for (uint32_t t = 0; t < kManyTiles; ++t) now[b][t] = next[b][t];
     }
 
-    // register r = (t, m, i) of a lane is output 16 (tile0 + t) + column and row 16 m + 4 quad + i
-    const auto store = [&](float4v (&v)[kManyTiles][kRows]) {
+    // register (t, m, i) of a lane is output 16 (tile0 + t) + column and row 16 m + 4 quad + i
 #pragma unroll
-        for (uint32_t t = 0; t < kManyTiles; ++t) {
-            const uint32_t output = (tile0 + t) * kTile + column;
-            if (output >= a.outputs) continue;
-            const float bias = a.bias ? a.bias[output] : 0.0f;
+    for (uint32_t t = 0; t < kManyTiles; ++t) {
+        const uint32_t output = (tile0 + t) * kTile + column;
+        if (output >= a.outputs) continue;
+        const float bias = a.bias && a.slices == 1 ? a.bias[output] : 0.0f;
 #pragma unroll
-            for (uint32_t m = 0; m < kRows; ++m)
+        for (uint32_t m = 0; m < kRows; ++m)
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    const uint32_t row = row0 + m * 16 + quad * 4 + i;
-                    if (row < a.rows) store_any(a.y, row * a.y_stride + output, v[t][m][i] + bias, a.y_type);
-                }
-        }
-    };
-    if (a.slices == 1) {
-        store(sum);
-        return;
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t row = row0 + m * 16 + quad * 4 + i;
+                if (row >= a.rows) continue;
+                if (a.slices == 1) store_any(a.y, row * a.y_stride + output, sum[t][m][i] + bias, a.y_type);
+                else a.partials[(static_cast<uint64_t>(blockIdx.y) * a.rows + row) * (a.tiles * kTile) + output] = sum[t][m][i];
+            }
     }
-    // as in leo_q4_few
-    constexpr uint32_t kShare = kRegs * kManyWaves * 64;
-    const uint64_t group = static_cast<uint64_t>(blockIdx.z) * gridDim.x + blockIdx.x;
-    float* mine = a.partials + group * a.slices * kShare + wave * (kRegs * 64) + lane;
-#pragma unroll
-    for (uint32_t r = 0; r < kRegs; ++r)
-        hand_over(mine + blockIdx.y * kShare + r * 64, sum[r / (4 * kRows)][r / 4 % kRows][r % 4]);
-    if (!last_to_arrive(a.counters + group, a.slices)) return;
-    float4v total[kManyTiles][kRows] = {};
-    for (uint32_t s = 0; s < a.slices; ++s) {
-        float v[kRegs];
-#pragma unroll
-        for (uint32_t r = 0; r < kRegs; ++r) v[r] = take_over(mine + s * kShare + r * 64);
-#pragma unroll
-        for (uint32_t r = 0; r < kRegs; ++r) total[r / (4 * kRows)][r / 4 % kRows][r % 4] += v[r];
-    }
-    store(total);
 }
 
-constexpr uint32_t kStageBytes = 32 << 10, kFewGroups = 1024, kManyGroups = 512;
+// Adds the slices of 256 / kLanes outputs of one row, kLanes threads an output,
+// always in the same order.
+template <uint32_t kLanes>
+__global__ __launch_bounds__(256) void leo_q4_join(TileArgs a) {
+    constexpr uint32_t kOutputs = 256 / kLanes;
+    __shared__ float joined[kLanes][kOutputs];
+    const uint32_t output = blockIdx.x * kOutputs + threadIdx.x % kOutputs, part = threadIdx.x / kOutputs;
+    const uint32_t row = blockIdx.y + blockIdx.z * 32768;
+    const uint32_t width = a.tiles * kTile;
+    float sum = 0.0f;
+    if (output < a.outputs && row < a.rows) {
+        const float* at = a.partials + static_cast<uint64_t>(row) * width + output;
+        const uint64_t step = static_cast<uint64_t>(a.rows) * width;
+        for (uint32_t s = part; s < a.slices; s += kLanes * 8) {
+            float v[8];
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u)  // in flight together
+                v[u] = at[min(s + u * kLanes, a.slices - 1) * step];
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u) sum += s + u * kLanes < a.slices ? v[u] : 0.0f;
+        }
+    }
+    if constexpr (kLanes > 1) {
+        joined[part][threadIdx.x % kOutputs] = sum;
+        __syncthreads();
+        if (part != 0) return;
+#pragma unroll
+        for (uint32_t p = 1; p < kLanes; ++p) sum += joined[p][threadIdx.x];
+    }
+    if (output < a.outputs && row < a.rows)
+        store_any(a.y, row * a.y_stride + output, sum + (a.bias ? a.bias[output] : 0.0f), a.y_type);
+}
+
+constexpr uint32_t kStageBytes = 32 << 10, kFewGroups = 768, kManyGroups = 512, kFewRows = 4;
 
 struct Plan {
     bool few;         // leo_q4_few, else leo_q4_many
@@ -600,32 +617,28 @@ Plan plan_of(const LeoQ4Shape& s, uint64_t rows, int32_t x_type) {
     const uint32_t blocks = static_cast<uint32_t>(l.blocks);
     const auto over = [](uint64_t n, uint64_t d) { return static_cast<uint32_t>((n + d - 1) / d); };
     Plan p{};
-    p.few = rows <= 16;
-    uint32_t share;  // floats that a workgroup hands over
+    p.few = rows <= kFewRows;
     if (p.few) {
         const uint32_t parts = x_type == LEO_TYPE_F32 ? 2 : 1;
         p.rows = 1;
         p.slabs = 1;
-        p.groups = static_cast<uint32_t>(l.tiles);
+        p.groups = over(l.tiles, kFewTiles);
         while ((1u << p.row_bits) < rows) ++p.row_bits;
         const uint32_t block_bytes = (parts * 256 << p.row_bits) + 4 * std::max(1u << p.row_bits, 4u);
         const uint32_t most = std::max(kFewWaves, (kStageBytes / block_bytes) / kFewWaves * kFewWaves);
         p.slices = std::min(over(kFewGroups, p.groups), std::max(1u, blocks / (kFewWaves * 2)));
         p.slice_blocks = over(blocks, p.slices);
         p.stage_blocks = std::min(p.slice_blocks, most);
-        p.lds = std::max(p.stage_blocks * block_bytes, kFewWaves * 64 * 16);
-        share = 256;
+        p.lds = std::max(p.stage_blocks * block_bytes, kFewTiles * kFewWaves * 64 * 16);
     } else {
-        p.rows = rows <= 32 || x_type == LEO_TYPE_F32 ? 2 : 4;
+        p.rows = rows <= 16 ? 1 : rows <= 32 || x_type == LEO_TYPE_F32 ? 2 : 4;
         p.slabs = over(rows, 16 * p.rows);
         p.groups = over(l.tiles, kManyWaves * kManyTiles);
         p.slices = std::min(over(kManyGroups, static_cast<uint64_t>(p.groups) * p.slabs), std::max(1u, blocks / 4));
-        share = kManyWaves * kManyTiles * p.rows * 256;
     }
-    if (static_cast<uint64_t>(p.groups) * p.slabs > kCounters) p.slices = 1;
     p.slice_blocks = over(blocks, p.slices);
     p.slices = over(blocks, p.slice_blocks);
-    p.workspace = p.slices == 1 ? 0 : kCounterBytes + 4ull * share * p.groups * p.slabs * p.slices;
+    p.workspace = p.slices == 1 ? 0 : 4ull * p.slices * rows * l.tiles * kTile;
     return p;
 }
 
@@ -635,7 +648,8 @@ void launch_tiles(const Plan& p, const TileArgs& a, hipStream_t stream) {
     if (p.few) return launch(leo_q4_few<X, kGroups, kZero, kWide>, grid, dim3(kFewWaves * 64), p.lds, stream, a);
     if constexpr (!__is_same(X, F32))
         if (p.rows == 4) return launch(leo_q4_many<X, kGroups, kZero, kWide, 4>, grid, dim3(kManyWaves * 64), 0, stream, a);
-    launch(leo_q4_many<X, kGroups, kZero, kWide, 2>, grid, dim3(kManyWaves * 64), 0, stream, a);
+    if (p.rows == 2) return launch(leo_q4_many<X, kGroups, kZero, kWide, 2>, grid, dim3(kManyWaves * 64), 0, stream, a);
+    launch(leo_q4_many<X, kGroups, kZero, kWide, 1>, grid, dim3(kManyWaves * 64), 0, stream, a);
 }
 
 template <class X, int kGroups>
@@ -739,12 +753,16 @@ int32_t leo_q4_matvec(const LeoQ4Product* product, void* stream) {
         a.slice_blocks = plan.slice_blocks;
         a.row_bits = plan.row_bits;
         a.stage_blocks = plan.stage_blocks;
-        a.counters = static_cast<uint32_t*>(p.workspace);
-        a.partials = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + (plan.workspace ? kCounterBytes : 0));
+        a.partials = static_cast<float*>(p.workspace);
         const auto at = static_cast<hipStream_t>(stream);
         if (p.x_type == LEO_TYPE_F32) launch_products<F32>(p.shape, plan, a, at);
         else if (p.x_type == LEO_TYPE_F16) launch_products<F16>(p.shape, plan, a, at);
         else launch_products<BF16>(p.shape, plan, a, at);
+        if (plan.slices == 1) return;
+        const bool many = plan.slices >= 16;  // slices enough to share among threads
+        const uint32_t outputs = many ? 32 : 256, rows = std::min(a.rows, 32768u);
+        const dim3 grid((a.outputs + outputs - 1) / outputs, rows, (a.rows + rows - 1) / rows);
+        launch(many ? leo_q4_join<8> : leo_q4_join<1>, grid, dim3(256), 0, at, a);
     });
 }
 

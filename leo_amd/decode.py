@@ -8,8 +8,7 @@ tensors: 4-bit readout products, control of logits, and the draw.
 Each call goes through the C-ABI of include/leo_decode.h into libleo_hip.so and
 enqueues its work on the current stream of its tensors' device. Failed checks
 raise ``LeoError`` with ``native.ERR_INVALID_ARGUMENT``. There is no CPU
-fallback. Calls may be captured into a graph (their workspace is then the
-graph's own).
+fallback. Calls may be captured into a graph.
 
 The step runtime does not use torch; this module does, and torch brings a HIP
 runtime of its own. One process must have one: import torch (or this module)
@@ -30,7 +29,6 @@ if "torch" not in sys.modules and native._lib is not None:
 import torch  # noqa: E402
 
 _TYPES = {torch.float32: native.TYPE_F32, torch.float16: native.TYPE_F16, torch.bfloat16: native.TYPE_BF16}
-_workspaces: Dict[Tuple[int, int], torch.Tensor] = {}
 
 
 def _refuse(message: str) -> None:
@@ -67,26 +65,15 @@ def _vector(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, device: to
     return t.data_ptr()
 
 
-def _workspace(device: torch.device, stream: int, need: int) -> torch.Tensor:
-    """A zeroed buffer that calls on this stream share; calls leave zero what has to be zero."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(need, dtype=torch.uint8, device=device)
-    key = (device.index, stream)
-    found = _workspaces.get(key)
-    if found is None or found.numel() < need:
-        found = _workspaces[key] = torch.zeros(max(need, 1 << 20), dtype=torch.uint8, device=device)
-    return found
-
-
 def _call(function: str, args: ctypes.Structure, device: torch.device, need: int = 0) -> None:
     lib = native.load()
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return _call(function, args, device, need)
     stream = torch.cuda.current_stream(device).cuda_stream
-    if need:
-        space = _workspace(device, stream, need)
-        args.workspace, args.workspace_bytes = space.data_ptr(), space.numel()
+    if need:      # the caching allocator's: free again in the stream's order
+        space = torch.empty(need, dtype=torch.uint8, device=device)
+        args.workspace, args.workspace_bytes = space.data_ptr(), need
     native.check(lib, getattr(lib, function)(ctypes.byref(args), stream))
 
 
