@@ -9,19 +9,31 @@
 
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "leo_decode.h"
 #include "leo_host.h"
 
 namespace leo {
 
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+
+// Element e of 16 bytes of a type is at(words, e).
 struct F32 {
     using type = float;
+    using bits = uint32_t;
+    static constexpr uint32_t kNegativeInfinity = 0xff800000u;
+    static __device__ __forceinline__ float at(const uint4v& w, uint32_t e) { return __uint_as_float(w[e]); }
     static __device__ __forceinline__ float load(const void* p, int64_t i) { return static_cast<const float*>(p)[i]; }
     static __device__ __forceinline__ void store(void* p, int64_t i, float v) { static_cast<float*>(p)[i] = v; }
 };
 struct F16 {
     using type = _Float16;
+    using bits = uint16_t;
+    static constexpr uint32_t kNegativeInfinity = 0xfc00u;
+    static __device__ __forceinline__ float at(const uint4v& w, uint32_t e) {
+        return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[e / 2] >> (16 * (e % 2)))));
+    }
     static __device__ __forceinline__ float load(const void* p, int64_t i) {
         return static_cast<float>(static_cast<const _Float16*>(p)[i]);
     }
@@ -31,6 +43,11 @@ struct F16 {
 };
 struct BF16 {
     using type = __bf16;
+    using bits = uint16_t;
+    static constexpr uint32_t kNegativeInfinity = 0xff80u;
+    static __device__ __forceinline__ float at(const uint4v& w, uint32_t e) {
+        return __uint_as_float(e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    }
     static __device__ __forceinline__ float load(const void* p, int64_t i) {
         return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p)[i]) << 16);
     }
@@ -38,6 +55,65 @@ struct BF16 {
         static_cast<__bf16*>(p)[i] = static_cast<__bf16>(v);
     }
 };
+
+// Reductions over the 64 lanes of a wave in the register file (six DPP steps);
+// every lane gets the result.
+template <class F>
+__device__ __forceinline__ uint32_t wave_reduce(uint32_t v, uint32_t identity, F&& f) {
+    const auto step = [&](auto ctrl, auto rows) {
+        v = f(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(identity), static_cast<int>(v),
+                                                                  decltype(ctrl)::value, decltype(rows)::value, 0xf, false)));
+    };
+    step(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // within rows of 16, by 1, 2, 4 and 8
+    step(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+    step(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+    step(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+    step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // rows 0 and 2 into 1 and 3
+    step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // the lower half into the upper
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
+}
+__device__ __forceinline__ float wave_max(float v) {
+    return __uint_as_float(wave_reduce(__float_as_uint(v), 0xff800000u, [](uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    return __uint_as_float(wave_reduce(__float_as_uint(v), 0u, [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
+}
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
+    return wave_reduce(v, 0u, [](uint32_t a, uint32_t b) { return a + b; });
+}
+__device__ __forceinline__ uint32_t wave_min(uint32_t v) {
+    return wave_reduce(v, 0xffffffffu, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+}
+
+// 16 bytes from any address: rows need no alignment.
+__device__ __forceinline__ uint4v load_16(const void* p) {
+    uint4v v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+
+// 16 bytes of a row of n elements from element i on; -inf beyond its end.
+template <class T>
+__device__ __forceinline__ uint4v load_row(const void* row, uint32_t i, uint32_t n) {
+    constexpr uint32_t kWide = 16 / sizeof(typename T::bits), kInWord = 4 / sizeof(typename T::bits);
+    const auto* p = static_cast<const typename T::bits*>(row);
+    if (i + kWide <= n) return load_16(p + i);
+    uint4v v;
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) {
+        v[w] = 0;
+#pragma unroll
+        for (uint32_t e = 0; e < kInWord; ++e) {
+            const uint32_t at = i + w * kInWord + e;
+            v[w] |= (at < n ? static_cast<uint32_t>(p[at]) : T::kNegativeInfinity) << (32 / kInWord * e);
+        }
+    }
+    return v;
+}
 
 inline bool valid_type(int32_t type) { return type == LEO_TYPE_F32 || type == LEO_TYPE_F16 || type == LEO_TYPE_BF16; }
 inline uint64_t type_bytes(int32_t type) { return type == LEO_TYPE_F32 ? 4 : 2; }

@@ -75,6 +75,8 @@ __device__ __forceinline__ float from_order_key(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
+// --- the draw ---------------------------------------------------------------
+// The race: the symbol with the largest key z + noise, the lowest of equals.
 struct Racer {
     float key;
     uint32_t at;
@@ -92,133 +94,404 @@ struct Racer {
 };
 __device__ __forceinline__ Racer nobody() { return {negative_infinity(), 0xffffffffu, negative_infinity()}; }
 
-constexpr uint32_t kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64;
+__device__ __forceinline__ Racer wave_race(Racer r) {
+    const float key = wave_max(r.key);
+    const uint32_t at = wave_min(r.key == key ? r.at : 0xffffffffu);
+    const uint64_t here = __ballot(r.key == key && r.at == at);
+    const int lane = __ffsll(static_cast<unsigned long long>(here)) - 1;
+    return {key, at, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(r.z), lane))};
+}
 
-struct SampleShared {
-    Racer racer[kSampleWaves];
-    float value[kSampleWaves];
-    uint32_t count[kSampleWaves];
+// exp of a difference that is not above 0, 1 for a difference of infinities;
+// its error grows with the size of the difference, as its share of a sum falls.
+__device__ __forceinline__ float mass_of(float z, float top) {
+    return z == top ? 1.0f : __builtin_amdgcn_exp2f((z - top) * 1.44269504f);
+}
+
+// A row's parameters.
+struct Rules {
+    float t, inverse, top_p, min_p;
+    uint32_t top_k;
+    bool greedy, ordinary, filtered;
+
+    // logit / t, -inf for NaN: a product with the reciprocal and one correction
+    // by its remainder round as the division does.
+    __device__ __forceinline__ float divided(float logit) const {
+        float q = logit * inverse;
+        if (ordinary) {
+            const float exact = __builtin_fmaf(__builtin_fmaf(-q, t, logit), inverse, q);
+            q = fabsf(q) < __builtin_inff() ? exact : q;
+        } else {
+            q = logit / t;
+        }
+        return q == q ? q : negative_infinity();
+    }
 };
-
-__device__ Racer block_racer(Racer r, SampleShared& s) {
-    for (uint32_t d = 32; d; d /= 2) r.meet(__shfl_xor(r.key, d), __shfl_xor(r.at, d), __shfl_xor(r.z, d));
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) s.racer[threadIdx.x / 64] = r;
-    __syncthreads();
-    for (uint32_t w = 0; w < kSampleWaves; ++w) r.meet(s.racer[w].key, s.racer[w].at, s.racer[w].z);
+__device__ __forceinline__ Rules rules_of(const LeoSample& a, uint64_t row) {
+    Rules r;
+    r.t = a.noise ? (a.temperature ? a.temperature[row] : 1.0f) : 0.0f;
+    r.greedy = !(r.t > 0.0f);
+    if (r.greedy) r.t = 1.0f;
+    r.inverse = 1.0f / r.t;
+    r.ordinary = r.t > 0x1p-100f && r.t < 0x1p100f;
+    r.top_k = a.top_k ? static_cast<uint32_t>(max(a.top_k[row], 1)) : 0x7fffffffu;
+    r.top_p = a.top_p ? a.top_p[row] : 1.0f;
+    r.min_p = a.min_p ? a.min_p[row] : 0.0f;
+    r.filtered = !r.greedy && !(r.top_k >= a.symbols && r.top_p >= 1.0f && r.min_p <= 0.0f);
     return r;
 }
-__device__ float block_max(float v, SampleShared& s) {
-    for (uint32_t d = 32; d; d /= 2) v = fmaxf(v, __shfl_xor(v, d));
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) s.value[threadIdx.x / 64] = v;
-    __syncthreads();
-    for (uint32_t w = 0; w < kSampleWaves; ++w) v = fmaxf(v, s.value[w]);
-    return v;
-}
-__device__ float block_sum(float v, SampleShared& s) {
-    for (uint32_t d = 32; d; d /= 2) v += __shfl_xor(v, d);
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) s.value[threadIdx.x / 64] = v;
-    __syncthreads();
-    float sum = 0.0f;
-    for (uint32_t w = 0; w < kSampleWaves; ++w) sum += s.value[w];
-    return sum;
-}
-__device__ uint32_t block_count(uint32_t v, SampleShared& s) {
-    for (uint32_t d = 32; d; d /= 2) v += __shfl_xor(v, d);
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) s.count[threadIdx.x / 64] = v;
-    __syncthreads();
-    uint32_t sum = 0;
-    for (uint32_t w = 0; w < kSampleWaves; ++w) sum += s.count[w];
-    return sum;
-}
 
-// One workgroup a row. What stays is a prefix of the values in falling order,
-// so one value decides: the race's winner over the whole row is the answer if
-// it stays; if not, no value up to its own stays, and the race is held again
-// above. A second value halfway (in the order of floats) to the lowest one known to stay is tried in
-// the same pass, which bounds the passes by the 32 bits of a float.
+// 1,024 neighbouring symbols of a row in the registers of a wave, 16 a lane in
+// rising order: z, -inf for NaN and beyond the row's end, and the noise.
+constexpr uint32_t kSpan = 1024, kEach = 16;
+
 template <class T>
-__global__ __launch_bounds__(kSampleThreads) void leo_sample_rows(LeoSample a) {
-    __shared__ SampleShared shared;
-    const uint64_t row = blockIdx.x;
-    const uint32_t n = static_cast<uint32_t>(a.symbols);
-    const float t = a.noise ? (a.temperature ? a.temperature[row] : 1.0f) : 0.0f;
-    const bool greedy = !(t > 0.0f);
-    const float divide = greedy ? 1.0f : t;
-    const auto value = [&](uint32_t i) {
-        const float z = T::load(a.logits, row * a.logits_stride + i) / divide;
-        return z == z ? z : negative_infinity();
-    };
-    const float* noise = a.noise ? a.noise + row * a.noise_stride : nullptr;
-    Racer best = nobody();
-    float top = negative_infinity();
-    for (uint32_t i = threadIdx.x; i < n; i += kSampleThreads) {
-        const float z = value(i);
-        top = fmaxf(top, z);
-        if (z > negative_infinity()) best.meet(greedy ? z : z + noise[i], i, z);
+struct Span {
+    static constexpr uint32_t kWide = 16 / sizeof(typename T::type);  // elements of a 16-byte load
+    float z[kEach], noise[kEach];
+
+    static __device__ __forceinline__ uint32_t index(uint32_t base, uint32_t i) {
+        return base + i / kWide * (64 * kWide) + threadIdx.x % 64 * kWide + i % kWide;
     }
-    top = block_max(top, shared);
-    best = block_racer(best, shared);
-    const auto mass_of = [&](float z) { return z == top ? 1.0f : expf(z - top); };
-    float whole = 0.0f;
-    if (top > negative_infinity())
-        for (uint32_t i = threadIdx.x; i < n; i += kSampleThreads) whole += mass_of(value(i));
-    whole = block_sum(whole, shared);
-    if (top == negative_infinity()) {
-        if (threadIdx.x == 0) {
-            a.out_symbols[row] = -1;
-            a.out_logprobs[row] = negative_infinity();
+    __device__ __forceinline__ void load(const LeoSample& a, const Rules& r, uint64_t row, uint32_t base) {
+        const uint32_t n = static_cast<uint32_t>(a.symbols);
+        const auto* logits = static_cast<const typename T::type*>(a.logits) + row * a.logits_stride;
+        const float* from = a.noise + row * a.noise_stride;
+#pragma unroll
+        for (uint32_t v = 0; v < kEach; v += kWide) {
+            const uint32_t at = index(base, v);
+            const uint4v raw = load_row<T>(logits, at, n);
+#pragma unroll
+            for (uint32_t e = 0; e < kWide; ++e) z[v + e] = T::at(raw, e);
         }
-        return;
+#pragma unroll
+        for (uint32_t v = 0; v < kEach; v += 4) {
+            const uint32_t at = index(base, v);
+            if (r.greedy) {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) noise[v + e] = 0.0f;
+            } else {
+                const uint4v raw = load_row<F32>(from, at, n);
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) noise[v + e] = __uint_as_float(raw[e]);
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) z[i] = r.divided(z[i]);
     }
-    if (!greedy) {
-        const uint32_t k = a.top_k ? static_cast<uint32_t>(max(a.top_k[row], 1)) : n;
-        const float p = a.top_p ? a.top_p[row] : 1.0f;
-        const float floor_p = a.min_p ? a.min_p[row] : 0.0f;
+    __device__ __forceinline__ float key(const Rules& r, uint32_t i) const { return r.greedy ? z[i] : z[i] + noise[i]; }
+
+    __device__ __forceinline__ float top() const {
+        float m = z[0];
+#pragma unroll
+        for (uint32_t i = 1; i < kEach; ++i) m = fmaxf(m, z[i]);
+        return wave_max(m);
+    }
+    // The lane's mass, against `top`, which is not -inf.
+    __device__ __forceinline__ float mass(float top) const {
+        float sum = 0.0f;
+        if (top < __builtin_inff()) {
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; ++i) sum += __builtin_amdgcn_exp2f((z[i] - top) * 1.44269504f);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; ++i) sum += z[i] == top ? 1.0f : 0.0f;
+        }
+        return sum;
+    }
+    // The wave's winner. In rising order a larger key is enough; symbols whose
+    // key is no number or -inf race only where a lane holds no others.
+    __device__ __forceinline__ Racer race(const Rules& r, uint32_t base) const {
+        Racer best = nobody();
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const float k = key(r, i);
+            if (k > best.key) best = {k, index(base, i), z[i]};
+        }
+        if (__any(best.at == 0xffffffffu)) {
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; ++i)
+                if (best.at == 0xffffffffu && z[i] > negative_infinity()) best = {negative_infinity(), index(base, i), z[i]};
+        }
+        return wave_race(best);
+    }
+};
+
+// What lies above a value: how many, their mass, the race among them.
+struct Above {
+    uint32_t count;
+    float mass;
+    Racer best;
+    __device__ __forceinline__ void add(float w, float key, uint32_t at, float z) {
+        count += 1;
+        mass += w;
+        best.meet(key, at, z);
+    }
+};
+
+constexpr uint32_t kMostWaves = 16, kRowWaves = 8;
+struct SampleShared {
+    Racer best[kMostWaves];
+    float top[kMostWaves], mass[kMostWaves];
+    Above above[2][2][kMostWaves];  // two pivots, alternating between sweeps
+};
+
+// What stays is a prefix of the values in falling order, so one value decides:
+// the race's winner over the whole row is the answer if it stays; if not, no
+// value up to its own stays, and the race is held again above. A second value,
+// halfway (in the order of floats) to the lowest one known to stay, is tried in
+// the same sweep, which bounds the sweeps by the 32 bits of a float. sweep(low,
+// high, above) adds what a thread holds above either; all threads take part.
+// `probe`, where it lies above the winner, is tried first: a value that is
+// likely not to stay and has little above it.
+template <class Sweep>
+__device__ __forceinline__ void settle(const LeoSample& a, const Rules& r, uint64_t row, float top, float whole, Racer best,
+                                       float probe, SampleShared& shared, Sweep&& sweep) {
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64;
+    if (r.filtered && top > negative_infinity()) {
+        const auto stays = [&](float z, const Above& v) {
+            return v.count < r.top_k && (r.top_p >= 1.0f || v.mass < r.top_p * whole) && mass_of(z, top) >= r.min_p;
+        };
         float lowest = top;  // of the values known to stay
-        while (best.z < lowest) {
-            const float low = best.z;
+        for (uint32_t turn = 0; best.z < lowest; turn ^= 1) {
+            const bool probing = probe > best.z && probe < lowest;
+            const float low = probing ? probe : best.z;
             const uint32_t key = order_key(low);
             const float high = from_order_key(key + (order_key(lowest) - key) / 2);
-            uint32_t larger[2] = {0, 0};
-            float mass[2] = {0.0f, 0.0f};
-            Racer next[2] = {nobody(), nobody()};
-            for (uint32_t i = threadIdx.x; i < n; i += kSampleThreads) {
-                const float z = value(i);
-                if (!(z > low)) continue;
-                const float w = mass_of(z), race = z + noise[i];
-                larger[0] += 1;
-                mass[0] += w;
-                next[0].meet(race, i, z);
-                if (!(z > high)) continue;
-                larger[1] += 1;
-                mass[1] += w;
-                next[1].meet(race, i, z);
-            }
-            const auto stays = [&](float z, uint32_t above, float before) {
-                return above < k && (p >= 1.0f || before < p * whole) && mass_of(z) >= floor_p;
-            };
+            Above above[2] = {{0, 0.0f, nobody()}, {0, 0.0f, nobody()}};
+            sweep(low, high, above);
+#pragma unroll
             for (int h = 0; h < 2; ++h) {
-                larger[h] = block_count(larger[h], shared);
-                mass[h] = block_sum(mass[h], shared);
-                next[h] = block_racer(next[h], shared);
+                above[h] = {wave_sum(above[h].count), wave_sum(above[h].mass), wave_race(above[h].best)};
+                if (waves > 1 && lane == 0) shared.above[turn][h][wave] = above[h];
             }
-            if (stays(low, larger[0], mass[0])) break;
-            if (stays(high, larger[1], mass[1])) {
+            if (waves > 1) {
+                __syncthreads();
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const Above v = lane < waves ? shared.above[turn][h][lane] : Above{0, 0.0f, nobody()};
+                    above[h] = {wave_sum(v.count), wave_sum(v.mass), wave_race(v.best)};
+                }
+            }
+            if (stays(low, above[0])) {
+                if (!probing) break;
+                lowest = low;
+            } else if (stays(high, above[1])) {
                 lowest = high;
-                best = next[0];
+                best = above[0].best;
             } else {
-                best = next[1];
+                best = above[1].best;
             }
+            probe = negative_infinity();
         }
     }
     if (threadIdx.x == 0) {
-        a.out_symbols[row] = static_cast<int32_t>(best.at);
-        a.out_logprobs[row] = (best.z == top ? 0.0f : best.z - top) - logf(whole);
+        const bool empty = top == negative_infinity();
+        a.out_symbols[row] = empty ? -1 : static_cast<int32_t>(best.at);
+        a.out_logprobs[row] = empty ? negative_infinity() : (best.z == top ? 0.0f : best.z - top) - logf(whole);
     }
+}
+
+__device__ __forceinline__ void add_above(float low, float high, float top, float z, float key, uint32_t at, Above (&above)[2]) {
+    if (z > low) {
+        const float w = mass_of(z, top);
+        above[0].add(w, key, at, z);
+        if (z > high) above[1].add(w, key, at, z);
+    }
+}
+
+// A short row, in the registers of one workgroup: one span a wave.
+template <class T>
+__global__ __launch_bounds__(kRowWaves * 64) void leo_sample_row(LeoSample a) {
+    __shared__ SampleShared shared;
+    const uint64_t row = blockIdx.x;
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64;
+    const Rules r = rules_of(a, row);
+    Span<T> span;
+    span.load(a, r, row, wave * kSpan);
+    float top = span.top();
+    Racer best = span.race(r, wave * kSpan);
+    float mass = top > negative_infinity() ? wave_sum(span.mass(top)) : 0.0f;
+    if (waves > 1) {
+        if (lane == 0) {
+            shared.best[wave] = best;
+            shared.top[wave] = top;
+            shared.mass[wave] = mass;
+        }
+        __syncthreads();
+        const float theirs = lane < waves ? shared.top[lane] : negative_infinity();
+        top = wave_max(theirs);
+        mass = wave_sum(theirs > negative_infinity() ? shared.mass[lane] * mass_of(theirs, top) : 0.0f);
+        best = wave_race(lane < waves ? shared.best[lane] : nobody());
+    }
+    settle(a, r, row, top, mass, best, negative_infinity(), shared, [&](float low, float high, Above (&above)[2]) {
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i)
+            add_above(low, high, top, span.z[i], span.key(r, i), Span<T>::index(wave * kSpan, i), above);
+    });
+}
+
+// Longer rows: one wave a span leaves its part of the result, and one workgroup
+// a row settles the rest.
+struct SpanRecord {
+    Racer best;
+    float top, mass;
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void leo_sample_spans(LeoSample a, uint32_t spans, SpanRecord* records) {
+    const uint64_t row = blockIdx.y;
+    const uint32_t which = blockIdx.x * 4 + threadIdx.x / 64;
+    if (which >= spans) return;
+    const Rules r = rules_of(a, row);
+    Span<T> span;
+    span.load(a, r, row, which * kSpan);
+    SpanRecord rec;
+    rec.top = span.top();
+    rec.best = span.race(r, which * kSpan);
+    rec.mass = rec.top > negative_infinity() ? wave_sum(span.mass(rec.top)) : 0.0f;
+    if (threadIdx.x % 64 == 0) records[row * spans + which] = rec;
+}
+
+// What lies above a pivot is first gathered in LDS, by each lane in its own
+// column, and counted and weighed from there: a row has few such values where
+// its rules leave few, and one compare a value passes over the others. If no
+// column runs over, later pivots, which are higher, need the columns alone.
+constexpr uint32_t kColumn = 12, kTogether = 2;
+struct Column {
+    float z[kColumn][64], key[kColumn][64];
+    uint32_t at[kColumn][64];
+};
+
+template <class T>
+__global__ __launch_bounds__(kMostWaves * 64) void leo_sample_settle(LeoSample a, uint32_t spans, const SpanRecord* records) {
+    __shared__ SampleShared shared;
+    __shared__ Column columns[kMostWaves];
+    constexpr uint32_t kWide = Span<T>::kWide, kLoads = kEach / kWide;
+    const uint64_t row = blockIdx.x;
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const uint32_t n = static_cast<uint32_t>(a.symbols);
+    const Rules r = rules_of(a, row);
+    records += row * spans;
+    const auto* logits = static_cast<const typename T::type*>(a.logits) + row * a.logits_stride;
+    const float* noise = a.noise + row * a.noise_stride;
+    // every wave takes all records: no wave waits for another
+    float top = negative_infinity(), mass = 0.0f, sum = 0.0f, squares = 0.0f;
+    uint32_t counted = 0;
+    Racer best = nobody();
+    for (uint32_t s = lane; s < spans; s += 64) {
+        const SpanRecord rec = records[s];
+        if (rec.top == negative_infinity()) continue;
+        const float higher = fmaxf(top, rec.top);
+        mass = (top > negative_infinity() ? mass * mass_of(top, higher) : 0.0f) + rec.mass * mass_of(rec.top, higher);
+        top = higher;
+        best.meet(rec.best.key, rec.best.at, rec.best.z);
+        counted += 1;
+        sum += rec.top;
+        squares += rec.top * rec.top;
+    }
+    const float mine = top;
+    top = wave_max(top);
+    mass = wave_sum(mine > negative_infinity() ? mass * mass_of(mine, top) : 0.0f);
+    best = wave_race(best);
+    // A first pivot with a few values of each span above it: one and a half
+    // standard deviations below the mean of the spans' largest values, or where
+    // min_p cuts, if that is higher.
+    float probe = negative_infinity();
+    if (r.filtered && top > negative_infinity()) {
+        const float count = static_cast<float>(wave_sum(counted)), mean = wave_sum(sum) / count;
+        probe = mean - 1.5f * sqrtf(fmaxf(wave_sum(squares) / count - mean * mean, 0.0f));
+        if (r.min_p > 0.0f) probe = fmaxf(probe, top + logf(r.min_p) * 1.0001f - 0.0001f);
+    }
+
+    Column& column = columns[wave];
+    uint32_t filled = 0;     // of this lane's column
+    float held = __builtin_inff();  // the wave's columns hold all there is above this
+    settle(a, r, row, top, mass, best, probe, shared, [&](float low, float high, Above (&above)[2]) {
+        const auto weigh = [&](bool fresh) {
+            if (fresh) {  // logits so far; their noise comes all at once
+                float race[kColumn];
+#pragma unroll
+                for (uint32_t c = 0; c < kColumn; ++c)
+                    if (c < filled) race[c] = noise[column.at[c][lane]];
+#pragma unroll
+                for (uint32_t c = 0; c < kColumn; ++c)
+                    if (c < filled) {
+                        const float z = r.divided(column.z[c][lane]);
+                        column.z[c][lane] = z;
+                        column.key[c][lane] = z + race[c];
+                    }
+            }
+            for (uint32_t c = 0; __any(c < filled); ++c)
+                if (c < filled) add_above(low, high, top, column.z[c][lane], column.key[c][lane], column.at[c][lane], above);
+        };
+        if (low >= held) return weigh(false);
+        // z above low needs a logit above this, whatever the division rounds
+        const float bar = low * r.t - (fabsf(low * r.t) * 0x1p-20f + 0x1p-120f);
+        held = low;
+        filled = 0;
+        for (uint32_t from = wave; from < spans; from += kMostWaves * 64) {
+            const uint32_t mine_at = from + lane * kMostWaves;
+            uint64_t left = __ballot(mine_at < spans && records[min(mine_at, spans - 1)].top > low);
+            while (left) {
+                uint32_t base[kTogether];
+                bool some[kTogether];
+                uint4v raw[kTogether][kLoads];
+#pragma unroll
+                for (uint32_t u = 0; u < kTogether; ++u) {  // in flight together
+                    some[u] = left != 0;
+                    if (!some[u]) continue;
+                    base[u] = (from + static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(left)) - 1) * kMostWaves) * kSpan;
+                    left &= left - 1;
+#pragma unroll
+                    for (uint32_t v = 0; v < kLoads; ++v) raw[u][v] = load_row<T>(logits, Span<T>::index(base[u], v * kWide), n);
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < kTogether; ++u) {
+                    if (!some[u]) continue;
+#pragma unroll
+                    for (uint32_t i = 0; i < kEach; ++i) {
+                        if (i % 4 == 0 && __any(filled > kColumn - 4)) {
+                            weigh(true);
+                            filled = 0;
+                            held = __builtin_inff();
+                        }
+                        const float logit = T::at(raw[u][i / kWide], i % kWide);
+                        if (logit > bar) {
+                            column.z[filled][lane] = logit;
+                            column.at[filled][lane] = Span<T>::index(base[u], i);
+                            filled += 1;
+                        }
+                    }
+                }
+            }
+        }
+        weigh(true);
+    });
+}
+
+struct SamplePlan {
+    uint32_t spans;
+    bool whole;  // leo_sample_row takes a row at once
+    uint64_t workspace;
+};
+SamplePlan sample_plan(uint64_t rows, uint64_t symbols) {
+    SamplePlan p{};
+    p.spans = static_cast<uint32_t>((symbols + kSpan - 1) / kSpan);
+    p.whole = p.spans <= kRowWaves;
+    if (p.whole) return p;
+    p.workspace = rows * p.spans * sizeof(SpanRecord);
+    return p;
+}
+
+template <class T>
+void launch_sample(const SamplePlan& p, const LeoSample& s, hipStream_t stream) {
+    const uint32_t rows = static_cast<uint32_t>(s.rows);
+    if (p.whole) return launch(leo_sample_row<T>, dim3(rows), dim3(p.spans * 64), 0, stream, s);
+    auto* records = static_cast<SpanRecord*>(s.workspace);
+    launch(leo_sample_spans<T>, dim3((p.spans + 3) / 4, rows), dim3(256), 0, stream, s, p.spans, records);
+    launch(leo_sample_settle<T>, dim3(rows), dim3(kMostWaves * 64), 0, stream, s, p.spans,
+           static_cast<const SpanRecord*>(records));
 }
 
 }  // namespace
@@ -261,7 +534,7 @@ int32_t leo_sample_workspace_bytes(uint64_t rows, uint64_t symbols, uint64_t* by
     return guarded([&] {
         require(bytes, "leo_sample_workspace_bytes: null argument");
         require(rows <= 65535 && symbols <= 0x7fffffffu, "leo_sample_workspace_bytes: too many rows or symbols");
-        *bytes = 0;
+        *bytes = sample_plan(rows, symbols).workspace;
     });
 }
 
@@ -276,10 +549,14 @@ int32_t leo_sample(const LeoSample* sample, void* stream) {
         require(s.symbols >= 1, "leo_sample: no symbols to draw from");
         require(s.logits && s.out_symbols && s.out_logprobs, "leo_sample: null argument");
         require(s.logits_stride >= 0 && s.noise_stride >= 0, "leo_sample: strides must not be negative");
-        const auto kernel = s.type == LEO_TYPE_F32   ? leo_sample_rows<F32>
-                            : s.type == LEO_TYPE_F16 ? leo_sample_rows<F16>
-                                                     : leo_sample_rows<BF16>;
-        launch(kernel, dim3(static_cast<uint32_t>(s.rows)), dim3(kSampleThreads), 0, static_cast<hipStream_t>(stream), s);
+        const SamplePlan p = sample_plan(s.rows, s.symbols);
+        require(p.workspace == 0 || (s.workspace && reinterpret_cast<uintptr_t>(s.workspace) % 256 == 0 &&
+                                     s.workspace_bytes >= p.workspace),
+                "leo_sample: workspace is missing, too small or not 256-byte aligned");
+        const auto at = static_cast<hipStream_t>(stream);
+        if (s.type == LEO_TYPE_F32) launch_sample<F32>(p, s, at);
+        else if (s.type == LEO_TYPE_F16) launch_sample<F16>(p, s, at);
+        else launch_sample<BF16>(p, s, at);
     });
 }
 

@@ -114,7 +114,6 @@ __device__ __forceinline__ void store_any(void* p, int64_t i, float v, int32_t t
 typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float float4v __attribute__((ext_vector_type(4)));
-typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
 struct TileArgs {
     const char* codes;
