@@ -18,12 +18,13 @@ namespace leo {
 
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
-// Element e of 16 bytes of a type is at(words, e).
+// Element e of 16 bytes of a type is at(words, e); put rounds into it.
 struct F32 {
     using type = float;
     using bits = uint32_t;
     static constexpr uint32_t kNegativeInfinity = 0xff800000u;
     static __device__ __forceinline__ float at(const uint4v& w, uint32_t e) { return __uint_as_float(w[e]); }
+    static __device__ __forceinline__ void put(uint4v& w, uint32_t e, float v) { w[e] = __float_as_uint(v); }
     static __device__ __forceinline__ float load(const void* p, int64_t i) { return static_cast<const float*>(p)[i]; }
     static __device__ __forceinline__ void store(void* p, int64_t i, float v) { static_cast<float*>(p)[i] = v; }
 };
@@ -33,6 +34,10 @@ struct F16 {
     static constexpr uint32_t kNegativeInfinity = 0xfc00u;
     static __device__ __forceinline__ float at(const uint4v& w, uint32_t e) {
         return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[e / 2] >> (16 * (e % 2)))));
+    }
+    static __device__ __forceinline__ void put(uint4v& w, uint32_t e, float v) {
+        const uint32_t half = __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
+        w[e / 2] = e % 2 ? w[e / 2] | half << 16 : half;
     }
     static __device__ __forceinline__ float load(const void* p, int64_t i) {
         return static_cast<float>(static_cast<const _Float16*>(p)[i]);
@@ -47,6 +52,10 @@ struct BF16 {
     static constexpr uint32_t kNegativeInfinity = 0xff80u;
     static __device__ __forceinline__ float at(const uint4v& w, uint32_t e) {
         return __uint_as_float(e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    }
+    static __device__ __forceinline__ void put(uint4v& w, uint32_t e, float v) {
+        const uint32_t half = __builtin_bit_cast(uint16_t, static_cast<__bf16>(v));
+        w[e / 2] = e % 2 ? w[e / 2] | half << 16 : half;
     }
     static __device__ __forceinline__ float load(const void* p, int64_t i) {
         return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p)[i]) << 16);

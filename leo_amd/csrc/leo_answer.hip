@@ -1,10 +1,10 @@
 // Control of a row's logits and the draw of its next symbol.
+#include <algorithm>
+
 #include "decode_common.h"
 
 namespace leo {
 namespace {
-
-constexpr uint32_t kChunk = 4096;  // logits of one workgroup of the control
 
 __device__ __forceinline__ float negative_infinity() { return -__builtin_inff(); }
 
@@ -20,29 +20,25 @@ __device__ __forceinline__ Run row_run(const int64_t* offsets, uint64_t row, uin
     return {inside(offsets[row]), inside(offsets[row + 1])};
 }
 
-// One workgroup a row and chunk of symbols: it counts the row's history over
-// its chunk in LDS (whole-number adds, whose order does not matter), notes the
-// last bias entry of each symbol, and passes once over the logits.
+// One workgroup a row and chunk of symbols. It notes in LDS, for each symbol of
+// its chunk, the row's last bias entry and how often the history holds it
+// (whole-number operations, whose order does not matter), and passes once over
+// the logits, 16 bytes a lane. A word holds both, 16 bits each; a row with more
+// entries than that takes its chunk by halves, with a word for each.
+constexpr uint32_t kTable = 16384, kControlThreads = 1024;
+
 template <class T>
-__global__ __launch_bounds__(256) void leo_control_rows(LeoLogitControl a) {
-    __shared__ uint32_t count[kChunk];
-    __shared__ uint32_t bias_at[kChunk];  // last entry + 1, counted from the row's first
+__global__ __launch_bounds__(kControlThreads, 8) void leo_control_rows(LeoLogitControl a, uint32_t chunk) {
+    extern __shared__ __attribute__((aligned(16))) uint32_t table[];
+    constexpr uint32_t kWide = 16 / sizeof(typename T::type), kHeld = kTable / kControlThreads / kWide;
     const uint64_t row = blockIdx.y;
-    const int64_t base = static_cast<int64_t>(blockIdx.x) * kChunk;
-    const int64_t width = min(static_cast<int64_t>(kChunk), static_cast<int64_t>(a.symbols) - base);
-    for (uint32_t i = threadIdx.x; i < kChunk; i += 256) count[i] = bias_at[i] = 0;
-    __syncthreads();
+    const uint32_t n = static_cast<uint32_t>(a.symbols), threads = blockDim.x;
+    const uint32_t begin = blockIdx.x * chunk, end = min(begin + chunk, n);
     const Run history = row_run(a.history_offsets, row, a.history_count);
-    for (int64_t i = history.begin + threadIdx.x; i < history.end; i += 256) {
-        const int64_t at = a.history[i] - base;
-        if (at >= 0 && at < width) atomicAdd(&count[at], 1u);
-    }
     const Run bias = row_run(a.bias_offsets, row, a.bias_count);
-    for (int64_t i = bias.begin + threadIdx.x; i < bias.end; i += 256) {
-        const int64_t at = a.bias_ids[i] - base;
-        if (at >= 0 && at < width) atomicMax(&bias_at[at], static_cast<uint32_t>(i - bias.begin) + 1);
-    }
-    __syncthreads();
+    const bool listed = history.end > history.begin || bias.end > bias.begin;
+    const bool wide = max(history.end - history.begin, bias.end - bias.begin) >= 0xffff;
+    const uint32_t step = wide ? chunk / 2 : chunk;
     const float repetition = a.repetition ? a.repetition[row] : 1.0f;
     const float presence = a.presence ? a.presence[row] : 0.0f;
     const float frequency = a.frequency ? a.frequency[row] : 0.0f;
@@ -53,16 +49,89 @@ __global__ __launch_bounds__(256) void leo_control_rows(LeoLogitControl a) {
         shut = which < -1 || which >= static_cast<int64_t>(a.mask_count);
         if (!shut && which >= 0) mask = a.masks + which * a.masks_stride;
     }
-    for (int64_t i = threadIdx.x; i < width; i += 256) {
-        const int64_t v = base + i;
-        float z = T::load(a.logits, row * a.logits_stride + v);
-        if (const uint32_t c = count[i]) {
+    const auto* logits = static_cast<const typename T::type*>(a.logits) + row * a.logits_stride;
+    auto* out = static_cast<typename T::type*>(a.out) + row * a.out_stride;
+    const auto bits_of = [&](uint32_t v) {  // from symbol v's bit on
+        return shut ? 0u : mask ? static_cast<uint32_t>(mask[v / 32]) >> (v % 32) : ~0u;
+    };
+    const auto adjusted = [&](float z, uint32_t count, uint32_t entry) {
+        if (count) {
             z = z > 0.0f ? z / repetition : z * repetition;
-            z = z - (presence + frequency * static_cast<float>(c));
+            z = z - (presence + frequency * static_cast<float>(count));
         }
-        if (const uint32_t b = bias_at[i]) z = z + a.bias_values[bias.begin + b - 1];
-        if (shut || (mask && !(static_cast<uint32_t>(mask[v / 32]) >> (v % 32) & 1u))) z = negative_infinity();
-        T::store(a.out, row * a.out_stride + v, z);
+        if (entry) z = z + a.bias_values[bias.begin + entry - 1];
+        return z;
+    };
+    for (uint32_t from = begin; from < end; from += step) {
+        const uint32_t width = min(step, end - from), whole = wide ? 0 : width / kWide * kWide;  // wide rows go one by one
+        // Chunks and halves begin at multiples of 32: the symbols of 16 bytes share a mask word. Logits and mask words
+        // are on their way while the lists are read.
+        uint4v raw[kHeld];
+        uint32_t allowed[kHeld];
+#pragma unroll
+        for (uint32_t h = 0; h < kHeld; ++h)
+            if (const uint32_t i = (threadIdx.x + h * threads) * kWide; i < whole) {
+                raw[h] = load_16(logits + from + i);
+                allowed[h] = bits_of(from + i);
+            }
+        if (listed) {
+            if (from != begin) __syncthreads();
+            for (uint32_t i = threadIdx.x * 4; i < chunk; i += threads * 4)
+                *reinterpret_cast<uint4v*>(table + i) = uint4v{0, 0, 0, 0};
+            __syncthreads();
+            // an entry counts from the row's first, 0 is none
+            for (int64_t i = bias.begin + threadIdx.x; i < bias.end; i += threads) {
+                const uint32_t at = static_cast<uint32_t>(a.bias_ids[i]) - from, entry = static_cast<uint32_t>(i - bias.begin) + 1;
+                if (at < width) atomicMax(&table[wide ? chunk / 2 + at : at], wide ? entry : entry << 16);
+            }
+            if (!wide && bias.end > bias.begin) __syncthreads();
+            const auto note = [&](uint32_t symbol) {
+                if (symbol - from < width) atomicAdd(&table[symbol - from], 1u);
+            };
+            const int64_t fours = history.begin + (history.end - history.begin) / 4 * 4;
+            for (int64_t first = history.begin + threadIdx.x * 4; first < fours; first += threads * 8) {
+                const int64_t second = first + threads * 4;
+                const uint4v four = load_16(a.history + first);
+                uint4v more = {~0u, ~0u, ~0u, ~0u};
+                if (second < fours) more = load_16(a.history + second);
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) note(four[e]);
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) note(more[e]);
+            }
+            if (fours + threadIdx.x < history.end) note(static_cast<uint32_t>(a.history[fours + threadIdx.x]));
+            __syncthreads();
+        }
+#pragma unroll
+        for (uint32_t h = 0; h < kHeld; ++h) {
+            const uint32_t i = (threadIdx.x + h * threads) * kWide;
+            if (i >= whole) break;
+            uint32_t word[kWide] = {}, any = 0;
+            if (listed) {
+#pragma unroll
+                for (uint32_t e = 0; e < kWide; e += 4) {
+                    const uint4v w = *reinterpret_cast<const uint4v*>(table + i + e);
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) any |= word[e + k] = w[k];
+                }
+            }
+            float z[kWide];
+#pragma unroll
+            for (uint32_t e = 0; e < kWide; ++e) z[e] = T::at(raw[h], e);
+            if (any) {
+#pragma unroll
+                for (uint32_t e = 0; e < kWide; ++e) z[e] = adjusted(z[e], word[e] & 0xffffu, word[e] >> 16);
+            }
+            uint4v to;
+#pragma unroll
+            for (uint32_t e = 0; e < kWide; ++e) T::put(to, e, allowed[h] >> e & 1u ? z[e] : negative_infinity());
+            __builtin_memcpy(out + from + i, &to, 16);
+        }
+        for (uint32_t i = whole + threadIdx.x; i < width; i += threads) {
+            float z = T::load(logits, from + i);
+            if (listed) z = wide ? adjusted(z, table[i], table[chunk / 2 + i]) : adjusted(z, table[i] & 0xffffu, table[i] >> 16);
+            T::store(out, from + i, bits_of(from + i) & 1u ? z : negative_infinity());
+        }
     }
 }
 
@@ -522,11 +591,16 @@ int32_t leo_control_logits(const LeoLogitControl* control, void* stream) {
             require(c.mask_rows || c.mask_count == 1 || c.mask_count == c.rows,
                     "leo_control_logits: masks need one row, a row for each of the logits, or mask_rows");
         }
-        const dim3 grid(static_cast<uint32_t>((c.symbols + kChunk - 1) / kChunk), static_cast<uint32_t>(c.rows));
+        // Chunks small enough for some 512 workgroups, but of 2,048 symbols at least (each reads the row's lists
+        // again) and of a table's size at most: 16 symbols a thread.
+        const uint64_t least = (c.symbols + kTable - 1) / kTable, most = (c.symbols + 2047) / 2048;
+        const uint64_t chunks = std::max(least, std::min(most, (512 + c.rows - 1) / c.rows));
+        const uint32_t chunk = static_cast<uint32_t>(((c.symbols + chunks - 1) / chunks + 63) / 64 * 64);
+        const dim3 grid(static_cast<uint32_t>((c.symbols + chunk - 1) / chunk), static_cast<uint32_t>(c.rows));
         const auto kernel = c.type == LEO_TYPE_F32   ? leo_control_rows<F32>
                             : c.type == LEO_TYPE_F16 ? leo_control_rows<F16>
                                                      : leo_control_rows<BF16>;
-        launch(kernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), c);
+        launch(kernel, grid, dim3(chunk > 8192 ? kControlThreads : chunk > 4096 ? kControlThreads / 2 : kControlThreads / 4), chunk * 4, static_cast<hipStream_t>(stream), c, chunk);
     });
 }
 
