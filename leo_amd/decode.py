@@ -35,46 +35,59 @@ def _refuse(message: str) -> None:
     raise native.LeoError(native.ERR_INVALID_ARGUMENT, message)
 
 
-def _matrix(name: str, t: torch.Tensor, dtypes, device: Optional[torch.device] = None) -> None:
-    """`t` is a 2-D device tensor of one of `dtypes` whose last axis is dense."""
+def _device(name: str, t: torch.Tensor) -> int:
+    """The number of the GPU that `t` is on."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         _refuse(f"{name} must be a tensor on the GPU")
-    if device is not None and t.device != device:
-        _refuse(f"{name} is on {t.device}, not on {device}")
-    if t.dtype not in dtypes:
-        _refuse(f"{name} has type {t.dtype}")
-    if t.dim() != 2:
-        _refuse(f"{name} must have two axes, not {t.dim()}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    return t.get_device()
+
+
+def _matrix(name: str, t: torch.Tensor, dtypes, index: int) -> Tuple[int, int, int]:
+    """(rows, width, row stride) of a 2-D tensor of one of `dtypes` on GPU `index` whose last axis is dense."""
+    if isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype in dtypes and t.dim() == 2:
+        rows, width = t.shape
+        stride, last = t.stride()
+        if last == 1 or width <= 1:
+            return rows, width, stride
         _refuse(f"{name}'s last axis must be dense")
+    if _device(name, t) != index:
+        _refuse(f"{name} is on GPU {t.get_device()}, not on {index}")
+    _refuse(f"{name} has type {t.dtype}" if t.dtype not in dtypes else f"{name} must have two axes, not {t.dim()}")
 
 
-def _vector(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, device: torch.device,
-            count: Optional[int] = None) -> Optional[int]:
-    """The address of a dense 1-D tensor (None for none)."""
+def _vector(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, index: int, count: int) -> Optional[int]:
+    """The address of a dense 1-D tensor of `count` entries (any number below 0), None for none."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.device != device:
-        _refuse(f"{name} must be a tensor on {device}")
-    if t.dtype != dtype:
+    if (isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype is dtype and t.dim() == 1
+            and t.is_contiguous() and (count < 0 or t.numel() == count)):
+        return t.data_ptr()
+    if _device(name, t) != index:
+        _refuse(f"{name} is on GPU {t.get_device()}, not on {index}")
+    if t.dtype is not dtype:
         _refuse(f"{name} must have type {dtype}, not {t.dtype}")
-    if t.dim() != 1 or not t.is_contiguous():
-        _refuse(f"{name} must be a dense vector")
-    if count is not None and t.shape[0] != count:
-        _refuse(f"{name} has {t.shape[0]} entries, not {count}")
-    return t.data_ptr()
+    _refuse(f"{name} must be a dense vector" + (f" of {count} entries" if count >= 0 else ""))
 
 
-def _call(function: str, args: ctypes.Structure, device: torch.device, need: int = 0) -> None:
+def _public_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# torch's own accessor of the same number, without the Stream object that costs more than a small launch's checks
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", _public_stream)
+
+
+def _call(function: str, args: ctypes.Structure, index: int, need: int = 0) -> None:
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _call(function, args, index, need)
     lib = native.load()
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _call(function, args, device, need)
-    stream = torch.cuda.current_stream(device).cuda_stream
     if need:      # the caching allocator's: free again in the stream's order
-        space = torch.empty(need, dtype=torch.uint8, device=device)
+        space = torch.empty(need, dtype=torch.uint8, device=index)
         args.workspace, args.workspace_bytes = space.data_ptr(), need
-    native.check(lib, getattr(lib, function)(ctypes.byref(args), stream))
+    status = getattr(lib, function)(ctypes.byref(args), _stream_of(index))
+    if status:
+        native.check(lib, status)
 
 
 class Q4Weight:
@@ -92,19 +105,22 @@ class Q4Weight:
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
                  inputs: int, group: int):
-        _matrix("codes", codes, (torch.uint8,))
+        self.index = _device("codes", codes)
         self.device = codes.device
-        _matrix("scales", scales, _TYPES, self.device)
-        if zeros is not None:
-            _matrix("zeros", zeros, (torch.uint8,), self.device)
+        outputs, width, codes_stride = _matrix("codes", codes, (torch.uint8,), self.index)
         if group not in (32, 64, 128):
             _refuse(f"group must be 32, 64 or 128, not {group}")
-        outputs, groups = codes.shape[0], -(-inputs // group)
-        if inputs < 1 or outputs < 1 or codes.shape[1] != (inputs + 1) // 2:
-            _refuse(f"codes of {inputs} inputs have {(inputs + 1) // 2} bytes a row, not {codes.shape[1]}")
-        for name, t in (("scales", scales), ("zeros", zeros)):
-            if t is not None and tuple(t.shape) != (outputs, groups):
-                _refuse(f"{name} must be {(outputs, groups)}, not {tuple(t.shape)}")
+        if inputs < 1 or outputs < 1 or width != (inputs + 1) // 2:
+            _refuse(f"codes of {inputs} inputs have {(inputs + 1) // 2} bytes a row, not {width}")
+        strides = []
+        for name, t, dtypes in (("scales", scales, _TYPES), ("zeros", zeros, (torch.uint8,))):
+            if t is None and name == "zeros":
+                strides.append(0)
+                continue
+            *shape, stride = _matrix(name, t, dtypes, self.index)
+            if shape != [outputs, -(-inputs // group)]:
+                _refuse(f"{name} must be {(outputs, -(-inputs // group))}, not {tuple(shape)}")
+            strides.append(stride)
         self.outputs, self.inputs, self.group = outputs, inputs, group
         self.shape = native.LeoQ4Shape(outputs=outputs, inputs=inputs, group=group, scale_type=_TYPES[scales.dtype],
                                        has_zeros=zeros is not None)
@@ -112,11 +128,10 @@ class Q4Weight:
         native.check(lib, lib.leo_q4_layout_bytes(ctypes.byref(self.shape), ctypes.byref(size)))
         self.layout = torch.empty(size.value, dtype=torch.uint8, device=self.device)
         source = native.LeoQ4Source(
-            shape=self.shape, codes=codes.data_ptr(), codes_stride=codes.stride(0), scales=scales.data_ptr(),
-            scales_stride=scales.stride(0), zeros=None if zeros is None else zeros.data_ptr(),
-            zeros_stride=0 if zeros is None else zeros.stride(0), layout=self.layout.data_ptr(),
-            layout_bytes=size.value)
-        _call("leo_q4_layout", source, self.device)
+            shape=self.shape, codes=codes.data_ptr(), codes_stride=codes_stride, scales=scales.data_ptr(),
+            scales_stride=strides[0], zeros=None if zeros is None else zeros.data_ptr(), zeros_stride=strides[1],
+            layout=self.layout.data_ptr(), layout_bytes=size.value)
+        _call("leo_q4_layout", source, self.index)
         self._workspace_bytes: Dict[Tuple[int, int], int] = {}
 
     def workspace_bytes(self, rows: int, x_type: int) -> int:
@@ -154,20 +169,22 @@ def q4_matvec(x: torch.Tensor, weight: Q4Weight, bias: Optional[torch.Tensor] = 
         if out is not None:
             _refuse("out needs x with two axes")
         return q4_matvec(x[None], weight, bias, out_dtype=out_dtype)[0]
-    _matrix("x", x, _TYPES, weight.device)
-    rows = x.shape[0]
-    if x.shape[1] != weight.inputs:
-        _refuse(f"x has {x.shape[1]} inputs, the weight {weight.inputs}")
+    index = weight.index
+    rows, width, x_stride = _matrix("x", x, _TYPES, index)
+    if width != weight.inputs:
+        _refuse(f"x has {width} inputs, the weight {weight.inputs}")
     if out is None:
-        out = torch.empty((rows, weight.outputs), dtype=out_dtype or x.dtype, device=x.device)
-    _matrix("out", out, _TYPES, weight.device)
-    if out.shape[0] != rows or out.shape[1] != weight.outputs or (out_dtype is not None and out.dtype != out_dtype):
-        _refuse(f"out must be {(rows, weight.outputs)} of {out_dtype or out.dtype}")
+        out = torch.empty((rows, weight.outputs), dtype=out_dtype or x.dtype, device=weight.device)
+        y_stride = weight.outputs
+    else:
+        *shape, y_stride = _matrix("out", out, _TYPES, index)
+        if shape != [rows, weight.outputs] or (out_dtype is not None and out.dtype is not out_dtype):
+            _refuse(f"out must be {(rows, weight.outputs)} of {out_dtype or out.dtype}")
+    x_type = _TYPES[x.dtype]
     args = native.LeoQ4Product(
-        shape=weight.shape, layout=weight.layout.data_ptr(), layout_bytes=weight.layout.numel(), rows=rows,
-        x=x.data_ptr(), x_stride=x.stride(0), bias=_vector("bias", bias, torch.float32, weight.device, weight.outputs),
-        y=out.data_ptr(), y_stride=out.stride(0), x_type=_TYPES[x.dtype], y_type=_TYPES[out.dtype])
-    _call("leo_q4_matvec", args, weight.device, weight.workspace_bytes(rows, args.x_type))
+        weight.shape, weight.layout.data_ptr(), weight.layout.numel(), rows, x.data_ptr(), x_stride,
+        _vector("bias", bias, torch.float32, index, weight.outputs), out.data_ptr(), y_stride, x_type, _TYPES[out.dtype])
+    _call("leo_q4_matvec", args, index, weight.workspace_bytes(rows, x_type))
     return out
 
 
@@ -189,39 +206,43 @@ def control_logits(logits: torch.Tensor, *, history: Optional[Tuple[torch.Tensor
                without it n is 1 or the number of rows
     out        may be `logits`
     """
-    _matrix("logits", logits, _TYPES)
-    device = logits.device
-    rows, symbols = logits.shape
+    index = _device("logits", logits)
+    rows, symbols, stride = _matrix("logits", logits, _TYPES, index)
     if out is None:
-        out = torch.empty((rows, symbols), dtype=logits.dtype, device=device)
+        out = torch.empty((rows, symbols), dtype=logits.dtype, device=logits.device)
+        out_stride = symbols
     else:
-        _matrix("out", out, (logits.dtype,), device)
-        if out.shape != logits.shape:
+        *shape, out_stride = _matrix("out", out, (logits.dtype,), index)
+        if shape != [rows, symbols]:
             _refuse(f"out must be {(rows, symbols)}")
-    args = native.LeoLogitControl(rows=rows, symbols=symbols, logits=logits.data_ptr(),
-                                  logits_stride=logits.stride(0), out=out.data_ptr(), out_stride=out.stride(0),
-                                  type=_TYPES[logits.dtype])
+    args = native.LeoLogitControl(rows, symbols, logits.data_ptr(), stride, out.data_ptr(), out_stride,
+                                  _TYPES[logits.dtype])
     if history is not None:
-        args.history = _vector("history", history[0], torch.int32, device)
-        args.history_offsets = _vector("history offsets", history[1], torch.int64, device, rows + 1)
-        args.history_count = history[0].shape[0]
-    args.repetition = _vector("repetition", repetition, torch.float32, device, rows)
-    args.presence = _vector("presence", presence, torch.float32, device, rows)
-    args.frequency = _vector("frequency", frequency, torch.float32, device, rows)
+        entries, offsets = history
+        args.history = _vector("history", entries, torch.int32, index, -1)
+        args.history_offsets = _vector("history offsets", offsets, torch.int64, index, rows + 1)
+        args.history_count = entries.numel()
+    if repetition is not None:
+        args.repetition = _vector("repetition", repetition, torch.float32, index, rows)
+    if presence is not None:
+        args.presence = _vector("presence", presence, torch.float32, index, rows)
+    if frequency is not None:
+        args.frequency = _vector("frequency", frequency, torch.float32, index, rows)
     if bias is not None:
-        args.bias_ids = _vector("bias ids", bias[0], torch.int32, device)
-        args.bias_count = bias[0].shape[0]
-        args.bias_values = _vector("bias values", bias[1], torch.float32, device, args.bias_count)
-        args.bias_offsets = _vector("bias offsets", bias[2], torch.int64, device, rows + 1)
+        ids, values, offsets = bias
+        args.bias_ids = _vector("bias ids", ids, torch.int32, index, -1)
+        args.bias_count = ids.numel()
+        args.bias_values = _vector("bias values", values, torch.float32, index, args.bias_count)
+        args.bias_offsets = _vector("bias offsets", offsets, torch.int64, index, rows + 1)
     if masks is not None:
-        _matrix("masks", masks, (torch.int32,), device)
-        if masks.shape[1] != (symbols + 31) // 32:
-            _refuse(f"masks of {symbols} symbols have {(symbols + 31) // 32} words, not {masks.shape[1]}")
-        args.masks, args.masks_stride, args.mask_count = masks.data_ptr(), masks.stride(0), masks.shape[0]
+        args.mask_count, words, args.masks_stride = _matrix("masks", masks, (torch.int32,), index)
+        if words != (symbols + 31) // 32:
+            _refuse(f"masks of {symbols} symbols have {(symbols + 31) // 32} words, not {words}")
+        args.masks = masks.data_ptr()
+        args.mask_rows = _vector("mask_rows", mask_rows, torch.int32, index, rows)
     elif mask_rows is not None:
         _refuse("mask_rows without masks")
-    args.mask_rows = _vector("mask_rows", mask_rows, torch.int32, device, rows)
-    _call("leo_control_logits", args, device)
+    _call("leo_control_logits", args, index)
     return out
 
 
@@ -240,27 +261,24 @@ def sample(logits: torch.Tensor, noise: Optional[torch.Tensor] = None, *, temper
     -inf alone gives -1 and -inf. temperature, top_p, min_p float32 [rows] and
     top_k int32 [rows]; without them 1, 1, 0 and all.
     """
-    _matrix("logits", logits, _TYPES)
-    device = logits.device
-    rows, symbols = logits.shape
+    index = _device("logits", logits)
+    rows, symbols, stride = _matrix("logits", logits, _TYPES, index)
     if symbols < 1:
         _refuse("no symbols to draw from")
+    noise_at, noise_stride = None, 0
     if noise is not None:
-        _matrix("noise", noise, (torch.float32,), device)
-        if noise.shape != logits.shape:
-            _refuse(f"noise must be {(rows, symbols)}, not {tuple(noise.shape)}")
-    drawn = torch.empty(rows, dtype=torch.int32, device=device)
-    logprobs = torch.empty(rows, dtype=torch.float32, device=device)
+        *shape, noise_stride = _matrix("noise", noise, (torch.float32,), index)
+        if shape != [rows, symbols]:
+            _refuse(f"noise must be {(rows, symbols)}, not {tuple(shape)}")
+        noise_at = noise.data_ptr()
+    drawn = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
     args = native.LeoSample(
-        rows=rows, symbols=symbols, logits=logits.data_ptr(), logits_stride=logits.stride(0),
-        type=_TYPES[logits.dtype], noise=None if noise is None else noise.data_ptr(),
-        noise_stride=0 if noise is None else noise.stride(0),
-        temperature=_vector("temperature", temperature, torch.float32, device, rows),
-        top_k=_vector("top_k", top_k, torch.int32, device, rows),
-        top_p=_vector("top_p", top_p, torch.float32, device, rows),
-        min_p=_vector("min_p", min_p, torch.float32, device, rows),
-        out_symbols=drawn.data_ptr(), out_logprobs=logprobs.data_ptr())
-    _call("leo_sample", args, device, _sample_workspace(rows, symbols))
+        rows, symbols, logits.data_ptr(), stride, _TYPES[logits.dtype], 0, noise_at, noise_stride,
+        _vector("temperature", temperature, torch.float32, index, rows), _vector("top_k", top_k, torch.int32, index, rows),
+        _vector("top_p", top_p, torch.float32, index, rows), _vector("min_p", min_p, torch.float32, index, rows),
+        drawn.data_ptr(), logprobs.data_ptr())
+    _call("leo_sample", args, index, _sample_workspace(rows, symbols))
     return drawn, logprobs
 
 
