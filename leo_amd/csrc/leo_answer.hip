@@ -298,6 +298,10 @@ struct Above {
     }
 };
 
+__device__ __forceinline__ Above wave_above(const Above& v) {
+    return {wave_sum(v.count), wave_sum(v.mass), wave_race(v.best)};
+}
+
 constexpr uint32_t kMostWaves = 16, kRowWaves = 8;
 struct SampleShared {
     Racer best[kMostWaves];
@@ -307,57 +311,74 @@ struct SampleShared {
 
 // What stays is a prefix of the values in falling order, so one value decides:
 // the race's winner over the whole row is the answer if it stays; if not, no
-// value up to its own stays, and the race is held again above. A second value,
-// halfway (in the order of floats) to the lowest one known to stay, is tried in
-// the same sweep, which bounds the sweeps by the 32 bits of a float. sweep(low,
-// high, above) adds what a thread holds above either; all threads take part.
-// `probe`, where it lies above the winner, is tried first: a value that is
-// likely not to stay and has little above it.
-template <class Sweep>
-__device__ __forceinline__ void settle(const LeoSample& a, const Rules& r, uint64_t row, float top, float whole, Racer best,
-                                       float probe, SampleShared& shared, Sweep&& sweep) {
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64;
-    if (r.filtered && top > negative_infinity()) {
-        const auto stays = [&](float z, const Above& v) {
-            return v.count < r.top_k && (r.top_p >= 1.0f || v.mass < r.top_p * whole) && mass_of(z, top) >= r.min_p;
-        };
-        float lowest = top;  // of the values known to stay
-        for (uint32_t turn = 0; best.z < lowest; turn ^= 1) {
-            const bool probing = probe > best.z && probe < lowest;
-            const float low = probing ? probe : best.z;
-            const uint32_t key = order_key(low);
-            const float high = from_order_key(key + (order_key(lowest) - key) / 2);
-            Above above[2] = {{0, 0.0f, nobody()}, {0, 0.0f, nobody()}};
-            sweep(low, high, above);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                above[h] = {wave_sum(above[h].count), wave_sum(above[h].mass), wave_race(above[h].best)};
-                if (waves > 1 && lane == 0) shared.above[turn][h][wave] = above[h];
-            }
-            if (waves > 1) {
-                __syncthreads();
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const Above v = lane < waves ? shared.above[turn][h][lane] : Above{0, 0.0f, nobody()};
-                    above[h] = {wave_sum(v.count), wave_sum(v.mass), wave_race(v.best)};
-                }
-            }
-            if (stays(low, above[0])) {
-                if (!probing) break;
-                lowest = low;
-            } else if (stays(high, above[1])) {
-                lowest = high;
-                best = above[0].best;
-            } else {
-                best = above[1].best;
-            }
-            probe = negative_infinity();
+// value up to its own stays, and the race is held again above.
+struct Search {
+    float top, whole;  // the row's largest value and its mass
+    float lowest;      // of the values known to stay
+    Racer best;        // the winner among what is not known not to stay
+
+    __device__ __forceinline__ bool open(const Rules& r) const { return r.filtered && best.z < lowest; }
+    // Halfway, in the order of floats, to the lowest value known to stay.
+    __device__ __forceinline__ float halfway(float low) const {
+        const uint32_t key = order_key(low);
+        return from_order_key(key + (order_key(lowest) - key) / 2);
+    }
+    // Whether a value stays that has this above it.
+    __device__ __forceinline__ bool stays(const Rules& r, float z, const Above& v) const {
+        return v.count < r.top_k && (r.top_p >= 1.0f || v.mass < r.top_p * whole) && mass_of(z, top) >= r.min_p;
+    }
+    // Takes what lies above a value that is not below the winner's, and above a
+    // higher one, if that was tried.
+    __device__ __forceinline__ void narrow(const Rules& r, float low, float high, const Above (&above)[2], bool both) {
+        if (stays(r, low, above[0])) {
+            lowest = low;
+        } else if (!both) {
+            best = above[0].best;
+        } else if (stays(r, high, above[1])) {
+            lowest = high;
+            best = above[0].best;
+        } else {
+            best = above[1].best;
         }
     }
+};
+
+// Narrows a search until it is decided, and stores its answer. `probe`, where it
+// lies above the winner, is tried before: a value that is likely not to stay and
+// has little above it. Few turns are enough where the noise is what it should
+// be; from the fifth on a second value is tried with each, halfway to the lowest
+// one known to stay, which bounds the turns by the 32 bits of a float. sweep(low,
+// high, above) adds what a thread holds above either; all threads take part.
+template <class Sweep>
+__device__ __forceinline__ void settle(const LeoSample& a, const Rules& r, uint64_t row, Search s, float probe, SampleShared& shared,
+                                       Sweep&& sweep) {
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64;
+    for (uint32_t turn = 0; s.open(r); ++turn) {
+        const bool probing = probe > s.best.z && probe < s.lowest, both = turn >= 4;
+        const float low = probing ? probe : s.best.z, high = both ? s.halfway(low) : __builtin_inff();
+        Above above[2] = {{0, 0.0f, nobody()}, {0, 0.0f, nobody()}};
+        sweep(low, high, above);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (h == 1 && !both) break;
+            above[h] = wave_above(above[h]);
+            if (waves > 1 && lane == 0) shared.above[turn % 2][h][wave] = above[h];
+        }
+        if (waves > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (h == 1 && !both) break;
+                above[h] = wave_above(lane < waves ? shared.above[turn % 2][h][lane] : Above{0, 0.0f, nobody()});
+            }
+        }
+        s.narrow(r, low, high, above, both);
+        probe = negative_infinity();
+    }
     if (threadIdx.x == 0) {
-        const bool empty = top == negative_infinity();
-        a.out_symbols[row] = empty ? -1 : static_cast<int32_t>(best.at);
-        a.out_logprobs[row] = empty ? negative_infinity() : (best.z == top ? 0.0f : best.z - top) - logf(whole);
+        const bool empty = s.top == negative_infinity();
+        a.out_symbols[row] = empty ? -1 : static_cast<int32_t>(s.best.at);
+        a.out_logprobs[row] = empty ? negative_infinity() : (s.best.z == s.top ? 0.0f : s.best.z - s.top) - logf(s.whole);
     }
 }
 
@@ -393,15 +414,15 @@ __global__ __launch_bounds__(kRowWaves * 64) void leo_sample_row(LeoSample a) {
         mass = wave_sum(theirs > negative_infinity() ? shared.mass[lane] * mass_of(theirs, top) : 0.0f);
         best = wave_race(lane < waves ? shared.best[lane] : nobody());
     }
-    settle(a, r, row, top, mass, best, negative_infinity(), shared, [&](float low, float high, Above (&above)[2]) {
+    settle(a, r, row, {top, mass, top, best}, negative_infinity(), shared, [&](float low, float high, Above (&above)[2]) {
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i)
             add_above(low, high, top, span.z[i], span.key(r, i), Span<T>::index(wave * kSpan, i), above);
     });
 }
 
-// Longer rows: one wave a span leaves its part of the result, and one workgroup
-// a row settles the rest.
+// Longer rows take two launches: one wave a span weighs it and holds its race,
+// and one workgroup a row settles the rest from the spans' records.
 struct SpanRecord {
     Racer best;
     float top, mass;
@@ -422,11 +443,12 @@ __global__ __launch_bounds__(256) void leo_sample_spans(LeoSample a, uint32_t sp
     if (threadIdx.x % 64 == 0) records[row * spans + which] = rec;
 }
 
-// What lies above a pivot is first gathered in LDS, by each lane in its own
-// column, and counted and weighed from there: a row has few such values where
-// its rules leave few, and one compare a value passes over the others. If no
-// column runs over, later pivots, which are higher, need the columns alone.
+// What lies above a value is first gathered in LDS, by each lane in its own
+// column, and counted and weighed from there: one compare a logit passes over
+// the others. If no column runs over, later values, which are higher, need the
+// columns alone.
 constexpr uint32_t kColumn = 12, kTogether = 2;
+constexpr float kProbe = 1.5f;
 struct Column {
     float z[kColumn][64], key[kColumn][64];
     uint32_t at[kColumn][64];
@@ -448,8 +470,9 @@ __global__ __launch_bounds__(kMostWaves * 64) void leo_sample_settle(LeoSample a
     float top = negative_infinity(), mass = 0.0f, sum = 0.0f, squares = 0.0f;
     uint32_t counted = 0;
     Racer best = nobody();
-    for (uint32_t s = lane; s < spans; s += 64) {
-        const SpanRecord rec = records[s];
+#pragma unroll 2
+    for (uint32_t i = lane; i < spans; i += 64) {
+        const SpanRecord rec = records[i];
         if (rec.top == negative_infinity()) continue;
         const float higher = fmaxf(top, rec.top);
         mass = (top > negative_infinity() ? mass * mass_of(top, higher) : 0.0f) + rec.mass * mass_of(rec.top, higher);
@@ -462,46 +485,47 @@ __global__ __launch_bounds__(kMostWaves * 64) void leo_sample_settle(LeoSample a
     const float mine = top;
     top = wave_max(top);
     mass = wave_sum(mine > negative_infinity() ? mass * mass_of(mine, top) : 0.0f);
-    best = wave_race(best);
-    // A first pivot with a few values of each span above it: one and a half
-    // standard deviations below the mean of the spans' largest values, or where
-    // min_p cuts, if that is higher.
+    const Search s = {top, mass, top, wave_race(best)};
+    // The value that is tried first, with a few of each span's above it: kProbe
+    // standard deviations below the mean of the spans' largest, or where min_p
+    // cuts.
     float probe = negative_infinity();
-    if (r.filtered && top > negative_infinity()) {
+    if (s.open(r)) {
         const float count = static_cast<float>(wave_sum(counted)), mean = wave_sum(sum) / count;
-        probe = mean - 1.5f * sqrtf(fmaxf(wave_sum(squares) / count - mean * mean, 0.0f));
+        probe = mean - kProbe * sqrtf(fmaxf(wave_sum(squares) / count - mean * mean, 0.0f));
         if (r.min_p > 0.0f) probe = fmaxf(probe, top + logf(r.min_p) * 1.0001f - 0.0001f);
     }
 
     Column& column = columns[wave];
-    uint32_t filled = 0;     // of this lane's column
+    uint32_t filled = 0;            // of this lane's column
     float held = __builtin_inff();  // the wave's columns hold all there is above this
-    settle(a, r, row, top, mass, best, probe, shared, [&](float low, float high, Above (&above)[2]) {
-        const auto weigh = [&](bool fresh) {
-            if (fresh) {  // logits so far; their noise comes all at once
-                float race[kColumn];
-#pragma unroll
-                for (uint32_t c = 0; c < kColumn; ++c)
-                    if (c < filled) race[c] = noise[column.at[c][lane]];
-#pragma unroll
-                for (uint32_t c = 0; c < kColumn; ++c)
-                    if (c < filled) {
-                        const float z = r.divided(column.z[c][lane]);
-                        column.z[c][lane] = z;
-                        column.key[c][lane] = z + race[c];
-                    }
-            }
+    settle(a, r, row, s, probe, shared, [&](float low, float high, Above (&above)[2]) {
+        const auto weigh = [&] {
             for (uint32_t c = 0; __any(c < filled); ++c)
                 if (c < filled) add_above(low, high, top, column.z[c][lane], column.key[c][lane], column.at[c][lane], above);
         };
-        if (low >= held) return weigh(false);
+        if (low >= held) return weigh();
+        const auto weigh_logits = [&] {  // their noise comes all at once
+            float race[kColumn];
+#pragma unroll
+            for (uint32_t c = 0; c < kColumn; ++c)
+                if (c < filled) race[c] = noise[column.at[c][lane]];
+#pragma unroll
+            for (uint32_t c = 0; c < kColumn; ++c)
+                if (c < filled) {
+                    const float z = r.divided(column.z[c][lane]);
+                    column.z[c][lane] = z;
+                    column.key[c][lane] = z + race[c];
+                }
+            weigh();
+        };
         // z above low needs a logit above this, whatever the division rounds
-        const float bar = low * r.t - (fabsf(low * r.t) * 0x1p-20f + 0x1p-120f);
+        const float least = low * r.t - (fabsf(low * r.t) * 0x1p-20f + 0x1p-120f);
         held = low;
         filled = 0;
         for (uint32_t from = wave; from < spans; from += kMostWaves * 64) {
-            const uint32_t mine_at = from + lane * kMostWaves;
-            uint64_t left = __ballot(mine_at < spans && records[min(mine_at, spans - 1)].top > low);
+            const uint32_t mine = from + lane * kMostWaves;
+            uint64_t left = __ballot(mine < spans && records[min(mine, spans - 1)].top > low);
             while (left) {
                 uint32_t base[kTogether];
                 bool some[kTogether];
@@ -521,12 +545,12 @@ __global__ __launch_bounds__(kMostWaves * 64) void leo_sample_settle(LeoSample a
 #pragma unroll
                     for (uint32_t i = 0; i < kEach; ++i) {
                         if (i % 4 == 0 && __any(filled > kColumn - 4)) {
-                            weigh(true);
+                            weigh_logits();
                             filled = 0;
                             held = __builtin_inff();
                         }
                         const float logit = T::at(raw[u][i / kWide], i % kWide);
-                        if (logit > bar) {
+                        if (logit > least) {
                             column.z[filled][lane] = logit;
                             column.at[filled][lane] = Span<T>::index(base[u], i);
                             filled += 1;
@@ -535,7 +559,7 @@ __global__ __launch_bounds__(kMostWaves * 64) void leo_sample_settle(LeoSample a
                 }
             }
         }
-        weigh(true);
+        weigh_logits();
     });
 }
 
@@ -548,8 +572,7 @@ SamplePlan sample_plan(uint64_t rows, uint64_t symbols) {
     SamplePlan p{};
     p.spans = static_cast<uint32_t>((symbols + kSpan - 1) / kSpan);
     p.whole = p.spans <= kRowWaves;
-    if (p.whole) return p;
-    p.workspace = rows * p.spans * sizeof(SpanRecord);
+    p.workspace = p.whole ? 0 : rows * p.spans * sizeof(SpanRecord);
     return p;
 }
 
@@ -559,8 +582,7 @@ void launch_sample(const SamplePlan& p, const LeoSample& s, hipStream_t stream) 
     if (p.whole) return launch(leo_sample_row<T>, dim3(rows), dim3(p.spans * 64), 0, stream, s);
     auto* records = static_cast<SpanRecord*>(s.workspace);
     launch(leo_sample_spans<T>, dim3((p.spans + 3) / 4, rows), dim3(256), 0, stream, s, p.spans, records);
-    launch(leo_sample_settle<T>, dim3(rows), dim3(kMostWaves * 64), 0, stream, s, p.spans,
-           static_cast<const SpanRecord*>(records));
+    launch(leo_sample_settle<T>, dim3(rows), dim3(kMostWaves * 64), 0, stream, s, p.spans, static_cast<const SpanRecord*>(records));
 }
 
 }  // namespace
