@@ -115,6 +115,9 @@ typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 
+// The same for all of a wave's lanes, so what follows from it is scalar.
+__device__ __forceinline__ uint32_t wave_of_workgroup() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64); }
+
 struct TileArgs {
     const char* codes;
     const char* scales;
@@ -130,6 +133,9 @@ struct TileArgs {
     uint32_t slices, slice_blocks;
     uint32_t row_bits, stage_blocks;  // of leo_q4_few: its rows rounded up to a power of two, blocks of x in LDS at a time
     float* partials;  // [slice][row][16 tiles], where there are several slices
+    const half8* ready;
+    const float* factors;
+    uint32_t row_tiles;
 };
 
 // Eight neighbouring inputs of a row, as the type has them in memory.
@@ -217,6 +223,14 @@ __device__ __forceinline__ void halves(const Eight<X>& v, float factor, half8 (&
     }
 }
 
+// word & mask | high in one instruction: two constants in one need a register,
+// which the compiler does not spend by itself.
+__device__ __forceinline__ uint32_t and_or(uint32_t word, uint32_t mask, uint32_t high) {
+    uint32_t v;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(v) : "v"(word), "s"(mask), "v"(high));
+    return v;
+}
+
 // Four pairs of codes less their zero, exactly: in half precision 1024 + u is
 // the bits 0x6400 | u and 1024 + 16 u the bits 0x6400 | u << 4.
 __device__ __forceinline__ half8 weights_of(uint32_t word, half2 minus, half2 minus_high) {
@@ -227,10 +241,10 @@ __device__ __forceinline__ half8 weights_of(uint32_t word, half2 minus, half2 mi
         half8 v;
     } u;
     const uint32_t next = word >> 8;
-    u.w[0] = (word & 0x000f000fu) | 0x64006400u;
-    u.w[1] = (word & 0x00f000f0u) | 0x64006400u;
-    u.w[2] = (next & 0x000f000fu) | 0x64006400u;
-    u.w[3] = (next & 0x00f000f0u) | 0x64006400u;
+    u.w[0] = and_or(word, 0x000f000fu, 0x64006400u);
+    u.w[1] = and_or(word, 0x00f000f0u, 0x64006400u);
+    u.w[2] = and_or(next, 0x000f000fu, 0x64006400u);
+    u.w[3] = and_or(next, 0x00f000f0u, 0x64006400u);
     u.h[0] = u.h[0] + minus;
     u.h[1] = __builtin_elementwise_fma(u.h[1], sixteenth, minus_high);
     u.h[2] = u.h[2] + minus;
@@ -246,28 +260,32 @@ struct WeightBlock {
     uint32_t scale[kScaleWords];
     uint32_t zero;
 
+    // `at` is the same for the whole wave: its addresses are a scalar and an
+    // offset that stays.
     __device__ __forceinline__ void load(const TileArgs& a, uint64_t at, uint32_t lane) {
         const uint32_t column = lane % kTile;
-        code = reinterpret_cast<const uint4v*>(a.codes)[at * 64 + lane];
-        const uint64_t group = (at * kTile + column) * kGroups;
+        code = reinterpret_cast<const uint4v*>(a.codes + at * kBlockBytes)[lane];
+        const char* of_block = a.scales + at * (kTile * kGroups * (kWide ? 4 : 2));
         if constexpr (!kWide && kGroups == 1) {
-            scale[0] = reinterpret_cast<const uint16_t*>(a.scales)[group];
+            scale[0] = reinterpret_cast<const uint16_t*>(of_block)[column];
         } else {
-            __builtin_memcpy(scale, __builtin_assume_aligned(a.scales + group * (kWide ? 4 : 2), sizeof(scale)),
+            __builtin_memcpy(scale, __builtin_assume_aligned(of_block + column * (kGroups * (kWide ? 4 : 2)), sizeof(scale)),
                              sizeof(scale));
         }
         if constexpr (kZero) {
-            if constexpr (kGroups == 4) zero = reinterpret_cast<const uint16_t*>(a.zeros)[at * kTile + column];
-            else zero = reinterpret_cast<const uint8_t*>(a.zeros)[at * kTile + column];
+            if constexpr (kGroups == 4) zero = reinterpret_cast<const uint16_t*>(a.zeros + at * (kTile * 2))[column];
+            else zero = reinterpret_cast<const uint8_t*>(a.zeros + at * kTile)[column];
         }
     }
-    __device__ __forceinline__ float scale_of(int g, bool bf16) const {
+    // `bf16` has every bit set where the scales are bf16; a branch here would
+    // part the matrix instructions of one group from the next's.
+    __device__ __forceinline__ float scale_of(int g, uint32_t bf16) const {
         if constexpr (kWide) {
             return __uint_as_float(scale[g]);
         } else {
-            const uint32_t bits = scale[g / 2] >> (16 * (g % 2)) & 0xffffu;
-            return bf16 ? __uint_as_float(bits << 16)
-                        : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+            const uint32_t bits = scale[g / 2] >> (16 * (g % 2));
+            const uint32_t half = __float_as_uint(static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits))));
+            return __uint_as_float((bits << 16 & bf16) | (half & ~bf16));
         }
     }
     // The 8 weights of a lane in matrix instruction j of the block.
@@ -290,19 +308,24 @@ template <class X>
 struct XBlock {
     static constexpr bool kScaled = !__is_same(X, F16);  // x goes to half precision by a power of two a row and block
     static constexpr int kParts = __is_same(X, F32) ? 2 : 1;
+    static constexpr bool kWhole = false;
     Eight<X> v[4];
 
+    static __device__ __forceinline__ int64_t place(const TileArgs& a, uint32_t row, uint32_t block, uint32_t quad) {
+        return min(row, a.rows - 1) * a.x_stride + static_cast<int64_t>(block) * kBlock + quad * 8;
+    }
+    // A block inside the row.
     __device__ __forceinline__ void load(const TileArgs& a, uint32_t row, uint32_t block, uint32_t quad) {
-        const int64_t at = min(row, a.rows - 1) * a.x_stride + static_cast<int64_t>(block) * kBlock + quad * 8;
-        const uint32_t inside = a.inputs - block * kBlock;
-        if (inside >= kBlock) {
+        const int64_t at = place(a, row, block, quad);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = load_eight<X>(a.x, at + 32 * j);
-        } else {
+        for (int j = 0; j < 4; ++j) v[j] = load_eight<X>(a.x, at + 32 * j);
+    }
+    // The block in which it ends.
+    __device__ __forceinline__ void load_last(const TileArgs& a, uint32_t row, uint32_t block, uint32_t quad) {
+        const int64_t at = place(a, row, block, quad);
+        const int32_t inside = static_cast<int32_t>(a.inputs - block * kBlock) - 8 * static_cast<int32_t>(quad);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                v[j] = load_some<X>(a.x, at + 32 * j, static_cast<int32_t>(inside) - 32 * j - 8 * static_cast<int32_t>(quad));
-        }
+        for (int j = 0; j < 4; ++j) v[j] = load_some<X>(a.x, at + 32 * j, inside - 32 * j);
     }
     // Writes part p of instruction j to at(p, j); returns the factor that takes
     // sums over the block back to x's values. Lanes of one row take part together.
@@ -328,6 +351,56 @@ struct XBlock {
     }
 };
 
+// x as leo_q4_prepare leaves it: [block][16 rows][part][instruction][lane], then
+// the factors [block][row].
+template <int kPartsOf, bool kScaledOf>
+struct Ready {};
+
+template <int kPartsOf, bool kScaledOf>
+struct XBlock<Ready<kPartsOf, kScaledOf>> {
+    static constexpr bool kScaled = kScaledOf;
+    static constexpr int kParts = kPartsOf;
+    static constexpr bool kWhole = true;  // a row's end is filled up
+    half8 v[kParts][4];
+    float factor;
+
+    static __device__ __forceinline__ uint64_t place(const TileArgs& a, uint32_t row, uint32_t block) {
+        return static_cast<uint64_t>(block) * a.row_tiles + row / 16;
+    }
+    __device__ __forceinline__ void load(const TileArgs& a, uint32_t row, uint32_t block, uint32_t) {
+        const half8* from = a.ready + place(a, row, block) * (kParts * 256) + threadIdx.x % 64;
+#pragma unroll
+        for (int p = 0; p < kParts; ++p)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[p][j] = from[(p * 4 + j) * 64];
+        if constexpr (kScaled) factor = a.factors[place(a, row, block) * 16 + row % 16];
+    }
+    template <class At>
+    __device__ __forceinline__ float store(At&& at) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) *at(p, j) = v[p][j];
+        return kScaled ? factor : 1.0f;
+    }
+};
+
+// Brings x into that form once for all workgroups of a product: one wave 16 rows
+// of a block.
+template <class X>
+__global__ __launch_bounds__(256) void leo_q4_prepare(TileArgs a, half8* ready, float* factors) {
+    const uint32_t lane = threadIdx.x % 64, block = blockIdx.x, tile = blockIdx.y * 4 + threadIdx.x / 64;
+    if (tile >= a.row_tiles) return;
+    const uint32_t row = tile * 16 + lane % 16, quad = lane / 16;
+    XBlock<X> x;
+    if ((block + 1) * kBlock <= a.inputs) x.load(a, row, block, quad);
+    else x.load_last(a, row, block, quad);
+    const uint64_t place = static_cast<uint64_t>(block) * a.row_tiles + tile;
+    half8* to = ready + place * (XBlock<X>::kParts * 256) + lane;
+    const float factor = x.store([&](uint32_t p, uint32_t j) { return to + (p * 4 + j) * 64; });
+    if (XBlock<X>::kScaled && quad == 0) factors[place * 16 + lane] = factor;
+}
+
 // Few rows: one workgroup takes kFewTiles tiles of 16 outputs and a slice of
 // the inputs, its eight waves the slice's blocks in turn. x goes through LDS
 // once a workgroup, in the order in which matrix instructions take it; the 16
@@ -340,7 +413,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void leo_q4_few(TileArgs a) {
     constexpr bool kScaled = XBlock<X>::kScaled;
     constexpr int kParts = XBlock<X>::kParts;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const uint32_t lane = threadIdx.x % 64, wave = wave_of_workgroup();
     const uint32_t column = lane % 16, quad = lane / 16;
     const uint32_t bits = a.row_bits;
     const uint32_t begin = blockIdx.y * a.slice_blocks, end = min(begin + a.slice_blocks, a.blocks);
@@ -358,18 +431,22 @@ __global__ __launch_bounds__(kFewWaves * 64) void leo_q4_few(TileArgs a) {
     for (uint32_t from = begin; from < end; from += a.stage_blocks) {
         const uint32_t to = min(from + a.stage_blocks, end);
         WeightBlock<kGroups, kZero, kWide> ring[kAhead][kFewTiles];
+        // Loads run on past the stage's end, to its last block again: a load under a condition would make every wait one
+        // for all of them.
+        const auto load_weights = [&](uint32_t u, uint32_t block) {
 #pragma unroll
-        for (uint32_t u = 0; u < kAhead; ++u)
-            if (from + wave + u * kFewWaves < to)
+            for (uint32_t t = 0; t < kFewTiles; ++t) ring[u][t].load(a, tile_at[t] + min(block, to - 1), lane);
+        };
 #pragma unroll
-                for (uint32_t t = 0; t < kFewTiles; ++t) ring[u][t].load(a, tile_at[t] + from + wave + u * kFewWaves, lane);
+        for (uint32_t u = 0; u < kAhead; ++u) load_weights(u, from + wave + u * kFewWaves);
         if (from != begin) __syncthreads();
         const uint32_t row = column & ((1u << bits) - 1), ahead = column >> bits, step = 16u >> bits;
         for (uint32_t first = from + wave * step; first < to; first += kFewWaves * step) {
             const uint32_t block = first + ahead, in_stage = block - from;
             if (block < to) {
                 XBlock<X> x;
-                x.load(a, row, block, quad);
+                if ((block + 1) * kBlock <= a.inputs) x.load(a, row, block, quad);
+                else x.load_last(a, row, block, quad);
                 const float factor = x.store([&](uint32_t p, uint32_t j) { return parts + part_at(in_stage, p, j, quad) + row; });
                 if (kScaled && quad == 0) back[in_stage * back_rows + row] = factor;
             }
@@ -416,11 +493,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void leo_q4_few(TileArgs a) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) sum[t][i] = __builtin_fmaf(f[i], whole[t][i], sum[t][i]);
                     }
-                    if (block + kAhead * kFewWaves < to)
-#pragma unroll
-                        for (uint32_t t = 0; t < kFewTiles; ++t)
-                            ring[u][t].load(a, tile_at[t] + block + kAhead * kFewWaves, lane);
                 }
+                load_weights(u, block + kAhead * kFewWaves);
             }
         }
     }
@@ -450,17 +524,19 @@ __global__ __launch_bounds__(kFewWaves * 64) void leo_q4_few(TileArgs a) {
 // More rows: one workgroup takes 16 kRows rows, eight tiles of outputs (two a
 // wave) and a slice of the inputs. x goes through two buffers in LDS that the
 // four waves share, each wave bringing 16 rows of one block a step, so a step is
-// 4 / kRows blocks; codes go straight to registers.
+// 4 / kRows blocks; codes go straight to registers, some blocks ahead.
 constexpr uint32_t kManyWaves = 4, kManyTiles = 2;
 
 template <class X, int kGroups, bool kZero, bool kWide, int kRows>
 __global__ __launch_bounds__(kManyWaves * 64, 2) void leo_q4_many(TileArgs a) {
     constexpr bool kScaled = XBlock<X>::kScaled;
     constexpr int kParts = XBlock<X>::kParts;
-    constexpr uint32_t kStep = kManyWaves / kRows;
+    constexpr uint32_t kRing = kRows == 4 ? 2 : 4;  // blocks ahead, as the registers allow
+    constexpr uint32_t kStep = kManyWaves / kRows, kSteps = kRing / kStep;
+    constexpr uint32_t kSets = kSteps == 1 ? 1 : 2;  // steps of x on their way; one is enough where a step is long
     __shared__ half8 parts[2][kStep][kRows][kParts][4][64];
     __shared__ __attribute__((aligned(16))) float back[2][kStep][kRows * 16];
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const uint32_t lane = threadIdx.x % 64, wave = wave_of_workgroup();
     const uint32_t column = lane % 16, quad = lane / 16;
     const uint32_t tile0 = (blockIdx.x * kManyWaves + wave) * kManyTiles, row0 = blockIdx.z * kRows * 16;
     const uint32_t begin = blockIdx.y * a.slice_blocks, end = min(begin + a.slice_blocks, a.blocks);
@@ -469,85 +545,100 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void leo_q4_many(TileArgs a) {
 #pragma unroll
     for (uint32_t t = 0; t < kManyTiles; ++t) tile_at[t] = static_cast<uint64_t>(min(tile0 + t, a.tiles - 1)) * a.blocks;
 
-    // blocks beyond the slice's last are read as that one; they are not multiplied
-    const auto stage = [&](const XBlock<X>& x, uint32_t buffer) {
-        const float factor = x.store([&](uint32_t p, uint32_t j) { return &parts[buffer][my_block][my_rows][p][j][lane]; });
+    // Blocks inside the row go through the pipeline, the one in which it ends after it. Loads run on past the last
+    // block, to that one again: a load under a condition would make every wait one for all of them.
+    const uint32_t full = XBlock<X>::kWhole ? end : min(end, a.inputs / kBlock);
+    XBlock<X> x[kSets];
+    const auto load_x = [&](XBlock<X>& v, uint32_t block) {
+        v.load(a, row0 + my_rows * 16 + column, min(block + my_block, full - 1), quad);
+    };
+    const auto stage = [&](const XBlock<X>& v, uint32_t buffer) {
+        const float factor = v.store([&](uint32_t p, uint32_t j) { return &parts[buffer][my_block][my_rows][p][j][lane]; });
         if (kScaled && quad == 0) back[buffer][my_block][my_rows * 16 + column] = factor;
     };
-    const auto load_x = [&](XBlock<X>& x, uint32_t block) {
-        x.load(a, row0 + my_rows * 16 + column, min(block + my_block, end - 1), quad);
-    };
     float4v sum[kManyTiles][kRows] = {};
-    WeightBlock<kGroups, kZero, kWide> now[kStep][kManyTiles], next[kStep][kManyTiles];
-    const auto load_weights = [&](WeightBlock<kGroups, kZero, kWide> (&w)[kStep][kManyTiles], uint32_t block) {
+    WeightBlock<kGroups, kZero, kWide> ring[kRing][kManyTiles];
+    const auto load_weights = [&](uint32_t u, uint32_t block) {
 #pragma unroll
-        for (uint32_t b = 0; b < kStep; ++b)
-#pragma unroll
-            for (uint32_t t = 0; t < kManyTiles; ++t) w[b][t].load(a, tile_at[t] + min(block + b, end - 1), lane);
+        for (uint32_t t = 0; t < kManyTiles; ++t) ring[u][t].load(a, tile_at[t] + block, lane);
     };
-    XBlock<X> x;
-    load_weights(now, begin);
-    load_x(x, begin);
-    stage(x, 0);
-    __syncthreads();
-    uint32_t buffer = 0;
-    for (uint32_t block = begin; block < end; block += kStep, buffer = 1 - buffer) {
-        const bool more = block + kStep < end;
-        if (more) {
-            load_weights(next, block + kStep);
-            load_x(x, block + kStep);
-        }
+    const auto multiply = [&](uint32_t u, uint32_t buffer, uint32_t b) {
+        float4v whole[kManyTiles][kRows] = {};
 #pragma unroll
-        for (uint32_t b = 0; b < kStep; ++b) {
-            if (block + b >= end) break;
-            float4v whole[kManyTiles][kRows] = {};
+        for (int g = 0; g < kGroups; ++g) {
+            float4v d[kManyTiles][kRows] = {};
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
-                float4v d[kManyTiles][kRows] = {};
+            for (int j = g * 4 / kGroups; j < (g + 1) * 4 / kGroups; ++j) {
+                half8 w[kManyTiles];
 #pragma unroll
-                for (int j = g * 4 / kGroups; j < (g + 1) * 4 / kGroups; ++j) {
-                    half8 w[kManyTiles];
+                for (uint32_t t = 0; t < kManyTiles; ++t) w[t] = ring[u][t].weights(j);
 #pragma unroll
-                    for (uint32_t t = 0; t < kManyTiles; ++t) w[t] = now[b][t].weights(j);
+                for (int m = 0; m < kRows; ++m)
 #pragma unroll
-                    for (int m = 0; m < kRows; ++m)
+                    for (int p = 0; p < kParts; ++p) {
+                        const half8 v = parts[buffer][b][m][p][j][lane];
 #pragma unroll
-                        for (int p = 0; p < kParts; ++p) {
-                            const half8 v = parts[buffer][b][m][p][j][lane];
-#pragma unroll
-                            for (uint32_t t = 0; t < kManyTiles; ++t)
-                                d[t][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[t], d[t][m], 0, 0, 0);
-                        }
-                }
-#pragma unroll
-                for (uint32_t t = 0; t < kManyTiles; ++t) {
-                    const float scale = now[b][t].scale_of(g, a.scale_bf16);
-#pragma unroll
-                    for (int m = 0; m < kRows; ++m)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if constexpr (kScaled) whole[t][m][i] = __builtin_fmaf(scale, d[t][m][i], whole[t][m][i]);
-                            else sum[t][m][i] = __builtin_fmaf(scale, d[t][m][i], sum[t][m][i]);
-                        }
-                }
+                        for (uint32_t t = 0; t < kManyTiles; ++t)
+                            d[t][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[t], d[t][m], 0, 0, 0);
+                    }
             }
-            if constexpr (kScaled) {
 #pragma unroll
-                for (int m = 0; m < kRows; ++m) {
-                    const float4v f = *reinterpret_cast<const float4v*>(&back[buffer][b][m * 16 + quad * 4]);
+            for (uint32_t t = 0; t < kManyTiles; ++t) {
+                const float scale = ring[u][t].scale_of(g, a.scale_bf16);
 #pragma unroll
-                    for (uint32_t t = 0; t < kManyTiles; ++t)
+                for (int m = 0; m < kRows; ++m)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) sum[t][m][i] = __builtin_fmaf(f[i], whole[t][m][i], sum[t][m][i]);
-                }
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (kScaled) whole[t][m][i] = __builtin_fmaf(scale, d[t][m][i], whole[t][m][i]);
+                        else sum[t][m][i] = __builtin_fmaf(scale, d[t][m][i], sum[t][m][i]);
+                    }
             }
         }
-        if (more) stage(x, 1 - buffer);
+        if constexpr (kScaled) {
+#pragma unroll
+            for (int m = 0; m < kRows; ++m) {
+                const float4v f = *reinterpret_cast<const float4v*>(&back[buffer][b][m * 16 + quad * 4]);
+#pragma unroll
+                for (uint32_t t = 0; t < kManyTiles; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[t][m][i] = __builtin_fmaf(f[i], whole[t][m][i], sum[t][m][i]);
+            }
+        }
+    };
+    if (begin < full) {
+        load_x(x[0], begin);
+        if constexpr (kSets == 2) load_x(x[1], begin + kStep);
+#pragma unroll
+        for (uint32_t u = 0; u < kRing; ++u) load_weights(u, min(begin + u, full - 1));
+        stage(x[0], 0);
         __syncthreads();
+        uint32_t odd = 0;  // the buffer of a round of one step
+        for (uint32_t block = begin; block < full; block += kRing, odd ^= 1) {
 #pragma unroll
-        for (uint32_t b = 0; b < kStep; ++b)
+            for (uint32_t s = 0; s < kSteps; ++s) {
+                const uint32_t at = block + s * kStep, buffer = kSets == 2 ? s % 2 : odd;
+                if (at >= full) break;
+                load_x(x[s % kSets], at + kSets * kStep);
 #pragma unroll
-            for (uint32_t t = 0; t < kManyTiles; ++t) now[b][t] = next[b][t];
+                for (uint32_t b = 0; b < kStep; ++b) {
+                    if (at + b < full) multiply(s * kStep + b, buffer, b);
+                    load_weights(s * kStep + b, min(at + b + kRing, full - 1));
+                }
+                stage(x[(s + 1) % kSets], 1 - buffer);
+                __syncthreads();
+            }
+        }
+    }
+    if constexpr (!XBlock<X>::kWhole) {
+        if (full < end && begin <= full) {
+            load_weights(0, full);
+            if (my_block == 0) {
+                x[0].load_last(a, row0 + my_rows * 16 + column, full, quad);
+                stage(x[0], 0);
+            }
+            __syncthreads();
+            multiply(0, 0, 0);
+        }
     }
 
     // register (t, m, i) of a lane is output 16 (tile0 + t) + column and row 16 m + 4 quad + i
@@ -601,14 +692,14 @@ __global__ __launch_bounds__(256) void leo_q4_join(TileArgs a) {
         store_any(a.y, row * a.y_stride + output, sum + (a.bias ? a.bias[output] : 0.0f), a.y_type);
 }
 
-constexpr uint32_t kStageBytes = 32 << 10, kFewGroups = 768, kManyGroups = 512, kFewRows = 4;
+constexpr uint32_t kStageBytes = 64 << 10, kFewGroups = 512, kManyGroups = 512, kFewRows = 4;
 
 struct Plan {
     bool few;         // leo_q4_few, else leo_q4_many
     uint32_t rows;    // of 16, of one workgroup
     uint32_t groups, slabs, slices, slice_blocks;
     uint32_t row_bits, stage_blocks, lds;
-    uint64_t workspace;
+    uint64_t ready, factors, workspace;  // places in the workspace, after the slices' sums
 };
 
 Plan plan_of(const LeoQ4Shape& s, uint64_t rows, int32_t x_type) {
@@ -625,7 +716,7 @@ Plan plan_of(const LeoQ4Shape& s, uint64_t rows, int32_t x_type) {
         while ((1u << p.row_bits) < rows) ++p.row_bits;
         const uint32_t block_bytes = (parts * 256 << p.row_bits) + 4 * std::max(1u << p.row_bits, 4u);
         const uint32_t most = std::max(kFewWaves, (kStageBytes / block_bytes) / kFewWaves * kFewWaves);
-        p.slices = std::min(over(kFewGroups, p.groups), std::max(1u, blocks / (kFewWaves * 2)));
+        p.slices = p.groups >= kFewGroups / 4 ? 1 : std::min(kFewGroups / p.groups, std::max(1u, blocks / (kFewWaves * 2)));
         p.slice_blocks = over(blocks, p.slices);
         p.stage_blocks = std::min(p.slice_blocks, most);
         p.lds = std::max(p.stage_blocks * block_bytes, kFewTiles * kFewWaves * 64 * 16);
@@ -633,22 +724,32 @@ Plan plan_of(const LeoQ4Shape& s, uint64_t rows, int32_t x_type) {
         p.rows = rows <= 16 ? 1 : rows <= 32 || x_type == LEO_TYPE_F32 ? 2 : 4;
         p.slabs = over(rows, 16 * p.rows);
         p.groups = over(l.tiles, kManyWaves * kManyTiles);
-        p.slices = std::min(over(kManyGroups, static_cast<uint64_t>(p.groups) * p.slabs), std::max(1u, blocks / 4));
+        p.slices = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(kManyGroups / (static_cast<uint64_t>(p.groups) * p.slabs), blocks / 4)));
     }
     p.slice_blocks = over(blocks, p.slices);
     p.slices = over(blocks, p.slice_blocks);
-    p.workspace = p.slices == 1 ? 0 : 4ull * p.slices * rows * l.tiles * kTile;
+    const auto up = [](uint64_t v) { return (v + 255) / 256 * 256; };
+    p.ready = p.factors = p.workspace = p.slices == 1 ? 0 : up(4ull * p.slices * rows * l.tiles * kTile);
+    if (p.rows > 1 && x_type != LEO_TYPE_F32) {  // where its rows turn out not to be aligned
+        const uint64_t places = static_cast<uint64_t>(blocks) * p.slabs * p.rows;
+        p.factors = p.ready + places * 4096;
+        p.workspace = p.factors + (x_type == LEO_TYPE_F16 ? 0 : places * 64);
+    }
     return p;
 }
 
 template <class X, int kGroups, bool kZero, bool kWide>
 void launch_tiles(const Plan& p, const TileArgs& a, hipStream_t stream) {
-    const dim3 grid(p.groups, p.slices, p.slabs);
+    using Prepared = Ready<XBlock<X>::kParts, XBlock<X>::kScaled>;
+    const dim3 grid(p.groups, p.slices, p.slabs), block(kManyWaves * 64);
     if (p.few) return launch(leo_q4_few<X, kGroups, kZero, kWide>, grid, dim3(kFewWaves * 64), p.lds, stream, a);
-    if constexpr (!__is_same(X, F32))
-        if (p.rows == 4) return launch(leo_q4_many<X, kGroups, kZero, kWide, 4>, grid, dim3(kManyWaves * 64), 0, stream, a);
-    if (p.rows == 2) return launch(leo_q4_many<X, kGroups, kZero, kWide, 2>, grid, dim3(kManyWaves * 64), 0, stream, a);
-    launch(leo_q4_many<X, kGroups, kZero, kWide, 1>, grid, dim3(kManyWaves * 64), 0, stream, a);
+    if (p.rows == 1) return launch(leo_q4_many<X, kGroups, kZero, kWide, 1>, grid, block, 0, stream, a);
+    if constexpr (!__is_same(X, F32)) {
+        if (a.ready && p.rows == 2) return launch(leo_q4_many<Prepared, kGroups, kZero, kWide, 2>, grid, block, 0, stream, a);
+        if (a.ready) return launch(leo_q4_many<Prepared, kGroups, kZero, kWide, 4>, grid, block, 0, stream, a);
+        if (p.rows == 4) return launch(leo_q4_many<X, kGroups, kZero, kWide, 4>, grid, block, 0, stream, a);
+    }
+    launch(leo_q4_many<X, kGroups, kZero, kWide, 2>, grid, block, 0, stream, a);
 }
 
 template <class X, int kGroups>
@@ -662,6 +763,9 @@ void launch_groups(const LeoQ4Shape& s, const Plan& p, const TileArgs& a, hipStr
 
 template <class X>
 void launch_products(const LeoQ4Shape& s, const Plan& p, const TileArgs& a, hipStream_t stream) {
+    if constexpr (!__is_same(X, F32))
+        if (a.ready) launch(leo_q4_prepare<X>, dim3(a.blocks, (a.row_tiles + 3) / 4), dim3(256), 0, stream, a,
+                            const_cast<half8*>(a.ready), const_cast<float*>(a.factors));
     if (s.group == 32) launch_groups<X, 4>(s, p, a, stream);
     else if (s.group == 64) launch_groups<X, 2>(s, p, a, stream);
     else launch_groups<X, 1>(s, p, a, stream);
@@ -742,7 +846,7 @@ int32_t leo_q4_matvec(const LeoQ4Product* product, void* stream) {
         a.y = p.y;
         a.y_stride = p.y_stride;
         a.y_type = p.y_type;
-        a.scale_bf16 = p.shape.scale_type == LEO_TYPE_BF16;
+        a.scale_bf16 = p.shape.scale_type == LEO_TYPE_BF16 ? ~0u : 0u;
         a.rows = static_cast<uint32_t>(p.rows);
         a.inputs = static_cast<uint32_t>(p.shape.inputs);
         a.outputs = static_cast<uint32_t>(p.shape.outputs);
@@ -752,7 +856,16 @@ int32_t leo_q4_matvec(const LeoQ4Product* product, void* stream) {
         a.slice_blocks = plan.slice_blocks;
         a.row_bits = plan.row_bits;
         a.stage_blocks = plan.stage_blocks;
-        a.partials = static_cast<float*>(p.workspace);
+        char* space = static_cast<char*>(p.workspace);
+        a.partials = reinterpret_cast<float*>(space);
+        // Loads of 16 bytes are fast at multiples of 4 only, and eight tiles a workgroup read x again for each: 64 rows of
+        // 5,001 16-bit inputs against 11,007 outputs took 43 us, and 30 with x brought into place first, 5,000 inputs 28
+        // and 29.
+        if (plan.rows > 1 && p.x_type != LEO_TYPE_F32 && (reinterpret_cast<uintptr_t>(p.x) % 4 || p.x_stride % 2)) {
+            a.ready = reinterpret_cast<const half8*>(space + plan.ready);
+            a.factors = reinterpret_cast<const float*>(space + plan.factors);
+        }
+        a.row_tiles = plan.slabs * plan.rows;
         const auto at = static_cast<hipStream_t>(stream);
         if (p.x_type == LEO_TYPE_F32) launch_products<F32>(p.shape, plan, a, at);
         else if (p.x_type == LEO_TYPE_F16) launch_products<F16>(p.shape, plan, a, at);
