@@ -17,8 +17,10 @@ before the first call into libleo_hip.so.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import sys
-from typing import Dict, Optional, Tuple
+from typing import Optional, Tuple
 
 from . import native
 
@@ -55,20 +57,6 @@ def _matrix(name: str, t: torch.Tensor, dtypes, index: int) -> Tuple[int, int, i
     _refuse(f"{name} has type {t.dtype}" if t.dtype not in dtypes else f"{name} must have two axes, not {t.dim()}")
 
 
-def _vector(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, index: int, count: int) -> Optional[int]:
-    """The address of a dense 1-D tensor of `count` entries (any number below 0), None for none."""
-    if t is None:
-        return None
-    if (isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype is dtype and t.dim() == 1
-            and t.is_contiguous() and (count < 0 or t.numel() == count)):
-        return t.data_ptr()
-    if _device(name, t) != index:
-        _refuse(f"{name} is on GPU {t.get_device()}, not on {index}")
-    if t.dtype is not dtype:
-        _refuse(f"{name} must have type {dtype}, not {t.dtype}")
-    _refuse(f"{name} must be a dense vector" + (f" of {count} entries" if count >= 0 else ""))
-
-
 def _public_stream(index: int) -> int:
     return torch.cuda.current_stream(index).cuda_stream
 
@@ -77,17 +65,19 @@ def _public_stream(index: int) -> int:
 _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", _public_stream)
 
 
-def _call(function: str, args: ctypes.Structure, index: int, need: int = 0) -> None:
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return _call(function, args, index, need)
-    lib = native.load()
-    if need:      # the caching allocator's: free again in the stream's order
-        space = torch.empty(need, dtype=torch.uint8, device=index)
-        args.workspace, args.workspace_bytes = space.data_ptr(), need
-    status = getattr(lib, function)(ctypes.byref(args), _stream_of(index))
-    if status:
-        native.check(lib, status)
+def _load_binding():
+    path = native.LIB_PATH.with_name("leo_decode_binding.so")
+    if not path.exists():
+        raise ImportError(f"{path} is missing: build it with `python -m leo_amd.build` (no fallback exists)")
+    native.load()
+    loader = importlib.machinery.ExtensionFileLoader("leo_decode_binding", str(path))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
+    loader.exec_module(module)
+    module.setup(native.LeoError, _stream_of)
+    return module
+
+
+_binding = _load_binding()   # the products', the control's and the draw's checks, results and calls
 
 
 class Q4Weight:
@@ -131,17 +121,9 @@ class Q4Weight:
             shape=self.shape, codes=codes.data_ptr(), codes_stride=codes_stride, scales=scales.data_ptr(),
             scales_stride=strides[0], zeros=None if zeros is None else zeros.data_ptr(), zeros_stride=strides[1],
             layout=self.layout.data_ptr(), layout_bytes=size.value)
-        _call("leo_q4_layout", source, self.index)
-        self._workspace_bytes: Dict[Tuple[int, int], int] = {}
-
-    def workspace_bytes(self, rows: int, x_type: int) -> int:
-        """Bytes of workspace that a product with `rows` rows of x needs."""
-        found = self._workspace_bytes.get((rows, x_type))
-        if found is None:
-            lib, size = native.load(), ctypes.c_uint64()
-            native.check(lib, lib.leo_q4_workspace_bytes(ctypes.byref(self.shape), rows, x_type, ctypes.byref(size)))
-            found = self._workspace_bytes[rows, x_type] = size.value
-        return found
+        with torch.cuda.device(self.index):
+            native.check(lib, lib.leo_q4_layout(ctypes.byref(source), _stream_of(self.index)))
+        self._shape = bytes(self.shape)
 
     @classmethod
     def quantize(cls, weight: torch.Tensor, group: int = 32, scale_dtype: torch.dtype = torch.float16) -> "Q4Weight":
@@ -169,23 +151,11 @@ def q4_matvec(x: torch.Tensor, weight: Q4Weight, bias: Optional[torch.Tensor] = 
         if out is not None:
             _refuse("out needs x with two axes")
         return q4_matvec(x[None], weight, bias, out_dtype=out_dtype)[0]
-    index = weight.index
-    rows, width, x_stride = _matrix("x", x, _TYPES, index)
-    if width != weight.inputs:
-        _refuse(f"x has {width} inputs, the weight {weight.inputs}")
     if out is None:
-        out = torch.empty((rows, weight.outputs), dtype=out_dtype or x.dtype, device=weight.device)
-        y_stride = weight.outputs
-    else:
-        *shape, y_stride = _matrix("out", out, _TYPES, index)
-        if shape != [rows, weight.outputs] or (out_dtype is not None and out.dtype is not out_dtype):
-            _refuse(f"out must be {(rows, weight.outputs)} of {out_dtype or out.dtype}")
-    x_type = _TYPES[x.dtype]
-    args = native.LeoQ4Product(
-        weight.shape, weight.layout.data_ptr(), weight.layout.numel(), rows, x.data_ptr(), x_stride,
-        _vector("bias", bias, torch.float32, index, weight.outputs), out.data_ptr(), y_stride, x_type, _TYPES[out.dtype])
-    _call("leo_q4_matvec", args, index, weight.workspace_bytes(rows, x_type))
-    return out
+        out = -1 if out_dtype is None else _TYPES.get(out_dtype, len(_TYPES))
+    elif out_dtype is not None and getattr(out, "dtype", None) is not out_dtype:
+        _refuse(f"out must have type {out_dtype}")
+    return _binding.q4_matvec(x, weight.layout, weight._shape, bias, out)
 
 
 def control_logits(logits: torch.Tensor, *, history: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
@@ -206,44 +176,10 @@ def control_logits(logits: torch.Tensor, *, history: Optional[Tuple[torch.Tensor
                without it n is 1 or the number of rows
     out        may be `logits`
     """
-    index = _device("logits", logits)
-    rows, symbols, stride = _matrix("logits", logits, _TYPES, index)
-    if out is None:
-        out = torch.empty((rows, symbols), dtype=logits.dtype, device=logits.device)
-        out_stride = symbols
-    else:
-        *shape, out_stride = _matrix("out", out, (logits.dtype,), index)
-        if shape != [rows, symbols]:
-            _refuse(f"out must be {(rows, symbols)}")
-    args = native.LeoLogitControl(rows, symbols, logits.data_ptr(), stride, out.data_ptr(), out_stride,
-                                  _TYPES[logits.dtype])
-    if history is not None:
-        entries, offsets = history
-        args.history = _vector("history", entries, torch.int32, index, -1)
-        args.history_offsets = _vector("history offsets", offsets, torch.int64, index, rows + 1)
-        args.history_count = entries.numel()
-    if repetition is not None:
-        args.repetition = _vector("repetition", repetition, torch.float32, index, rows)
-    if presence is not None:
-        args.presence = _vector("presence", presence, torch.float32, index, rows)
-    if frequency is not None:
-        args.frequency = _vector("frequency", frequency, torch.float32, index, rows)
-    if bias is not None:
-        ids, values, offsets = bias
-        args.bias_ids = _vector("bias ids", ids, torch.int32, index, -1)
-        args.bias_count = ids.numel()
-        args.bias_values = _vector("bias values", values, torch.float32, index, args.bias_count)
-        args.bias_offsets = _vector("bias offsets", offsets, torch.int64, index, rows + 1)
-    if masks is not None:
-        args.mask_count, words, args.masks_stride = _matrix("masks", masks, (torch.int32,), index)
-        if words != (symbols + 31) // 32:
-            _refuse(f"masks of {symbols} symbols have {(symbols + 31) // 32} words, not {words}")
-        args.masks = masks.data_ptr()
-        args.mask_rows = _vector("mask_rows", mask_rows, torch.int32, index, rows)
-    elif mask_rows is not None:
-        _refuse("mask_rows without masks")
-    _call("leo_control_logits", args, index)
-    return out
+    entries, offsets = (None, None) if history is None else history
+    ids, values, bias_offsets = (None, None, None) if bias is None else bias
+    return _binding.control_logits(logits, entries, offsets, repetition, presence, frequency, ids, values, bias_offsets,
+                                   masks, mask_rows, out)
 
 
 def sample(logits: torch.Tensor, noise: Optional[torch.Tensor] = None, *, temperature: Optional[torch.Tensor] = None,
@@ -261,34 +197,4 @@ def sample(logits: torch.Tensor, noise: Optional[torch.Tensor] = None, *, temper
     -inf alone gives -1 and -inf. temperature, top_p, min_p float32 [rows] and
     top_k int32 [rows]; without them 1, 1, 0 and all.
     """
-    index = _device("logits", logits)
-    rows, symbols, stride = _matrix("logits", logits, _TYPES, index)
-    if symbols < 1:
-        _refuse("no symbols to draw from")
-    noise_at, noise_stride = None, 0
-    if noise is not None:
-        *shape, noise_stride = _matrix("noise", noise, (torch.float32,), index)
-        if shape != [rows, symbols]:
-            _refuse(f"noise must be {(rows, symbols)}, not {tuple(shape)}")
-        noise_at = noise.data_ptr()
-    drawn = torch.empty(rows, dtype=torch.int32, device=logits.device)
-    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    args = native.LeoSample(
-        rows, symbols, logits.data_ptr(), stride, _TYPES[logits.dtype], 0, noise_at, noise_stride,
-        _vector("temperature", temperature, torch.float32, index, rows), _vector("top_k", top_k, torch.int32, index, rows),
-        _vector("top_p", top_p, torch.float32, index, rows), _vector("min_p", min_p, torch.float32, index, rows),
-        drawn.data_ptr(), logprobs.data_ptr())
-    _call("leo_sample", args, index, _sample_workspace(rows, symbols))
-    return drawn, logprobs
-
-
-_sample_spaces: Dict[Tuple[int, int], int] = {}
-
-
-def _sample_workspace(rows: int, symbols: int) -> int:
-    found = _sample_spaces.get((rows, symbols))
-    if found is None:
-        lib, size = native.load(), ctypes.c_uint64()
-        native.check(lib, lib.leo_sample_workspace_bytes(rows, symbols, ctypes.byref(size)))
-        found = _sample_spaces[rows, symbols] = size.value
-    return found
+    return _binding.sample(logits, noise, temperature, top_k, top_p, min_p)
