@@ -24,7 +24,11 @@ __device__ __forceinline__ Run row_run(const int64_t* offsets, uint64_t row, uin
 // its chunk, the row's last bias entry and how often the history holds it
 // (whole-number operations, whose order does not matter), and passes once over
 // the logits, 16 bytes a lane. A word holds both, 16 bits each; a row with more
-// entries than that takes its chunk by halves, with a word for each.
+// entries than that takes its chunk by halves, with a word for each. Memory bounds
+// the large calls: 128 rows of 131,075 float32 symbols with 8,192 symbols of history
+// and 300 biases a row, 138 MB, take 33 to 40 us (3.5 to 4.2 TB/s), of which the lists,
+// read once a chunk, are some 9 (31 us without them); hence the widest chunk that the
+// LDS of two workgroups a CU holds: 64 KB. A launch bounds the small: 3.7 us for 257.
 constexpr uint32_t kTable = 16384, kControlThreads = 1024;
 
 template <class T>
@@ -302,7 +306,7 @@ __device__ __forceinline__ Above wave_above(const Above& v) {
     return {wave_sum(v.count), wave_sum(v.mass), wave_race(v.best)};
 }
 
-constexpr uint32_t kMostWaves = 16, kRowWaves = 8;
+constexpr uint32_t kMostWaves = 16;
 struct SampleShared {
     Racer best[kMostWaves];
     float top[kMostWaves], mass[kMostWaves];
@@ -390,9 +394,13 @@ __device__ __forceinline__ void add_above(float low, float high, float top, floa
     }
 }
 
-// A short row, in the registers of one workgroup: one span a wave.
+// A short row, in the registers of one workgroup: one span a wave, so that logits
+// and noise are read once and every turn works on registers. A launch bounds it
+// (257 symbols: 4.5 us), then one workgroup's turns.
+// Up to 16 spans: 128 rows of 12,000 symbols took 23.0 us in the two launches below
+// and 19.5 so, of 16,000 32.1 and 20.4, one row of 12,000 9.8 and 6.8.
 template <class T>
-__global__ __launch_bounds__(kRowWaves * 64) void leo_sample_row(LeoSample a) {
+__global__ __launch_bounds__(kMostWaves * 64) void leo_sample_row(LeoSample a) {
     __shared__ SampleShared shared;
     const uint64_t row = blockIdx.x;
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64;
@@ -422,7 +430,9 @@ __global__ __launch_bounds__(kRowWaves * 64) void leo_sample_row(LeoSample a) {
 }
 
 // Longer rows take two launches: one wave a span weighs it and holds its race,
-// and one workgroup a row settles the rest from the spans' records.
+// and one workgroup a row settles the rest from the spans' records. This one reads
+// everything once and is bound by memory: 128 rows of 131,075 float32 logits with
+// noise, 134 MB, take 22.8 us (5.9 TB/s).
 struct SpanRecord {
     Racer best;
     float top, mass;
@@ -446,7 +456,12 @@ __global__ __launch_bounds__(256) void leo_sample_spans(LeoSample a, uint32_t sp
 // What lies above a value is first gathered in LDS, by each lane in its own
 // column, and counted and weighed from there: one compare a logit passes over
 // the others. If no column runs over, later values, which are higher, need the
-// columns alone.
+// columns alone. One CU's loads bound it: it reads again the spans that reach above
+// the value, a megabyte for 262,147 symbols, and 128 rows of 131,075 take 24.6 us, 16
+// rows of 32,001 11.1 and two of 262,147 14 to 46, as the values fall. A third launch
+// that gathered over all CUs gave back in latency what it saved (32,001: 5 + 7 + 10 us
+// for 5 + 11, 131,075: 23 + 22 + 21 for 23 + 25). kProbe: 1.5, 2 and 2.5 deviations
+// took 48.2, 50.6 and 58 us for both kernels at 128 rows of 131,075.
 constexpr uint32_t kColumn = 12, kTogether = 2;
 constexpr float kProbe = 1.5f;
 struct Column {
@@ -571,7 +586,7 @@ struct SamplePlan {
 SamplePlan sample_plan(uint64_t rows, uint64_t symbols) {
     SamplePlan p{};
     p.spans = static_cast<uint32_t>((symbols + kSpan - 1) / kSpan);
-    p.whole = p.spans <= kRowWaves;
+    p.whole = p.spans <= kMostWaves;
     p.workspace = p.whole ? 0 : rows * p.spans * sizeof(SpanRecord);
     return p;
 }

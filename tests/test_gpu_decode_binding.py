@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from leo_amd import decode, native
+from tests.test_gpu_decode_symbols import compare, gumbel
 
 pytestmark = pytest.mark.gpu
 DEVICE = "cuda:0"
@@ -77,3 +78,20 @@ def test_what_is_no_tensor_is_refused(require_gpu):
         with pytest.raises(native.LeoError) as err:
             call()
         assert err.value.code == native.ERR_INVALID_ARGUMENT and str(err.value)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("symbols", [16_383, 16_384, 16_385, 20_001])
+def test_draws_around_the_longest_row_of_one_workgroup(require_gpu, dtype, symbols):
+    # quarters and temperatures that are powers of two: every z is exact
+    gen = torch.Generator(DEVICE).manual_seed(symbols)
+    rows = 12
+    wide = (torch.randn(rows, symbols + 1, generator=gen, device=DEVICE) * 10).round() / 4
+    wide[3] = -torch.inf
+    noise = gumbel(gen, rows, symbols)
+    # two rows whose race the lowest value left wins each time: many turns before one that stays
+    wide[4:6] = -(torch.arange(symbols + 1, device=DEVICE) % 47) / 4
+    noise[4:6] = -5 * wide[4:6, 1:]
+    compare(wide.to(dtype)[:, 1:], noise, [0.0, 0.5, 1.0, 1.0, 1.0, 1.0] + [1.0, 2.0] * 3,
+            [40, 40, 1, 5, 3, symbols] + [symbols, 2, 40] * 2, [1.0, 0.9137, 0.5113, 1.0, 2.0, 0.9137] + [0.9137, 1.0, 0.0517] * 2,
+            [0.0, 0.0317, 0.0, 0.0, 0.0, 0.0317] + [0.0, 0.0317, 0.41] * 2)
