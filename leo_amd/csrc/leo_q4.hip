@@ -386,7 +386,7 @@ struct XBlock<Ready<kPartsOf, kScaledOf>> {
 };
 
 // Brings x into that form once for all workgroups of a product: one wave 16 rows
-// of a block.
+// of a block. A launch bounds it: 3 to 4.2 us for 64 rows of 5,001.
 template <class X>
 __global__ __launch_bounds__(256) void leo_q4_prepare(TileArgs a, half8* ready, float* factors) {
     const uint32_t lane = threadIdx.x % 64, block = blockIdx.x, tile = blockIdx.y * 4 + threadIdx.x / 64;
@@ -405,7 +405,12 @@ __global__ __launch_bounds__(256) void leo_q4_prepare(TileArgs a, half8* ready, 
 // the inputs, its eight waves the slice's blocks in turn. x goes through LDS
 // once a workgroup, in the order in which matrix instructions take it; the 16
 // row lanes of a staging wave cover several blocks, so that no lane converts a
-// row that is not there.
+// row that is not there. Instructions bound it, not memory: a tile and block of
+// 1,024 bytes of codes takes 60 to 90 of them to widen the codes and apply the
+// scales, while the matrix instructions have 15 of 16 rows idle. One row of 1,048,576
+// float32 inputs to 257 outputs (147 MB) takes 35.1 us, 4.2 TB/s; 8,192 to 8,192 in
+// bfloat16 (35 MB) 9.3 us, 3.7 TB/s; 1,024 to 257 a launch, 4.7 us. Two tiles a
+// workgroup: x is brought into LDS half as often.
 constexpr uint32_t kFewWaves = 8, kAhead = 2, kFewTiles = 2;
 
 template <class X, int kGroups, bool kZero, bool kWide>
@@ -524,7 +529,11 @@ __global__ __launch_bounds__(kFewWaves * 64) void leo_q4_few(TileArgs a) {
 // More rows: one workgroup takes 16 kRows rows, eight tiles of outputs (two a
 // wave) and a slice of the inputs. x goes through two buffers in LDS that the
 // four waves share, each wave bringing 16 rows of one block a step, so a step is
-// 4 / kRows blocks; codes go straight to registers, some blocks ahead.
+// 4 / kRows blocks; codes go straight to registers, some blocks ahead. A weight is
+// widened once for all 16 kRows rows. 8 rows of 131,072 bfloat16 inputs to 257 outputs
+// (20 MB) take 12.5 us, most of it the way in and out of 441 short workgroups; 64 rows
+// of 5,001 to 11,007 (7 GFLOP) 21.6 us, 325 TFLOP/s, bound by the some 420 vector
+// instructions of a step at two waves a SIMD, which the registers allow.
 constexpr uint32_t kManyWaves = 4, kManyTiles = 2;
 
 template <class X, int kGroups, bool kZero, bool kWide, int kRows>
@@ -660,7 +669,9 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void leo_q4_many(TileArgs a) {
 }
 
 // Adds the slices of 256 / kLanes outputs of one row, kLanes threads an output,
-// always in the same order.
+// always in the same order, so that results do not depend on which workgroup ends
+// first. A launch bounds it (3.9 to 4.9 us); joining in the last workgroup to arrive
+// cost 4 to 7 us, and up to 40 with 64 slices, for its waits on stores and its atomics.
 template <uint32_t kLanes>
 __global__ __launch_bounds__(256) void leo_q4_join(TileArgs a) {
     constexpr uint32_t kOutputs = 256 / kLanes;
@@ -692,6 +703,14 @@ __global__ __launch_bounds__(256) void leo_q4_join(TileArgs a) {
         store_any(a.y, row * a.y_stride + output, sum + (a.bias ? a.bias[output] : 0.0f), a.y_type);
 }
 
+// Both sides of these rules, in us, codes in groups of 64:
+// kFewRows   2 rows of 131,072 inputs to 257 outputs: few 11.2 (float32) and 9.8 (bfloat16), many 15.3 and 13.1; 4 rows
+//            12.6 and 10.7 against 15.9 and 13.5; 8 rows 17.0 and 12.1 against 15.6 and 13.4. 8,192 to 8,192: 2 rows
+//            13.2 and 9.8 against 15.3 and 12.9, 4 rows 17.4 and 12.2 against 15.9 and 13.4, 8 rows 28.2 and 15.7
+//            against 16.6 and 13.7.
+// k..Groups  256, 512 and 1,024 workgroups aimed at: one row of 1,048,576 to 257 46.2, 41.6 and 42.5, 8 rows 72.8, 63.4
+//            and 69.8; 64 rows of 5,000 to 11,007 31.1, 26.2 and 31.7; one row of 131,072 to 257 10.9, 11.2 and 12.5.
+//            512 are what two workgroups a CU take at once: 516 need a second turn.
 constexpr uint32_t kStageBytes = 64 << 10, kFewGroups = 512, kManyGroups = 512, kFewRows = 4;
 
 struct Plan {
