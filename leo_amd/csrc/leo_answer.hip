@@ -460,7 +460,10 @@ __global__ __launch_bounds__(256) void leo_sample_spans(LeoSample a, uint32_t sp
 // the value, a megabyte for 262,147 symbols, and 128 rows of 131,075 take 24.6 us, 16
 // rows of 32,001 11.1 and two of 262,147 14 to 46, as the values fall. A third launch
 // that gathered over all CUs gave back in latency what it saved (32,001: 5 + 7 + 10 us
-// for 5 + 11, 131,075: 23 + 22 + 21 for 23 + 25). kProbe: 1.5, 2 and 2.5 deviations
+// for 5 + 11, 131,075: 23 + 22 + 21 for 23 + 25). Two launches that take the first two
+// turns with a wave a span held calls of one to four rows of 262,147 to 25 to 30 us
+// under min_p, which take 17 to 46 so, but not their mean (28.0, 28.2 and 29.3 against
+// 24.3, 27.4 and 30.4), and cost top_k 3 to 63 us below a million symbols. kProbe: 1.5, 2 and 2.5 deviations
 // took 48.2, 50.6 and 58 us for both kernels at 128 rows of 131,075.
 constexpr uint32_t kColumn = 12, kTogether = 2;
 constexpr float kProbe = 1.5f;
