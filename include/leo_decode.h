@@ -114,7 +114,7 @@ typedef struct LeoLogitControl {
     const float* bias_values;
     const int64_t* bias_offsets; /* rows + 1, or NULL: no biases */
     uint64_t bias_count;
-    const int32_t* masks; /* NULL: no masks */
+    const int32_t* masks; /* NULL: no masks; then mask_count is 0 and mask_rows NULL */
     int64_t masks_stride;
     uint64_t mask_count;
     const int32_t* mask_rows;

@@ -219,6 +219,7 @@ PyObject* control_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
             if (m.width != (z.width + 31) / 32)
                 refuse("masks of " + std::to_string(z.width) + " symbols have " + std::to_string((z.width + 31) / 32) +
                        " words, not " + std::to_string(m.width));
+            if (m.rows < 1) refuse("masks have no rows");
             c.masks = static_cast<const int32_t*>(m.data);
             c.masks_stride = m.stride;
             c.mask_count = static_cast<uint64_t>(m.rows);

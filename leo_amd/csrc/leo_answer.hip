@@ -630,6 +630,8 @@ int32_t leo_control_logits(const LeoLogitControl* control, void* stream) {
             require(c.masks_stride >= 0, "leo_control_logits: masks_stride must not be negative");
             require(c.mask_rows || c.mask_count == 1 || c.mask_count == c.rows,
                     "leo_control_logits: masks need one row, a row for each of the logits, or mask_rows");
+        } else {  // an empty table has no memory: it must not open what its rows' numbers shut
+            require(c.mask_count == 0 && !c.mask_rows, "leo_control_logits: mask_count or mask_rows without masks");
         }
         // Chunks small enough for some 512 workgroups, but of 2,048 symbols at least (each reads the row's lists
         // again) and of a table's size at most: 16 symbols a thread.

@@ -171,7 +171,7 @@ def control_logits(logits: torch.Tensor, *, history: Optional[Tuple[torch.Tensor
     history    (symbols int32, offsets int64 [rows + 1]); entries outside the vocabulary are ignored
     repetition, presence, frequency   float32 [rows]; without them 1, 0 and 0
     bias       (ids int32, values float32, offsets int64 [rows + 1]); a row's last entry for a symbol counts
-    masks      int32 [n, ceil(symbols / 32)], symbol v at bit v % 32 of word v // 32
+    masks      int32 [n, ceil(symbols / 32)] with n >= 1, symbol v at bit v % 32 of word v // 32
     mask_rows  int32 [rows]: each row's mask, -1 for none, any other number outside 0..n-1 allows nothing;
                without it n is 1 or the number of rows
     out        may be `logits`
