@@ -12,21 +12,23 @@ fallback. Calls may be captured into a graph.
 
 The step runtime does not use torch; this module does, and torch brings a HIP
 runtime of its own. One process must have one: import torch (or this module)
-before the first call into libleo_hip.so.
+before the first call into libleo_hip.so; any other order raises ``ImportError``.
 """
 from __future__ import annotations
 
 import ctypes
 import importlib.machinery
 import importlib.util
+import pathlib
 import sys
 from typing import Optional, Tuple
 
 from . import native
 
+_ORDER = ("import torch (or leo_amd.decode) before the first HipRuntime: libleo_hip.so is already bound to another HIP "
+          "runtime than torch's")
 if "torch" not in sys.modules and native._lib is not None:
-    raise ImportError("import torch (or leo_amd.decode) before the first HipRuntime: libleo_hip.so is already bound "
-                      "to another HIP runtime than torch's")
+    raise ImportError(_ORDER)
 
 import torch  # noqa: E402
 
@@ -65,11 +67,21 @@ def _public_stream(index: int) -> int:
 _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", _public_stream)
 
 
+def _check_runtime(lib: ctypes.CDLL) -> None:
+    """Refuses a library that calls another HIP runtime than torch: torch may have
+    come after the library, and then each is bound to its own."""
+    hip = pathlib.Path(torch.__file__).with_name("lib") / "libtorch_hip.so"
+    if hip.exists():
+        ours, theirs = (ctypes.cast(l.hipLaunchKernel, ctypes.c_void_p).value for l in (lib, ctypes.CDLL(str(hip))))
+        if ours != theirs:
+            raise ImportError(_ORDER)
+
+
 def _load_binding():
     path = native.LIB_PATH.with_name("leo_decode_binding.so")
     if not path.exists():
         raise ImportError(f"{path} is missing: build it with `python -m leo_amd.build` (no fallback exists)")
-    native.load()
+    _check_runtime(native.load())
     loader = importlib.machinery.ExtensionFileLoader("leo_decode_binding", str(path))
     module = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
     loader.exec_module(module)
