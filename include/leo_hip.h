@@ -430,6 +430,10 @@ int32_t leo_hip_read_list(LeoHipRuntime* runtime, int32_t which, uint64_t* out,
  * up to `capacity` entries of each array that is non-null. */
 int32_t leo_hip_read_active(LeoHipRuntime* runtime, uint64_t* neurons, float* activations,
                             uint64_t capacity, uint64_t* count);
+/* The readout's current parameters, as leo_hip_download_model gives them:
+ * out_weight [257, neurons] and bias [257]; either may be NULL. Unlike a whole
+ * download it changes no mark: what a mirror has still to synchronise stays so. */
+int32_t leo_hip_read_readout(LeoHipRuntime* runtime, float* out_weight, float* bias);
 /* Transient state of the canonical runtime for parity checks; `count` must
  * equal the state's element count. */
 int32_t leo_hip_read_state(LeoHipRuntime* runtime, int32_t which, float* out, uint64_t count);

@@ -1827,6 +1827,18 @@ void upload_topology(LeoHipRuntime* h, const LeoModelView& m) {
     sync(s);
 }
 
+void download_readout(LeoHipRuntime* h, float* out_weight, float* bias) {
+    const Sizes& z = h->z;
+    std::vector<float> rows(out_weight ? z.n * kOutStride : 0), biases(bias ? kOutStride : 0);
+    if (out_weight) download(rows.data(), h->canon.out_w, rows.size() * 4, h->stream);
+    if (bias) download(biases.data(), h->canon.bias, kOutStride * 4, h->stream);
+    sync(h->stream);
+    if (out_weight)
+        for (uint64_t o = 0; o < kOutputs; ++o)
+            for (uint64_t n = 0; n < z.n; ++n) out_weight[o * z.n + n] = rows[n * kOutStride + o];
+    if (bias) std::copy(biases.begin(), biases.begin() + kOutputs, bias);
+}
+
 void download_model(LeoHipRuntime* h, LeoModelView& m) {
     const Sizes& z = h->z;
     hipStream_t s = h->stream;
@@ -1840,18 +1852,12 @@ void download_model(LeoHipRuntime* h, LeoModelView& m) {
     download(m.threshold, h->canon.threshold, z.n * 4, s);
     download(m.rec_weight, h->canon.rec_weight, z.ns * 4, s);
     download(m.in_weight, h->canon.in_weight, z.ni * 4, s);
-    std::vector<float> rows(z.n * kOutStride);
-    download(rows.data(), h->canon.out_w, rows.size() * 4, s);
-    std::vector<float> bias(kOutStride);
-    download(bias.data(), h->canon.bias, kOutStride * 4, s);
     download(m.ctx_keys, h->canon.ctx_keys, z.slots * 8, s);
     download(m.ctx_emb, h->canon.ctx_emb, z.slots * z.e * 4, s);
     download(m.ctx_obs, h->canon.ctx_obs, z.slots * 4, s);
     download(m.ctx_out, h->canon.ctx_out, kOutputs * z.e * 4, s);
     sync(s);
-    for (uint64_t o = 0; o < kOutputs; ++o)
-        for (uint64_t n = 0; n < z.n; ++n) m.out_weight[o * z.n + n] = rows[n * kOutStride + o];
-    std::copy(bias.begin(), bias.begin() + kOutputs, m.bias);
+    download_readout(h, m.out_weight, m.bias);
     m.generation = h->generation;
     m.parameter_revision = h->revision;
     m.statistics = h->stats;
@@ -3399,6 +3405,13 @@ int32_t leo_hip_read_active(LeoHipRuntime* h, uint64_t* neurons, float* activati
             if (neurons) neurons[i] = ids[i];
             if (activations) activations[i] = values[i];
         }
+    });
+}
+
+int32_t leo_hip_read_readout(LeoHipRuntime* h, float* out_weight, float* bias) {
+    return guarded([&] {
+        leo::BusyGuard g(h);
+        leo::download_readout(h, out_weight, bias);
     });
 }
 

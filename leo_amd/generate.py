@@ -69,10 +69,9 @@ class Generator:
         self.weight: Optional[decode.Q4Weight] = None
         self.bias: Optional[torch.Tensor] = None
         if readout == "q4":
-            model = runtime.model()
-            rows = torch.from_numpy(model.out_weight.reshape(OUTPUT_CLASSES, self.neurons)).to(self.device)
-            self.weight = decode.Q4Weight.quantize(rows, group)
-            self.bias = torch.from_numpy(model.bias).to(self.device)
+            rows, bias = runtime._read_readout()
+            self.weight = decode.Q4Weight.quantize(torch.from_numpy(rows).to(self.device), group)
+            self.bias = torch.from_numpy(bias).to(self.device)
         self._active = torch.zeros(1, self.neurons, device=self.device)
         self._noise = torch.Generator(self.device).manual_seed(seed)
         self._next = utf8_table()

@@ -353,6 +353,13 @@ class HipRuntime:
         hit = np.nonzero(ids == neuron)[0]
         return float(values[hit[0]]) if hit.size else 0.0
 
+    def _read_readout(self) -> Tuple[np.ndarray, np.ndarray]:
+        """The output weights [257, neurons] and the bias; no mirror's marks change."""
+        weight = np.zeros((257, self.config.model.neuron_count), dtype=np.float32)
+        bias = np.zeros(257, dtype=np.float32)
+        self._call("leo_hip_read_readout", weight.ctypes.data, bias.ctypes.data)
+        return weight, bias
+
     def read_state(self, name: str) -> np.ndarray:
         n = self.config.model.neuron_count
         sizes = {"branches": 4 * n, "logits": 257, "probabilities": 257, "errors": 257}

@@ -1,0 +1,61 @@
+"""What a generator keeps and what it must not: a mirror's marks, the model's weights
+after training, documents that have ended, whole UTF-8."""
+from __future__ import annotations
+
+import codecs
+
+import numpy as np
+import pytest
+import torch
+
+from leo_amd import native
+from leo_amd.generate import END, Generator
+from leo_amd.model import Model
+from leo_amd.runtime import HipRuntime
+from tests.helpers import assert_models_equal, small_redundant_config, story
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def runtime():
+    with HipRuntime(Model.synthetic(small_redundant_config(), weight_sigma=0.05), max_lanes=2) as r:
+        r.train_batch([story(0, 200)], native.TRAINING, replay=False)
+        yield r
+
+
+@pytest.mark.parametrize("tracked", [False, True])
+def test_a_mirror_still_gets_its_changes(require_gpu, runtime, tracked):
+    mirror = runtime.model()
+    if tracked:
+        runtime.enable_parameter_tracking()
+    runtime.train_batch([story(1, 200), story(2, 200)], native.TRAINING, replay=True)
+    if tracked:
+        runtime.enable_parameter_tracking()
+    Generator(runtime)
+    runtime.synchronize_model(mirror)
+    assert_models_equal(mirror, runtime.model())
+
+
+def no_document(call):
+    with pytest.raises(native.LeoError) as err:
+        call()
+    assert err.value.code == native.ERR_INVALID_ARGUMENT and "document" in str(err.value)
+
+
+def learn_by_batch(r):
+    r.train_batch([story(1, 300)], native.TRAINING, replay=False)
+
+
+def learn_by_lanes(r):
+    r.train_batch([story(1, 300), story(2, 300)], native.TRAINING, replay=True)
+
+
+def learn_by_steps(r):
+    r.begin_document()
+    for a, b in zip(b"once upon a tim", b"nce upon a time"):
+        r.step(a, b, native.TRAINING)
+
+
+def take_another_model(r):
+    r.set_model(Model.synthetic(r.config, weight_sigma=0.2))
