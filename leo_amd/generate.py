@@ -66,12 +66,12 @@ class Generator:
         self.device = torch.device("cuda", runtime.device)
         self.neurons = runtime.config.model.neuron_count
         self.readout = readout
+        self.group = group
         self.weight: Optional[decode.Q4Weight] = None
         self.bias: Optional[torch.Tensor] = None
+        self._version = -1      # of the parameters that weight and bias were made from
         if readout == "q4":
-            rows, bias = runtime._read_readout()
-            self.weight = decode.Q4Weight.quantize(torch.from_numpy(rows).to(self.device), group)
-            self.bias = torch.from_numpy(bias).to(self.device)
+            self._take_weights()
         self._active = torch.zeros(1, self.neurons, device=self.device)
         self._noise = torch.Generator(self.device).manual_seed(seed)
         self._next = utf8_table()
@@ -79,10 +79,19 @@ class Generator:
         self._state = 0
         self._written: List[int] = []
 
+    def _take_weights(self) -> None:
+        version = self.runtime.parameter_version
+        if version != self._version:
+            rows, bias = self.runtime._read_readout()
+            self.weight = decode.Q4Weight.quantize(torch.from_numpy(rows).to(self.device), self.group)
+            self.bias = torch.from_numpy(bias).to(self.device)
+            self._version = version
+
     def logits(self) -> torch.Tensor:
-        """[1, 257]: the readout of the last step."""
-        if self.weight is None:
+        """[1, 257]: the readout of the last step, with the model's weights as they are now."""
+        if self.readout == "device":
             return torch.from_numpy(self.runtime.read_state("logits")).to(self.device)[None]
+        self._take_weights()
         ids, values = self.runtime._read_active()
         self._active.zero_()
         self._active[0, torch.from_numpy(ids).to(self.device)] = torch.from_numpy(values).to(self.device)

@@ -159,6 +159,8 @@ class HipRuntime:
                                                           max_lanes, ctypes.byref(self._handle)))
         self._template = model
         self.device = device
+        # rises with every call that may change parameters: what is made from them holds while it stays
+        self.parameter_version = 0
 
     def fork(self, model: Model) -> "HipRuntime":
         """RuntimeBackend::fork (backend.rs:623-633 -> cuda.rs:2347-2356): a
@@ -187,6 +189,10 @@ class HipRuntime:
     def _call(self, name: str, *args) -> None:
         native.check(self._lib, getattr(self._lib, name)(self._handle, *args))
 
+    def _learns(self, permission: int) -> None:
+        if permission != native.FROZEN:
+            self.parameter_version += 1
+
     # --- RuntimeBackend -------------------------------------------------------
     def model(self) -> Model:
         """synchronize_model() + model() (backend.rs:355-356)."""
@@ -198,6 +204,7 @@ class HipRuntime:
 
     def set_model(self, model: Model) -> None:
         """model_mut() replacement: upload a whole model (backend.rs:357)."""
+        self.parameter_version += 1
         view = model.view()
         self._call("leo_hip_upload_model", ctypes.byref(view))
 
@@ -210,11 +217,13 @@ class HipRuntime:
 
     def synchronize_packed_model(self, update: PackedUpdate) -> None:
         """backend.rs:374-376 / cuda.rs:2844-2857: scatter; tracking ends."""
+        self.parameter_version += 1
         u = update.to_c()
         self._call("leo_hip_synchronize_packed_model", ctypes.byref(u))
 
     def commit_packed_host_model(self, update: PackedUpdate) -> None:
         """backend.rs:378-387 / cuda.rs:2859-2868: scatter; tracking kept."""
+        self.parameter_version += 1
         u = update.to_c()
         self._call("leo_hip_commit_packed_host_model", ctypes.byref(u))
 
@@ -232,6 +241,7 @@ class HipRuntime:
 
     def step(self, symbol: int, target: Optional[int], permission: int) -> StepMetrics:
         m = native.LeoStepMetrics()
+        self._learns(permission)
         self._call("leo_hip_step", symbol, -1 if target is None else target, permission, ctypes.byref(m))
         return StepMetrics.from_c(m)
 
@@ -242,6 +252,7 @@ class HipRuntime:
         symbols = np.array([s for s, _ in steps], dtype=np.uint32)
         targets = np.array([-1 if t is None else t for _, t in steps], dtype=np.int32)
         out = (native.LeoStepMetrics * n)()
+        self._learns(permission)
         self._call("leo_hip_training_step_batch", symbols.ctypes.data, targets.ctypes.data, n, permission, out)
         return [StepMetrics.from_c(m) for m in out]
 
@@ -260,6 +271,7 @@ class HipRuntime:
         targets = np.array([-1 if t is None else t for _, t in steps], dtype=np.int32)
         out = (native.LeoStepMetrics * n)()
         supervised = ctypes.c_uint32()
+        self._learns(permission)
         self._call("leo_hip_replay_streaming_batch", symbols.ctypes.data, targets.ctypes.data, n, permission, out,
                    ctypes.byref(supervised))
         return [StepMetrics.from_c(out[i]) for i in range(supervised.value)]
@@ -269,6 +281,7 @@ class HipRuntime:
         data, offsets = pack_stories(stories)
         losses = np.zeros(int(offsets[-1]) + len(stories), dtype=np.float32)
         rep = native.LeoBatchReport()
+        self._learns(permission)
         self._call("leo_hip_training_story_batch", data.ctypes.data, offsets.ctypes.data, len(stories), permission,
                    losses.ctypes.data, ctypes.byref(rep))
         return BatchReport.from_c(rep), _split_losses(losses, stories)
@@ -279,6 +292,7 @@ class HipRuntime:
         data, offsets = pack_stories(stories)
         losses = np.zeros(int(offsets[-1]) + len(stories), dtype=np.float32)
         rep = native.LeoBatchReport()
+        self._learns(permission)
         self._call("leo_hip_train_batch", data.ctypes.data, offsets.ctypes.data, len(stories), permission,
                    1 if replay else 0, losses.ctypes.data, ctypes.byref(rep))
         return BatchReport.from_c(rep), _split_losses(losses, stories)
@@ -299,6 +313,7 @@ class HipRuntime:
                            ) -> BatchReport:
         """train_batch over pre-packed stories (no per-story loss copy-out)."""
         rep = native.LeoBatchReport()
+        self._learns(permission)
         self._call("leo_hip_train_batch", data.ctypes.data, offsets.ctypes.data, len(offsets) - 1, permission,
                    1 if replay else 0, None, ctypes.byref(rep))
         return BatchReport.from_c(rep)

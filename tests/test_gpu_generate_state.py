@@ -59,3 +59,29 @@ def learn_by_steps(r):
 
 def take_another_model(r):
     r.set_model(Model.synthetic(r.config, weight_sigma=0.2))
+
+
+@pytest.mark.parametrize("change", [learn_by_batch, learn_by_lanes, learn_by_steps, take_another_model])
+def test_answers_come_from_the_current_model(require_gpu, runtime, change):
+    generator = Generator(runtime)
+    generator.prompt(b"once upon ")
+    generator.write(5, temperature=0.0, allow_end=False)
+    change(runtime)
+    answers = []
+    for g in (generator, Generator(runtime)):
+        g.prompt(b"once upon ")
+        logits = g.logits().clone()
+        answers.append((logits, *g.write(20, temperature=0.0, allow_end=False)))
+    assert torch.equal(answers[0][0], answers[1][0])
+    assert answers[0][1:] == answers[1][1:]
+
+
+def test_weights_are_kept_while_the_model_stays(require_gpu, runtime):
+    generator = Generator(runtime)
+    kept = generator.weight
+    generator.prompt(b"once upon ")
+    generator.write(5)
+    runtime.evaluate([story(3, 50)])
+    generator.prompt(b"the ")
+    generator.write(5)
+    assert generator.weight is kept
