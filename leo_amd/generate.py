@@ -78,6 +78,7 @@ class Generator:
         self._masks = torch.from_numpy(utf8_masks()).to(self.device)
         self._state = 0
         self._written: List[int] = []
+        self._document: Optional[int] = None      # the runtime's count while the prompt's document is open
 
     def _take_weights(self) -> None:
         version = self.runtime.parameter_version
@@ -110,13 +111,19 @@ class Generator:
         self.runtime.step(symbols[-1], None, native.FROZEN)
         self._state = state
         self._written = list(text)
+        self._document = self.runtime.documents
 
     def write(self, count: int, *, temperature: float = 0.8, top_k: int = 40, top_p: float = 0.95, min_p: float = 0.0,
               repetition: float = 1.0, presence: float = 0.0, frequency: float = 0.0, history: int = 64,
               bias: Optional[Dict[int, float]] = None, allow_end: bool = True) -> Tuple[bytes, List[float]]:
         """Up to `count` bytes after the prompt, and their logprobs; fewer where the
-        model ends the document. The penalties look at the last `history` bytes,
-        the prompt's among them; `bias` adds to single bytes' logits (256: the end)."""
+        model ends the document. Needs the document that `prompt` began, ended neither
+        by the model nor by another use of the runtime. The penalties look at the last
+        `history` bytes, the prompt's among them; `bias` adds to single bytes' logits
+        (256: the end)."""
+        if self._document != self.runtime.documents:
+            raise native.LeoError(native.ERR_INVALID_ARGUMENT, "no document is open: begin one with prompt()")
+
         def one(value, dtype=torch.float32):
             return torch.tensor([value], dtype=dtype, device=self.device)
 

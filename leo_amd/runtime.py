@@ -161,6 +161,8 @@ class HipRuntime:
         self.device = device
         # rises with every call that may change parameters: what is made from them holds while it stays
         self.parameter_version = 0
+        # rises with every call that begins or ends a document, or resets what one has left
+        self.documents = 0
 
     def fork(self, model: Model) -> "HipRuntime":
         """RuntimeBackend::fork (backend.rs:623-633 -> cuda.rs:2347-2356): a
@@ -205,6 +207,7 @@ class HipRuntime:
     def set_model(self, model: Model) -> None:
         """model_mut() replacement: upload a whole model (backend.rs:357)."""
         self.parameter_version += 1
+        self.documents += 1
         view = model.view()
         self._call("leo_hip_upload_model", ctypes.byref(view))
 
@@ -228,12 +231,15 @@ class HipRuntime:
         self._call("leo_hip_commit_packed_host_model", ctypes.byref(u))
 
     def begin_document(self) -> None:
+        self.documents += 1
         self._call("leo_hip_begin_document")
 
     def finish_document(self) -> None:
+        self.documents += 1
         self._call("leo_hip_finish_document")
 
     def reset_transient_state(self) -> None:
+        self.documents += 1
         self._call("leo_hip_reset_transient_state")
 
     def enable_parameter_tracking(self) -> None:
@@ -282,6 +288,7 @@ class HipRuntime:
         losses = np.zeros(int(offsets[-1]) + len(stories), dtype=np.float32)
         rep = native.LeoBatchReport()
         self._learns(permission)
+        self.documents += 1
         self._call("leo_hip_training_story_batch", data.ctypes.data, offsets.ctypes.data, len(stories), permission,
                    losses.ctypes.data, ctypes.byref(rep))
         return BatchReport.from_c(rep), _split_losses(losses, stories)
@@ -293,6 +300,7 @@ class HipRuntime:
         losses = np.zeros(int(offsets[-1]) + len(stories), dtype=np.float32)
         rep = native.LeoBatchReport()
         self._learns(permission)
+        self.documents += 1
         self._call("leo_hip_train_batch", data.ctypes.data, offsets.ctypes.data, len(stories), permission,
                    1 if replay else 0, losses.ctypes.data, ctypes.byref(rep))
         return BatchReport.from_c(rep), _split_losses(losses, stories)
@@ -304,6 +312,7 @@ class HipRuntime:
         data, offsets = pack_stories(stories)
         losses = np.zeros(int(offsets[-1]) + len(stories), dtype=np.float32)
         rep = native.LeoEvaluationReport()
+        self.documents += 1
         self._call("leo_hip_evaluate", data.ctypes.data, offsets.ctypes.data, len(stories), losses.ctypes.data,
                    ctypes.byref(rep))
         report = {name: getattr(rep, name) for name, _ in native.LeoEvaluationReport._fields_ if name != "pad0"}
@@ -314,6 +323,7 @@ class HipRuntime:
         """train_batch over pre-packed stories (no per-story loss copy-out)."""
         rep = native.LeoBatchReport()
         self._learns(permission)
+        self.documents += 1
         self._call("leo_hip_train_batch", data.ctypes.data, offsets.ctypes.data, len(offsets) - 1, permission,
                    1 if replay else 0, None, ctypes.byref(rep))
         return BatchReport.from_c(rep)

@@ -85,3 +85,20 @@ def test_weights_are_kept_while_the_model_stays(require_gpu, runtime):
     generator.prompt(b"the ")
     generator.write(5)
     assert generator.weight is kept
+
+
+@pytest.mark.parametrize("readout", ["q4", "device"])
+def test_writing_needs_an_open_document(require_gpu, runtime, readout):
+    generator = Generator(runtime, readout=readout)
+    no_document(lambda: generator.write(3))
+    generator.prompt(b"a")
+    assert generator.write(5, bias={END: 1e4}) == (b"", [])
+    no_document(lambda: generator.write(5))
+    generator.prompt(b"a")
+    assert len(generator.write(5, allow_end=False)[0]) == 5
+    assert len(generator.write(5, allow_end=False)[0]) == 5      # it is still open
+    for ends in (runtime.finish_document, runtime.begin_document, runtime.reset_transient_state, lambda: learn_by_batch(runtime),
+                 lambda: runtime.evaluate([story(3, 50)]), lambda: Generator(runtime).prompt(b"b")):
+        generator.prompt(b"a")
+        ends()
+        no_document(lambda: generator.write(5))
