@@ -60,9 +60,9 @@ int32_t leo_q4_layout(const LeoQ4Source* source, void* stream);
 
 /* y[m, n] = bias[n] + sum over k of x[m, k] * w[n, k] for `rows` rows of x.
  * Sums are held in 32 bits and rounded once to y_type; bias (float) may be
- * NULL. `workspace`: at least leo_q4_workspace_bytes() bytes (none where that is
- * 0), 256-byte aligned, whatever they hold; free again when the call's work is
- * done. */
+ * NULL. y and x share no memory. `workspace`: at least leo_q4_workspace_bytes()
+ * bytes (none where that is 0), 256-byte aligned, whatever they hold; free again
+ * when the call's work is done. */
 typedef struct LeoQ4Product {
     LeoQ4Shape shape;
     const void* layout;
@@ -94,7 +94,8 @@ int32_t leo_q4_matvec(const LeoQ4Product* product, void* stream);
  * rows of ceil(symbols / 32) words, symbol v at bit v % 32 of word v / 32;
  * mask_rows chooses one for each row, -1 for none; any other number outside
  * 0 .. mask_count-1 allows nothing. Without mask_rows, row r uses mask r, or
- * mask 0 where mask_count is 1. out may be the logits themselves. */
+ * mask 0 where mask_count is 1. out may be the logits themselves, but not overlap
+ * them otherwise. */
 typedef struct LeoLogitControl {
     uint64_t rows;
     uint64_t symbols;

@@ -131,6 +131,29 @@ inline void require(bool ok, const char* what) {
     if (!ok) throw Error(LEO_ERR_INVALID_ARGUMENT, what);
 }
 
+// The bytes of a matrix with dense rows.
+struct Rows {
+    uintptr_t at;
+    uint64_t count, width, stride;
+};
+inline Rows rows_of(const void* p, uint64_t count, uint64_t width, int64_t stride, int32_t type) {
+    const uint64_t e = type_bytes(type);
+    return {reinterpret_cast<uintptr_t>(p), count, width * e, count > 1 ? static_cast<uint64_t>(stride) * e : 0};
+}
+// Whether two of them share a byte. Columns of one buffer do not, though their
+// ranges do: only then are the rows gone through, in the order of both.
+inline bool overlap(const Rows& a, const Rows& b) {
+    const auto end = [](const Rows& r) { return r.at + (r.count - 1) * r.stride + r.width; };
+    if (end(a) <= b.at || end(b) <= a.at) return false;
+    for (uint64_t i = 0, j = 0; i < a.count && j < b.count;) {
+        const uintptr_t in_a = a.at + i * a.stride, in_b = b.at + j * b.stride;
+        if (in_a + a.width <= in_b) ++i;
+        else if (in_b + b.width <= in_a) ++j;
+        else return true;
+    }
+    return false;
+}
+
 // Launches through the returned status, not the thread's last error, which an
 // earlier call of the program may have left.
 template <class... Args>

@@ -621,6 +621,10 @@ int32_t leo_control_logits(const LeoLogitControl* control, void* stream) {
         require(c.logits && c.out, "leo_control_logits: null argument");
         require(c.logits_stride >= 0, "leo_control_logits: logits_stride must not be negative");
         require(c.rows == 1 || c.out_stride >= static_cast<int64_t>(c.symbols), "leo_control_logits: out_stride is too small");
+        require((c.out == c.logits && (c.rows == 1 || c.out_stride == c.logits_stride)) ||
+                    !overlap(rows_of(c.logits, c.rows, c.symbols, c.logits_stride, c.type),
+                             rows_of(c.out, c.rows, c.symbols, c.out_stride, c.type)),
+                "leo_control_logits: out overlaps the logits without being them");
         require(!c.history_offsets || c.history || c.history_count == 0, "leo_control_logits: offsets without a history");
         require(!c.bias_offsets || (c.bias_ids && c.bias_values) || c.bias_count == 0,
                 "leo_control_logits: offsets without biases");

@@ -847,6 +847,8 @@ int32_t leo_q4_matvec(const LeoQ4Product* product, void* stream) {
         require(p.layout && p.x && p.y, "leo_q4_matvec: null argument");
         require(p.x_stride >= 0, "leo_q4_matvec: x_stride must not be negative");
         require(p.y_stride >= static_cast<int64_t>(p.shape.outputs) || p.rows == 1, "leo_q4_matvec: y_stride is too small");
+        require(!overlap(rows_of(p.x, p.rows, p.shape.inputs, p.x_stride, p.x_type),
+                         rows_of(p.y, p.rows, p.shape.outputs, p.y_stride, p.y_type)), "leo_q4_matvec: y overlaps x");
         require(reinterpret_cast<uintptr_t>(p.layout) % 256 == 0, "leo_q4_matvec: layout must be 256-byte aligned");
         const Q4Layout l = layout_of(p.shape);
         require(p.layout_bytes >= l.bytes, "leo_q4_matvec: layout is too small for its shape");

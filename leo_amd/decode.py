@@ -158,7 +158,7 @@ def q4_matvec(x: torch.Tensor, weight: Q4Weight, bias: Optional[torch.Tensor] = 
               out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """bias + x W^T for x [rows, inputs] (or [inputs]) of float32, float16 or
     bfloat16: sums in 32 bits, rounded once to `out_dtype` (x's type by default).
-    bias: float32 [outputs]."""
+    bias: float32 [outputs]. `out` and x share no memory."""
     if isinstance(x, torch.Tensor) and x.dim() == 1:
         if out is not None:
             _refuse("out needs x with two axes")
@@ -186,7 +186,7 @@ def control_logits(logits: torch.Tensor, *, history: Optional[Tuple[torch.Tensor
     masks      int32 [n, ceil(symbols / 32)] with n >= 1, symbol v at bit v % 32 of word v // 32
     mask_rows  int32 [rows]: each row's mask, -1 for none, any other number outside 0..n-1 allows nothing;
                without it n is 1 or the number of rows
-    out        may be `logits`
+    out        may be `logits`, but share no memory with them otherwise
     """
     entries, offsets = (None, None) if history is None else history
     ids, values, bias_offsets = (None, None, None) if bias is None else bias

@@ -1,5 +1,5 @@
 """Refusals of the decoding operators that need no GPU: masks that are not there, a
-second HIP runtime in the process."""
+second HIP runtime in the process, results over their operands."""
 from __future__ import annotations
 
 import ctypes
@@ -37,3 +37,29 @@ def test_torch_before_the_library_is_one_runtime():
     code = ("import torch\nfrom leo_amd import native\nnative.load()\nimport leo_amd.decode, leo_amd.generate\n"
             "assert len({l.split()[-1] for l in open('/proc/self/maps') if 'libamdhip64' in l}) == 1\n")
     subprocess.run([sys.executable, "-c", code], check=True, cwd=str(ROOT))
+
+
+MATRIX = dict(rows=4, x_stride=128, y_stride=128)
+
+
+@pytest.mark.parametrize("x,y,change", [
+    (1 << 20, 1 << 20, {}), (1 << 20, (1 << 20) + 4, {}), ((1 << 20) + 4 * 127, 1 << 20, {}),
+    (1 << 20, (1 << 20) + 4 * 128 * 4 - 4, {}), (1 << 20, (1 << 20) + 4 * 100, dict(x_stride=300, y_stride=300)),
+    (1 << 20, (1 << 20) + 4 * 250, dict(x_stride=300, y_stride=300)), (1 << 20, (1 << 20) + 4 * 64, dict(x_stride=0)),
+    (1 << 20, (1 << 20) + 4 * 130, dict(x_stride=257, y_stride=200))])
+def test_results_over_their_operand_are_refused(x, y, change):
+    # other workgroups read x while the first results are stored
+    shape = native.LeoQ4Shape(outputs=128, inputs=128, group=128, scale_type=native.TYPE_F32, has_zeros=0)
+    assert "overlaps x" in refusal("leo_q4_matvec", native.LeoQ4Product, dict(
+        shape=shape, layout=1 << 30, layout_bytes=1 << 20, x=x, y=y, x_type=native.TYPE_F32, y_type=native.TYPE_F32,
+        workspace=1 << 31, workspace_bytes=1 << 30, **{**MATRIX, **change}))
+
+
+@pytest.mark.parametrize("out,change", [
+    (4, {}), (-4, {}), (4 * 256, {}), (4 * 257 * 3, {}), (0, dict(out_stride=300)), (0, dict(logits_stride=0)),
+    (4 * 200, dict(logits_stride=400, out_stride=400))])
+def test_controlled_logits_beside_the_logits_are_refused(out, change):
+    # in place is exactly in place
+    assert "overlaps the logits" in refusal("leo_control_logits", native.LeoLogitControl, {**dict(
+        rows=4, symbols=257, logits=1 << 20, logits_stride=257, out=(1 << 20) + out, out_stride=257,
+        type=native.TYPE_F32), **change})
