@@ -122,7 +122,8 @@ typedef struct LeoLogitControl {
 } LeoLogitControl;
 int32_t leo_control_logits(const LeoLogitControl* control, void* stream);
 
-/* One symbol a row of logits [rows, symbols]. With z = logit / temperature and
+/* One symbol a row of logits [rows, symbols]. With z = logit / temperature in
+ * float (a finite logit's does not fall below the lowest finite value) and
  * w = exp(z - max z), a symbol stays if fewer than top_k symbols have a larger z,
  * those have less than top_p of the whole mass (top_p >= 1: any), and
  * w >= min_p; the largest always stays. The symbol is the one that stays with

@@ -181,14 +181,20 @@ __device__ __forceinline__ float mass_of(float z, float top) {
     return z == top ? 1.0f : __builtin_amdgcn_exp2f((z - top) * 1.44269504f);
 }
 
+constexpr float kMost = 0x1.fffffep127f;
+
 // A row's parameters.
 struct Rules {
     float t, inverse, top_p, min_p;
     uint32_t top_k;
     bool greedy, ordinary, filtered;
 
-    // logit / t, -inf for NaN: a product with the reciprocal and one correction
-    // by its remainder round as the division does.
+    // logit / t, -inf for NaN. A finite logit's quotient does not fall to -inf: a row
+    // that a mask left at its type's lowest value is not an empty one. A product with
+    // the reciprocal and one correction by its remainder rounds as the division does
+    // (3e8 random pairs, none apart) from logits of 2^-90 on; below, where the remainder
+    // leaves float's range, it may be a unit in the last place off, and is still in the
+    // logits' order.
     __device__ __forceinline__ float divided(float logit) const {
         float q = logit * inverse;
         if (ordinary) {
@@ -197,7 +203,7 @@ struct Rules {
         } else {
             q = logit / t;
         }
-        return q == q ? q : negative_infinity();
+        return logit > negative_infinity() ? fmaxf(q, -kMost) : negative_infinity();
     }
 };
 __device__ __forceinline__ Rules rules_of(const LeoSample& a, uint64_t row) {
@@ -538,7 +544,7 @@ __global__ __launch_bounds__(kMostWaves * 64) void leo_sample_settle(LeoSample a
             weigh();
         };
         // z above low needs a logit above this, whatever the division rounds
-        const float least = low * r.t - (fabsf(low * r.t) * 0x1p-20f + 0x1p-120f);
+        const float cut = __builtin_amdgcn_fmed3f(low * r.t, -kMost, kMost), least = cut - (fabsf(cut) * 0x1p-20f + 0x1p-120f);
         held = low;
         filled = 0;
         for (uint32_t from = wave; from < spans; from += kMostWaves * 64) {

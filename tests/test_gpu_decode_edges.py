@@ -31,6 +31,34 @@ def test_an_empty_table_of_masks_is_refused(require_gpu):
     refused(lambda: decode.control_logits(z, masks=empty, mask_rows=torch.full((3,), -1, dtype=torch.int32, device=DEVICE)))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("symbols", [5, 257, 20_001])
+def test_rows_of_the_types_lowest_value_have_a_symbol(require_gpu, dtype, symbols):
+    # finite logits that a temperature below 1 takes out of float32: the row is not one of -inf
+    lowest, t = torch.finfo(dtype).min, [0.7, 1.0, 1.3, 0.0, 0.5, 0.7]
+    logits = torch.full((6, symbols), lowest, device=DEVICE, dtype=dtype)
+    logits[4, 0] = -math.inf
+    logits[5] = -lowest
+    noise = torch.zeros(6, symbols, device=DEVICE)
+    noise[:, 3] = 1.0
+    for extra in ({}, {"top_k": torch.full((6,), 2, dtype=torch.int32, device=DEVICE)}, {"top_p": per_row([0.5] * 6)},
+                  {"min_p": per_row([0.5] * 6)}):
+        got, logprob = decode.sample(logits, noise, temperature=per_row(t), **extra)
+        # next to such a logit the noise is below a float32 step: all are equal, the lowest comes first
+        assert got.tolist() == [0, 0, 0, 0, 1, 0]
+        want = torch.full((6,), -math.log(symbols), device=DEVICE)
+        want[4] = -math.log(symbols - 1)
+        assert bool(((logprob - want).abs() <= 1e-5 * (1 + want.abs())).all())
+
+
+def test_a_lowest_value_among_others_is_out_of_the_race(require_gpu):
+    logits = torch.full((2, 300), torch.finfo(torch.float32).min, device=DEVICE)
+    logits[0, 77] = -3.0
+    logits[1, 44] = 3e38
+    got, logprob = decode.sample(logits, torch.zeros(2, 300, device=DEVICE), temperature=per_row([0.6, 0.6]))
+    assert got.tolist() == [77, 44] and logprob.tolist() == [0.0, 0.0]
+
+
 @pytest.mark.parametrize("rows", [1, 3, 20, 70])
 def test_results_beside_their_operands(require_gpu, rows):
     # columns of one buffer, and neighbours in memory, share nothing
