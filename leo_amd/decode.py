@@ -140,7 +140,9 @@ class Q4Weight:
     @classmethod
     def quantize(cls, weight: torch.Tensor, group: int = 32, scale_dtype: torch.dtype = torch.float16) -> "Q4Weight":
         """A floating matrix [outputs, inputs] rounded to codes about 8: a group's
-        scale is its largest magnitude over 7 (0 for a group of zeros)."""
+        scale is its largest magnitude over 7 (0 for a group of zeros). Refuses a
+        weight with a scale that `scale_dtype` does not hold; the check waits for the
+        GPU and is left out while a graph is captured."""
         if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not weight.is_floating_point():
             _refuse("weight must be a floating matrix")
         if group not in (32, 64, 128):
@@ -148,6 +150,8 @@ class Q4Weight:
         outputs, inputs = weight.shape
         padded = torch.nn.functional.pad(weight.float(), (0, -inputs % group)).view(outputs, -1, group)
         scales = (padded.abs().amax(dim=2) / 7.0).to(scale_dtype)
+        if not torch.cuda.is_current_stream_capturing() and not bool(scales.isfinite().all()):
+            _refuse(f"a group's largest magnitude over 7 is no finite {scale_dtype}")
         divide = torch.where(scales == 0, torch.ones_like(scales), scales).float()
         codes = ((padded / divide[:, :, None]).round().clamp(-8, 7) + 8).to(torch.uint8)
         codes = codes.view(outputs, -1)[:, :inputs + inputs % 2].contiguous()

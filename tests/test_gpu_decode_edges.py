@@ -59,6 +59,18 @@ def test_a_lowest_value_among_others_is_out_of_the_race(require_gpu):
     assert got.tolist() == [77, 44] and logprob.tolist() == [0.0, 0.0]
 
 
+def test_scales_that_their_type_cannot_hold_are_refused(require_gpu):
+    w = torch.randn(4, 64, device=DEVICE)
+    for value in (460_000.0, 1e30, math.inf, math.nan):
+        large = w.clone()
+        large[1, 40] = value
+        refused(lambda: decode.Q4Weight.quantize(large, 32, torch.float16))
+    large[1, 40] = 460_000.0
+    for dtype in (torch.float32, torch.bfloat16):
+        y = decode.q4_matvec(torch.eye(64, device=DEVICE), decode.Q4Weight.quantize(large, 32, dtype))
+        assert bool(torch.isfinite(y).all()) and abs(y[40, 1].item() / 460_000.0 - 1) <= 2.0 ** -8
+
+
 @pytest.mark.parametrize("rows", [1, 3, 20, 70])
 def test_results_beside_their_operands(require_gpu, rows):
     # columns of one buffer, and neighbours in memory, share nothing
@@ -82,3 +94,19 @@ def test_results_beside_their_operands(require_gpu, rows):
     assert torch.equal(decode.control_logits(z[:, 200:380], out=z[:, 20:200]), want)
     refused(lambda: decode.control_logits(z[:, :180], out=z[:, 20:200]))
     assert torch.equal(decode.control_logits(z[:, 20:200], out=z[:, 20:200]), want)
+
+
+def test_a_weight_is_rounded_inside_a_graph(require_gpu):
+    w, x = torch.randn(40, 96, device=DEVICE), torch.randn(2, 96, device=DEVICE)
+    fixed = w.clone()
+    decode.q4_matvec(x, decode.Q4Weight.quantize(w))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = decode.q4_matvec(x, decode.Q4Weight.quantize(fixed))
+    for factor in (1.0, 3.0, -0.5):
+        fixed.copy_(w * factor)
+        graph.replay()
+        eager = decode.q4_matvec(x, decode.Q4Weight.quantize(w * factor))
+        torch.cuda.synchronize()
+        assert torch.equal(y, eager)
