@@ -145,6 +145,7 @@ class Q4Weight:
         GPU and is left out while a graph is captured."""
         if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not weight.is_floating_point():
             _refuse("weight must be a floating matrix")
+        _device("weight", weight)
         if group not in (32, 64, 128):
             _refuse(f"group must be 32, 64 or 128, not {group}")
         outputs, inputs = weight.shape

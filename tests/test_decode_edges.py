@@ -63,3 +63,10 @@ def test_controlled_logits_beside_the_logits_are_refused(out, change):
     assert "overlaps the logits" in refusal("leo_control_logits", native.LeoLogitControl, {**dict(
         rows=4, symbols=257, logits=1 << 20, logits_stride=257, out=(1 << 20) + out, out_stride=257,
         type=native.TYPE_F32), **change})
+
+
+def test_a_weight_off_the_gpu_is_refused():
+    code = ("import torch\nfrom leo_amd import decode, native\ntry:\n    decode.Q4Weight.quantize(torch.ones(4, 64))\n"
+            "except native.LeoError as e:\n    assert e.code == native.ERR_INVALID_ARGUMENT and 'on the GPU' in str(e)\n"
+            "else:\n    raise SystemExit(1)\n")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=str(ROOT))
