@@ -148,9 +148,15 @@ class Q4Weight:
         _device("weight", weight)
         if group not in (32, 64, 128):
             _refuse(f"group must be 32, 64 or 128, not {group}")
+        if scale_dtype not in _TYPES:
+            _refuse(f"scales have type float32, float16 or bfloat16, not {scale_dtype}")
         outputs, inputs = weight.shape
-        padded = torch.nn.functional.pad(weight.float(), (0, -inputs % group)).view(outputs, -1, group)
-        scales = (padded.abs().amax(dim=2) / 7.0).to(scale_dtype)
+        padded = torch.nn.functional.pad(weight.detach().float(), (0, -inputs % group)).view(outputs, -1, group)
+        largest = padded.abs().amax(dim=2)
+        scales = (largest / 7.0).to(scale_dtype)
+        # among the type's smallest values, where rounding may have left too little, its next one
+        bits = scales.view(torch.int32 if scale_dtype is torch.float32 else torch.int16)
+        scales = (bits + (largest > 7.5 * scales.float())).view(scale_dtype)
         if not torch.cuda.is_current_stream_capturing() and not bool(scales.isfinite().all()):
             _refuse(f"a group's largest magnitude over 7 is no finite {scale_dtype}")
         divide = torch.where(scales == 0, torch.ones_like(scales), scales).float()

@@ -71,6 +71,21 @@ def test_scales_that_their_type_cannot_hold_are_refused(require_gpu):
         assert bool(torch.isfinite(y).all()) and abs(y[40, 1].item() / 460_000.0 - 1) <= 2.0 ** -8
 
 
+@pytest.mark.parametrize("scale", TYPES)
+def test_small_weights_move_by_half_a_step_at_most(require_gpu, scale):
+    # groups whose scale is a few of the smallest steps of float16: the scale in its type is the step
+    for size in (1e-9, 1e-7, 2.5e-7, 6e-7, 1e-6, 3e-5, 1e-3):
+        w = torch.randn(64, 96, device=DEVICE) * size
+        weight = decode.Q4Weight.quantize(w, 32, scale)
+        got = decode.q4_matvec(torch.eye(96, device=DEVICE), weight, out_dtype=torch.float32).t()
+        largest = w.abs().view(64, 3, 32).amax(2)
+        # the step is the scale as its type holds it: the largest over 7, or the next of the type's values above it
+        grid = {torch.float32: 2.0 ** -23, torch.bfloat16: 2.0 ** -7, torch.float16: 2.0 ** -10}[scale]
+        step = largest / 7 * (1 + grid) + (2.0 ** -24 if scale == torch.float16 else 0.0)
+        off = (got - w).abs().view(64, 3, 32)
+        assert bool((off <= (step * (0.5 + 1e-5))[:, :, None]).all()), (size, (off / step[:, :, None]).max().item())
+
+
 @pytest.mark.parametrize("rows", [1, 3, 20, 70])
 def test_results_beside_their_operands(require_gpu, rows):
     # columns of one buffer, and neighbours in memory, share nothing
@@ -110,3 +125,13 @@ def test_a_weight_is_rounded_inside_a_graph(require_gpu):
         eager = decode.q4_matvec(x, decode.Q4Weight.quantize(w * factor))
         torch.cuda.synchronize()
         assert torch.equal(y, eager)
+
+
+def test_a_parameter_is_rounded(require_gpu):
+    w = torch.nn.Parameter(torch.randn(20, 64, device=DEVICE))
+    x = torch.randn(3, 64, device=DEVICE)
+    for scale in TYPES:
+        got = decode.q4_matvec(x, decode.Q4Weight.quantize(w, 64, scale))
+        assert torch.equal(got, decode.q4_matvec(x, decode.Q4Weight.quantize(w.detach().clone(), 64, scale)))
+    for scale in (torch.float64, torch.int32, torch.uint8, None):
+        refused(lambda: decode.Q4Weight.quantize(w, 64, scale))
