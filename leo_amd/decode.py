@@ -176,7 +176,9 @@ def q4_matvec(x: torch.Tensor, weight: Q4Weight, bias: Optional[torch.Tensor] = 
         return q4_matvec(x[None], weight, bias, out_dtype=out_dtype)[0]
     if out is None:
         out = -1 if out_dtype is None else _TYPES.get(out_dtype, len(_TYPES))
-    elif out_dtype is not None and getattr(out, "dtype", None) is not out_dtype:
+    elif not isinstance(out, torch.Tensor):      # a number would pass for a type
+        _refuse("out must be a tensor on the GPU")
+    elif out_dtype is not None and out.dtype is not out_dtype:
         _refuse(f"out must have type {out_dtype}")
     return _binding.q4_matvec(x, weight.layout, weight._shape, bias, out)
 

@@ -86,6 +86,14 @@ def test_small_weights_move_by_half_a_step_at_most(require_gpu, scale):
         assert bool((off <= (step * (0.5 + 1e-5))[:, :, None]).all()), (size, (off / step[:, :, None]).max().item())
 
 
+def test_results_are_tensors(require_gpu):
+    weight = decode.Q4Weight.quantize(torch.randn(8, 64, device=DEVICE))
+    x = torch.randn(2, 64, device=DEVICE)
+    for out in (0, 1, 2, -1, True, 1 << 70):
+        refused(lambda: decode.q4_matvec(x, weight, out=out))
+        refused(lambda: decode.q4_matvec(x, weight, out_dtype=torch.float32, out=out))
+
+
 @pytest.mark.parametrize("rows", [1, 3, 20, 70])
 def test_results_beside_their_operands(require_gpu, rows):
     # columns of one buffer, and neighbours in memory, share nothing
