@@ -677,10 +677,10 @@ __global__ __launch_bounds__(256) void leo_q4_join(TileArgs a) {
     constexpr uint32_t kOutputs = 256 / kLanes;
     __shared__ float joined[kLanes][kOutputs];
     const uint32_t output = blockIdx.x * kOutputs + threadIdx.x % kOutputs, part = threadIdx.x / kOutputs;
-    const uint32_t row = blockIdx.y + blockIdx.z * 32768;
+    const uint32_t row = blockIdx.y;
     const uint32_t width = a.tiles * kTile;
     float sum = 0.0f;
-    if (output < a.outputs && row < a.rows) {
+    if (output < a.outputs) {
         const float* at = a.partials + static_cast<uint64_t>(row) * width + output;
         const uint64_t step = static_cast<uint64_t>(a.rows) * width;
         for (uint32_t s = part; s < a.slices; s += kLanes * 8) {
@@ -699,7 +699,7 @@ __global__ __launch_bounds__(256) void leo_q4_join(TileArgs a) {
 #pragma unroll
         for (uint32_t p = 1; p < kLanes; ++p) sum += joined[p][threadIdx.x];
     }
-    if (output < a.outputs && row < a.rows)
+    if (output < a.outputs)
         store_any(a.y, row * a.y_stride + output, sum + (a.bias ? a.bias[output] : 0.0f), a.y_type);
 }
 
@@ -893,8 +893,9 @@ int32_t leo_q4_matvec(const LeoQ4Product* product, void* stream) {
         else launch_products<BF16>(p.shape, plan, a, at);
         if (plan.slices == 1) return;
         const bool many = plan.slices >= 16;  // slices enough to share among threads
-        const uint32_t outputs = many ? 32 : 256, rows = std::min(a.rows, 32768u);
-        const dim3 grid((a.outputs + outputs - 1) / outputs, rows, (a.rows + rows - 1) / rows);
+        // slices are several only where groups times slabs are half of kManyGroups at most: 16,384 rows
+        const uint32_t outputs = many ? 32 : 256;
+        const dim3 grid((a.outputs + outputs - 1) / outputs, a.rows);
         launch(many ? leo_q4_join<8> : leo_q4_join<1>, grid, dim3(256), 0, at, a);
     });
 }

@@ -143,3 +143,12 @@ def test_a_parameter_is_rounded(require_gpu):
         assert torch.equal(got, decode.q4_matvec(x, decode.Q4Weight.quantize(w.detach().clone(), 64, scale)))
     for scale in (torch.float64, torch.int32, torch.uint8, None):
         refused(lambda: decode.Q4Weight.quantize(w, 64, scale))
+
+
+@pytest.mark.parametrize("rows", [16_000, 16_384, 16_400])
+def test_slices_of_the_most_rows(require_gpu, rows):
+    # up to 16,384 rows a product is split over its inputs and joined
+    codes, scales, z = make(16, 1100, 32, torch.float16, True, rows)
+    weight = decode.Q4Weight(codes, scales, z, inputs=1100, group=32)
+    x = torch.randn(rows, 1100, device=DEVICE).to(torch.bfloat16)
+    check(decode.q4_matvec(x, weight), x, dense(codes, scales, z, 1100, 32), None, torch.bfloat16)
