@@ -59,6 +59,19 @@ def test_a_lowest_value_among_others_is_out_of_the_race(require_gpu):
     assert got.tolist() == [77, 44] and logprob.tolist() == [0.0, 0.0]
 
 
+@pytest.mark.parametrize("rows,inputs,outputs", [(17, 128, 64), (32, 640, 100), (32, 1000, 257), (24, 24_002, 40), (40, 1002, 70)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_on_and_off_word_boundaries(require_gpu, rows, inputs, outputs, dtype):
+    # rows at multiples of 4 bytes (even base and stride), a base off them with an even stride, and an odd stride
+    for group, scale, zeros in ((32, torch.float16, True), (64, torch.bfloat16, False), (128, torch.float32, True)):
+        codes, scales, z = make(outputs, inputs, group, scale, zeros, rows + inputs)
+        weight = decode.Q4Weight(codes, scales, z, inputs=inputs, group=group)
+        w = dense(codes, scales, z, inputs, group)
+        for pad, begin in ((0, 0), (4, 1), (2, 2), (5, 0), (5, 3)):
+            x = torch.randn(rows, inputs + pad, device=DEVICE).to(dtype)[:, begin:begin + inputs]
+            check(decode.q4_matvec(x, weight), x, w, None, dtype)
+
+
 def test_scales_that_their_type_cannot_hold_are_refused(require_gpu):
     w = torch.randn(4, 64, device=DEVICE)
     for value in (460_000.0, 1e30, math.inf, math.nan):
