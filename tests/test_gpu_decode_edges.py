@@ -59,6 +59,42 @@ def test_a_lowest_value_among_others_is_out_of_the_race(require_gpu):
     assert got.tolist() == [77, 44] and logprob.tolist() == [0.0, 0.0]
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("symbols", [3000, 16_384, 16_385, 40_001])
+def test_temperatures_that_are_no_powers_of_two(require_gpu, dtype, symbols):
+    # top-k counts are whole numbers, so the symbol is exact where z is the float32 quotient: this holds the corrected
+    # product with the reciprocal to a division, and the undivided bound that values are gathered by to its margin
+    gen = torch.Generator(DEVICE).manual_seed(symbols)
+    t = [0.7, 0.8, 1.3, 0.6, 3.1, 0.05, 17.3, 1e-3, 911.0, 0.9999999, 1.0000001, 0.333]
+    rows = len(t)
+    logits = (torch.randn(rows, symbols, generator=gen, device=DEVICE) * 2.5).to(dtype)
+    noise = gumbel(gen, rows, symbols)
+    for scale in (1.0, -3.0):      # against the order of the values: many turns before one that stays
+        for k in ([1, 2, 40, 500, 7, 3, 1000, symbols, 40, 5, 60, 20], [40] * rows):
+            compare(logits, noise + (scale < 0) * scale * logits.float() / per_row(t)[:, None], t, k, [1.0] * rows, [0.0] * rows)
+
+
+@pytest.mark.parametrize("symbols", [3000, 40_001])
+@pytest.mark.parametrize("size", [1e-20, 1e20])
+def test_temperatures_with_small_and_large_logits(require_gpu, symbols, size):
+    gen = torch.Generator(DEVICE).manual_seed(symbols + 1)
+    logits = torch.randn(6, symbols, generator=gen, device=DEVICE) * size
+    t = [0.7 * size, 1.3 * size, 0.8, 0.011 * size, 2.9 * size, 0.6]
+    compare(logits, gumbel(gen, 6, symbols), t, [40, 3, 1000, 40, 500, 2], [1.0] * 6, [0.0] * 6)
+
+
+@pytest.mark.parametrize("symbols", [3000, 40_001])
+def test_min_p_at_temperatures_that_are_no_powers_of_two(require_gpu, symbols):
+    # quarters over t: the distances to the largest are k / 4 t, and the cut lies between two of them, 2 % of it away
+    gen = torch.Generator(DEVICE).manual_seed(symbols + 2)
+    t = [0.7, 0.8, 1.3, 0.6]
+    logits = (torch.randn(4, symbols, generator=gen, device=DEVICE) * 10).round() / 4
+    floor = [math.exp(-(k + 0.5) / 4 / u) for k, u in zip([3, 9, 14, 20], t)]
+    noise = gumbel(gen, 4, symbols)
+    compare(logits, noise, t, [symbols] * 4, [1.0] * 4, floor)
+    compare(logits, noise - 3 * logits / per_row(t)[:, None], t, [symbols, 50, symbols, 400], [1.0] * 4, floor)
+
+
 @pytest.mark.parametrize("rows,inputs,outputs", [(17, 128, 64), (32, 640, 100), (32, 1000, 257), (24, 24_002, 40), (40, 1002, 70)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_rows_on_and_off_word_boundaries(require_gpu, rows, inputs, outputs, dtype):
