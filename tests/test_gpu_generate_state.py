@@ -102,3 +102,15 @@ def test_writing_needs_an_open_document(require_gpu, runtime, readout):
         generator.prompt(b"a")
         ends()
         no_document(lambda: generator.write(5))
+
+
+@pytest.mark.parametrize("readout", ["q4", "device"])
+def test_every_prefix_is_utf8(require_gpu, runtime, readout):
+    for seed in range(6):
+        generator = Generator(runtime, readout=readout, seed=seed)
+        start = "café ".encode()[:-2]                            # ends inside a character
+        generator.prompt(start)
+        text, _ = generator.write(60, temperature=2.0, top_k=257, top_p=1.0, allow_end=False)
+        decoder = codecs.getincrementaldecoder("utf-8")("strict")
+        decoder.decode(start + text, final=False)                # raises at the first byte that cannot stand there
+        assert (generator._state == 0) == (decoder.getstate()[0] == b"")
