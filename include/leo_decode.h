@@ -59,8 +59,12 @@ typedef struct LeoQ4Source {
 int32_t leo_q4_layout(const LeoQ4Source* source, void* stream);
 
 /* y[m, n] = bias[n] + sum over k of x[m, k] * w[n, k] for `rows` rows of x.
- * Sums are held in 32 bits and rounded once to y_type; bias (float) may be
- * NULL. y and x share no memory. `workspace`: at least leo_q4_workspace_bytes()
+ * Sums are held in 32 bits and rounded once to y_type. x enters its products in
+ * half precision, float16 as it is, others under a power of two for each row and
+ * 128 inputs: bfloat16 in one part, float in two (22 bits), both to 2^-39 of the
+ * largest of those 128. Scales have to stay below 2^100 in magnitude: a group's sum
+ * is scaled before that power of two is taken back. bias (float) may be NULL. y and
+ * x share no memory. `workspace`: at least leo_q4_workspace_bytes()
  * bytes (none where that is 0), 256-byte aligned, whatever they hold; free again
  * when the call's work is done. */
 typedef struct LeoQ4Product {

@@ -28,7 +28,7 @@ __device__ __forceinline__ Run row_run(const int64_t* offsets, uint64_t row, uin
 // the large calls: 128 rows of 131,075 float32 symbols with 8,192 symbols of history
 // and 300 biases a row, 138 MB, take 33 to 40 us (3.5 to 4.2 TB/s), of which the lists,
 // read once a chunk, are some 9 (31 us without them); hence the widest chunk that the
-// LDS of two workgroups a CU holds: 64 KB. A launch bounds the small: 3.7 us for 257.
+// LDS of two workgroups a CU holds: 64 KB. A launch bounds the small: 3.4 to 5 us for 257.
 constexpr uint32_t kTable = 16384, kControlThreads = 1024;
 
 template <class T>
@@ -402,7 +402,7 @@ __device__ __forceinline__ void add_above(float low, float high, float top, floa
 
 // A short row, in the registers of one workgroup: one span a wave, so that logits
 // and noise are read once and every turn works on registers. A launch bounds it
-// (257 symbols: 4.5 us), then one workgroup's turns.
+// (257 symbols: 4.6 us), then one workgroup's turns.
 // Up to 16 spans: 128 rows of 12,000 symbols took 23.0 us in the two launches below
 // and 19.5 so, of 16,000 32.1 and 20.4, one row of 12,000 9.8 and 6.8.
 template <class T>
@@ -438,7 +438,7 @@ __global__ __launch_bounds__(kMostWaves * 64) void leo_sample_row(LeoSample a) {
 // Longer rows take two launches: one wave a span weighs it and holds its race,
 // and one workgroup a row settles the rest from the spans' records. This one reads
 // everything once and is bound by memory: 128 rows of 131,075 float32 logits with
-// noise, 134 MB, take 22.8 us (5.9 TB/s).
+// noise, 134 MB, take 22.4 us (6.0 TB/s).
 struct SpanRecord {
     Racer best;
     float top, mass;
@@ -463,14 +463,17 @@ __global__ __launch_bounds__(256) void leo_sample_spans(LeoSample a, uint32_t sp
 // column, and counted and weighed from there: one compare a logit passes over
 // the others. If no column runs over, later values, which are higher, need the
 // columns alone. One CU's loads bound it: it reads again the spans that reach above
-// the value, a megabyte for 262,147 symbols, and 128 rows of 131,075 take 24.6 us, 16
-// rows of 32,001 11.1 and two of 262,147 14 to 46, as the values fall. A third launch
-// that gathered over all CUs gave back in latency what it saved (32,001: 5 + 7 + 10 us
-// for 5 + 11, 131,075: 23 + 22 + 21 for 23 + 25). Two launches that take the first two
-// turns with a wave a span held calls of one to four rows of 262,147 to 25 to 30 us
-// under min_p, which take 17 to 46 so, but not their mean (28.0, 28.2 and 29.3 against
-// 24.3, 27.4 and 30.4), and cost top_k 3 to 63 us below a million symbols. kProbe: 1.5, 2 and 2.5 deviations
-// took 48.2, 50.6 and 58 us for both kernels at 128 rows of 131,075.
+// the value, a megabyte for 262,147 symbols, and 128 rows of 131,075 take 24.3 us, 16
+// rows of 32,001 11.1 and two of 262,147 10 to 146 as the values fall (24 states: half
+// of them below 22). A third launch that gathered over all CUs gave back in latency what
+// it saved (32,001: 5 + 7 + 10 us for 5 + 11, 131,075: 23 + 22 + 21 for 23 + 25). Two
+// launches that take the first two turns with a wave a span: calls of 1, 2, 4 and 8 rows
+// of 262,147 under min_p took 28.0, 28.2, 29.3 and 31.8 us against 24.3, 27.4, 30.4 and
+// 60.9 so, the mean of 4 states, and of a million symbols 46 to 134 against 26 to 225;
+// with top_k they cost 3 to 63 us below a million symbols. Not taken: the sizes do not
+// tell the two apart, and which filters a call has was not made part of the rule. kProbe:
+// 1.5, 2 and 2.5 deviations took 48.2, 50.6 and 58 us for both kernels at 128 rows of
+// 131,075 normal logits; other sizes and distributions were not tried.
 constexpr uint32_t kColumn = 12, kTogether = 2;
 constexpr float kProbe = 1.5f;
 struct Column {

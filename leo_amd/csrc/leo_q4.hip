@@ -206,7 +206,11 @@ __device__ __forceinline__ uint32_t top_exponent(const Eight<X> (&v)[4]) {
 }
 
 // Half precision halves of x * factor: the value to 11 bits and, of a 32-bit x,
-// the 11 below them.
+// the 11 below them. With the block's largest at 2^14 .. 2^15 and half precision's
+// smallest at 2^-24, a bfloat16 x is exact down to 2^-31 of the largest, and nothing
+// is further off than its last bit or 2^-39 of the largest: a third half would add
+// half as many matrix instructions for bits that a float sum of a block drops too,
+// unless the largest meet weights of 0.
 template <class X, int kParts>
 __device__ __forceinline__ void halves(const Eight<X>& v, float factor, half8 (&a)[kParts]) {
     float f[8];
@@ -231,8 +235,9 @@ __device__ __forceinline__ uint32_t and_or(uint32_t word, uint32_t mask, uint32_
     return v;
 }
 
-// Four pairs of codes less their zero, exactly: in half precision 1024 + u is
-// the bits 0x6400 | u and 1024 + 16 u the bits 0x6400 | u << 4.
+// Four pairs of codes less their zero, exactly, by the known way of placing a whole
+// number in a float's last bits: in half precision 1024 + u is the bits 0x6400 | u
+// and 1024 + 16 u the bits 0x6400 | u << 4.
 __device__ __forceinline__ half8 weights_of(uint32_t word, half2 minus, half2 minus_high) {
     const half2 sixteenth = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
     union {
@@ -408,8 +413,8 @@ __global__ __launch_bounds__(256) void leo_q4_prepare(TileArgs a, half8* ready, 
 // row that is not there. Instructions bound it, not memory: a tile and block of
 // 1,024 bytes of codes takes 60 to 90 of them to widen the codes and apply the
 // scales, while the matrix instructions have 15 of 16 rows idle. One row of 1,048,576
-// float32 inputs to 257 outputs (147 MB) takes 35.1 us, 4.2 TB/s; 8,192 to 8,192 in
-// bfloat16 (35 MB) 9.3 us, 3.7 TB/s; 1,024 to 257 a launch, 4.7 us. Two tiles a
+// float32 inputs to 257 outputs (147 MB) takes 35.7 us, 4.1 TB/s; 8,192 to 8,192 in
+// bfloat16 (35 MB) 9.6 us, 3.6 TB/s; 1,024 to 257 a launch, 4.7 us. Two tiles a
 // workgroup: x is brought into LDS half as often.
 constexpr uint32_t kFewWaves = 8, kAhead = 2, kFewTiles = 2;
 
@@ -531,9 +536,11 @@ __global__ __launch_bounds__(kFewWaves * 64) void leo_q4_few(TileArgs a) {
 // four waves share, each wave bringing 16 rows of one block a step, so a step is
 // 4 / kRows blocks; codes go straight to registers, some blocks ahead. A weight is
 // widened once for all 16 kRows rows. 8 rows of 131,072 bfloat16 inputs to 257 outputs
-// (20 MB) take 12.5 us, most of it the way in and out of 441 short workgroups; 64 rows
-// of 5,001 to 11,007 (7 GFLOP) 21.6 us, 325 TFLOP/s, bound by the some 420 vector
-// instructions of a step at two waves a SIMD, which the registers allow.
+// (20 MB) take 12.5 us: the way in and out of 441 short workgroups, and 257 outputs are
+// 17 tiles in 24 places, of which 7 read and multiply the last tile again. 64 rows
+// of 5,001 to 11,007 (7 GFLOP) 21.4 us, 330 TFLOP/s, bound by the some 420 vector
+// instructions of a step at two waves a SIMD, which the registers allow; its 430
+// workgroups leave 82 of the 256 CUs with one where the others have two.
 constexpr uint32_t kManyWaves = 4, kManyTiles = 2;
 
 template <class X, int kGroups, bool kZero, bool kWide, int kRows>
@@ -670,7 +677,7 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void leo_q4_many(TileArgs a) {
 
 // Adds the slices of 256 / kLanes outputs of one row, kLanes threads an output,
 // always in the same order, so that results do not depend on which workgroup ends
-// first. A launch bounds it (3.9 to 4.9 us); joining in the last workgroup to arrive
+// first. A launch bounds it (3.8 to 4.8 us); joining in the last workgroup to arrive
 // cost 4 to 7 us, and up to 40 with 64 slices, for its waits on stores and its atomics.
 template <uint32_t kLanes>
 __global__ __launch_bounds__(256) void leo_q4_join(TileArgs a) {

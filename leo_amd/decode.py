@@ -168,8 +168,10 @@ class Q4Weight:
 def q4_matvec(x: torch.Tensor, weight: Q4Weight, bias: Optional[torch.Tensor] = None, *,
               out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """bias + x W^T for x [rows, inputs] (or [inputs]) of float32, float16 or
-    bfloat16: sums in 32 bits, rounded once to `out_dtype` (x's type by default).
-    bias: float32 [outputs]. `out` and x share no memory."""
+    bfloat16: sums in 32 bits, rounded once to `out_dtype` (x's type by default). A
+    float32 x enters with 22 bits of each value, and to 2^-39 of the largest of its
+    row's 128 neighbouring inputs, to which a bfloat16 x is held too; scales have to
+    stay below 2^100. bias: float32 [outputs]. `out` and x share no memory."""
     if isinstance(x, torch.Tensor) and x.dim() == 1:
         if out is not None:
             _refuse("out needs x with two axes")

@@ -9,9 +9,12 @@ that UTF-8 allows next) and the draw. The loop is that of the reference's
 generation (crates/leo-cli/src/main.rs:834-1009), with its UTF-8 state
 (crates/leo-core/src/utf8.rs:4-87) as a grammar mask.
 
-The 4-bit readout takes an eighth of the output weights' memory and answers from
-the neurons alone, without the context's share; readout="device" takes the
-runtime's own logits instead.
+The 4-bit readout answers from the neurons alone, without the context's share. Its
+weights are an eighth of the output weights' size, beside those, which the runtime
+keeps. readout="device" takes the runtime's own logits, which every step leaves and
+which are quicker to have: 58 us a byte against 180 at 1,024 neurons, 60 against 132
+at 1,048,576, where the product of all weights alone takes 39 us and the active
+neurons come by way of the host.
 """
 from __future__ import annotations
 
@@ -120,7 +123,7 @@ class Generator:
         model ends the document. Needs the document that `prompt` began, ended neither
         by the model nor by another use of the runtime. The penalties look at the last
         `history` bytes, the prompt's among them; `bias` adds to single bytes' logits
-        (256: the end)."""
+        (256: the end). A top_k below 1 keeps the largest alone, as 1 does."""
         if self._document != self.runtime.documents:
             raise native.LeoError(native.ERR_INVALID_ARGUMENT, "no document is open: begin one with prompt()")
 
@@ -187,7 +190,7 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
     for name, default in (("temperature", 0.8), ("top-p", 0.95), ("min-p", 0.0), ("repetition", 1.1), ("presence", 0.0),
                           ("frequency", 0.0)):
         parser.add_argument("--" + name, type=float, default=default)
-    parser.add_argument("--top-k", type=int, default=40)
+    parser.add_argument("--top-k", type=int, default=40, help="bytes to draw from; below 2 the likeliest alone, 257 for all")
     parser.add_argument("--history", type=int, default=64)
     args = parser.parse_args(argv)
     if args.checkpoint:
