@@ -6,7 +6,6 @@ from __future__ import annotations
 
 import math
 
-import numpy as np
 import pytest
 import torch
 
@@ -95,7 +94,8 @@ def test_min_p_at_temperatures_that_are_no_powers_of_two(require_gpu, symbols):
     compare(logits, noise - 3 * logits / per_row(t)[:, None], t, [symbols, 50, symbols, 400], [1.0] * 4, floor)
 
 
-@pytest.mark.parametrize("rows,inputs,outputs", [(17, 128, 64), (32, 640, 100), (32, 1000, 257), (24, 24_002, 40), (40, 1002, 70)])
+@pytest.mark.parametrize("rows,inputs,outputs", [(17, 128, 64), (32, 640, 100), (32, 1000, 257), (24, 24_002, 40),
+                                                 (40, 1002, 70)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_rows_on_and_off_word_boundaries(require_gpu, rows, inputs, outputs, dtype):
     # rows at multiples of 4 bytes (even base and stride), a base off them with an even stride, and an odd stride

@@ -4,7 +4,6 @@ from __future__ import annotations
 
 import codecs
 
-import numpy as np
 import pytest
 import torch
 
