@@ -2,12 +2,14 @@
  * leo_decode.h -- C-ABI of the operators that take a model from activations to
  * its next symbol: matrix-vector products with 4-bit weights and group scales
  * (the readout of a served model), the control of logits (penalties for
- * repeated symbols, biases, grammar masks) and the draw of one symbol a row.
+ * repeated symbols, biases, grammar masks) and the draw of one symbol a row; and
+ * of those that answer with several hypotheses at once: products with 8-bit
+ * weights and activations, the selection of beams and the reordering of their states.
  *
  * Same manner as leo_hip.h: every call returns an int32 status (0 = ok) and
  * leo_hip_last_error() returns the message of the last failure on the calling
- * thread. All pointers inside the argument structs are device memory of the
- * device that `stream` (a hipStream_t; NULL = the default stream) belongs to,
+ * thread. All pointers inside the argument structs (but LeoReorder's `arrays`) are
+ * device memory of the device that `stream` (a hipStream_t; NULL = the default stream) belongs to,
  * which must be the calling thread's current device. Calls enqueue work on
  * `stream` and return without waiting; they allocate nothing, so they may be
  * captured into a HIP graph. Strides count elements; the last axis is dense.
@@ -158,6 +160,126 @@ typedef struct LeoSample {
 } LeoSample;
 int32_t leo_sample_workspace_bytes(uint64_t rows, uint64_t symbols, uint64_t* bytes);
 int32_t leo_sample(const LeoSample* sample, void* stream);
+
+/* An 8-bit weight matrix [outputs, inputs]: w[n, k] = scale[n] * code[n, k] with
+ * codes -128..127. */
+typedef struct LeoQ8Shape {
+    uint64_t outputs;
+    uint64_t inputs;
+} LeoQ8Shape;
+
+/* Bytes of the device layout that leo_q8_layout writes. */
+int32_t leo_q8_layout_bytes(const LeoQ8Shape* shape, uint64_t* bytes);
+
+/* Lays a matrix out once for leo_q8_matmul. codes: int8, codes_stride from row to
+ * row; scales: `outputs` values of scale_type. `layout` (256-byte aligned)
+ * receives layout_bytes. */
+typedef struct LeoQ8Source {
+    LeoQ8Shape shape;
+    const void* codes;
+    int64_t codes_stride;
+    const void* scales;
+    int32_t scale_type; /* LEO_TYPE_* */
+    uint32_t pad0;
+    void* layout;
+    uint64_t layout_bytes;
+} LeoQ8Source;
+int32_t leo_q8_layout(const LeoQ8Source* source, void* stream);
+
+/* y[m, n] = bias[n] + s[m] * scale[n] * sum over k of q[m, k] * code[n, k], where
+ * s[m] is the larger of 2^-126 and the largest magnitude of row m of x over 127,
+ * rounded to float, and q[m, k] the whole number nearest to x[m, k] / s[m], of two
+ * the even one. Sums of codes are exact, the rest is held in 64 bits, and one
+ * rounding takes it to y_type. A row of x with an infinity or NaN gives NaN. bias
+ * (float) may be NULL. y and x share no memory. `workspace`: at least
+ * leo_q8_workspace_bytes() bytes (none where that is 0), 256-byte aligned, whatever
+ * they hold; free again when the call's work is done. */
+typedef struct LeoQ8Product {
+    LeoQ8Shape shape;
+    const void* layout;
+    uint64_t layout_bytes;
+    uint64_t rows;
+    const void* x;
+    int64_t x_stride;
+    const float* bias;
+    void* y;
+    int64_t y_stride;
+    int32_t x_type;
+    int32_t y_type;
+    void* workspace;
+    uint64_t workspace_bytes;
+} LeoQ8Product;
+int32_t leo_q8_workspace_bytes(const LeoQ8Shape* shape, uint64_t rows, int32_t x_type, uint64_t* bytes);
+int32_t leo_q8_matmul(const LeoQ8Product* product, void* stream);
+
+/* Beam search's selection, `groups` searches of `beams` hypotheses each. logits has
+ * a row of `symbols` for each hypothesis, scores [groups, beams] the sums of log
+ * probabilities so far, -inf where there is none (NaN counts as -inf). Candidates:
+ *     symbol v after hypothesis b:  score + z[v] - log sum exp z  (those above -inf)
+ *     a finished hypothesis itself:  its score; its logits are not read
+ * and the `kept` (at most 64, as are the beams) with the largest score / length^length_penalty
+ * are taken, largest first; of equals the lower hypothesis, the larger logit, the
+ * lower symbol. length counts the symbol that comes in: lengths[b] + 1, lengths[b]
+ * of a finished one, at least 1; lengths may be NULL where length_penalty is 0.
+ * Logits count as in leo_sample, those of +inf share all probability. Ranks are
+ * held in 64 bits.
+ * out_parents is the hypothesis within its search; out_symbols is -1 for a finished
+ * one. Places that no candidate takes have symbol -1, parent 0 and score -inf.
+ * finished (bytes, 0 or not) may be NULL: none is. out_finished (may be NULL) is 1
+ * for finished ones and where the symbol is `end` (-1: no symbol ends), else 0;
+ * out_lengths (may be NULL, needs lengths) the lengths, hypothesis 0's at places that
+ * no candidate takes. Outputs have [groups, kept] entries. `workspace` as in leo_q4_matvec. */
+typedef struct LeoBeams {
+    uint64_t groups;
+    uint64_t beams;
+    uint64_t kept;
+    uint64_t symbols;
+    const void* logits;
+    int64_t logits_stride;
+    int32_t type;
+    uint32_t pad0;
+    const float* scores;
+    const uint8_t* finished;
+    const int32_t* lengths;
+    double length_penalty;
+    int64_t end;
+    int32_t* out_symbols;
+    int32_t* out_parents;
+    float* out_scores;
+    uint8_t* out_finished;
+    int32_t* out_lengths;
+    void* workspace;
+    uint64_t workspace_bytes;
+} LeoBeams;
+int32_t leo_beam_workspace_bytes(uint64_t groups, uint64_t beams, uint64_t kept, uint64_t symbols, uint64_t* bytes);
+int32_t leo_beam_select(const LeoBeams* beams, void* stream);
+
+/* Rows of `count` arrays in the order of their parents: row g * kept + k of the target
+ * becomes row g * beams + parents[g, k] of the source, zeros where the parent is
+ * outside 0 .. beams-1. A row is `outer` pieces of `width` bytes; strides are
+ * bytes, not negative. An array may be its own target (same address and strides,
+ * kept = beams); otherwise no target shares memory with any source or other target,
+ * which arrays that interleave have to show by common divisors of their strides.
+ * `arrays` is host memory, read during the call. */
+typedef struct LeoStateArray {
+    const void* source;
+    void* target;
+    uint64_t outer;
+    uint64_t width;
+    int64_t source_row;
+    int64_t source_outer;
+    int64_t target_row;
+    int64_t target_outer;
+} LeoStateArray;
+typedef struct LeoReorder {
+    const LeoStateArray* arrays;
+    uint64_t count;
+    uint64_t groups;
+    uint64_t beams; /* at most 64, as is kept */
+    uint64_t kept;
+    const int32_t* parents; /* [groups, kept] */
+} LeoReorder;
+int32_t leo_reorder_states(const LeoReorder* reorder, void* stream);
 
 #ifdef __cplusplus
 }

@@ -54,7 +54,7 @@ def build_library() -> pathlib.Path:
     BUILD.mkdir(exist_ok=True)
     LIB_DIR.mkdir(exist_ok=True)
     commands, objects = [], []
-    for src in ("leo_kernels.hip", "leo_runtime.hip", "leo_q4.hip", "leo_answer.hip"):
+    for src in ("leo_kernels.hip", "leo_runtime.hip", "leo_q4.hip", "leo_answer.hip", "leo_q8.hip", "leo_beams.hip"):
         objects.append(BUILD / (src + ".o"))
         commands.append([HIPCC, *HIP_FLAGS, "-c", CSRC / src, "-o", objects[-1]])
     for src in ("host_model.cpp", "formats.cpp"):

@@ -15,6 +15,7 @@
 
 #include <cstring>
 #include <string>
+#include <vector>
 
 #include "leo_decode.h"
 #include "leo_hip.h"
@@ -131,14 +132,28 @@ bool given(Py_ssize_t n, Py_ssize_t wanted) {
     return false;
 }
 
-// q4_matvec(x, layout, shape as bytes, bias, out or the result's type as LEO_TYPE_* (-1: x's))
-PyObject* q4_matvec(PyObject*, PyObject* const* args, Py_ssize_t n) {
+struct Q4 {
+    using Product = LeoQ4Product;
+    static constexpr const char* kShape = "shape must be a LeoQ4Shape";
+    static constexpr auto workspace_bytes = leo_q4_workspace_bytes;
+    static constexpr auto call = leo_q4_matvec;
+};
+struct Q8 {
+    using Product = LeoQ8Product;
+    static constexpr const char* kShape = "shape must be a LeoQ8Shape";
+    static constexpr auto workspace_bytes = leo_q8_workspace_bytes;
+    static constexpr auto call = leo_q8_matmul;
+};
+
+// product(x, layout, shape as bytes, bias, out or the result's type as LEO_TYPE_* (-1: x's))
+template <class Q>
+PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!given(n, 5)) return nullptr;
     return guarded([&]() -> PyObject* {
         const at::Tensor& layout = tensor(args[1], "layout");
         const int index = layout.get_device();
-        LeoQ4Product p{};
-        if (!PyBytes_Check(args[2]) || PyBytes_GET_SIZE(args[2]) != sizeof(p.shape)) refuse("shape must be a LeoQ4Shape");
+        typename Q::Product p{};
+        if (!PyBytes_Check(args[2]) || PyBytes_GET_SIZE(args[2]) != sizeof(p.shape)) refuse(Q::kShape);
         memcpy(&p.shape, PyBytes_AS_STRING(args[2]), sizeof(p.shape));
         const at::Tensor& input = tensor(args[0], "x");
         const Matrix x = matrix(input, "x", index, kFloating);
@@ -168,13 +183,13 @@ PyObject* q4_matvec(PyObject*, PyObject* const* args, Py_ssize_t n) {
         p.y_stride = y.stride;
         p.y_type = y.type;
         const c10::DeviceGuard guard(input.device());
-        check(leo_q4_workspace_bytes(&p.shape, p.rows, p.x_type, &p.workspace_bytes));
+        check(Q::workspace_bytes(&p.shape, p.rows, p.x_type, &p.workspace_bytes));
         at::Tensor space;
         if (p.workspace_bytes) {
             space = workspace(p.workspace_bytes, input);
             p.workspace = space.data_ptr();
         }
-        check(leo_q4_matvec(&p, stream_of(index)));
+        check(Q::call(&p, stream_of(index)));
         return THPVariable_Wrap(out);
     });
 }
@@ -279,6 +294,194 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// A dense 2-D tensor of a type.
+const at::Tensor& table(PyObject* o, const char* name, at::ScalarType type, int index) {
+    const at::Tensor& t = tensor(o, name);
+    same_device(t, name, index);
+    if (t.scalar_type() != type)
+        refuse(std::string(name) + " must have type " + c10::toString(type) + ", not " + c10::toString(t.scalar_type()));
+    if (t.dim() != 2 || !t.is_contiguous()) refuse(std::string(name) + " must be dense with two axes");
+    return t;
+}
+
+// beam_select(logits, scores, kept, finished, lengths, length_penalty, end); None for what is not given
+PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (!given(n, 7)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const at::Tensor& logits = tensor(args[0], "logits");
+        const int index = logits.get_device();
+        const Matrix z = matrix(logits, "logits", index, kFloating);
+        const at::Tensor& scores = table(args[1], "scores", at::kFloat, index);
+        LeoBeams b{};
+        const int64_t groups = scores.size(0), beams = scores.size(1);
+        const int64_t kept = args[2] == Py_None ? beams : PyLong_AsLongLong(args[2]);
+        if (PyErr_Occurred()) throw python_error();
+        if (beams < 1 || beams > 64) refuse("scores have 1 to 64 beams, not " + std::to_string(beams));
+        if (z.rows != groups * beams)
+            refuse("logits have " + std::to_string(z.rows) + " rows, the scores " + std::to_string(groups * beams) + " entries");
+        b.groups = static_cast<uint64_t>(groups);
+        b.beams = static_cast<uint64_t>(beams);
+        b.kept = static_cast<uint64_t>(kept);
+        b.symbols = static_cast<uint64_t>(z.width);
+        b.logits = z.data;
+        b.logits_stride = z.stride;
+        b.type = z.type;
+        b.scores = static_cast<const float*>(scores.const_data_ptr());
+        const auto beside = [&](PyObject* o, const char* name, at::ScalarType type) -> const void* {
+            if (o == Py_None) return nullptr;
+            const at::Tensor& t = table(o, name, type, index);
+            if (t.size(0) != groups || t.size(1) != beams)
+                refuse(std::string(name) + " must be (" + std::to_string(groups) + ", " + std::to_string(beams) + ")");
+            return t.const_data_ptr();
+        };
+        b.finished = static_cast<const uint8_t*>(beside(args[3], "finished", at::kBool));
+        b.lengths = static_cast<const int32_t*>(beside(args[4], "lengths", at::kInt));
+        b.length_penalty = PyFloat_AsDouble(args[5]);
+        if (PyErr_Occurred()) throw python_error();
+        b.end = -1;
+        if (args[6] != Py_None) {
+            b.end = PyLong_AsLongLong(args[6]);
+            if (PyErr_Occurred()) throw python_error();
+            if (b.end < 0) refuse("end must be a symbol");
+        }
+        const c10::DeviceGuard guard(logits.device());
+        check(leo_beam_workspace_bytes(b.groups, b.beams, b.kept, b.symbols, &b.workspace_bytes));
+        at::Tensor outs[5];
+        const auto out = [&](int i, at::ScalarType type) {
+            outs[i] = at::empty({groups, kept}, logits.options().dtype(type));
+            return outs[i].data_ptr();
+        };
+        b.out_symbols = static_cast<int32_t*>(out(0, at::kInt));
+        b.out_parents = static_cast<int32_t*>(out(1, at::kInt));
+        b.out_scores = static_cast<float*>(out(2, at::kFloat));
+        if (b.finished || args[6] != Py_None) b.out_finished = static_cast<uint8_t*>(out(3, at::kBool));
+        if (b.lengths) b.out_lengths = static_cast<int32_t*>(out(4, at::kInt));
+        at::Tensor space;
+        if (b.workspace_bytes) {
+            space = workspace(b.workspace_bytes, logits);
+            b.workspace = space.data_ptr();
+        }
+        check(leo_beam_select(&b, stream_of(index)));
+        PyObject* result = PyTuple_New(5);
+        if (!result) throw python_error();
+        for (int i = 0; i < 5; ++i) {
+            PyObject* o = Py_None;
+            if (outs[i].defined()) o = THPVariable_Wrap(outs[i]);
+            else Py_INCREF(o);
+            if (!o) {
+                Py_DECREF(result);
+                throw python_error();
+            }
+            PyTuple_SET_ITEM(result, i, o);
+        }
+        return result;
+    });
+}
+
+// A state's rows as pieces of dense bytes: every axis but the first joined to the
+// one behind it where it can be, and one more beside.
+struct Pieces {
+    int64_t row, outer, width;  // bytes
+    uint64_t count;
+    bool fits;
+};
+Pieces pieces(const at::Tensor& t) {
+    const int64_t e = static_cast<int64_t>(t.element_size());
+    Pieces p{t.stride(0) * e, 0, e, 1, true};
+    for (int64_t d = t.dim() - 1; d > 0; --d) {
+        const int64_t size = t.size(d), stride = t.stride(d) * e;
+        if (size == 1) continue;
+        if (p.count == 1 && stride == p.width) {
+            p.width *= size;
+        } else if (p.count == 1) {
+            p.outer = stride;
+            p.count = static_cast<uint64_t>(size);
+        } else if (stride == p.outer * static_cast<int64_t>(p.count)) {
+            p.count *= static_cast<uint64_t>(size);
+        } else {
+            p.fits = false;
+        }
+    }
+    return p;
+}
+
+// reorder_states(states as a tuple, parents, outs as a tuple or None): a list of the results
+PyObject* reorder_states(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (!given(n, 3)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        if (!PyTuple_Check(args[0]) || (args[2] != Py_None && !PyTuple_Check(args[2]))) refuse("states and outs must be tuples");
+        const at::Tensor& order = tensor(args[1], "parents");
+        const int index = order.get_device();
+        table(args[1], "parents", at::kInt, index);
+        const Py_ssize_t count = PyTuple_GET_SIZE(args[0]);
+        if (args[2] != Py_None && PyTuple_GET_SIZE(args[2]) != count) refuse("out needs a tensor for each of the states");
+        const int64_t groups = order.size(0), kept = order.size(1);
+        if (kept < 1 || kept > 64) refuse("parents have 1 to 64 places a row, not " + std::to_string(kept));
+        const c10::DeviceGuard guard(order.device());
+        std::vector<at::Tensor> outs;
+        std::vector<LeoStateArray> arrays;
+        int64_t beams = 0;
+        for (Py_ssize_t i = 0; i < count; ++i) {
+            const at::Tensor& t = tensor(PyTuple_GET_ITEM(args[0], i), "a state");
+            same_device(t, "a state", index);
+            if (t.layout() != at::kStrided || t.is_conj() || t.is_neg()) refuse("a state must be a dense tensor, its values as they are in memory");
+            if (t.dim() < 1) refuse("a state needs an axis of rows");
+            if (groups > 0 && (t.size(0) % groups || t.size(0) == 0 || (i && t.size(0) != groups * beams)))
+                refuse("a state has " + std::to_string(t.size(0)) + " rows for " + std::to_string(groups) + " groups" +
+                       (i ? " of " + std::to_string(beams) + " beams" : ""));
+            if (groups == 0 && t.size(0)) refuse("a state has rows, the parents none");
+            beams = groups ? t.size(0) / groups : 1;
+            std::vector<int64_t> sizes(t.sizes().begin(), t.sizes().end());
+            sizes[0] = groups * kept;
+            if (args[2] == Py_None) {
+                outs.push_back(at::empty(sizes, t.options()));
+            } else {
+                const at::Tensor& out = tensor(PyTuple_GET_ITEM(args[2], i), "out");
+                same_device(out, "out", index);
+                if (out.layout() != at::kStrided || out.is_conj() || out.is_neg() || out.scalar_type() != t.scalar_type() || out.sizes() != at::IntArrayRef(sizes))
+                    refuse("out must have the states' types, and their shapes with " + std::to_string(groups * kept) + " rows");
+                outs.push_back(out);
+            }
+            if (t.numel() == 0) continue;
+            Pieces from = pieces(t), to = pieces(outs.back());
+            if (!from.fits || !to.fits) refuse("a state's axes behind the first must join to two at most, the last of them dense");
+            // the wider side in the other's pieces
+            if (from.count == 1 && to.count > 1) {
+                from.outer = to.width;
+                from.width = to.width;
+                from.count = to.count;
+            } else if (to.count == 1 && from.count > 1) {
+                to.outer = from.width;
+                to.width = from.width;
+                to.count = from.count;
+            }
+            if (from.count != to.count || from.width != to.width) refuse("a state and its out must join to the same pieces");
+            arrays.push_back({t.const_data_ptr(), outs.back().data_ptr(), from.count, static_cast<uint64_t>(from.width),
+                              from.row, from.outer, to.row, to.outer});
+        }
+        if (beams > 64) refuse("64 beams are the most, not " + std::to_string(beams));
+        LeoReorder r{};
+        r.arrays = arrays.data();
+        r.count = arrays.size();
+        r.groups = static_cast<uint64_t>(groups);
+        r.beams = static_cast<uint64_t>(count ? beams : 1);
+        r.kept = static_cast<uint64_t>(kept);
+        r.parents = static_cast<const int32_t*>(order.const_data_ptr());
+        check(leo_reorder_states(&r, stream_of(index)));
+        PyObject* result = PyList_New(count);
+        if (!result) throw python_error();
+        for (Py_ssize_t i = 0; i < count; ++i) {
+            PyObject* o = THPVariable_Wrap(outs[static_cast<size_t>(i)]);
+            if (!o) {
+                Py_DECREF(result);
+                throw python_error();
+            }
+            PyList_SET_ITEM(result, i, o);
+        }
+        return result;
+    });
+}
+
 // setup(LeoError, stream_of)
 PyObject* setup(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!given(n, 2)) return nullptr;
@@ -289,9 +492,12 @@ PyObject* setup(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyMethodDef kMethods[] = {
-    {"q4_matvec", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(q4_matvec)), METH_FASTCALL, nullptr},
+    {"q4_matvec", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(product<Q4>)), METH_FASTCALL, nullptr},
+    {"q8_matmul", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(product<Q8>)), METH_FASTCALL, nullptr},
     {"control_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(control_logits)), METH_FASTCALL, nullptr},
     {"sample", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sample)), METH_FASTCALL, nullptr},
+    {"beam_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(beam_select)), METH_FASTCALL, nullptr},
+    {"reorder_states", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(reorder_states)), METH_FASTCALL, nullptr},
     {"setup", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(setup)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -1,9 +1,13 @@
 """The operators that take a model from activations to its next symbol, on torch
-tensors: 4-bit readout products, control of logits, and the draw.
+tensors: readout products, control of logits, the draw, and what a search over
+several hypotheses needs beside them.
 
     Q4Weight, q4_matvec   y = b + x W^T with 4-bit codes and group scales
+    Q8Weight, q8_matmul   y = b + x W^T with 8-bit codes and scales, x in 8 bits too
     control_logits        penalties for repeated symbols, biases, grammar masks
     sample                temperature, top-k, top-p, min-p and the draw
+    beam_select           the best hypotheses over all beams and symbols
+    reorder_states        states in the order of the hypotheses' parents
 
 Each call goes through the C-ABI of include/leo_decode.h into libleo_hip.so and
 enqueues its work on the current stream of its tensors' device. Failed checks
@@ -21,7 +25,7 @@ import importlib.machinery
 import importlib.util
 import pathlib
 import sys
-from typing import Optional, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
 from . import native
 
@@ -185,6 +189,80 @@ def q4_matvec(x: torch.Tensor, weight: Q4Weight, bias: Optional[torch.Tensor] = 
     return _binding.q4_matvec(x, weight.layout, weight._shape, bias, out)
 
 
+class Q8Weight:
+    """An 8-bit weight matrix [outputs, inputs], laid out once for `q8_matmul`:
+
+        w[n, k] = scales[n] * codes[n, k]
+
+    codes   int8 [outputs, inputs]
+    scales  float32, float16 or bfloat16 [outputs]
+
+    The layout is the object's own; the arguments are not kept.
+    """
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        self.index = _device("codes", codes)
+        self.device = codes.device
+        outputs, inputs, stride = _matrix("codes", codes, (torch.int8,), self.index)
+        if outputs < 1 or inputs < 1:
+            _refuse("codes have no rows or no columns")
+        if _device("scales", scales) != self.index:
+            _refuse(f"scales is on GPU {scales.get_device()}, not on {self.index}")
+        if scales.dtype not in _TYPES or scales.shape != (outputs,) or not scales.is_contiguous():
+            _refuse(f"scales must be a dense vector of {outputs} float32, float16 or bfloat16 entries")
+        self.outputs, self.inputs = outputs, inputs
+        self.shape = native.LeoQ8Shape(outputs=outputs, inputs=inputs)
+        lib, size = native.load(), ctypes.c_uint64()
+        native.check(lib, lib.leo_q8_layout_bytes(ctypes.byref(self.shape), ctypes.byref(size)))
+        self.layout = torch.empty(size.value, dtype=torch.uint8, device=self.device)
+        source = native.LeoQ8Source(
+            shape=self.shape, codes=codes.data_ptr(), codes_stride=stride, scales=scales.data_ptr(),
+            scale_type=_TYPES[scales.dtype], layout=self.layout.data_ptr(), layout_bytes=size.value)
+        with torch.cuda.device(self.index):
+            native.check(lib, lib.leo_q8_layout(ctypes.byref(source), _stream_of(self.index)))
+        self._shape = bytes(self.shape)
+
+    @classmethod
+    def quantize(cls, weight: torch.Tensor) -> "Q8Weight":
+        """A floating matrix [outputs, inputs] rounded to codes -127..127: a row's
+        scale is its largest magnitude over 127 in float32, at least 2^-126 (0 for a
+        row of zeros). Refuses a weight that is not finite; the check waits for the GPU
+        and is left out while a graph is captured."""
+        if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not weight.is_floating_point():
+            _refuse("weight must be a floating matrix")
+        _device("weight", weight)
+        values = weight.detach().float()
+        if values.numel() == 0:
+            _refuse("weight has no rows or no columns")
+        scales = values.abs().amax(dim=1) / 127.0
+        if not torch.cuda.is_current_stream_capturing() and not bool(scales.isfinite().all()):
+            _refuse("weight is not finite in float32")
+        scales = torch.where(scales > 0, scales.clamp_min(2.0 ** -126), scales)
+        divide = torch.where(scales == 0, torch.ones_like(scales), scales)
+        return cls((values / divide[:, None]).round().clamp(-127, 127).to(torch.int8), scales)
+
+
+def q8_matmul(x: torch.Tensor, weight: Q8Weight, bias: Optional[torch.Tensor] = None, *,
+              out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """bias + x W^T for x [rows, inputs] (or [inputs]) of float32, float16 or
+    bfloat16, with x in 8 bits: a row's scale is its largest magnitude over 127 in
+    float32 (at least 2^-126), its codes the nearest whole numbers to x over that, of
+    two the even one. Sums of codes are exact, the rest has 64 bits and is rounded once
+    to `out_dtype` (x's type by default). A row with an infinity or NaN gives NaN.
+    bias: float32 [outputs]. `out` and x share no memory."""
+    if isinstance(x, torch.Tensor) and x.dim() == 1:
+        if out is not None:
+            _refuse("out needs x with two axes")
+        return q8_matmul(x[None], weight, bias, out_dtype=out_dtype)[0]
+    if out is None:
+        out = -1 if out_dtype is None else _TYPES.get(out_dtype, len(_TYPES))
+    elif not isinstance(out, torch.Tensor):      # a number would pass for a type
+        _refuse("out must be a tensor on the GPU")
+    elif out_dtype is not None and out.dtype is not out_dtype:
+        _refuse(f"out must have type {out_dtype}")
+    return _binding.q8_matmul(x, weight.layout, weight._shape, bias, out)
+
+
 def control_logits(logits: torch.Tensor, *, history: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
                    repetition: Optional[torch.Tensor] = None, presence: Optional[torch.Tensor] = None,
                    frequency: Optional[torch.Tensor] = None,
@@ -225,3 +303,58 @@ def sample(logits: torch.Tensor, noise: Optional[torch.Tensor] = None, *, temper
     top_k int32 [rows]; without them 1, 1, 0 and all.
     """
     return _binding.sample(logits, noise, temperature, top_k, top_p, min_p)
+
+
+class Beams(NamedTuple):
+    """What `beam_select` kept, [groups, kept], the best first."""
+
+    symbols: torch.Tensor              # int32, -1 after a finished hypothesis and where there is none
+    parents: torch.Tensor              # int32, the hypothesis within its group
+    scores: torch.Tensor               # float32, -inf where there is none
+    finished: Optional[torch.Tensor]   # bool, with `finished` or `end` given
+    lengths: Optional[torch.Tensor]    # int32, with `lengths` given
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, kept: Optional[int] = None, *,
+                finished: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                length_penalty: float = 0.0, end: Optional[int] = None) -> Beams:
+    """The `kept` best of all hypotheses' next symbols, for scores [groups, beams]
+    and logits [groups * beams, symbols]; as many as there are beams by default, 64
+    at most.
+
+    A hypothesis continues with symbol v at scores + z[v] - log sum exp z, a finished
+    one stays as it is and its logits are not read. The order is that of score /
+    length^length_penalty, with the length that the hypothesis then has; of equals
+    the lower hypothesis comes first, then the larger logit, then the lower symbol.
+    Ranks have 64 bits. Logits of -inf or NaN are no way on, nor are hypotheses whose
+    score is -inf or NaN. Where fewer than `kept` are left, the others have symbol
+    -1, parent 0, score -inf, and the length of hypothesis 0.
+
+    scores     float32, sums of log probabilities; -inf for beams that do not count, as
+               all but the first where a search begins with one hypothesis
+    finished   bool [groups, beams]
+    lengths    int32 [groups, beams], symbols so far; a length_penalty needs them
+    end        the symbol that finishes a hypothesis
+    """
+    return Beams(*_binding.beam_select(logits, scores, kept, finished, lengths, length_penalty, end))
+
+
+def reorder_states(states: Union[torch.Tensor, Sequence[torch.Tensor]], parents: torch.Tensor, *,
+                   out: Union[None, torch.Tensor, Sequence[torch.Tensor]] = None
+                   ) -> Union[torch.Tensor, List[torch.Tensor]]:
+    """States in the order of their parents [groups, kept] (int32): row g * kept + k
+    of a result is row g * beams + parents[g, k] of a state, zeros where the parent is
+    no row of the group.
+
+    states   one tensor or several, of any types, groups * beams rows on the first
+             axis (64 beams at most); the axes behind join to two, the last of them
+             dense: a cache's filled part of each head, cache[:, :, :length], does
+    out      tensors for the results. The states themselves, where kept is beams: then
+             only rows that move are read and written. Otherwise they share no memory
+             with the states or each other; tensors that interleave have common strides
+    """
+    one = isinstance(states, torch.Tensor)
+    if one:
+        states, out = (states,), out if out is None else (out,)
+    found = _binding.reorder_states(tuple(states), parents, out if out is None else tuple(out))
+    return found[0] if one else found

@@ -308,6 +308,36 @@ class LeoSample(ctypes.Structure):
                 ("workspace_bytes", _U64)]
 
 
+class LeoQ8Shape(ctypes.Structure):
+    _fields_ = [("outputs", _U64), ("inputs", _U64)]
+
+
+class LeoQ8Source(ctypes.Structure):
+    _fields_ = [("shape", LeoQ8Shape), ("codes", _P), ("codes_stride", _I64), ("scales", _P), ("scale_type", _I32),
+                ("pad0", _U32), ("layout", _P), ("layout_bytes", _U64)]
+
+
+class LeoQ8Product(ctypes.Structure):
+    _fields_ = [("shape", LeoQ8Shape), *LeoQ4Product._fields_[1:]]
+
+
+class LeoBeams(ctypes.Structure):
+    _fields_ = [("groups", _U64), ("beams", _U64), ("kept", _U64), ("symbols", _U64), ("logits", _P),
+                ("logits_stride", _I64), ("type", _I32), ("pad0", _U32), ("scores", _P), ("finished", _P),
+                ("lengths", _P), ("length_penalty", ctypes.c_double), ("end", _I64), ("out_symbols", _P),
+                ("out_parents", _P), ("out_scores", _P), ("out_finished", _P), ("out_lengths", _P), ("workspace", _P),
+                ("workspace_bytes", _U64)]
+
+
+class LeoStateArray(ctypes.Structure):
+    _fields_ = [("source", _P), ("target", _P), ("outer", _U64), ("width", _U64), ("source_row", _I64),
+                ("source_outer", _I64), ("target_row", _I64), ("target_outer", _I64)]
+
+
+class LeoReorder(ctypes.Structure):
+    _fields_ = [("arrays", _P), ("count", _U64), ("groups", _U64), ("beams", _U64), ("kept", _U64), ("parents", _P)]
+
+
 DECODE_SIGNATURES = {
     "leo_q4_layout_bytes": (_I32, [_P, _P]),
     "leo_q4_layout": (_I32, [_P, _P]),
@@ -316,6 +346,13 @@ DECODE_SIGNATURES = {
     "leo_control_logits": (_I32, [_P, _P]),
     "leo_sample_workspace_bytes": (_I32, [_U64, _U64, _P]),
     "leo_sample": (_I32, [_P, _P]),
+    "leo_q8_layout_bytes": (_I32, [_P, _P]),
+    "leo_q8_layout": (_I32, [_P, _P]),
+    "leo_q8_workspace_bytes": (_I32, [_P, _U64, _I32, _P]),
+    "leo_q8_matmul": (_I32, [_P, _P]),
+    "leo_beam_workspace_bytes": (_I32, [_U64, _U64, _U64, _U64, _P]),
+    "leo_beam_select": (_I32, [_P, _P]),
+    "leo_reorder_states": (_I32, [_P, _P]),
 }
 
 

@@ -1,0 +1,252 @@
+"""Beam selection on the GPU against its definition in 64 bits.
+
+A score is the sum of a score, a logit less the largest, and the log of a sum of
+exponentials, rounded to float: half a step of its value, and the error of the sum, each
+of whose float terms may be off by 2^-22 of itself: 2^-21 covers it."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from leo_amd import decode, native
+
+pytestmark = pytest.mark.gpu
+DEVICE = "cuda:0"
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def reference(logits, scores, kept, finished=None, lengths=None, penalty=0.0, end=None):
+    """(symbols, parents, scores, finished, lengths) as nested lists, from the definition."""
+    z = logits.detach().cpu().double().numpy()
+    s = scores.cpu().double().numpy()
+    groups, beams = s.shape
+    done = np.zeros_like(s, dtype=bool) if finished is None else finished.cpu().numpy()
+    length = np.zeros_like(s, dtype=np.int64) if lengths is None else lengths.cpu().numpy().astype(np.int64)
+    z = np.where(np.isnan(z), -np.inf, z)
+    out = []
+    for g in range(groups):
+        found = []      # (-rank, hypothesis, place in its row's order, symbol, score)
+        for b in range(beams):
+            if not s[g, b] > -np.inf:
+                continue
+
+            def rank(score, n):
+                return score / float(max(n, 1)) ** penalty
+
+            if done[g, b]:
+                found.append((-rank(s[g, b], length[g, b]), b, 0, -1, s[g, b]))
+                continue
+            row = z[g * beams + b]
+            top = row.max()
+            if top == -np.inf:
+                continue
+            with np.errstate(invalid="ignore"):
+                d = np.where(row == top, 0.0, row - top)
+            lse = math.log(np.exp(d).sum())
+            for place, v in enumerate(np.lexsort((np.arange(row.size), -row))[:kept]):
+                if row[v] > -np.inf and d[v] > -np.inf:
+                    score = s[g, b] + (d[v] - lse)
+                    found.append((-rank(score, length[g, b] + 1), b, place, int(v), score))
+        found.sort()
+        found = found[:kept]
+        rest = kept - len(found)
+        out.append(([f[3] for f in found] + [-1] * rest, [f[1] for f in found] + [0] * rest,
+                    [f[4] for f in found] + [-np.inf] * rest,
+                    [bool(done[g, f[1]]) or (end is not None and f[3] == end) for f in found] + [False] * rest,
+                    [int(length[g, f[1]]) + (0 if done[g, f[1]] else 1) for f in found] + [int(length[g, 0])] * rest))
+    return [[o[i] for o in out] for i in range(5)]
+
+
+def compare(logits, scores, kept, finished=None, lengths=None, penalty=0.0, end=None):
+    got = decode.beam_select(logits, scores, kept, finished=finished, lengths=lengths, length_penalty=penalty, end=end)
+    want = reference(logits, scores, kept, finished, lengths, penalty, end)
+    assert got.symbols.tolist() == want[0]
+    assert got.parents.tolist() == want[1]
+    w, g = np.array(want[2]), got.scores.cpu().double().numpy()
+    with np.errstate(over="ignore"):
+        fine = np.isfinite(w.astype(np.float32))
+    assert np.array_equal(np.isneginf(g), ~fine)
+    assert (np.abs(g[fine] - w[fine]) <= np.abs(w[fine]) * 2.0 ** -24 + 2.0 ** -21).all()
+    assert (got.finished is None) == (finished is None and end is None)
+    if got.finished is not None:
+        assert got.finished.dtype is torch.bool and got.finished.tolist() == want[3]
+    assert (got.lengths is None) == (lengths is None)
+    if got.lengths is not None:
+        assert got.lengths.dtype is torch.int32 and got.lengths.tolist() == want[4]
+    return got
+
+
+def make(seed, groups, beams, symbols, dtype, pad=0):
+    gen = torch.Generator(DEVICE).manual_seed(seed)
+    z = torch.randn(groups * beams, symbols + pad, generator=gen, device=DEVICE) * 3
+    z = torch.where(torch.rand(z.shape, generator=gen, device=DEVICE) < 0.1, torch.full_like(z, -torch.inf), z)
+    scores = -10 - 3 * torch.rand(groups, beams, generator=gen, device=DEVICE)
+    return z.to(dtype)[:, pad:], scores, gen
+
+
+SIZES = [(1, 1, 1, 1), (1, 1, 5, 3), (2, 3, 4, 2), (1, 4, 257, 4), (3, 4, 257, 8), (2, 8, 1000, 8), (1, 16, 257, 32), (2, 5, 4099, 5),
+         (1, 64, 257, 64), (2, 64, 50, 64), (1, 3, 32_001, 6), (1, 8, 70_003, 16), (1, 1, 262_147, 64), (4, 2, 16_385, 1),
+         (1, 2, 131_075, 33), (70, 2, 300, 2)]
+
+
+@pytest.mark.parametrize("groups, beams, symbols, kept", SIZES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sizes_and_types(require_gpu, groups, beams, symbols, kept, dtype):
+    z, scores, gen = make(symbols + kept, groups, beams, symbols, TYPES[dtype])
+    compare(z, scores, kept)
+    finished = torch.rand(groups, beams, generator=gen, device=DEVICE) < 0.3
+    lengths = torch.randint(0, 300, (groups, beams), generator=gen, device=DEVICE, dtype=torch.int32)
+    compare(z, scores, kept, finished, lengths, 0.7, symbols - 1)
+    compare(z, scores, kept, None, lengths, -0.3, 0)
+    first = torch.full_like(scores, -torch.inf)
+    first[:, 0] = 0.0
+    compare(z, first, kept, end=int(z[0].argmax()))
+
+
+@pytest.mark.parametrize("symbols", [257, 5003, 40_001])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_off_word_boundaries(require_gpu, symbols, dtype):
+    for pad in (1, 2, 3, 5):
+        z, scores, _ = make(pad, 2, 3, symbols, TYPES[dtype], pad)
+        compare(z, scores, 6)
+
+
+@pytest.mark.parametrize("symbols", [64, 257, 3000, 33_000])
+@pytest.mark.parametrize("beams, kept", [(1, 7), (4, 4), (5, 64)])
+def test_ties_go_to_the_lowest(require_gpu, symbols, beams, kept):
+    groups = 2
+    scores = torch.full((groups, beams), -3.0, device=DEVICE)
+    z = torch.zeros(groups * beams, symbols, device=DEVICE)
+    compare(z, scores, kept)                                        # everything ties
+    z = (torch.arange(symbols, device=DEVICE) % 5).float().repeat(groups * beams, 1)
+    compare(z, scores, kept)
+    compare(-z.flip(1), scores, kept)
+    z[:] = -torch.inf
+    z[:, -1] = 1.0
+    compare(z, scores, kept)                                        # one symbol a row
+    z[:, 0] = -0.0
+    z[:, symbols // 2] = 0.0
+    z[:, -1] = -torch.inf
+    compare(z, scores, kept)                                        # zeros of either sign are equal
+
+
+@pytest.mark.parametrize("symbols", [130, 2049, 20_000])
+@pytest.mark.parametrize("kept", [1, 4, 16, 64])
+def test_order_of_rows(require_gpu, symbols, kept):
+    """Rows in rising and falling order, and with their largest side by side in every place."""
+    rising = torch.linspace(-20, 20, symbols, device=DEVICE)
+    rows = [rising, rising.flip(0)]
+    for at in (0, 1, 63, 64, symbols // 2, symbols - 65, symbols - 64, symbols - 1):
+        row = torch.randn(symbols, device=DEVICE, generator=torch.Generator(DEVICE).manual_seed(at))
+        row[max(0, at):at + kept] = 30 + rising[:kept][:max(0, symbols - at)]
+        rows.append(row)
+    z = torch.stack(rows)
+    scores = torch.full((len(rows), 1), -1.0, device=DEVICE)
+    for dtype in (torch.float32, torch.bfloat16):
+        compare(z.to(dtype), scores, kept)
+    compare(z, scores.view(2, -1), kept)
+
+
+@pytest.mark.parametrize("symbols", [40, 300, 17_000])
+def test_special_values(require_gpu, symbols):
+    z, scores, _ = make(3, 10, 2, symbols, torch.float32)
+    z[0] = -torch.inf                       # a row without a way
+    z[2] = z[3] = -torch.inf                # a group without one
+    z[4, 5] = torch.nan
+    z[5] = torch.nan
+    z[6, [3, 7, 11]] = torch.inf            # share all probability
+    z[7, 9] = torch.inf
+    z[8] = torch.finfo(torch.float32).min   # the type's lowest value
+    z[9] = torch.finfo(torch.float32).min
+    z[9, 4] = torch.finfo(torch.float32).max
+    scores[5] = -torch.inf
+    scores[6, 0] = torch.nan
+    scores[7] = -1e30
+    scores[8] = 0.0
+    z[18, 1:] = -torch.inf                  # a probability of 1
+    for kept in (1, 2, 5, 64):
+        compare(z, scores, kept)
+        finished = torch.zeros(10, 2, dtype=torch.bool, device=DEVICE)
+        finished[1] = True                  # their logits hold nothing, and are not read
+        finished[5] = True
+        finished[7, 1] = True
+        compare(z, scores, kept, finished, torch.full((10, 2), 7, device=DEVICE, dtype=torch.int32), 1.0, 2)
+
+
+def test_lengths(require_gpu):
+    z, scores, _ = make(4, 3, 4, 100, torch.float32)
+    lengths = torch.tensor([[0, 1, 2, 3], [-5, 2**31 - 2, 0, 10], [2**31 - 2, 1, 1, 1]], device=DEVICE, dtype=torch.int32)
+    finished = torch.tensor([[False, True, False, True], [True, False, True, False], [False] * 4], device=DEVICE)
+    for penalty in (0.0, 1.0, 2.5, -1.0, 30.0):
+        compare(z, scores, 6, finished, lengths, penalty, 7)
+    compare(z, scores, 6, torch.ones_like(finished), lengths, 0.5)
+
+
+def test_results_are_the_same_each_time(require_gpu):
+    z, scores, _ = make(6, 2, 8, 90_001, torch.bfloat16)
+    first = decode.beam_select(z, scores, 16)
+    for _ in range(5):
+        again = decode.beam_select(z, scores, 16)
+        assert all(torch.equal(a, b) for a, b in zip(first[:3], again[:3]))
+
+
+def test_streams_and_graphs(require_gpu):
+    cases = [make(7, 2, 4, 257, torch.float32)[:2], make(8, 1, 8, 50_001, torch.bfloat16)[:2]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, held = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    with torch.cuda.stream(side):
+        for graph in graphs:
+            with torch.cuda.graph(graph, stream=side):
+                held.append([decode.beam_select(z, s, 8, end=1) for z, s in cases])
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for z, s in cases:
+            z.normal_()
+            s.uniform_(-9, -7)
+        eager = [decode.beam_select(z, s, 8, end=1) for z, s in cases]
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for got in held:
+            for a, b, (z, s) in zip(got, eager, cases):
+                assert all(torch.equal(x, y) for x, y in zip(a[:4], b[:4]))
+        compare(*cases[0], 8, end=1)
+
+
+def test_refusals(require_gpu):
+    z, scores, _ = make(9, 2, 3, 50, torch.float32)
+    flags, lengths = torch.zeros(2, 3, dtype=torch.bool, device=DEVICE), torch.ones(2, 3, dtype=torch.int32, device=DEVICE)
+    for call in (
+        lambda: decode.beam_select(z[:5], scores),
+        lambda: decode.beam_select(z.t(), scores),
+        lambda: decode.beam_select(z.cpu(), scores),
+        lambda: decode.beam_select(z.double(), scores),
+        lambda: decode.beam_select(z[:, :0], scores),
+        lambda: decode.beam_select(z, scores.cpu()),
+        lambda: decode.beam_select(z, scores.half()),
+        lambda: decode.beam_select(z, scores.view(6)),
+        lambda: decode.beam_select(z, scores.t()),
+        lambda: decode.beam_select(z, scores, 0),
+        lambda: decode.beam_select(z, scores, 65),
+        lambda: decode.beam_select(z, scores, -1),
+        lambda: decode.beam_select(torch.zeros(65, 50, device=DEVICE), torch.zeros(1, 65, device=DEVICE)),
+        lambda: decode.beam_select(z, scores, finished=lengths),
+        lambda: decode.beam_select(z, scores, finished=flags[:1]),
+        lambda: decode.beam_select(z, scores, lengths=lengths.long()),
+        lambda: decode.beam_select(z, scores, lengths=lengths[:, :2]),
+        lambda: decode.beam_select(z, scores, length_penalty=1.0),
+        lambda: decode.beam_select(z, scores, lengths=lengths, length_penalty=float("nan")),
+        lambda: decode.beam_select(z, scores, end=50),
+        lambda: decode.beam_select(z, scores, end=-1),
+        lambda: decode.beam_select(None, scores),
+        lambda: decode.beam_select(z, None),
+    ):
+        with pytest.raises(native.LeoError) as err:
+            call()
+        assert err.value.code == native.ERR_INVALID_ARGUMENT and str(err.value)
+    empty = decode.beam_select(z[:0], scores[:0], 4)
+    assert empty.symbols.shape == (0, 4)
