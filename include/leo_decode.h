@@ -162,7 +162,7 @@ int32_t leo_sample_workspace_bytes(uint64_t rows, uint64_t symbols, uint64_t* by
 int32_t leo_sample(const LeoSample* sample, void* stream);
 
 /* An 8-bit weight matrix [outputs, inputs]: w[n, k] = scale[n] * code[n, k] with
- * codes -128..127. */
+ * codes -128..127 and at most 2^27 inputs. */
 typedef struct LeoQ8Shape {
     uint64_t outputs;
     uint64_t inputs;
@@ -187,8 +187,8 @@ typedef struct LeoQ8Source {
 int32_t leo_q8_layout(const LeoQ8Source* source, void* stream);
 
 /* y[m, n] = bias[n] + s[m] * scale[n] * sum over k of q[m, k] * code[n, k], where
- * s[m] is the larger of 2^-126 and the largest magnitude of row m of x over 127,
- * rounded to float, and q[m, k] the whole number nearest to x[m, k] / s[m], of two
+ * s[m] is the larger of 2^-126 and the largest magnitude of row m of x times the
+ * float nearest to 1 / 127, rounded to float, and q[m, k] the whole number nearest to x[m, k] / s[m], of two
  * the even one. Sums of codes are exact, the rest is held in 64 bits, and one
  * rounding takes it to y_type. A row of x with an infinity or NaN gives NaN. bias
  * (float) may be NULL. y and x share no memory. `workspace`: at least

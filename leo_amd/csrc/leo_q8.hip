@@ -1,7 +1,7 @@
 // Products with 8-bit weights and 8-bit activations, and the layout they read.
 //
 //     y[m, n] = bias[n] + s[m] c[n] sum_k q[m, k] w[n, k]
-//     s[m] = max(max_k |x[m, k]| / 127, 2^-126),  q[m, k] = round(x[m, k] / s[m])
+//     s[m] = max(max_k |x[m, k]| * float(1 / 127), 2^-126),  q[m, k] = round(x[m, k] / s[m])
 //
 // Layout. Rows (outputs of the weights, rows of x) go in tiles of 16, inputs in
 // blocks of 64; the codes of one tile and block are 1,024 bytes, 16 for each lane
@@ -30,7 +30,7 @@ struct Q8Layout {
 
 void check_shape(const LeoQ8Shape& s) {
     require(s.outputs >= 1 && s.outputs <= (1ull << 31), "q8: outputs must be 1 .. 2^31");
-    require(s.inputs >= 1 && s.inputs <= (1ull << 31), "q8: inputs must be 1 .. 2^31");
+    require(s.inputs >= 1 && s.inputs <= (1ull << 27), "q8: inputs must be 1 .. 2^27");
 }
 
 uint64_t up(uint64_t v) { return (v + 255) / 256 * 256; }
@@ -82,115 +82,374 @@ struct ProductArgs {
     int32_t y_type;
     uint32_t rows, inputs, outputs, tiles, blocks, row_tiles;
     uint32_t slices, slice_blocks;
-    char* x_codes;    // x as a layout
-    float* x_scales;  // 16 a tile
-    int32_t* partials;  // [slice][row][16 tiles]
+    uint32_t parts, part_inputs;  // of a row, whose largest magnitudes were taken before; 0: none were
+    const uint32_t* largest;      // [row][part], bits of magnitudes
+    char* x_codes;                // x as a layout; what is beyond its rows and inputs holds anything: those
+                                  // rows' sums are not used, and the weights of those inputs are 0
+    float* x_scales;              // one a row
+    int32_t* partials;            // [slice][row][16 tiles]
 };
 
-// The whole number nearest to the exact quotient x / s, of two the even one: the
-// product with the rounded inverse is off by less than one half, and the remainder
-// x - n s, which needs no rounding where it is near s / 2, tells where it matters.
-__device__ __forceinline__ int32_t code_of(float x, float s, float inverse) {
-    const float n = __builtin_rintf(x * inverse), rest = __builtin_fmaf(-n, s, x), half = 0.5f * s;
-    const int32_t code = static_cast<int32_t>(n);
-    if (rest > half || (rest == half && (code & 1))) return code + 1;
-    if (rest < -half || (rest == -half && (code & 1))) return code - 1;
-    return code;
+__device__ __forceinline__ uint32_t wave_of_workgroup() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64); }
+__device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
+    return wave_reduce(v, 0u, [](uint32_t p, uint32_t q) { return p > q ? p : q; });
+}
+
+// 16 neighbouring inputs of a row from k on; 0 beyond its end.
+struct Sixteen {
+    float f[16];
+};
+template <class X>
+__device__ __forceinline__ Sixteen load_sixteen(const ProductArgs& a, uint32_t row, uint32_t k) {
+    constexpr uint32_t kWide = 16 / sizeof(typename X::type);
+    const auto* p = static_cast<const typename X::type*>(a.x) + static_cast<int64_t>(row) * a.x_stride + k;
+    Sixteen s;
+    if (k + 16 <= a.inputs) {
+        uint4v raw[16 / kWide];
+#pragma unroll
+        for (uint32_t v = 0; v < 16 / kWide; ++v) raw[v] = load_16(p + v * kWide);
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) s.f[i] = X::at(raw[i / kWide], i % kWide);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) s.f[i] = k + i < a.inputs ? X::load(p, i) : 0.0f;
+    }
+    return s;
+}
+__device__ __forceinline__ uint32_t largest_of(const Sixteen& s) {
+    uint32_t most = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) most = max(most, __float_as_uint(s.f[i]) & 0x7fffffffu);
+    return most;
 }
 
 // The scale of a row from the largest magnitude of its values, as bits; NaN where that is no finite number.
 __device__ __forceinline__ float scale_of(uint32_t largest) {
-    return largest < 0x7f800000u ? fmaxf(__uint_as_float(largest) / 127.0f, 0x1p-126f) : __builtin_nanf("");
+    return largest < 0x7f800000u ? fmaxf(__uint_as_float(largest) * (1.0f / 127.0f), 0x1p-126f) : __builtin_nanf("");
 }
 
-// One workgroup a row of a tile.
-template <class T>
-__global__ __launch_bounds__(256) void leo_q8_quantize(ProductArgs a) {
-    __shared__ uint32_t most[4];
-    const uint32_t row = blockIdx.x, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const bool inside = row < a.rows;
-    const auto* x = static_cast<const typename T::type*>(a.x) + static_cast<int64_t>(row) * a.x_stride;
-    uint32_t largest = 0;
-    if (inside)
-        for (uint32_t k = threadIdx.x; k < a.inputs; k += 256)
-            largest = max(largest, __float_as_uint(T::load(x, k)) & 0x7fffffffu);
-    largest = wave_reduce(largest, 0u, [](uint32_t p, uint32_t q) { return p > q ? p : q; });
-    if (lane == 0) most[wave] = largest;
-    __syncthreads();
-    const float scale = scale_of(max(max(most[0], most[1]), max(most[2], most[3]))), inverse = 1.0f / scale;
-    if (threadIdx.x == 0) a.x_scales[row] = inside ? scale : 0.0f;
-    const bool counts = inside && scale == scale;
-    for (uint32_t part = threadIdx.x; part < a.blocks * 4; part += 256) {
-        union {
-            uint4v words;
-            int8_t codes[16];
-        } u;
-        for (uint32_t i = 0; i < 16; ++i) {
-            const uint32_t k = part * 16 + i;
-            u.codes[i] = counts && k < a.inputs ? static_cast<int8_t>(code_of(T::load(x, k), scale, inverse)) : int8_t{0};
+// The whole numbers nearest to the exact quotients x / s, of two the even one: the
+// product with the rounded inverse is off by less than one half, and the remainder
+// x - n s, which needs no rounding where it is near s / 2, tells where it matters.
+__device__ __forceinline__ uint4v codes_of(const Sixteen& s, float scale) {
+    const float inverse = 1.0f / scale, half = 0.5f * scale;
+    uint4v words;
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) {
+        uint32_t word = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const float x = s.f[4 * w + i], n = __builtin_rintf(x * inverse), rest = __builtin_fmaf(-n, scale, x);
+            int32_t code = static_cast<int32_t>(n);
+            const int32_t odd = code & 1;
+            if (rest > half || (rest == half && odd)) code += 1;
+            if (rest < -half || (rest == -half && odd)) code -= 1;
+            word |= (static_cast<uint32_t>(code) & 0xffu) << (8 * i);
         }
-        char* to = a.x_codes + (static_cast<uint64_t>(row / kTile) * a.blocks + part / 4) * kBlockBytes;
-        reinterpret_cast<uint4v*>(to)[part % 4 * kTile + row % kTile] = u.words;
+        words[w] = word;
     }
+    return scale == scale ? words : uint4v{0, 0, 0, 0};
 }
 
-__device__ __forceinline__ void store_y(const ProductArgs& a, uint32_t row, uint32_t n, int64_t sum) {
-    const double v = static_cast<double>(sum) * a.x_scales[row] * a.scales[n] + (a.bias ? a.bias[n] : 0.0f);
+__device__ __forceinline__ void store_y(const ProductArgs& a, uint32_t row, uint32_t n, int64_t sum, float scale) {
+    const double v = static_cast<double>(sum) * scale * a.scales[n] + (a.bias ? a.bias[n] : 0.0f);
     const int64_t at = static_cast<int64_t>(row) * a.y_stride + n;
     if (a.y_type == LEO_TYPE_F32) static_cast<float*>(a.y)[at] = static_cast<float>(v);
     else if (a.y_type == LEO_TYPE_F16) static_cast<_Float16*>(a.y)[at] = static_cast<_Float16>(v);
     else static_cast<__bf16*>(a.y)[at] = static_cast<__bf16>(v);
 }
 
-// One wave 16 rows, 16 outputs and a slice of the inputs. x is the A operand, so lane
-// l gets output l % 16 of rows 4 (l / 16) + 0..3.
-__global__ __launch_bounds__(64) void leo_q8_multiply(ProductArgs a) {
-    const uint32_t tile = blockIdx.x, row_tile = blockIdx.y, slice = blockIdx.z, lane = threadIdx.x;
-    const uint32_t begin = slice * a.slice_blocks, end = min(begin + a.slice_blocks, a.blocks);
-    const char* w = a.codes + static_cast<uint64_t>(tile) * a.blocks * kBlockBytes;
-    const char* x = a.x_codes + static_cast<uint64_t>(row_tile) * a.blocks * kBlockBytes;
-    int4v sum = {0, 0, 0, 0};
-    for (uint32_t block = begin; block < end; ++block) {
-        const int4v p = reinterpret_cast<const int4v*>(x + static_cast<uint64_t>(block) * kBlockBytes)[lane];
-        const int4v q = reinterpret_cast<const int4v*>(w + static_cast<uint64_t>(block) * kBlockBytes)[lane];
-        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(p, q, sum, 0, 0, 0);
+// The largest magnitude of each part of a row.
+template <class X>
+__global__ __launch_bounds__(256) void leo_q8_largest(ProductArgs a, uint32_t* to) {
+    __shared__ uint32_t most[4];
+    const uint32_t row = blockIdx.x, begin = blockIdx.y * a.part_inputs, end = min(begin + a.part_inputs, a.inputs);
+    uint32_t largest = 0;
+    for (uint32_t k = begin + threadIdx.x * 16; k < end; k += 256 * 16) largest = max(largest, largest_of(load_sixteen<X>(a, row, k)));
+    largest = wave_largest(largest);
+    if (threadIdx.x % 64 == 0) most[threadIdx.x / 64] = largest;
+    __syncthreads();
+    if (threadIdx.x == 0) to[row * a.parts + blockIdx.y] = max(max(most[0], most[1]), max(most[2], most[3]));
+}
+
+constexpr uint32_t kMostParts = 64;
+__device__ __forceinline__ float scale_of_parts(const ProductArgs& a, uint32_t row) {  // by a whole wave
+    const uint32_t lane = threadIdx.x % 64;
+    return scale_of(wave_largest(lane < a.parts ? a.largest[row * a.parts + lane] : 0u));
+}
+
+__device__ __forceinline__ uint4v* place_of(const ProductArgs& a, uint32_t row, uint32_t sixteen) {
+    char* to = a.x_codes + (static_cast<uint64_t>(row / kTile) * a.blocks + sixteen / 4) * kBlockBytes;
+    return reinterpret_cast<uint4v*>(to) + (sixteen % 4 * kTile + row % kTile);
+}
+
+// x in 8 bits in the weights' layout, for the products of many rows: one workgroup a
+// row of up to 16,384 inputs, which its threads hold in registers, or a part of a longer one.
+constexpr uint32_t kHeldInputs = 16384;
+template <class X>
+__global__ __launch_bounds__(1024) void leo_q8_quantize_row(ProductArgs a) {
+    __shared__ uint32_t most[16];
+    const uint32_t row = blockIdx.x, lane = threadIdx.x % 64, k = threadIdx.x * 16;
+    const Sixteen s = load_sixteen<X>(a, row, k);
+    const uint32_t largest = wave_largest(largest_of(s));
+    if (lane == 0) most[threadIdx.x / 64] = largest;
+    __syncthreads();
+    const float scale = scale_of(wave_largest(lane < blockDim.x / 64 ? most[lane] : 0u));
+    if (threadIdx.x == 0) a.x_scales[row] = scale;
+    if (k < a.inputs) *place_of(a, row, threadIdx.x) = codes_of(s, scale);
+}
+template <class X>
+__global__ __launch_bounds__(256) void leo_q8_quantize_part(ProductArgs a) {
+    const uint32_t row = blockIdx.x, begin = blockIdx.y * a.part_inputs, end = min(begin + a.part_inputs, a.inputs);
+    const float scale = scale_of_parts(a, row);
+    if (begin == 0 && threadIdx.x == 0) a.x_scales[row] = scale;
+    for (uint32_t k = begin + threadIdx.x * 16; k < end; k += 256 * 16) *place_of(a, row, k / 16) = codes_of(load_sixteen<X>(a, row, k), scale);
+}
+
+// Up to 16 rows. A workgroup takes kTiles output tiles and a slice of the inputs,
+// and brings the slice of x to LDS in 8 bits itself; its eight waves share the
+// slice's blocks, each block's weights a run of 1,024 bytes a tile. x is the A
+// operand, so lane l gets output l % 16 of rows 4 (l / 16) + 0..3; rows beyond the
+// last read it again and are not stored. Whole sums go to LDS by whole-number
+// additions, whose order does not matter.
+constexpr uint32_t kFewThreads = 512, kFewWaves = kFewThreads / 64;
+constexpr uint32_t kFewStage = 48 << 10;  // bytes of x in LDS
+
+template <class X, int kTiles>
+__global__ __launch_bounds__(kFewThreads, 4) void leo_q8_few(ProductArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint4v staged[];
+    __shared__ int32_t sums[kTiles * 256];
+    __shared__ uint32_t most[16][kFewWaves];
+    __shared__ float scales[16];
+    constexpr uint32_t kAhead = kTiles >= 5 ? 1 : kTiles >= 3 ? 2 : kTiles == 2 ? 4 : 8;
+    const uint32_t lane = threadIdx.x % 64, wave = wave_of_workgroup();
+    const uint32_t first = blockIdx.y * a.slice_blocks, count = min(a.slice_blocks, a.blocks - first);
+    const uint32_t each = (count + kFewWaves - 1) / kFewWaves;
+    const uint32_t begin = min(first + wave * each, first + count), end = min(begin + each, first + count);
+    const char* weights[kTiles];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+        weights[t] = a.codes + static_cast<uint64_t>(min(blockIdx.x * kTiles + t, a.tiles - 1)) * a.blocks * kBlockBytes;
+    const auto fetch = [&](int4v (&to)[kAhead][kTiles], uint32_t block) {
+        if (block >= end) return;
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+                to[u][t] = reinterpret_cast<const int4v*>(weights[t] + static_cast<uint64_t>(min(block + u, end - 1)) * kBlockBytes)[lane];
+    };
+    int4v even[kAhead][kTiles], odd[kAhead][kTiles];
+    fetch(even, begin);  // on their way while x is prepared
+    for (uint32_t i = threadIdx.x; i < kTiles * 256; i += kFewThreads) sums[i] = 0;
+
+    if (a.parts) {
+        for (uint32_t row = wave; row < a.rows; row += kFewWaves) {
+            const float scale = scale_of_parts(a, row);
+            if (lane == 0) scales[row] = scale;
+        }
+    } else {
+        for (uint32_t row = 0; row < a.rows; ++row) {
+            uint32_t largest = 0;
+            for (uint32_t k = threadIdx.x * 16; k < a.inputs; k += kFewThreads * 16)
+                largest = max(largest, largest_of(load_sixteen<X>(a, row, k)));
+            largest = wave_largest(largest);
+            if (lane == 0) most[row][wave] = largest;
+        }
+        __syncthreads();
+        for (uint32_t row = wave; row < a.rows; row += kFewWaves) {
+            const float scale = scale_of(wave_largest(lane < kFewWaves ? most[row][lane] : 0u));
+            if (lane == 0) scales[row] = scale;
+        }
     }
-    const uint32_t n = tile * kTile + lane % kTile;
-    for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t row = row_tile * kTile + lane / kTile * 4 + i;
-        if (row >= a.rows) break;
-        if (a.slices == 1) {
-            if (n < a.outputs) store_y(a, row, n, sum[i]);
-        } else {
-            a.partials[(static_cast<uint64_t>(slice) * a.rows + row) * a.tiles * kTile + n] = sum[i];
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < a.rows * count * 4; i += kFewThreads) {
+        const uint32_t row = i / (count * 4), sixteen = i % (count * 4);
+        staged[sixteen * a.rows + row] = codes_of(load_sixteen<X>(a, row, (first * 4 + sixteen) * 16), scales[row]);
+    }
+    if (a.slices > 1 && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < a.rows) a.x_scales[threadIdx.x] = scales[threadIdx.x];
+    __syncthreads();
+
+    int4v sum[kTiles];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) sum[t] = int4v{0, 0, 0, 0};
+    const uint32_t mine = lane / kTile * a.rows + min(lane % kTile, a.rows - 1);
+    const auto multiply = [&](const int4v (&w)[kAhead][kTiles], uint32_t block) {
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u) {
+            if (block + u >= end) break;
+            const int4v x = __builtin_bit_cast(int4v, staged[(block + u - first) * 4 * a.rows + mine]);
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, w[u][t], sum[t], 0, 0, 0);
+        }
+    };
+    for (uint32_t block = begin; block < end; block += 2 * kAhead) {
+        fetch(odd, block + kAhead);
+        multiply(even, block);
+        fetch(even, block + 2 * kAhead);
+        multiply(odd, block + kAhead);
+    }
+    if (begin < end) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t row = lane / kTile * 4 + i;
+            if (row >= a.rows) break;
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) atomicAdd(&sums[row * (kTiles * kTile) + t * kTile + lane % kTile], sum[t][i]);
+        }
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < a.rows * (kTiles * kTile); i += kFewThreads) {
+        const uint32_t row = i / (kTiles * kTile), n = blockIdx.x * (kTiles * kTile) + i % (kTiles * kTile);
+        if (a.slices > 1) {
+            if (n < a.tiles * kTile) a.partials[(static_cast<uint64_t>(blockIdx.y) * a.rows + row) * a.tiles * kTile + n] = sums[i];
+        } else if (n < a.outputs) {
+            store_y(a, row, n, sums[i], scales[row]);
         }
     }
 }
 
+// More rows: 16 kRows rows and 16 kTiles outputs a workgroup, x and the weights
+// straight from their layouts to registers, the blocks of a slice shared by eight waves.
+constexpr int kManyRows = 4, kManyTiles = 2;
+__global__ __launch_bounds__(kFewThreads) void leo_q8_many(ProductArgs a) {
+    __shared__ int32_t sums[kManyRows * kManyTiles * 256];
+    constexpr uint32_t kOperands = kManyRows + kManyTiles, kWide = kManyTiles * kTile;
+    const uint32_t lane = threadIdx.x % 64, wave = wave_of_workgroup();
+    const uint32_t first = blockIdx.z * a.slice_blocks, count = min(a.slice_blocks, a.blocks - first);
+    const uint32_t each = (count + kFewWaves - 1) / kFewWaves;
+    const uint32_t begin = min(first + wave * each, first + count), end = min(begin + each, first + count);
+    const char* from[kOperands];
+#pragma unroll
+    for (uint32_t r = 0; r < kManyRows; ++r)
+        from[r] = a.x_codes + static_cast<uint64_t>(min(blockIdx.y * kManyRows + r, a.row_tiles - 1)) * a.blocks * kBlockBytes;
+#pragma unroll
+    for (uint32_t t = 0; t < kManyTiles; ++t)
+        from[kManyRows + t] = a.codes + static_cast<uint64_t>(min(blockIdx.x * kManyTiles + t, a.tiles - 1)) * a.blocks * kBlockBytes;
+    const auto fetch = [&](int4v (&to)[kOperands], uint32_t block) {
+        if (block >= end) return;
+#pragma unroll
+        for (uint32_t o = 0; o < kOperands; ++o) to[o] = reinterpret_cast<const int4v*>(from[o] + static_cast<uint64_t>(block) * kBlockBytes)[lane];
+    };
+    int4v sum[kManyRows][kManyTiles];
+#pragma unroll
+    for (int r = 0; r < kManyRows; ++r)
+#pragma unroll
+        for (int t = 0; t < kManyTiles; ++t) sum[r][t] = int4v{0, 0, 0, 0};
+    const auto multiply = [&](const int4v (&v)[kOperands], uint32_t block) {
+        if (block >= end) return;
+#pragma unroll
+        for (int r = 0; r < kManyRows; ++r)
+#pragma unroll
+            for (int t = 0; t < kManyTiles; ++t) sum[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[r], v[kManyRows + t], sum[r][t], 0, 0, 0);
+    };
+    int4v one[kOperands], two[kOperands];
+    fetch(one, begin);
+    for (uint32_t i = threadIdx.x; i < kManyRows * kManyTiles * 256; i += kFewThreads) sums[i] = 0;
+    __syncthreads();
+    for (uint32_t block = begin; block < end; block += 2) {
+        fetch(two, block + 1);
+        multiply(one, block);
+        fetch(one, block + 2);
+        multiply(two, block + 1);
+    }
+    if (begin < end) {
+#pragma unroll
+        for (int r = 0; r < kManyRows; ++r)
+#pragma unroll
+            for (int t = 0; t < kManyTiles; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    atomicAdd(&sums[(r * kTile + lane / kTile * 4 + i) * kWide + t * kTile + lane % kTile], sum[r][t][i]);
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < kManyRows * kManyTiles * 256; i += kFewThreads) {
+        const uint32_t row = blockIdx.y * (kManyRows * kTile) + i / kWide, n = blockIdx.x * kWide + i % kWide;
+        if (row >= a.rows) break;
+        if (a.slices > 1) {
+            if (n < a.tiles * kTile) a.partials[(static_cast<uint64_t>(blockIdx.z) * a.rows + row) * a.tiles * kTile + n] = sums[i];
+        } else if (n < a.outputs) {
+            store_y(a, row, n, sums[i], a.x_scales[row]);
+        }
+    }
+}
+
+// The slices of one output by kShare threads.
+template <uint32_t kShare>
 __global__ __launch_bounds__(256) void leo_q8_join(ProductArgs a) {
-    const uint32_t n = blockIdx.x * 256 + threadIdx.x, row = blockIdx.y;
-    if (n >= a.outputs) return;
+    constexpr uint32_t kOutputs = 256 / kShare;
+    __shared__ int64_t parts[kShare][kOutputs];
+    const uint32_t wide = (a.outputs + kOutputs - 1) / kOutputs, row = blockIdx.x / wide;
+    const uint32_t n = blockIdx.x % wide * kOutputs + threadIdx.x % kOutputs, share = threadIdx.x / kOutputs;
     int64_t sum = 0;
-    for (uint32_t s = 0; s < a.slices; ++s) sum += a.partials[(static_cast<uint64_t>(s) * a.rows + row) * a.tiles * kTile + n];
-    store_y(a, row, n, sum);
+    if (n < a.outputs) {
+#pragma unroll 8
+        for (uint32_t s = share; s < a.slices; s += kShare) sum += a.partials[(static_cast<uint64_t>(s) * a.rows + row) * a.tiles * kTile + n];
+    }
+    if constexpr (kShare > 1) {
+        parts[share][threadIdx.x % kOutputs] = sum;
+        __syncthreads();
+        if (share) return;
+#pragma unroll
+        for (uint32_t s = 1; s < kShare; ++s) sum += parts[s][threadIdx.x];
+    }
+    if (n < a.outputs) store_y(a, row, n, sum, a.x_scales[row]);
 }
 
 struct Plan {
+    bool few;
+    uint32_t group_tiles;  // of a workgroup of leo_q8_few
     uint32_t slices, slice_blocks;
-    uint64_t x_scales, partials, workspace;  // offsets behind x's codes, and the whole
+    uint32_t parts, part_inputs;
+    uint64_t x_scales, largest, partials, workspace;  // offsets behind x's codes, and the whole
 };
 Plan plan_of(const LeoQ8Shape& s, uint64_t rows) {
     const Q8Layout l = layout_of(s);
     const uint64_t row_tiles = (rows + kTile - 1) / kTile;
     Plan p{};
-    const uint64_t want = std::max<uint64_t>(1, 1024 / (l.tiles * row_tiles));
-    const uint64_t slices = std::max((l.blocks + kMostSliceBlocks - 1) / kMostSliceBlocks, std::min(want, (l.blocks + 15) / 16));
+    p.few = rows <= kTile;
+    uint64_t slices, groups;
+    if (p.few) {
+        // All tiles in groups that differ little, or where there are enough of them smaller groups and whole rows.
+        const bool whole = l.tiles >= 128;
+        p.group_tiles = static_cast<uint32_t>(whole ? std::min<uint64_t>(8, (l.tiles + 511) / 512) : (l.tiles + (l.tiles + 7) / 8 - 1) / ((l.tiles + 7) / 8));
+        groups = (l.tiles + p.group_tiles - 1) / p.group_tiles;
+        slices = whole ? 1 : std::max<uint64_t>(1, std::min<uint64_t>(512 / groups, (l.blocks + 7) / 8));
+        slices = std::max(slices, (l.blocks * rows * kBlock + kFewStage - 1) / kFewStage);
+    } else {
+        groups = (l.tiles + kManyTiles - 1) / kManyTiles * ((row_tiles + kManyRows - 1) / kManyRows);
+        slices = std::max<uint64_t>(1, std::min<uint64_t>(512 / groups, (l.blocks + 15) / 16));
+    }
+    slices = std::max(slices, (l.blocks + kMostSliceBlocks - 1) / kMostSliceBlocks);
     p.slice_blocks = static_cast<uint32_t>((l.blocks + slices - 1) / slices);
     p.slices = static_cast<uint32_t>((l.blocks + p.slice_blocks - 1) / p.slice_blocks);
-    p.x_scales = row_tiles * l.blocks * kBlockBytes;
-    p.partials = p.x_scales + up(row_tiles * kTile * sizeof(float));
+    if (p.few ? rows * s.inputs > 16384 : s.inputs > kHeldInputs) {
+        const uint64_t want = std::max<uint64_t>(4096, (s.inputs + kMostParts - 1) / kMostParts);
+        p.part_inputs = static_cast<uint32_t>((want + 15) / 16 * 16);
+        p.parts = static_cast<uint32_t>((s.inputs + p.part_inputs - 1) / p.part_inputs);
+    }
+    p.x_scales = p.few ? 0 : row_tiles * l.blocks * kBlockBytes;
+    p.largest = p.x_scales + (p.few && p.slices == 1 ? 0 : up(rows * sizeof(float)));
+    p.partials = p.largest + up(rows * p.parts * sizeof(uint32_t));
     p.workspace = p.partials + (p.slices > 1 ? up(p.slices * rows * l.tiles * kTile * sizeof(int32_t)) : 0);
     return p;
+}
+
+template <class X>
+void launch_few(const Plan& p, const ProductArgs& a, hipStream_t stream) {
+    const dim3 grid((a.tiles + p.group_tiles - 1) / p.group_tiles, a.slices);
+    const uint32_t lds = a.rows * a.slice_blocks * kBlock;
+    static constexpr void (*kKernels[])(ProductArgs) = {leo_q8_few<X, 1>, leo_q8_few<X, 2>, leo_q8_few<X, 3>, leo_q8_few<X, 4>,
+                                                        leo_q8_few<X, 5>, leo_q8_few<X, 6>, leo_q8_few<X, 7>, leo_q8_few<X, 8>};
+    launch(kKernels[p.group_tiles - 1], grid, dim3(kFewThreads), lds, stream, a);
+}
+
+template <class X>
+void launch_product(const Plan& p, const ProductArgs& a, uint32_t* largest, hipStream_t stream) {
+    if (a.parts) launch(leo_q8_largest<X>, dim3(a.rows, a.parts), dim3(256), 0, stream, a, largest);
+    if (p.few) return launch_few<X>(p, a, stream);
+    if (a.parts) launch(leo_q8_quantize_part<X>, dim3(a.rows, a.parts), dim3(256), 0, stream, a);
+    else launch(leo_q8_quantize_row<X>, dim3(a.rows), dim3((a.inputs + 1023) / 1024 * 64), 0, stream, a);
+    launch(leo_q8_many, dim3((a.tiles + kManyTiles - 1) / kManyTiles, (a.row_tiles + kManyRows - 1) / kManyRows, a.slices), dim3(kFewThreads), 0, stream, a);
 }
 
 }  // namespace
@@ -254,6 +513,7 @@ int32_t leo_q8_matmul(const LeoQ8Product* product, void* stream) {
         require(reinterpret_cast<uintptr_t>(p.layout) % 256 == 0, "leo_q8_matmul: layout must be 256-byte aligned");
         const Q8Layout l = layout_of(p.shape);
         require(p.layout_bytes >= l.bytes, "leo_q8_matmul: layout is too small for its shape");
+        require((p.shape.outputs + 31) / 32 * p.rows <= 0x7fffffffu, "leo_q8_matmul: the result is too large");
         const Plan plan = plan_of(p.shape, p.rows);
         require(plan.workspace == 0 || (p.workspace && reinterpret_cast<uintptr_t>(p.workspace) % 256 == 0 &&
                                         p.workspace_bytes >= plan.workspace),
@@ -275,14 +535,21 @@ int32_t leo_q8_matmul(const LeoQ8Product* product, void* stream) {
         a.row_tiles = (a.rows + kTile - 1) / kTile;
         a.slices = plan.slices;
         a.slice_blocks = plan.slice_blocks;
+        a.parts = plan.parts;
+        a.part_inputs = plan.part_inputs;
         a.x_codes = static_cast<char*>(p.workspace);
         a.x_scales = reinterpret_cast<float*>(a.x_codes + plan.x_scales);
+        auto* largest = reinterpret_cast<uint32_t*>(a.x_codes + plan.largest);
+        a.largest = largest;
         a.partials = reinterpret_cast<int32_t*>(a.x_codes + plan.partials);
         const auto at = static_cast<hipStream_t>(stream);
-        launch(p.x_type == LEO_TYPE_F32 ? leo_q8_quantize<F32> : p.x_type == LEO_TYPE_F16 ? leo_q8_quantize<F16> : leo_q8_quantize<BF16>,
-               dim3(a.row_tiles * kTile), dim3(256), 0, at, a);
-        launch(leo_q8_multiply, dim3(a.tiles, a.row_tiles, a.slices), dim3(64), 0, at, a);
-        if (a.slices > 1) launch(leo_q8_join, dim3((a.outputs + 255) / 256, a.rows), dim3(256), 0, at, a);
+        if (p.x_type == LEO_TYPE_F32) launch_product<F32>(plan, a, largest, at);
+        else if (p.x_type == LEO_TYPE_F16) launch_product<F16>(plan, a, largest, at);
+        else launch_product<BF16>(plan, a, largest, at);
+        if (plan.slices == 1) return;
+        const bool share = plan.slices >= 16;
+        const uint64_t count = (p.shape.outputs + (share ? 31 : 255)) / (share ? 32 : 256) * p.rows;
+        launch(share ? leo_q8_join<8> : leo_q8_join<1>, dim3(static_cast<uint32_t>(count)), dim3(256), 0, at, a);
     });
 }
 

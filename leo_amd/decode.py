@@ -245,7 +245,7 @@ class Q8Weight:
 def q8_matmul(x: torch.Tensor, weight: Q8Weight, bias: Optional[torch.Tensor] = None, *,
               out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """bias + x W^T for x [rows, inputs] (or [inputs]) of float32, float16 or
-    bfloat16, with x in 8 bits: a row's scale is its largest magnitude over 127 in
+    bfloat16, with x in 8 bits: a row's scale is its largest magnitude times 1 / 127 in
     float32 (at least 2^-126), its codes the nearest whole numbers to x over that, of
     two the even one. Sums of codes are exact, the rest has 64 bits and is rounded once
     to `out_dtype` (x's type by default). A row with an infinity or NaN gives NaN.

@@ -20,7 +20,7 @@ TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -24, torch.bfloat16: 2
 def quantized(x):
     """Codes and scales of x (float64 of values that float32 holds), as the formula says."""
     largest = x.abs().amax(dim=1)
-    scale = (largest.float() / 127.0).clamp_min(2.0 ** -126)
+    scale = (largest.float() * float(np.float32(1) / np.float32(127))).clamp_min(2.0 ** -126)
     good = torch.isfinite(largest)
     scale = torch.where(good, scale, torch.full_like(scale, torch.nan))
     codes = torch.where(good[:, None], torch.round(x / scale.double()[:, None]), torch.zeros_like(x))
