@@ -212,9 +212,10 @@ typedef struct LeoQ8Product {
 int32_t leo_q8_workspace_bytes(const LeoQ8Shape* shape, uint64_t rows, int32_t x_type, uint64_t* bytes);
 int32_t leo_q8_matmul(const LeoQ8Product* product, void* stream);
 
-/* Beam search's selection, `groups` searches of `beams` hypotheses each. logits has
- * a row of `symbols` for each hypothesis, scores [groups, beams] the sums of log
- * probabilities so far, -inf where there is none (NaN counts as -inf). Candidates:
+/* Beam search's selection, `groups` searches of `beams` hypotheses each (65,535
+ * hypotheses at most). logits has a row of `symbols` (2^26 at most) for each
+ * hypothesis, scores [groups, beams] the sums of log probabilities so far, -inf where
+ * there is none (NaN counts as -inf). Candidates:
  *     symbol v after hypothesis b:  score + z[v] - log sum exp z  (those above -inf)
  *     a finished hypothesis itself:  its score; its logits are not read
  * and the `kept` (at most 64, as are the beams) with the largest score / length^length_penalty

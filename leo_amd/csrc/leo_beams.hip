@@ -27,144 +27,408 @@ __device__ __forceinline__ float from_order_key(uint32_t k) {
 __device__ __forceinline__ uint64_t candidate(float z, uint32_t at) {
     return static_cast<uint64_t>(order_key(z + 0.0f)) << 32 | (0xffffffffu - at);
 }
-__device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
-    for (int step = 32; step; step /= 2) {
-        const uint64_t other = __shfl_xor(static_cast<unsigned long long>(v), step);
-        v = other > v ? other : v;
-    }
+__device__ __forceinline__ float logit_of(uint64_t c) { return from_order_key(static_cast<uint32_t>(c >> 32)); }
+__device__ __forceinline__ uint32_t symbol_of(uint64_t c) { return 0xffffffffu - static_cast<uint32_t>(c); }
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int step = 32; step; step /= 2) v += __shfl_xor(v, step);
     return v;
 }
 
-// What a row leaves for its search: its log of the sum of exponentials above its
-// largest logit, and its `kept` best candidates in falling order.
-struct BeamRecord {
-    float top;
-    uint32_t pad0;
-    double log_sum;
-};
-
-__device__ __forceinline__ bool is_finished(const LeoBeams& a, uint64_t row) { return a.finished && a.finished[row]; }
-
-// One workgroup a row.
-template <class T>
-__global__ __launch_bounds__(256) void leo_beam_rows(LeoBeams a, BeamRecord* records, uint64_t* candidates) {
-    __shared__ float tops[4];
-    __shared__ double sums[4];
-    __shared__ uint64_t bests[4];
-    const uint64_t row = blockIdx.x;
-    const uint32_t n = static_cast<uint32_t>(a.symbols), lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    if (is_finished(a, row) || !(a.scores[row] > negative_infinity())) return;
-    const auto* logits = static_cast<const typename T::type*>(a.logits) + row * a.logits_stride;
-    float top = negative_infinity();
-    for (uint32_t v = threadIdx.x; v < n; v += 256) top = fmaxf(top, T::load(logits, v));
-    top = wave_max(top);
-    if (lane == 0) tops[wave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    double sum = 0.0;
-    for (uint32_t v = threadIdx.x; v < n; v += 256) {
-        const float z = T::load(logits, v);
-        sum += z == top ? 1.0 : z > negative_infinity() ? exp(static_cast<double>(z) - top) : 0.0;
-    }
-    for (int step = 32; step; step /= 2) sum += __shfl_xor(sum, step);
-    if (lane == 0) sums[wave] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) records[row] = {top, 0, log(sums[0] + sums[1] + sums[2] + sums[3])};
-    uint64_t below = ~0ull;
-    for (uint32_t k = 0; k < a.kept; ++k) {
-        uint64_t best = 0;
-        if (below)
-            for (uint32_t v = threadIdx.x; v < n; v += 256) {
-                const float z = T::load(logits, v);
-                const uint64_t c = z > negative_infinity() ? candidate(z, v) : 0;
-                if (c < below && c > best) best = c;
-            }
-        best = wave_max64(best);
-        __syncthreads();
-        if (lane == 0) bests[wave] = best;
-        __syncthreads();
-        for (uint32_t w = 0; w < 4; ++w) best = bests[w] > best ? bests[w] : best;
-        if (threadIdx.x == 0) candidates[row * a.kept + k] = best;
-        below = best;
-    }
+// The largest of v in each group of `lanes` neighbouring lanes (a power of two up to 16).
+__device__ __forceinline__ uint32_t group_max(uint32_t v, uint32_t lanes) {
+    const auto step = [&](auto ctrl) {
+        v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), decltype(ctrl)::value, 0xf, 0xf, true)));
+    };
+    if (lanes >= 2) step(std::integral_constant<int, 0xb1>{});    // the neighbour in a pair
+    if (lanes >= 4) step(std::integral_constant<int, 0x4e>{});    // the other pair of four
+    if (lanes >= 8) step(std::integral_constant<int, 0x141>{});   // mirrored in eight
+    if (lanes >= 16) step(std::integral_constant<int, 0x140>{});  // mirrored in sixteen
+    return v;
 }
 
-struct Ranked {
-    double rank;
-    uint32_t at;  // hypothesis * kept + place in its row's order
-};
-__device__ __forceinline__ bool before(const Ranked& p, const Ranked& q) { return p.rank > q.rank || (p.rank == q.rank && p.at < q.at); }
+// A value that is not above the kept-th largest of a wave's 64, and equals it in its
+// upper 20 bits; 0 where fewer than `kept` are above 0.
+__device__ __forceinline__ uint32_t kth_of_wave(uint32_t v, uint32_t kept) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 12; --bit) {
+        const uint32_t higher = t | 1u << bit;
+        if (__popcll(__ballot(v >= higher)) >= static_cast<int>(kept)) t = higher;
+    }
+    return t;
+}
 
-// One wave a search.
-__global__ __launch_bounds__(64) void leo_beam_groups(LeoBeams a, const BeamRecord* records, const uint64_t* candidates) {
-    const uint64_t group = blockIdx.x, first = group * a.beams;
-    const uint32_t lane = threadIdx.x, kept = static_cast<uint32_t>(a.kept), count = static_cast<uint32_t>(a.beams) * kept;
-    const auto length_of = [&](uint64_t row) {
-        return a.lengths ? static_cast<int64_t>(a.lengths[row]) + (is_finished(a, row) ? 0 : 1) : 1;
+// The same over a workgroup of 1, 2, 4, 8 or 16 waves, whose lanes make 64 groups: so
+// many different groups hold something as large that the value bounds the kept-th
+// largest of all. `maxima`: 64 words of LDS, not used where kWave.
+template <bool kWave>
+__device__ __forceinline__ uint32_t bar_of(uint32_t largest, uint32_t kept, uint32_t* maxima) {
+    const uint32_t lane = threadIdx.x % 64, waves = kWave ? 1 : blockDim.x / 64;
+    if (waves > 1) {
+        const uint32_t m = group_max(largest, waves);
+        if (lane % waves == 0) maxima[(threadIdx.x / 64 * 64 + lane) / waves] = m;
+        __syncthreads();
+        largest = maxima[lane];
+    }
+    return kth_of_wave(largest, kept);
+}
+
+// Orders what one wave (kWave) or a workgroup wrote to LDS.
+template <bool kWave>
+__device__ __forceinline__ void settle_lds() {
+    if constexpr (kWave) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    else __syncthreads();
+}
+
+// A place behind what the wave's other lanes and the other waves take.
+__device__ __forceinline__ uint32_t place_for(bool taken, uint32_t* count) {
+    const uint64_t mask = __ballot(taken);
+    uint32_t base = 0;
+    if (threadIdx.x % 64 == 0) base = atomicAdd(count, static_cast<uint32_t>(__popcll(mask)));
+    base = __builtin_amdgcn_readfirstlane(base);
+    return base + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+}
+
+// 1,024 neighbouring symbols of a row in the registers of a wave, 16 a lane in
+// rising order; -inf for NaN and beyond the row's end.
+constexpr uint32_t kSpan = 1024, kEach = 16;
+
+template <class T>
+struct Span {
+    static constexpr uint32_t kWide = 16 / sizeof(typename T::type);  // elements of a 16-byte load
+    float z[kEach];
+
+    static __device__ __forceinline__ uint32_t index(uint32_t base, uint32_t i) {
+        return base + i / kWide * (64 * kWide) + threadIdx.x % 64 * kWide + i % kWide;
+    }
+    __device__ __forceinline__ void load(const LeoBeams& a, uint64_t row, uint32_t base) {
+        const uint32_t n = static_cast<uint32_t>(a.symbols);
+        const auto* logits = static_cast<const typename T::type*>(a.logits) + row * a.logits_stride;
+        uint4v raw[kEach / kWide];
+#pragma unroll
+        for (uint32_t v = 0; v < kEach / kWide; ++v) raw[v] = load_row<T>(logits, index(base, v * kWide), n);
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) z[i] = fmaxf(T::at(raw[i / kWide], i % kWide), negative_infinity());
+    }
+    __device__ __forceinline__ float top() const {
+        float m = z[0];
+#pragma unroll
+        for (uint32_t i = 1; i < kEach; ++i) m = fmaxf(m, z[i]);
+        return m;
+    }
+    __device__ __forceinline__ uint64_t key(uint32_t base, uint32_t i) const {
+        return z[i] > negative_infinity() ? candidate(z[i], index(base, i)) : 0;
+    }
+};
+
+// What a span leaves for its row: its largest logit and the sum of exponentials
+// against it. Lanes' sums of 16 are floats, what joins them has 64 bits.
+struct SpanRecord {
+    float top;
+    uint32_t pad0;
+    double mass;
+};
+template <class T>
+__device__ __forceinline__ SpanRecord weigh(const Span<T>& s, float lane_top) {
+    const float top = wave_max(lane_top);
+    float mass = 0.0f;
+    if (top == negative_infinity()) return {top, 0, 0.0};
+    if (top < __builtin_inff()) {
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) mass += __builtin_amdgcn_exp2f((s.z[i] - top) * 1.44269504f);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) mass += s.z[i] == top ? 1.0f : 0.0f;
+    }
+    return {top, 0, wave_sum(static_cast<double>(mass))};
+}
+
+// The `kept` best of the spans of a workgroup (or of one wave's span, kWave), in
+// falling order, 0 behind the last. All that is not below a bar is gathered in `pool`
+// and finds its place by counting. Where more lies there than the pool holds, as ties
+// may, the kept-th best is found bit by bit, which no other symbol equals.
+template <class T, bool kWave>
+__device__ __forceinline__ void pick(const Span<T>& s, uint32_t base, float lane_top, uint32_t kept, uint64_t* pool, uint32_t capacity,
+                                     uint32_t* counters, uint32_t* maxima, uint64_t* to) {
+    const uint32_t thread = kWave ? threadIdx.x % 64 : threadIdx.x, threads = kWave ? 64 : blockDim.x;
+    if (thread == 0) counters[0] = counters[1] = 0;
+    const uint32_t largest = lane_top > negative_infinity() ? order_key(lane_top + 0.0f) : 0;
+    uint64_t least = static_cast<uint64_t>(max(bar_of<kWave>(largest, kept, maxima), 1u)) << 32;
+    settle_lds<kWave>();
+    const auto gather = [&](uint32_t* count) {
+        if (!__any(largest >= least >> 32)) return;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const uint64_t key = s.key(base, i);
+            const bool taken = key >= least;
+            if (!__any(taken)) continue;
+            const uint32_t at = place_for(taken, count);
+            if (taken && at < capacity) pool[at] = key;
+        }
     };
-    const auto score_of = [&](uint32_t at) -> double {  // -inf where there is none
-        const uint64_t row = first + at / kept;
-        const float score = a.scores[row];
-        if (!(score > negative_infinity())) return -__builtin_inf();
-        if (is_finished(a, row)) return at % kept == 0 ? static_cast<double>(score) : -__builtin_inf();
-        const uint64_t c = candidates[row * kept + at % kept];
-        if (c == 0) return -__builtin_inf();
-        const float z = from_order_key(static_cast<uint32_t>(c >> 32));
-        return score + ((z == records[row].top ? 0.0 : static_cast<double>(z) - records[row].top) - records[row].log_sum);
-    };
-    Ranked last = {__builtin_inf(), 0};
-    bool any = false;  // `last` was taken
-    for (uint32_t k = 0; k < kept; ++k) {
-        Ranked best = {-__builtin_inf(), 0xffffffffu};
-        for (uint32_t at = lane; at < count; at += 64) {
-            const double score = score_of(at);
-            if (!(score > -__builtin_inf())) continue;
-            const int64_t length = length_of(first + at / kept);
-            const double norm = a.length_penalty == 0.0 ? 1.0 : pow(static_cast<double>(length < 1 ? 1 : length), a.length_penalty);
-            const Ranked mine = {score / norm, at};
-            if ((!any || before(last, mine)) && (best.at == 0xffffffffu || before(mine, best))) best = mine;
-        }
-        for (int step = 32; step; step /= 2) {
-            const Ranked other = {__shfl_xor(best.rank, step), static_cast<uint32_t>(__shfl_xor(static_cast<int>(best.at), step))};
-            if (other.at != 0xffffffffu && (best.at == 0xffffffffu || before(other, best))) best = other;
-        }
-        const bool found = best.at != 0xffffffffu;
-        if (lane == 0) {
-            const uint64_t to = group * kept + k;
-            const uint32_t beam = found ? best.at / kept : 0;
-            const uint64_t row = first + beam;
-            const bool was = found && is_finished(a, row);
-            const uint32_t symbol = found && !was ? 0xffffffffu - static_cast<uint32_t>(candidates[row * kept + best.at % kept]) : 0xffffffffu;
-            a.out_symbols[to] = static_cast<int32_t>(symbol);
-            a.out_parents[to] = static_cast<int32_t>(beam);
-            a.out_scores[to] = found ? static_cast<float>(score_of(best.at)) : negative_infinity();
-            if (a.out_finished) a.out_finished[to] = was || (found && !was && static_cast<int64_t>(symbol) == a.end);
-            if (a.out_lengths) a.out_lengths[to] = a.lengths[row] + (found && !was ? 1 : 0);
-        }
-        if (!found) {
-            for (uint32_t j = k + 1 + lane; j < kept; j += 64) {
-                const uint64_t to = group * kept + j;
-                a.out_symbols[to] = -1;
-                a.out_parents[to] = 0;
-                a.out_scores[to] = negative_infinity();
-                if (a.out_finished) a.out_finished[to] = 0;
-                if (a.out_lengths) a.out_lengths[to] = a.lengths[first];
+    gather(&counters[0]);
+    settle_lds<kWave>();
+    uint32_t count = counters[0];
+    if (count > capacity) {
+        least = 0;
+        for (int bit = 63; bit >= 0; --bit) {
+            const uint64_t higher = least | 1ull << bit;
+            uint32_t mine = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; ++i) mine += s.key(base, i) >= higher;
+            mine = wave_sum(mine);
+            if constexpr (!kWave) {
+                __syncthreads();
+                if (threadIdx.x == 0) counters[1] = 0;
+                __syncthreads();
+                if (threadIdx.x % 64 == 0) atomicAdd(&counters[1], mine);
+                __syncthreads();
+                mine = counters[1];
             }
+            if (mine >= kept) least = higher;
+        }
+        settle_lds<kWave>();
+        if (thread == 0) counters[0] = 0;
+        settle_lds<kWave>();
+        gather(&counters[0]);
+        settle_lds<kWave>();
+        count = counters[0];
+    }
+    for (uint32_t i = thread; i < count; i += threads) {
+        const uint64_t mine = pool[i];
+        uint32_t rank = 0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < count; ++j) rank += pool[j] > mine;
+        if (rank < kept) to[rank] = mine;
+    }
+    for (uint32_t i = count + thread; i < kept; i += threads) to[i] = 0;
+}
+
+__device__ __forceinline__ bool is_finished(const LeoBeams& a, uint64_t row) { return a.finished && a.finished[row]; }
+__device__ __forceinline__ bool is_open(const LeoBeams& a, uint64_t row) { return !is_finished(a, row) && a.scores[row] > negative_infinity(); }
+
+// What makes a hypothesis' logits comparable with another's.
+struct Hypothesis {
+    double score, log_mass, norm;
+    float top;
+    uint32_t kind;  // 0: none, 1: finished, 2: open
+};
+
+// A candidate on its way to its place: larger ranks first, of equals the lower
+// hypothesis, then the better candidate.
+struct Ranked {
+    uint64_t rank, key;
+    uint32_t beam, pad0;
+};
+__device__ __forceinline__ bool before(const Ranked& p, const Ranked& q) {
+    return p.rank != q.rank ? p.rank > q.rank : p.beam != q.beam ? p.beam < q.beam : p.key > q.key;
+}
+
+constexpr uint32_t kPool = 1024;  // of a search's candidates
+struct MergeShared {
+    Hypothesis hypotheses[kMostBeams];
+    Ranked pool[kPool];
+    Ranked best[16];
+    uint32_t maxima[64];
+    uint32_t count;
+};
+
+// A search's answer from its hypotheses' span records [beams][spans] and its lists of
+// candidates [beams][lists][kept], by a whole workgroup of 2^n waves.
+__device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const SpanRecord* records, uint32_t spans,
+                                      const uint64_t* candidates, uint32_t lists, MergeShared& shared) {
+    const uint64_t first = group * a.beams;
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64, beams = static_cast<uint32_t>(a.beams),
+                   kept = static_cast<uint32_t>(a.kept);
+    for (uint32_t b = wave; b < beams; b += waves) {
+        Hypothesis h{};
+        const uint64_t row = first + b;
+        h.score = a.scores[row];
+        h.kind = !(h.score > -__builtin_inf()) ? 0 : is_finished(a, row) ? 1 : 2;
+        if (h.kind == 2) {
+            float top = negative_infinity();
+            for (uint32_t i = lane; i < spans; i += 64) top = fmaxf(top, records[b * spans + i].top);
+            top = wave_max(top);
+            double mass = 0.0;
+            for (uint32_t i = lane; i < spans; i += 64) {
+                const SpanRecord r = records[b * spans + i];
+                if (r.top > negative_infinity()) mass += r.top == top ? r.mass : r.mass * exp(static_cast<double>(r.top) - top);
+            }
+            h.log_mass = log(wave_sum(mass));
+            h.top = top;
+        }
+        h.norm = 1.0;
+        if (a.length_penalty != 0.0) {
+            const int64_t length = static_cast<int64_t>(a.lengths[row]) + (h.kind == 1 ? 0 : 1);
+            h.norm = pow(static_cast<double>(length < 1 ? 1 : length), a.length_penalty);
+        }
+        if (lane == 0) shared.hypotheses[b] = h;
+    }
+    if (threadIdx.x == 0) shared.count = 0;
+    __syncthreads();
+    const auto score_of = [&](const Hypothesis& h, uint64_t key) {
+        if (h.kind == 1) return h.score;
+        const float z = logit_of(key);
+        return h.score + ((z == h.top ? 0.0 : static_cast<double>(z) - h.top) - h.log_mass);
+    };
+    // the best of all lists, then the second best, so that they fall to different threads; rank 0 is none
+    const uint32_t items = beams * lists * kept;
+    const auto item = [&](uint32_t i) -> Ranked {
+        const uint32_t place = i / (beams * lists), list = i % (beams * lists), beam = list / lists;
+        const Hypothesis& h = shared.hypotheses[beam];
+        uint64_t key = 0;
+        if (h.kind == 1) key = place == 0 && list % lists == 0 ? 1 : 0;
+        else if (h.kind == 2) key = candidates[static_cast<uint64_t>(list) * kept + place];
+        if (key == 0) return {0, 0, 0, 0};
+        const double score = score_of(h, key);
+        if (!(score > -__builtin_inf())) return {0, 0, 0, 0};
+        const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(score / h.norm + 0.0));
+        return {bits >> 63 ? ~bits : bits | 1ull << 63, key, beam, 0};
+    };
+    const auto answer = [&](uint32_t k, const Ranked& r) {
+        const uint64_t to = group * kept + k, row = first + r.beam;
+        const Hypothesis& h = shared.hypotheses[r.beam];
+        const bool found = r.rank != 0, grows = found && h.kind == 2;
+        const int32_t symbol = grows ? static_cast<int32_t>(symbol_of(r.key)) : -1;
+        a.out_symbols[to] = symbol;
+        a.out_parents[to] = static_cast<int32_t>(r.beam);
+        a.out_scores[to] = found ? static_cast<float>(score_of(h, r.key)) : negative_infinity();
+        if (a.out_finished) a.out_finished[to] = found && (!grows || symbol == a.end);
+        if (a.out_lengths) a.out_lengths[to] = a.lengths[row] + (grows ? 1 : 0);
+    };
+    uint32_t largest = 0;
+    for (uint32_t i = threadIdx.x; i < items; i += blockDim.x) largest = max(largest, static_cast<uint32_t>(item(i).rank >> 32));
+    const uint32_t bar = max(bar_of<false>(largest, kept, shared.maxima), 1u);
+    for (uint32_t from = 0; from < items; from += blockDim.x) {
+        if (!__any(largest >= bar)) break;
+        const uint32_t i = from + threadIdx.x;
+        const Ranked r = i < items ? item(i) : Ranked{0, 0, 0, 0};
+        const bool taken = r.rank >> 32 >= bar;
+        if (!__any(taken)) continue;
+        const uint32_t at = place_for(taken, &shared.count);
+        if (taken && at < kPool) shared.pool[at] = r;
+    }
+    __syncthreads();
+    const uint32_t count = shared.count;
+    if (count <= kPool) {
+        for (uint32_t i = threadIdx.x; i < count; i += blockDim.x) {
+            const Ranked mine = shared.pool[i];
+            uint32_t rank = 0;
+            for (uint32_t j = 0; j < count; ++j) rank += before(shared.pool[j], mine);
+            if (rank < kept) answer(rank, mine);
+        }
+        for (uint32_t k = count + threadIdx.x; k < kept; k += blockDim.x) answer(k, {0, 0, 0, 0});
+        return;
+    }
+    // more ties than the pool holds: one after the other
+    Ranked last = {~0ull, ~0ull, 0, 0};
+    for (uint32_t k = 0; k < kept; ++k) {
+        Ranked best = {0, 0, 0, 0};
+        for (uint32_t i = threadIdx.x; i < items; i += blockDim.x) {
+            const Ranked r = item(i);
+            if (r.rank && before(last, r) && (!best.rank || before(r, best))) best = r;
+        }
+        const auto meet = [&](const Ranked& other) {
+            if (other.rank && (!best.rank || before(other, best))) best = other;
+        };
+#pragma unroll
+        for (int step = 32; step; step /= 2)
+            meet({__shfl_xor(static_cast<unsigned long long>(best.rank), step), __shfl_xor(static_cast<unsigned long long>(best.key), step),
+                  static_cast<uint32_t>(__shfl_xor(static_cast<int>(best.beam), step)), 0});
+        if (lane == 0) shared.best[wave] = best;
+        __syncthreads();
+        for (uint32_t w = 0; w < waves; ++w) meet(shared.best[w]);
+        __syncthreads();
+        if (threadIdx.x == 0) answer(k, best);
+        if (!best.rank) {
+            for (uint32_t j = k + 1 + threadIdx.x; j < kept; j += blockDim.x) answer(j, {0, 0, 0, 0});
             return;
         }
         last = best;
-        any = true;
     }
 }
 
+// Searches whose rows make up to 16 spans take one workgroup each: a wave a span,
+// which picks from its registers, then the search's answer.
+constexpr uint32_t kMostWaves = 16, kWavePool = 192;
+template <class T>
+__global__ __launch_bounds__(kMostWaves * 64) void leo_beam_whole(LeoBeams a, uint32_t spans) {
+    union Shared {
+        uint64_t pools[kMostWaves][kWavePool];
+        MergeShared merge;
+    };
+    __shared__ Shared shared;
+    __shared__ uint64_t candidates[kMostWaves][kMostBeams];
+    __shared__ SpanRecord records[kMostWaves];
+    __shared__ uint32_t counters[kMostWaves][2];
+    const uint32_t wave = threadIdx.x / 64, beam = wave / spans, base = wave % spans * kSpan, kept = static_cast<uint32_t>(a.kept);
+    const uint64_t row = blockIdx.x * a.beams + beam;
+    if (beam < a.beams && is_open(a, row)) {
+        Span<T> s;
+        s.load(a, row, base);
+        const float lane_top = s.top();
+        const SpanRecord r = weigh(s, lane_top);
+        if (threadIdx.x % 64 == 0) records[wave] = r;
+        pick<T, true>(s, base, lane_top, kept, shared.pools[wave], kWavePool, counters[wave], nullptr, &candidates[0][0] + wave * kept);
+    }
+    __syncthreads();
+    merge(a, blockIdx.x, records, spans, &candidates[0][0], spans, shared.merge);
+}
+
+// Longer rows: a workgroup a run of spans, a wave each, which leave their records and
+// the run its best candidates; then a workgroup a search.
+constexpr uint32_t kRowPool = 2048;
+template <class T>
+__global__ __launch_bounds__(kMostWaves * 64) void leo_beam_rows(LeoBeams a, uint32_t spans, uint32_t lists, SpanRecord* records, uint64_t* candidates) {
+    __shared__ uint64_t pool[kRowPool];
+    __shared__ uint32_t maxima[64], counters[2];
+    const uint64_t row = blockIdx.y;
+    if (!is_open(a, row)) return;
+    const uint32_t span = blockIdx.x * (blockDim.x / 64) + threadIdx.x / 64;
+    Span<T> s;
+    s.load(a, row, span * kSpan);
+    const float lane_top = s.top();
+    const SpanRecord r = weigh(s, lane_top);
+    if (threadIdx.x % 64 == 0 && span < spans) records[row * spans + span] = r;
+    pick<T, false>(s, span * kSpan, lane_top, static_cast<uint32_t>(a.kept), pool, kRowPool, counters, maxima,
+                   candidates + (row * lists + blockIdx.x) * a.kept);
+}
+
+__global__ __launch_bounds__(kMostWaves * 64) void leo_beam_groups(LeoBeams a, uint32_t spans, uint32_t lists, const SpanRecord* records,
+                                                                  const uint64_t* candidates) {
+    __shared__ MergeShared shared;
+    const uint64_t first = blockIdx.x * a.beams;
+    merge(a, blockIdx.x, records + first * spans, spans, candidates + first * lists * a.kept, lists, shared);
+}
+
 struct BeamPlan {
+    uint32_t spans, lists;         // of a row
+    uint32_t waves, merge_waves;   // of a workgroup
+    bool whole;
     uint64_t candidates, workspace;  // the candidates' offset, and the whole
 };
-BeamPlan beam_plan(uint64_t groups, uint64_t beams, uint64_t kept) {
+BeamPlan beam_plan(uint64_t groups, uint64_t beams, uint64_t kept, uint64_t symbols) {
     const uint64_t rows = groups * beams;
     BeamPlan p{};
-    p.candidates = (rows * sizeof(BeamRecord) + 255) / 256 * 256;
-    p.workspace = p.candidates + rows * kept * sizeof(uint64_t);
+    const auto power = [](uint64_t most) {  // the least power of two that is no less
+        uint32_t v = 1;
+        while (v < most && v < kMostWaves) v *= 2;
+        return v;
+    };
+    p.spans = static_cast<uint32_t>((symbols + kSpan - 1) / kSpan);
+    p.whole = beams * p.spans <= kMostWaves;
+    if (p.whole) {
+        p.waves = power(beams * p.spans);
+        return p;
+    }
+    p.waves = power(p.spans);
+    if (p.waves == kMostWaves && rows * ((p.spans + kMostWaves - 1) / kMostWaves) < 256) p.waves = kMostWaves / 2;
+    p.lists = (p.spans + p.waves - 1) / p.waves;
+    p.merge_waves = power((beams * p.lists * kept + 63) / 64);
+    p.candidates = (rows * p.spans * sizeof(SpanRecord) + 255) / 256 * 256;
+    p.workspace = p.candidates + rows * p.lists * kept * sizeof(uint64_t);
     return p;
 }
 
@@ -174,16 +438,19 @@ void check_beams(const char* who, uint64_t groups, uint64_t beams, uint64_t kept
     };
     need(beams >= 1 && beams <= kMostBeams, "beams must be 1 .. 64");
     need(kept >= 1 && kept <= kMostBeams, "kept must be 1 .. 64");
-    need(groups <= 65535, "too many groups");
-    need(symbols >= 1 && symbols <= 0x7fffffffu, "symbols must be 1 .. 2^31 - 1");
+    need(groups * beams <= 65535, "too many hypotheses");
+    need(symbols >= 1 && symbols <= 1u << 26, "symbols must be 1 .. 2^26");
 }
 
 template <class T>
 void launch_beams(const BeamPlan& p, const LeoBeams& b, hipStream_t stream) {
-    auto* records = static_cast<BeamRecord*>(b.workspace);
+    const dim3 groups(static_cast<uint32_t>(b.groups));
+    if (p.whole) return launch(leo_beam_whole<T>, groups, dim3(p.waves * 64), 0, stream, b, p.spans);
+    auto* records = static_cast<SpanRecord*>(b.workspace);
     auto* candidates = reinterpret_cast<uint64_t*>(static_cast<char*>(b.workspace) + p.candidates);
-    launch(leo_beam_rows<T>, dim3(static_cast<uint32_t>(b.groups * b.beams)), dim3(256), 0, stream, b, records, candidates);
-    launch(leo_beam_groups, dim3(static_cast<uint32_t>(b.groups)), dim3(64), 0, stream, b, static_cast<const BeamRecord*>(records),
+    launch(leo_beam_rows<T>, dim3(p.lists, static_cast<uint32_t>(b.groups * b.beams)), dim3(p.waves * 64), 0, stream, b, p.spans, p.lists,
+           records, candidates);
+    launch(leo_beam_groups, groups, dim3(p.merge_waves * 64), 0, stream, b, p.spans, p.lists, static_cast<const SpanRecord*>(records),
            static_cast<const uint64_t*>(candidates));
 }
 
@@ -322,7 +589,7 @@ int32_t leo_beam_workspace_bytes(uint64_t groups, uint64_t beams, uint64_t kept,
     return guarded([&] {
         require(bytes, "leo_beam_workspace_bytes: null argument");
         check_beams("leo_beam_workspace_bytes", groups, beams, kept, symbols);
-        *bytes = groups ? beam_plan(groups, beams, kept).workspace : 0;
+        *bytes = groups ? beam_plan(groups, beams, kept, symbols).workspace : 0;
     });
 }
 
@@ -338,8 +605,8 @@ int32_t leo_beam_select(const LeoBeams* beams, void* stream) {
         require(std::isfinite(b.length_penalty), "leo_beam_select: length_penalty must be finite");
         require(b.lengths || (b.length_penalty == 0.0 && !b.out_lengths), "leo_beam_select: length_penalty or out_lengths without lengths");
         require(b.end >= -1 && b.end < static_cast<int64_t>(b.symbols), "leo_beam_select: end must be a symbol, or -1");
-        const BeamPlan p = beam_plan(b.groups, b.beams, b.kept);
-        require(b.workspace && reinterpret_cast<uintptr_t>(b.workspace) % 256 == 0 && b.workspace_bytes >= p.workspace,
+        const BeamPlan p = beam_plan(b.groups, b.beams, b.kept, b.symbols);
+        require(p.workspace == 0 || (b.workspace && reinterpret_cast<uintptr_t>(b.workspace) % 256 == 0 && b.workspace_bytes >= p.workspace),
                 "leo_beam_select: workspace is missing, too small or not 256-byte aligned");
         const auto at = static_cast<hipStream_t>(stream);
         if (b.type == LEO_TYPE_F32) launch_beams<F32>(p, b, at);

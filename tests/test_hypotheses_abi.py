@@ -73,13 +73,13 @@ def test_bad_products_are_refused():
 
 
 def test_bad_selections_are_refused():
-    good = dict(groups=2, beams=3, kept=3, symbols=257, logits=256, logits_stride=257, type=native.TYPE_F32, scores=256,
+    good = dict(groups=2, beams=3, kept=3, symbols=40_000, logits=256, logits_stride=40_000, type=native.TYPE_F32, scores=256,
                 out_symbols=256, out_parents=256, out_scores=256, end=-1, workspace=1 << 20, workspace_bytes=1 << 20)
-    for change in (dict(beams=0), dict(beams=65), dict(kept=0), dict(kept=65), dict(symbols=0), dict(symbols=1 << 31),
+    for change in (dict(beams=0), dict(beams=65), dict(kept=0), dict(kept=65), dict(symbols=0), dict(symbols=(1 << 26) + 1),
                    dict(groups=1 << 20), dict(type=4), dict(logits=None), dict(scores=None), dict(out_symbols=None),
                    dict(out_parents=None), dict(out_scores=None), dict(logits_stride=-1), dict(length_penalty=0.5),
                    dict(lengths=256, length_penalty=float("nan")), dict(lengths=256, length_penalty=float("inf")),
-                   dict(out_lengths=256), dict(end=257), dict(end=-2), dict(workspace=None), dict(workspace_bytes=8),
+                   dict(out_lengths=256), dict(end=40_000), dict(end=-2), dict(workspace=None), dict(workspace_bytes=8),
                    dict(workspace=(1 << 20) + 128)):
         _refused("leo_beam_select", ctypes.byref(native.LeoBeams(**{**good, **change})), None)
     size = ctypes.c_uint64()
