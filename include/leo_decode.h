@@ -188,10 +188,11 @@ int32_t leo_q8_layout(const LeoQ8Source* source, void* stream);
 
 /* y[m, n] = bias[n] + s[m] * scale[n] * sum over k of q[m, k] * code[n, k], where
  * s[m] is the larger of 2^-126 and the largest magnitude of row m of x times the
- * float nearest to 1 / 127, rounded to float, and q[m, k] the whole number nearest to x[m, k] / s[m], of two
- * the even one. Sums of codes are exact, the rest is held in 64 bits, and one
- * rounding takes it to y_type. A row of x with an infinity or NaN gives NaN. bias
- * (float) may be NULL. y and x share no memory. `workspace`: at least
+ * float nearest to 1 / 127, rounded to float, and q[m, k] the whole number nearest to
+ * x[m, k] / s[m], of two the even one. Sums of codes are exact; rounded to float they
+ * are multiplied by scale[n], which has to leave a finite float, then by s[m] with the
+ * bias in one fused operation, and rounded to y_type. A row of x with an infinity or
+ * NaN gives NaN. bias (float) may be NULL. y and x share no memory. `workspace`: at least
  * leo_q8_workspace_bytes() bytes (none where that is 0), 256-byte aligned, whatever
  * they hold; free again when the call's work is done. */
 typedef struct LeoQ8Product {

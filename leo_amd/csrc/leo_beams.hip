@@ -31,9 +31,30 @@ __device__ __forceinline__ float logit_of(uint64_t c) { return from_order_key(st
 __device__ __forceinline__ uint32_t symbol_of(uint64_t c) { return 0xffffffffu - static_cast<uint32_t>(c); }
 
 __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int step = 32; step; step /= 2) v += __shfl_xor(v, step);
-    return v;
+    const auto step = [&](auto ctrl, auto rows) {
+        const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(v));
+        const auto moved = [&](uint32_t half) {
+            return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(half), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+        };
+        const uint64_t other = static_cast<uint64_t>(moved(static_cast<uint32_t>(bits >> 32))) << 32 | moved(static_cast<uint32_t>(bits));
+        v += __longlong_as_double(static_cast<long long>(other));
+    };
+    step(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // as wave_reduce does
+    step(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+    step(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+    step(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+    step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
+    step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+    const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(v));
+    const auto last = [](uint32_t half) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(half), 63)); };
+    return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(last(static_cast<uint32_t>(bits >> 32))) << 32 | last(static_cast<uint32_t>(bits))));
+}
+
+// exp(d) for d <= 0, to some 2^-23 of itself: the product with log2(e) in two parts.
+__device__ __forceinline__ float exp_of(float d) {
+    const float high = d * 1.44269504f, low = __builtin_fmaf(d, 1.44269504f, -high) + d * 1.92596299e-8f;
+    const float e = __builtin_amdgcn_exp2f(high);
+    return e > 0.0f ? __builtin_fmaf(e, low * 0.693147181f, e) : 0.0f;
 }
 
 // The largest of v in each group of `lanes` neighbouring lanes (a power of two up to 16).
@@ -82,13 +103,17 @@ __device__ __forceinline__ void settle_lds() {
     else __syncthreads();
 }
 
+// The bits of a mask below this lane's.
+__device__ __forceinline__ uint32_t below_in(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+}
+
 // A place behind what the wave's other lanes and the other waves take.
 __device__ __forceinline__ uint32_t place_for(bool taken, uint32_t* count) {
     const uint64_t mask = __ballot(taken);
     uint32_t base = 0;
     if (threadIdx.x % 64 == 0) base = atomicAdd(count, static_cast<uint32_t>(__popcll(mask)));
-    base = __builtin_amdgcn_readfirstlane(base);
-    return base + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+    return __builtin_amdgcn_readfirstlane(base) + below_in(mask);
 }
 
 // 1,024 neighbouring symbols of a row in the registers of a wave, 16 a lane in
@@ -155,24 +180,32 @@ __device__ __forceinline__ void pick(const Span<T>& s, uint32_t base, float lane
     const uint32_t thread = kWave ? threadIdx.x % 64 : threadIdx.x, threads = kWave ? 64 : blockDim.x;
     if (thread == 0) counters[0] = counters[1] = 0;
     const uint32_t largest = lane_top > negative_infinity() ? order_key(lane_top + 0.0f) : 0;
-    uint64_t least = static_cast<uint64_t>(max(bar_of<kWave>(largest, kept, maxima), 1u)) << 32;
+    const float bar = from_order_key(max(bar_of<kWave>(largest, kept, maxima), 0x00800000u));  // the lowest finite value or more
     settle_lds<kWave>();
-    const auto gather = [&](uint32_t* count) {
-        if (!__any(largest >= least >> 32)) return;
+    const auto gather = [&](auto&& stays) {
+        if (!__any(lane_top >= bar)) return;
+        uint64_t masks[kEach];
+        uint32_t total = 0, at = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
-            const uint64_t key = s.key(base, i);
-            const bool taken = key >= least;
-            if (!__any(taken)) continue;
-            const uint32_t at = place_for(taken, count);
-            if (taken && at < capacity) pool[at] = key;
+            masks[i] = __ballot(stays(i));
+            total += static_cast<uint32_t>(__popcll(masks[i]));
+        }
+        if (threadIdx.x % 64 == 0) at = atomicAdd(&counters[0], total);
+        at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            if (!masks[i]) continue;
+            const uint32_t mine = at + below_in(masks[i]);
+            if (stays(i) && mine < capacity) pool[mine] = s.key(base, i);
+            at += static_cast<uint32_t>(__popcll(masks[i]));
         }
     };
-    gather(&counters[0]);
+    gather([&](uint32_t i) { return s.z[i] >= bar; });
     settle_lds<kWave>();
     uint32_t count = counters[0];
     if (count > capacity) {
-        least = 0;
+        uint64_t least = 0;
         for (int bit = 63; bit >= 0; --bit) {
             const uint64_t higher = least | 1ull << bit;
             uint32_t mine = 0;
@@ -192,14 +225,14 @@ __device__ __forceinline__ void pick(const Span<T>& s, uint32_t base, float lane
         settle_lds<kWave>();
         if (thread == 0) counters[0] = 0;
         settle_lds<kWave>();
-        gather(&counters[0]);
+        gather([&](uint32_t i) { return s.key(base, i) >= least; });
         settle_lds<kWave>();
         count = counters[0];
     }
     for (uint32_t i = thread; i < count; i += threads) {
         const uint64_t mine = pool[i];
         uint32_t rank = 0;
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t j = 0; j < count; ++j) rank += pool[j] > mine;
         if (rank < kept) to[rank] = mine;
     }
@@ -211,7 +244,7 @@ __device__ __forceinline__ bool is_open(const LeoBeams& a, uint64_t row) { retur
 
 // What makes a hypothesis' logits comparable with another's.
 struct Hypothesis {
-    double score, log_mass, norm;
+    double score, log_mass, inverse;  // 1 over the length's power
     float top;
     uint32_t kind;  // 0: none, 1: finished, 2: open
 };
@@ -219,11 +252,16 @@ struct Hypothesis {
 // A candidate on its way to its place: larger ranks first, of equals the lower
 // hypothesis, then the better candidate.
 struct Ranked {
-    uint64_t rank, key;
-    uint32_t beam, pad0;
+    uint64_t rank, second;
+    // 6 bits for the hypothesis, 32 for the logit, 26 for the symbol
+    static __device__ __forceinline__ uint64_t second_of(uint32_t beam, uint64_t key) {
+        return static_cast<uint64_t>(63 - beam) << 58 | (key >> 32) << 26 | (key & 0x3ffffffu);
+    }
+    __device__ __forceinline__ uint32_t beam() const { return 63 - static_cast<uint32_t>(second >> 58); }
+    __device__ __forceinline__ uint64_t key() const { return (second >> 26 & 0xffffffffu) << 32 | 0xfc000000u | (second & 0x3ffffffu); }
 };
 __device__ __forceinline__ bool before(const Ranked& p, const Ranked& q) {
-    return p.rank != q.rank ? p.rank > q.rank : p.beam != q.beam ? p.beam < q.beam : p.key > q.key;
+    return (p.rank > q.rank) | ((p.rank == q.rank) & (p.second > q.second));
 }
 
 constexpr uint32_t kPool = 1024;  // of a search's candidates
@@ -236,98 +274,147 @@ struct MergeShared {
 };
 
 // A search's answer from its hypotheses' span records [beams][spans] and its lists of
-// candidates [beams][lists][kept], by a whole workgroup of 2^n waves.
+// candidates [beams][lists][kept], by a whole workgroup of 2^n waves. What it reads is on
+// its way before anything is needed; the lists of finished hypotheses and of those with no
+// score hold anything, and count for nothing.
+constexpr uint32_t kAhead = 4;
 __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const SpanRecord* records, uint32_t spans,
                                       const uint64_t* candidates, uint32_t lists, MergeShared& shared) {
     const uint64_t first = group * a.beams;
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64, beams = static_cast<uint32_t>(a.beams),
-                   kept = static_cast<uint32_t>(a.kept);
+    const uint32_t thread = threadIdx.x, threads = blockDim.x, lane = thread % 64, wave = thread / 64, waves = threads / 64,
+                   beams = static_cast<uint32_t>(a.beams), kept = static_cast<uint32_t>(a.kept), all = beams * lists;
+    uint64_t ahead[kAhead];  // of this thread's first list
+#pragma unroll
+    for (uint32_t p = 0; p < kAhead; ++p) ahead[p] = thread < all && p < kept ? candidates[static_cast<uint64_t>(thread) * kept + p] : 0;
     for (uint32_t b = wave; b < beams; b += waves) {
-        Hypothesis h{};
         const uint64_t row = first + b;
-        h.score = a.scores[row];
-        h.kind = !(h.score > -__builtin_inf()) ? 0 : is_finished(a, row) ? 1 : 2;
+        const SpanRecord none = {negative_infinity(), 0, 0.0};
+        const SpanRecord mine = lane < spans ? records[b * spans + lane] : none;
+        const float score = a.scores[row];
+        const bool finished = is_finished(a, row);
+        const int32_t length = a.lengths ? a.lengths[row] : 0;
+        Hypothesis h{};
+        h.score = score;
+        h.kind = !(score > negative_infinity()) ? 0 : finished ? 1 : 2;
         if (h.kind == 2) {
-            float top = negative_infinity();
-            for (uint32_t i = lane; i < spans; i += 64) top = fmaxf(top, records[b * spans + i].top);
+            float top = mine.top;
+#pragma unroll 4
+            for (uint32_t i = lane + 64; i < spans; i += 64) top = fmaxf(top, records[b * spans + i].top);
             top = wave_max(top);
-            double mass = 0.0;
-            for (uint32_t i = lane; i < spans; i += 64) {
-                const SpanRecord r = records[b * spans + i];
-                if (r.top > negative_infinity()) mass += r.top == top ? r.mass : r.mass * exp(static_cast<double>(r.top) - top);
-            }
+            const auto against = [&](const SpanRecord& r) {
+                return r.top == top ? r.mass : r.top > negative_infinity() ? r.mass * exp_of(r.top - top) : 0.0;
+            };
+            double mass = against(mine);
+#pragma unroll 4
+            for (uint32_t i = lane + 64; i < spans; i += 64) mass += against(records[b * spans + i]);
             h.log_mass = log(wave_sum(mass));
             h.top = top;
         }
-        h.norm = 1.0;
+        h.inverse = 1.0;
         if (a.length_penalty != 0.0) {
-            const int64_t length = static_cast<int64_t>(a.lengths[row]) + (h.kind == 1 ? 0 : 1);
-            h.norm = pow(static_cast<double>(length < 1 ? 1 : length), a.length_penalty);
+            const int64_t grown = static_cast<int64_t>(length) + (h.kind == 1 ? 0 : 1);
+            h.inverse = 1.0 / pow(static_cast<double>(grown < 1 ? 1 : grown), a.length_penalty);
         }
         if (lane == 0) shared.hypotheses[b] = h;
     }
-    if (threadIdx.x == 0) shared.count = 0;
+    if (thread == 0) shared.count = 0;
     __syncthreads();
     const auto score_of = [&](const Hypothesis& h, uint64_t key) {
         if (h.kind == 1) return h.score;
         const float z = logit_of(key);
         return h.score + ((z == h.top ? 0.0 : static_cast<double>(z) - h.top) - h.log_mass);
     };
-    // the best of all lists, then the second best, so that they fall to different threads; rank 0 is none
-    const uint32_t items = beams * lists * kept;
-    const auto item = [&](uint32_t i) -> Ranked {
-        const uint32_t place = i / (beams * lists), list = i % (beams * lists), beam = list / lists;
+    // rank 0 is none
+    const auto ranked = [&](uint32_t list, uint32_t place, uint64_t key) -> Ranked {
+        const uint32_t beam = list / lists;
         const Hypothesis& h = shared.hypotheses[beam];
-        uint64_t key = 0;
         if (h.kind == 1) key = place == 0 && list % lists == 0 ? 1 : 0;
-        else if (h.kind == 2) key = candidates[static_cast<uint64_t>(list) * kept + place];
-        if (key == 0) return {0, 0, 0, 0};
         const double score = score_of(h, key);
-        if (!(score > -__builtin_inf())) return {0, 0, 0, 0};
-        const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(score / h.norm + 0.0));
-        return {bits >> 63 ? ~bits : bits | 1ull << 63, key, beam, 0};
+        const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(score * h.inverse + 0.0));
+        const bool none = h.kind == 0 || key == 0 || !(score > -__builtin_inf());
+        return {none ? 0 : bits >> 63 ? ~bits : bits | 1ull << 63, Ranked::second_of(beam, key)};
     };
+    const auto load_ranked = [&](uint32_t list, uint32_t place) { return ranked(list, place, candidates[static_cast<uint64_t>(list) * kept + place]); };
     const auto answer = [&](uint32_t k, const Ranked& r) {
-        const uint64_t to = group * kept + k, row = first + r.beam;
-        const Hypothesis& h = shared.hypotheses[r.beam];
-        const bool found = r.rank != 0, grows = found && h.kind == 2;
-        const int32_t symbol = grows ? static_cast<int32_t>(symbol_of(r.key)) : -1;
+        const bool found = r.rank != 0;
+        const uint32_t beam = found ? r.beam() : 0;
+        const uint64_t to = group * kept + k, row = first + beam;
+        const Hypothesis& h = shared.hypotheses[beam];
+        const bool grows = found && h.kind == 2;
+        const int32_t symbol = grows ? static_cast<int32_t>(symbol_of(r.key())) : -1;
         a.out_symbols[to] = symbol;
-        a.out_parents[to] = static_cast<int32_t>(r.beam);
-        a.out_scores[to] = found ? static_cast<float>(score_of(h, r.key)) : negative_infinity();
+        a.out_parents[to] = static_cast<int32_t>(beam);
+        a.out_scores[to] = found ? static_cast<float>(score_of(h, r.key())) : negative_infinity();
         if (a.out_finished) a.out_finished[to] = found && (!grows || symbol == a.end);
         if (a.out_lengths) a.out_lengths[to] = a.lengths[row] + (grows ? 1 : 0);
     };
-    uint32_t largest = 0;
-    for (uint32_t i = threadIdx.x; i < items; i += blockDim.x) largest = max(largest, static_cast<uint32_t>(item(i).rank >> 32));
-    const uint32_t bar = max(bar_of<false>(largest, kept, shared.maxima), 1u);
-    for (uint32_t from = 0; from < items; from += blockDim.x) {
-        if (!__any(largest >= bar)) break;
-        const uint32_t i = from + threadIdx.x;
-        const Ranked r = i < items ? item(i) : Ranked{0, 0, 0, 0};
+    const auto gather = [&](const Ranked& r, uint32_t bar) {  // whether any of the wave's was taken
         const bool taken = r.rank >> 32 >= bar;
-        if (!__any(taken)) continue;
+        if (!__any(taken)) return false;
         const uint32_t at = place_for(taken, &shared.count);
         if (taken && at < kPool) shared.pool[at] = r;
+        return true;
+    };
+    const Ranked nothing = {0, 0};
+    uint32_t largest = 0;
+    if (all >= kept) {
+        // the lists' best bound what can be kept, and each list is followed down to the bar
+        for (uint32_t list = thread; list < all; list += threads)
+            largest = max(largest, static_cast<uint32_t>((list == thread ? ranked(list, 0, ahead[0]) : load_ranked(list, 0)).rank >> 32));
+        const uint32_t bar = max(bar_of<false>(largest, kept, shared.maxima), 1u);
+        for (uint32_t from = 0; from < all; from += threads) {
+            if (!__any(largest >= bar)) break;
+            const uint32_t list = from + thread;
+            bool more = true;
+            if (from == 0) {  // one addition for what the lists' first places hold, which is mostly all
+                Ranked r[kAhead];
+                uint64_t masks[kAhead];
+                uint32_t total = 0, at = 0;
+#pragma unroll
+                for (uint32_t p = 0; p < kAhead; ++p) {
+                    r[p] = list < all && p < kept ? ranked(list, p, ahead[p]) : nothing;
+                    masks[p] = __ballot(r[p].rank >> 32 >= bar);
+                    total += static_cast<uint32_t>(__popcll(masks[p]));
+                }
+                if (lane == 0) at = atomicAdd(&shared.count, total);
+                at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+                for (uint32_t p = 0; p < kAhead; ++p) {
+                    const uint32_t mine = at + below_in(masks[p]);
+                    if (masks[p] >> lane & 1 && mine < kPool) shared.pool[mine] = r[p];
+                    at += static_cast<uint32_t>(__popcll(masks[p]));
+                }
+                more = masks[kAhead - 1] != 0;
+            }
+            for (uint32_t p = from == 0 ? kAhead : 0; more && p < kept; ++p) more = gather(list < all ? load_ranked(list, p) : nothing, bar);
+        }
+    } else {
+        // few lists: all their candidates, fewer than 64 * 64
+        const uint32_t items = all * kept;
+        const auto item = [&](uint32_t i) { return i < items ? load_ranked(i % all, i / all) : nothing; };
+        for (uint32_t i = thread; i < items; i += threads) largest = max(largest, static_cast<uint32_t>(item(i).rank >> 32));
+        const uint32_t bar = max(bar_of<false>(largest, kept, shared.maxima), 1u);
+        for (uint32_t from = 0; from < items; from += threads) gather(item(from + thread), bar);
     }
     __syncthreads();
     const uint32_t count = shared.count;
     if (count <= kPool) {
-        for (uint32_t i = threadIdx.x; i < count; i += blockDim.x) {
+        for (uint32_t i = thread; i < count; i += threads) {
             const Ranked mine = shared.pool[i];
             uint32_t rank = 0;
+#pragma unroll 8
             for (uint32_t j = 0; j < count; ++j) rank += before(shared.pool[j], mine);
             if (rank < kept) answer(rank, mine);
         }
-        for (uint32_t k = count + threadIdx.x; k < kept; k += blockDim.x) answer(k, {0, 0, 0, 0});
+        for (uint32_t k = count + thread; k < kept; k += threads) answer(k, nothing);
         return;
     }
     // more ties than the pool holds: one after the other
-    Ranked last = {~0ull, ~0ull, 0, 0};
+    Ranked last = {~0ull, ~0ull};
     for (uint32_t k = 0; k < kept; ++k) {
-        Ranked best = {0, 0, 0, 0};
-        for (uint32_t i = threadIdx.x; i < items; i += blockDim.x) {
-            const Ranked r = item(i);
+        Ranked best = nothing;
+        for (uint32_t i = thread; i < all * kept; i += threads) {
+            const Ranked r = load_ranked(i % all, i / all);
             if (r.rank && before(last, r) && (!best.rank || before(r, best))) best = r;
         }
         const auto meet = [&](const Ranked& other) {
@@ -335,15 +422,14 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const S
         };
 #pragma unroll
         for (int step = 32; step; step /= 2)
-            meet({__shfl_xor(static_cast<unsigned long long>(best.rank), step), __shfl_xor(static_cast<unsigned long long>(best.key), step),
-                  static_cast<uint32_t>(__shfl_xor(static_cast<int>(best.beam), step)), 0});
+            meet({__shfl_xor(static_cast<unsigned long long>(best.rank), step), __shfl_xor(static_cast<unsigned long long>(best.second), step)});
         if (lane == 0) shared.best[wave] = best;
         __syncthreads();
         for (uint32_t w = 0; w < waves; ++w) meet(shared.best[w]);
         __syncthreads();
-        if (threadIdx.x == 0) answer(k, best);
+        if (thread == 0) answer(k, best);
         if (!best.rank) {
-            for (uint32_t j = k + 1 + threadIdx.x; j < kept; j += blockDim.x) answer(j, {0, 0, 0, 0});
+            for (uint32_t j = k + 1 + thread; j < kept; j += threads) answer(j, nothing);
             return;
         }
         last = best;
@@ -365,9 +451,9 @@ __global__ __launch_bounds__(kMostWaves * 64) void leo_beam_whole(LeoBeams a, ui
     __shared__ uint32_t counters[kMostWaves][2];
     const uint32_t wave = threadIdx.x / 64, beam = wave / spans, base = wave % spans * kSpan, kept = static_cast<uint32_t>(a.kept);
     const uint64_t row = blockIdx.x * a.beams + beam;
-    if (beam < a.beams && is_open(a, row)) {
+    if (beam < a.beams) {
         Span<T> s;
-        s.load(a, row, base);
+        s.load(a, row, base);  // also where nothing comes of it: sooner than after asking
         const float lane_top = s.top();
         const SpanRecord r = weigh(s, lane_top);
         if (threadIdx.x % 64 == 0) records[wave] = r;
@@ -379,9 +465,9 @@ __global__ __launch_bounds__(kMostWaves * 64) void leo_beam_whole(LeoBeams a, ui
 
 // Longer rows: a workgroup a run of spans, a wave each, which leave their records and
 // the run its best candidates; then a workgroup a search.
-constexpr uint32_t kRowPool = 2048;
+constexpr uint32_t kRowPool = 1024;
 template <class T>
-__global__ __launch_bounds__(kMostWaves * 64) void leo_beam_rows(LeoBeams a, uint32_t spans, uint32_t lists, SpanRecord* records, uint64_t* candidates) {
+__global__ __launch_bounds__(256) void leo_beam_rows(LeoBeams a, uint32_t spans, uint32_t lists, SpanRecord* records, uint64_t* candidates) {
     __shared__ uint64_t pool[kRowPool];
     __shared__ uint32_t maxima[64], counters[2];
     const uint64_t row = blockIdx.y;
@@ -423,10 +509,9 @@ BeamPlan beam_plan(uint64_t groups, uint64_t beams, uint64_t kept, uint64_t symb
         p.waves = power(beams * p.spans);
         return p;
     }
-    p.waves = power(p.spans);
-    if (p.waves == kMostWaves && rows * ((p.spans + kMostWaves - 1) / kMostWaves) < 256) p.waves = kMostWaves / 2;
+    p.waves = std::min(power(p.spans), 4u);
     p.lists = (p.spans + p.waves - 1) / p.waves;
-    p.merge_waves = power((beams * p.lists * kept + 63) / 64);
+    p.merge_waves = power(std::max(beams, (beams * p.lists + 63) / 64));
     p.candidates = (rows * p.spans * sizeof(SpanRecord) + 255) / 256 * 256;
     p.workspace = p.candidates + rows * p.lists * kept * sizeof(uint64_t);
     return p;

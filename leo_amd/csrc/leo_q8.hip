@@ -22,6 +22,7 @@ constexpr uint64_t kMostRows = 1 << 20;
 constexpr uint32_t kMostSliceBlocks = 131072 / kBlock;
 
 typedef int32_t int4v __attribute__((ext_vector_type(4)));
+typedef float float4v __attribute__((ext_vector_type(4)));
 
 struct Q8Layout {
     uint64_t tiles, blocks;
@@ -62,7 +63,8 @@ __global__ __launch_bounds__(64) void leo_q8_lay_out(LeoQ8Source s, Q8Layout l) 
     u.words = uint4v{0, 0, 0, 0};
     if (n < s.shape.outputs) {
         const int8_t* row = static_cast<const int8_t*>(s.codes) + n * s.codes_stride;
-        for (uint32_t i = 0; i < 16; ++i)
+        if (k + 16 <= s.shape.inputs) u.words = load_16(row + k);
+        else for (uint32_t i = 0; i < 16; ++i)
             if (k + i < s.shape.inputs) u.codes[i] = row[k + i];
     }
     reinterpret_cast<uint4v*>(static_cast<char*>(s.layout) + at * kBlockBytes)[lane] = u.words;
@@ -128,31 +130,50 @@ __device__ __forceinline__ float scale_of(uint32_t largest) {
     return largest < 0x7f800000u ? fmaxf(__uint_as_float(largest) * (1.0f / 127.0f), 0x1p-126f) : __builtin_nanf("");
 }
 
-// The whole numbers nearest to the exact quotients x / s, of two the even one: the
-// product with the rounded inverse is off by less than one half, and the remainder
-// x - n s, which needs no rounding where it is near s / 2, tells where it matters.
+// The whole numbers nearest to the exact quotients x / s, of two the even one. The sum
+// with 1.5 * 2^23 of x and the rounded inverse rounds to a whole number once and has it in
+// its last byte. The inverse is off by 2^-24 of itself, so a quotient of 127 at most by
+// less than 2^-16: only where one lies as near to a half, as in some 3% of waves, the
+// remainder x - n s tells, which needs no rounding near s / 2.
 __device__ __forceinline__ uint4v codes_of(const Sixteen& s, float scale) {
-    const float inverse = 1.0f / scale, half = 0.5f * scale;
+    constexpr float kMagic = 12582912.0f;
+    const float inverse = 1.0f / scale;
+    float number[16], off = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {
+        number[i] = __builtin_fmaf(s.f[i], inverse, kMagic);
+        off = fmaxf(off, fabsf(__builtin_fmaf(s.f[i], inverse, kMagic - number[i])));
+    }
+    if (__any(off > 0.5f - 0x1p-16f)) {
+        const float half = 0.5f * scale;
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) {
+            const float n = number[i] - kMagic, rest = __builtin_fmaf(-n, scale, s.f[i]);
+            const bool odd = __float_as_uint(number[i]) & 1u;
+            if (rest > half || (rest == half && odd)) number[i] += 1.0f;
+            if (rest < -half || (rest == -half && odd)) number[i] -= 1.0f;
+        }
+    }
     uint4v words;
 #pragma unroll
     for (uint32_t w = 0; w < 4; ++w) {
-        uint32_t word = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            const float x = s.f[4 * w + i], n = __builtin_rintf(x * inverse), rest = __builtin_fmaf(-n, scale, x);
-            int32_t code = static_cast<int32_t>(n);
-            const int32_t odd = code & 1;
-            if (rest > half || (rest == half && odd)) code += 1;
-            if (rest < -half || (rest == -half && odd)) code -= 1;
-            word |= (static_cast<uint32_t>(code) & 0xffu) << (8 * i);
-        }
-        words[w] = word;
+        const uint32_t low = __builtin_amdgcn_perm(__float_as_uint(number[4 * w + 1]), __float_as_uint(number[4 * w]), 0x0c0c0400);
+        const uint32_t high = __builtin_amdgcn_perm(__float_as_uint(number[4 * w + 3]), __float_as_uint(number[4 * w + 2]), 0x04000c0c);
+        words[w] = low | high;
     }
     return scale == scale ? words : uint4v{0, 0, 0, 0};
 }
 
+// A whole sum as a value: three roundings of 2^-24, of which the second may be of a value
+// past the result's, then the one to y's type. 64 bits here took 11 us of a 256 x 256
+// tile's time, for bits that the 8-bit x does not have. The row's scale, which alone may be
+// next to the smallest float, comes last.
+__device__ __forceinline__ float value_of(float sum, float scale, float row_scale, float bias) {
+    return __builtin_fmaf(sum * scale, row_scale, bias);
+}
+
 __device__ __forceinline__ void store_y(const ProductArgs& a, uint32_t row, uint32_t n, int64_t sum, float scale) {
-    const double v = static_cast<double>(sum) * scale * a.scales[n] + (a.bias ? a.bias[n] : 0.0f);
+    const float v = value_of(static_cast<float>(static_cast<double>(sum)), a.scales[n], scale, a.bias ? a.bias[n] : 0.0f);
     const int64_t at = static_cast<int64_t>(row) * a.y_stride + n;
     if (a.y_type == LEO_TYPE_F32) static_cast<float*>(a.y)[at] = static_cast<float>(v);
     else if (a.y_type == LEO_TYPE_F16) static_cast<_Float16*>(a.y)[at] = static_cast<_Float16>(v);
@@ -189,7 +210,10 @@ constexpr uint32_t kHeldInputs = 16384;
 template <class X>
 __global__ __launch_bounds__(1024) void leo_q8_quantize_row(ProductArgs a) {
     __shared__ uint32_t most[16];
-    const uint32_t row = blockIdx.x, lane = threadIdx.x % 64, k = threadIdx.x * 16;
+    // Workgroups go to the XCDs in turn: the rows of a tile, which share lines, to one of them.
+    const uint32_t turn = blockIdx.x / 8, row = (turn / kTile * 8 + blockIdx.x % 8) * kTile + turn % kTile;
+    if (row >= a.rows) return;
+    const uint32_t lane = threadIdx.x % 64, k = threadIdx.x * 16;
     const Sixteen s = load_sixteen<X>(a, row, k);
     const uint32_t largest = wave_largest(largest_of(s));
     if (lane == 0) most[threadIdx.x / 64] = largest;
@@ -373,6 +397,167 @@ __global__ __launch_bounds__(kFewThreads) void leo_q8_many(ProductArgs a) {
     }
 }
 
+// Many rows: tiles of both operands go to LDS, in the order of their layouts, some
+// steps of 64 inputs ahead, and from there to registers one step ahead. The weights
+// are the A operand, so a lane gets four neighbouring outputs of one row.
+constexpr uint32_t kSlots = 4;  // steps in LDS
+
+// 16 bytes a lane from `from` + `offset` to 1,024 bytes of LDS. The instruction takes
+// no register, and nothing here waits for it: a step's waits are its own.
+__device__ __forceinline__ void load_to_lds(uint32_t lds, const char* from, uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(from) : "memory");
+}
+
+template <int kN, int kM, int kWavesN, int kWavesM>
+struct TileShape {
+    static constexpr int kWaves = kWavesN * kWavesM, kOutputs = kN * kWavesN, kRows = kM * kWavesM;  // in tiles of 16
+    static constexpr int kLoads = (kOutputs + kRows) / kWaves;  // of a wave and step
+    static constexpr uint32_t kSlotBytes = (kOutputs + kRows) * kBlockBytes;
+};
+
+template <int kN, int kM, int kWavesN, int kWavesM>
+__global__ __launch_bounds__(64 * kWavesN * kWavesM) void leo_q8_tiles(ProductArgs a, uint32_t across, uint32_t down) {
+    using Shape = TileShape<kN, kM, kWavesN, kWavesM>;
+    extern __shared__ __attribute__((aligned(16))) char slots[];
+    __shared__ float row_scales[Shape::kRows * kTile];
+    const uint32_t lane = threadIdx.x % 64, wave = wave_of_workgroup();
+    const uint32_t place = blockIdx.x;
+    const uint32_t tile_n = place % across * Shape::kOutputs, tile_m = place / across * Shape::kRows;
+    const uint32_t first = blockIdx.y * a.slice_blocks, last = min(first + a.slice_blocks, a.blocks) - 1;
+    const float scale_of_row = a.x_scales[min(tile_m * kTile + threadIdx.x, a.rows - 1)];
+    const char* from[Shape::kLoads];
+#pragma unroll
+    for (int j = 0; j < Shape::kLoads; ++j) {
+        const uint32_t f = wave * Shape::kLoads + j;
+        from[j] = f < Shape::kOutputs ? a.codes + static_cast<uint64_t>(min(tile_n + f, a.tiles - 1)) * a.blocks * kBlockBytes
+                                      : a.x_codes + static_cast<uint64_t>(min(tile_m + f - Shape::kOutputs, a.row_tiles - 1)) * a.blocks * kBlockBytes;
+    }
+    const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)slots));
+    const auto send = [&](uint32_t block, uint32_t slot) {
+        const uint32_t offset = min(block, last) * kBlockBytes + lane * 16;
+#pragma unroll
+        for (int j = 0; j < Shape::kLoads; ++j)
+            load_to_lds(base + slot * Shape::kSlotBytes + (wave * Shape::kLoads + j) * kBlockBytes, from[j], offset);
+    };
+    const uint32_t wave_n = wave % kWavesN * kN, wave_m = Shape::kOutputs + wave / kWavesN * kM;
+    const auto read = [&](int4v (&n)[kN], int4v (&m)[kM], uint32_t slot) {
+        const char* at = slots + slot * Shape::kSlotBytes + lane * 16;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) n[i] = *reinterpret_cast<const int4v*>(at + (wave_n + i) * kBlockBytes);
+#pragma unroll
+        for (int i = 0; i < kM; ++i) m[i] = *reinterpret_cast<const int4v*>(at + (wave_m + i) * kBlockBytes);
+    };
+    int4v sum[kN][kM];
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int m = 0; m < kM; ++m) sum[n][m] = int4v{0, 0, 0, 0};
+    const auto multiply = [&](const int4v (&n)[kN], const int4v (&m)[kM]) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+#pragma unroll
+            for (int j = 0; j < kM; ++j) sum[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(n[i], m[j], sum[i][j], 0, 0, 0);
+    };
+    // This wave's loads of all but the newest `kLeft` steps are done and its reads of
+    // LDS too; then those of all waves.
+    const auto arrive = [&](auto left) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(left)::value * Shape::kLoads) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    const auto step = [&](const int4v (&n)[kN], const int4v (&m)[kM], int4v (&next_n)[kN], int4v (&next_m)[kM], uint32_t block) {
+        const uint32_t slot = (block - first) % kSlots;
+        arrive(std::integral_constant<int, kSlots - 2>{});  // the next step has come, and nobody reads this one's slot any more
+        send(block + kSlots, slot);
+        __builtin_amdgcn_sched_barrier(0);
+        read(next_n, next_m, (slot + 1) % kSlots);
+        multiply(n, m);
+        // a read of LDS between the matrix instructions until all are on their way
+#pragma unroll
+        for (int i = 0; i < kN + kM; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, kN * kM / (kN + kM), 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (uint32_t s = 0; s < kSlots; ++s) send(first + s, s);
+    arrive(std::integral_constant<int, kSlots - 1>{});
+    int4v n0[kN], m0[kM], n1[kN], m1[kM];
+    read(n0, m0, 0);
+    uint32_t block = first;
+    for (; block + 1 <= last; block += 2) {
+        step(n0, m0, n1, m1, block);
+        step(n1, m1, n0, m0, block + 1);
+    }
+    if (block <= last) multiply(n0, m0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // LDS is another workgroup's after the end
+
+    if (threadIdx.x < Shape::kRows * kTile) row_scales[threadIdx.x] = scale_of_row;
+    const uint32_t n_of = (tile_n + wave_n) * kTile + lane / kTile * 4, m_of = (tile_m + wave_m - Shape::kOutputs) * kTile + lane % kTile;
+    if (a.slices > 1) {
+#pragma unroll
+        for (int j = 0; j < kM; ++j)
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                const uint32_t row = m_of + j * kTile, n = n_of + i * kTile;
+                if (row < a.rows && n < a.tiles * kTile)
+                    *reinterpret_cast<int4v*>(a.partials + (static_cast<uint64_t>(blockIdx.y) * a.rows + row) * a.tiles * kTile + n) = sum[i][j];
+            }
+        return;
+    }
+    // By way of LDS, each wave in a part of its own, so that rows leave in whole runs and the
+    // rounding stands in a loop: written out for all sums it was 100 KB of code, and most of
+    // a short product's time was spent fetching it.
+    __syncthreads();
+    constexpr uint32_t kQuads = kN * 4, kHalf = kM / 2 * kTile;  // fours of a row's outputs, rows at a time
+    int4v* held = reinterpret_cast<int4v*>(slots) + wave * (kQuads * kHalf);
+    const uint32_t quad = lane % kQuads, n = (tile_n + wave_n) * kTile + quad * 4;
+    float4v scales, bias;
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+        scales[e] = a.scales[min(n + e, a.outputs - 1)];
+        bias[e] = a.bias ? a.bias[min(n + e, a.outputs - 1)] : 0.0f;
+    }
+    const auto store = [&](auto type, uint32_t from) {
+        using Y = decltype(type);
+#pragma unroll 2
+        for (uint32_t r = lane / kQuads; r < kHalf; r += 64 / kQuads) {
+            const uint32_t of_tile = (wave_m - Shape::kOutputs) * kTile + from + r, row = tile_m * kTile + of_tile;
+            if (row >= a.rows) break;
+            const float scale = row_scales[of_tile];
+            const int4v whole = held[r * kQuads + (quad ^ (r % kQuads))];
+            typename Y::type four[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+                four[e] = static_cast<typename Y::type>(value_of(static_cast<float>(whole[e]), scales[e], scale, bias[e]));
+            auto* to = static_cast<typename Y::type*>(a.y) + static_cast<int64_t>(row) * a.y_stride + n;
+            if (n + 4 <= a.outputs) {
+                __builtin_memcpy(to, four, sizeof(four));  // rows need no alignment
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e)
+                    if (n + e < a.outputs) to[e] = four[e];
+            }
+        }
+    };
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int j = 0; j < kM / 2; ++j)
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                const uint32_t r = j * kTile + lane % kTile;
+                held[r * kQuads + ((i * 4 + lane / kTile) ^ (r % kQuads))] = sum[i][half * (kM / 2) + j];
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (a.y_type == LEO_TYPE_F32) store(F32{}, half * kHalf);
+        else if (a.y_type == LEO_TYPE_F16) store(F16{}, half * kHalf);
+        else store(BF16{}, half * kHalf);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+
 // The slices of one output by kShare threads.
 template <uint32_t kShare>
 __global__ __launch_bounds__(256) void leo_q8_join(ProductArgs a) {
@@ -396,7 +581,7 @@ __global__ __launch_bounds__(256) void leo_q8_join(ProductArgs a) {
 }
 
 struct Plan {
-    bool few;
+    bool few, tiles;
     uint32_t group_tiles;  // of a workgroup of leo_q8_few
     uint32_t slices, slice_blocks;
     uint32_t parts, part_inputs;
@@ -415,6 +600,9 @@ Plan plan_of(const LeoQ8Shape& s, uint64_t rows) {
         groups = (l.tiles + p.group_tiles - 1) / p.group_tiles;
         slices = whole ? 1 : std::max<uint64_t>(1, std::min<uint64_t>(512 / groups, (l.blocks + 7) / 8));
         slices = std::max(slices, (l.blocks * rows * kBlock + kFewStage - 1) / kFewStage);
+    } else if (rows >= 256 && l.tiles >= 16) {
+        p.tiles = true;
+        slices = 1;
     } else {
         groups = (l.tiles + kManyTiles - 1) / kManyTiles * ((row_tiles + kManyRows - 1) / kManyRows);
         slices = std::max<uint64_t>(1, std::min<uint64_t>(512 / groups, (l.blocks + 15) / 16));
@@ -448,7 +636,12 @@ void launch_product(const Plan& p, const ProductArgs& a, uint32_t* largest, hipS
     if (a.parts) launch(leo_q8_largest<X>, dim3(a.rows, a.parts), dim3(256), 0, stream, a, largest);
     if (p.few) return launch_few<X>(p, a, stream);
     if (a.parts) launch(leo_q8_quantize_part<X>, dim3(a.rows, a.parts), dim3(256), 0, stream, a);
-    else launch(leo_q8_quantize_row<X>, dim3(a.rows), dim3((a.inputs + 1023) / 1024 * 64), 0, stream, a);
+    else launch(leo_q8_quantize_row<X>, dim3((a.row_tiles + 7) / 8 * 8 * kTile), dim3((a.inputs + 1023) / 1024 * 64), 0, stream, a);
+    if (p.tiles) {
+        using Shape = TileShape<4, 8, 4, 2>;
+        const uint32_t across = (a.tiles + Shape::kOutputs - 1) / Shape::kOutputs, down = (a.row_tiles + Shape::kRows - 1) / Shape::kRows;
+        return launch(leo_q8_tiles<4, 8, 4, 2>, dim3(across * down, a.slices), dim3(64 * Shape::kWaves), kSlots * Shape::kSlotBytes, stream, a, across, down);
+    }
     launch(leo_q8_many, dim3((a.tiles + kManyTiles - 1) / kManyTiles, (a.row_tiles + kManyRows - 1) / kManyRows, a.slices), dim3(kFewThreads), 0, stream, a);
 }
 

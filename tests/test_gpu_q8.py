@@ -1,8 +1,9 @@
 """8-bit products on the GPU against the formula in whole numbers and 64 bits.
 
-The quantised rows, the sums of codes and the result in 64 bits are the formula's own, so
-a result is off by its type's rounding alone: half a step (one more 2^-50 of what it is
-summed from), or half of the type's smallest value."""
+The quantised rows and the sums of codes are the formula's own. A sum is rounded to float,
+so is its product with the output's scale, and the last product with the bias added: 2^-24
+each, two of the term and one of the result, which is no larger than the terms are together.
+Then half a step of the result's type, or half of its smallest value."""
 from __future__ import annotations
 
 import numpy as np
@@ -45,7 +46,7 @@ def check(got, x, codes, scales, bias):
     got, rounded = got.double(), want.to(dtype).double()
     fine = torch.isfinite(rounded) & ~nan
     assert torch.equal(got[~fine & ~nan], rounded[~fine & ~nan])
-    bound = want.abs() * (torch.finfo(dtype).eps / 2) + terms * 2.0 ** -50 + TINY[dtype] / 2
+    bound = want.abs() * (torch.finfo(dtype).eps / 2) + terms * (3.001 * 2.0 ** -24) + TINY[dtype] / 2
     off = ((got - want).abs() - bound)[fine]
     assert off.numel() == 0 or float(off.max()) <= 0, (float(off.max()), int(off.argmax()))
 
