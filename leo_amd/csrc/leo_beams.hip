@@ -148,13 +148,16 @@ struct Span {
     }
 };
 
-// What a span leaves for its row: its largest logit and the sum of exponentials
-// against it. Lanes' sums of 16 are floats, what joins them has 64 bits.
+// What a span, or a run of them, leaves for its row: its largest logit and the sum of
+// exponentials against it. Lanes' sums of 16 are floats, what joins them has 64 bits.
 struct SpanRecord {
     float top;
     uint32_t pad0;
     double mass;
 };
+__device__ __forceinline__ double against(const SpanRecord& r, float top) {
+    return r.top == top ? r.mass : r.top > negative_infinity() ? r.mass * exp_of(r.top - top) : 0.0;
+}
 template <class T>
 __device__ __forceinline__ SpanRecord weigh(const Span<T>& s, float lane_top) {
     const float top = wave_max(lane_top);
@@ -273,13 +276,13 @@ struct MergeShared {
     uint32_t count;
 };
 
-// A search's answer from its hypotheses' span records [beams][spans] and its lists of
-// candidates [beams][lists][kept], by a whole workgroup of 2^n waves. What it reads is on
+// A search's answer from its hypotheses' records and candidates, [beams][lists] and
+// [beams][lists][kept], by a whole workgroup of 2^n waves. What it reads is on
 // its way before anything is needed; the lists of finished hypotheses and of those with no
 // score hold anything, and count for nothing.
 constexpr uint32_t kAhead = 4;
-__device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const SpanRecord* records, uint32_t spans,
-                                      const uint64_t* candidates, uint32_t lists, MergeShared& shared) {
+__device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const SpanRecord* records, const uint64_t* candidates,
+                                      uint32_t lists, MergeShared& shared) {
     const uint64_t first = group * a.beams;
     const uint32_t thread = threadIdx.x, threads = blockDim.x, lane = thread % 64, wave = thread / 64, waves = threads / 64,
                    beams = static_cast<uint32_t>(a.beams), kept = static_cast<uint32_t>(a.kept), all = beams * lists;
@@ -289,7 +292,7 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const S
     for (uint32_t b = wave; b < beams; b += waves) {
         const uint64_t row = first + b;
         const SpanRecord none = {negative_infinity(), 0, 0.0};
-        const SpanRecord mine = lane < spans ? records[b * spans + lane] : none;
+        const SpanRecord mine = lane < lists ? records[b * lists + lane] : none;
         const float score = a.scores[row];
         const bool finished = is_finished(a, row);
         const int32_t length = a.lengths ? a.lengths[row] : 0;
@@ -299,14 +302,11 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const S
         if (h.kind == 2) {
             float top = mine.top;
 #pragma unroll 4
-            for (uint32_t i = lane + 64; i < spans; i += 64) top = fmaxf(top, records[b * spans + i].top);
+            for (uint32_t i = lane + 64; i < lists; i += 64) top = fmaxf(top, records[b * lists + i].top);
             top = wave_max(top);
-            const auto against = [&](const SpanRecord& r) {
-                return r.top == top ? r.mass : r.top > negative_infinity() ? r.mass * exp_of(r.top - top) : 0.0;
-            };
-            double mass = against(mine);
+            double mass = against(mine, top);
 #pragma unroll 4
-            for (uint32_t i = lane + 64; i < spans; i += 64) mass += against(records[b * spans + i]);
+            for (uint32_t i = lane + 64; i < lists; i += 64) mass += against(records[b * lists + i], top);
             h.log_mass = log(wave_sum(mass));
             h.top = top;
         }
@@ -460,33 +460,39 @@ __global__ __launch_bounds__(kMostWaves * 64) void leo_beam_whole(LeoBeams a, ui
         pick<T, true>(s, base, lane_top, kept, shared.pools[wave], kWavePool, counters[wave], nullptr, &candidates[0][0] + wave * kept);
     }
     __syncthreads();
-    merge(a, blockIdx.x, records, spans, &candidates[0][0], spans, shared.merge);
+    merge(a, blockIdx.x, records, &candidates[0][0], spans, shared.merge);
 }
 
-// Longer rows: a workgroup a run of spans, a wave each, which leave their records and
-// the run its best candidates; then a workgroup a search.
+// Longer rows: a workgroup a run of spans, a wave each, which leaves its record and its
+// best candidates; then a workgroup a search.
 constexpr uint32_t kRowPool = 1024;
 template <class T>
-__global__ __launch_bounds__(256) void leo_beam_rows(LeoBeams a, uint32_t spans, uint32_t lists, SpanRecord* records, uint64_t* candidates) {
+__global__ __launch_bounds__(256) void leo_beam_rows(LeoBeams a, uint32_t lists, SpanRecord* records, uint64_t* candidates) {
     __shared__ uint64_t pool[kRowPool];
     __shared__ uint32_t maxima[64], counters[2];
+    __shared__ SpanRecord parts[4];
     const uint64_t row = blockIdx.y;
     if (!is_open(a, row)) return;
-    const uint32_t span = blockIdx.x * (blockDim.x / 64) + threadIdx.x / 64;
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64, span = blockIdx.x * waves + wave;
     Span<T> s;
     s.load(a, row, span * kSpan);
     const float lane_top = s.top();
     const SpanRecord r = weigh(s, lane_top);
-    if (threadIdx.x % 64 == 0 && span < spans) records[row * spans + span] = r;
+    if (lane == 0) parts[wave] = r;
     pick<T, false>(s, span * kSpan, lane_top, static_cast<uint32_t>(a.kept), pool, kRowPool, counters, maxima,
                    candidates + (row * lists + blockIdx.x) * a.kept);
+    if (wave != 0) return;
+    const SpanRecord mine = lane < waves ? parts[lane] : SpanRecord{negative_infinity(), 0, 0.0};
+    const float top = wave_max(mine.top);
+    const double mass = wave_sum(against(mine, top));
+    if (lane == 0) records[row * lists + blockIdx.x] = {top, 0, top > negative_infinity() ? mass : 0.0};
 }
 
-__global__ __launch_bounds__(kMostWaves * 64) void leo_beam_groups(LeoBeams a, uint32_t spans, uint32_t lists, const SpanRecord* records,
+__global__ __launch_bounds__(kMostWaves * 64) void leo_beam_groups(LeoBeams a, uint32_t lists, const SpanRecord* records,
                                                                   const uint64_t* candidates) {
     __shared__ MergeShared shared;
     const uint64_t first = blockIdx.x * a.beams;
-    merge(a, blockIdx.x, records + first * spans, spans, candidates + first * lists * a.kept, lists, shared);
+    merge(a, blockIdx.x, records + first * lists, candidates + first * lists * a.kept, lists, shared);
 }
 
 struct BeamPlan {
@@ -512,7 +518,7 @@ BeamPlan beam_plan(uint64_t groups, uint64_t beams, uint64_t kept, uint64_t symb
     p.waves = std::min(power(p.spans), 4u);
     p.lists = (p.spans + p.waves - 1) / p.waves;
     p.merge_waves = power(std::max(beams, (beams * p.lists + 63) / 64));
-    p.candidates = (rows * p.spans * sizeof(SpanRecord) + 255) / 256 * 256;
+    p.candidates = (rows * p.lists * sizeof(SpanRecord) + 255) / 256 * 256;
     p.workspace = p.candidates + rows * p.lists * kept * sizeof(uint64_t);
     return p;
 }
@@ -533,9 +539,9 @@ void launch_beams(const BeamPlan& p, const LeoBeams& b, hipStream_t stream) {
     if (p.whole) return launch(leo_beam_whole<T>, groups, dim3(p.waves * 64), 0, stream, b, p.spans);
     auto* records = static_cast<SpanRecord*>(b.workspace);
     auto* candidates = reinterpret_cast<uint64_t*>(static_cast<char*>(b.workspace) + p.candidates);
-    launch(leo_beam_rows<T>, dim3(p.lists, static_cast<uint32_t>(b.groups * b.beams)), dim3(p.waves * 64), 0, stream, b, p.spans, p.lists,
-           records, candidates);
-    launch(leo_beam_groups, groups, dim3(p.merge_waves * 64), 0, stream, b, p.spans, p.lists, static_cast<const SpanRecord*>(records),
+    launch(leo_beam_rows<T>, dim3(p.lists, static_cast<uint32_t>(b.groups * b.beams)), dim3(p.waves * 64), 0, stream, b, p.lists, records,
+           candidates);
+    launch(leo_beam_groups, groups, dim3(p.merge_waves * 64), 0, stream, b, p.lists, static_cast<const SpanRecord*>(records),
            static_cast<const uint64_t*>(candidates));
 }
 
