@@ -193,10 +193,14 @@ __global__ __launch_bounds__(256) void leo_q8_largest(ProductArgs a, uint32_t* t
     if (threadIdx.x == 0) to[row * a.parts + blockIdx.y] = max(max(most[0], most[1]), max(most[2], most[3]));
 }
 
-constexpr uint32_t kMostParts = 64;
+constexpr uint32_t kMostParts = 256;
 __device__ __forceinline__ float scale_of_parts(const ProductArgs& a, uint32_t row) {  // by a whole wave
     const uint32_t lane = threadIdx.x % 64;
-    return scale_of(wave_largest(lane < a.parts ? a.largest[row * a.parts + lane] : 0u));
+    uint32_t largest = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kMostParts; i += 64)
+        if (i + lane < a.parts) largest = max(largest, a.largest[row * a.parts + i + lane]);
+    return scale_of(wave_largest(largest));
 }
 
 __device__ __forceinline__ uint4v* place_of(const ProductArgs& a, uint32_t row, uint32_t sixteen) {
@@ -334,7 +338,7 @@ __global__ __launch_bounds__(kFewThreads, 4) void leo_q8_few(ProductArgs a) {
 
 // More rows: 16 kRows rows and 16 kTiles outputs a workgroup, x and the weights
 // straight from their layouts to registers, the blocks of a slice shared by eight waves.
-constexpr int kManyRows = 4, kManyTiles = 2;
+template <int kManyRows, int kManyTiles>
 __global__ __launch_bounds__(kFewThreads) void leo_q8_many(ProductArgs a) {
     __shared__ int32_t sums[kManyRows * kManyTiles * 256];
     constexpr uint32_t kOperands = kManyRows + kManyTiles, kWide = kManyTiles * kTile;
@@ -416,7 +420,7 @@ struct TileShape {
 };
 
 template <int kN, int kM, int kWavesN, int kWavesM>
-__global__ __launch_bounds__(64 * kWavesN * kWavesM) void leo_q8_tiles(ProductArgs a, uint32_t across, uint32_t down) {
+__global__ __launch_bounds__(64 * kWavesN * kWavesM) void leo_q8_tiles(ProductArgs a, uint32_t across) {
     using Shape = TileShape<kN, kM, kWavesN, kWavesM>;
     extern __shared__ __attribute__((aligned(16))) char slots[];
     __shared__ float row_scales[Shape::kRows * kTile];
@@ -581,8 +585,10 @@ __global__ __launch_bounds__(256) void leo_q8_join(ProductArgs a) {
 }
 
 struct Plan {
-    bool few, tiles;
-    uint32_t group_tiles;  // of a workgroup of leo_q8_few
+    bool few;
+    uint32_t tiles;        // both sides of a workgroup of leo_q8_tiles, 0: none
+    uint32_t group_tiles;  // of a workgroup of leo_q8_few or leo_q8_many
+    uint32_t group_rows;   // in tiles, of a workgroup of leo_q8_many
     uint32_t slices, slice_blocks;
     uint32_t parts, part_inputs;
     uint64_t x_scales, largest, partials, workspace;  // offsets behind x's codes, and the whole
@@ -592,24 +598,39 @@ Plan plan_of(const LeoQ8Shape& s, uint64_t rows) {
     const uint64_t row_tiles = (rows + kTile - 1) / kTile;
     Plan p{};
     p.few = rows <= kTile;
-    uint64_t slices, groups;
+    uint64_t slices = 1;
+    const auto over = [](uint64_t v, uint64_t by) { return (v + by - 1) / by; };
     if (p.few) {
-        // All tiles in groups that differ little, or where there are enough of them smaller groups and whole rows.
-        const bool whole = l.tiles >= 128;
-        p.group_tiles = static_cast<uint32_t>(whole ? std::min<uint64_t>(8, (l.tiles + 511) / 512) : (l.tiles + (l.tiles + 7) / 8 - 1) / ((l.tiles + 7) / 8));
-        groups = (l.tiles + p.group_tiles - 1) / p.group_tiles;
-        slices = whole ? 1 : std::max<uint64_t>(1, std::min<uint64_t>(512 / groups, (l.blocks + 7) / 8));
-        slices = std::max(slices, (l.blocks * rows * kBlock + kFewStage - 1) / kFewStage);
-    } else if (rows >= 256 && l.tiles >= 16) {
-        p.tiles = true;
-        slices = 1;
+        // A workgroup a tile (or up to eight) over whole rows where that makes enough workgroups, or where rows are
+        // short: 8,192 -> 8,192 took 12.9 us with a tile each and 15.0 to 16.7 with more or in slices, 1,024 -> 257 3.3
+        // and 5.3. Else slices of 16 blocks, two a wave, and more where they would be over 512, for all tiles in groups
+        // that differ little: 8 rows of 131,072 -> 257 in 128 slices took 14.9 us, in 170 16.0, in 85 16.6.
+        const bool whole = l.tiles >= 128 || l.blocks <= 32;
+        p.group_tiles = static_cast<uint32_t>(whole ? std::min<uint64_t>(8, over(l.tiles, 512)) : over(l.tiles, over(l.tiles, 8)));
+        if (!whole) {
+            const uint64_t most = std::max<uint64_t>(1, 1024 / over(l.tiles, p.group_tiles));
+            slices = over(l.blocks, over(std::max<uint64_t>(16, over(l.blocks, most)), 8) * 8);
+        }
+        slices = std::max(slices, over(l.blocks * rows * kBlock, kFewStage));
+    } else if (row_tiles <= 8 || l.tiles < 8) {
+        // 64 rows of 8,192 -> 8,192 took 20.6 us with 512 workgroups of one tile and 23.0 with 256 of two, of 5,001 ->
+        // 11,007 20.3 with 688 and 18.9 with 344; 128 rows, each tile read twice, 24 with four tiles and 29 with two.
+        p.group_rows = row_tiles <= 2 ? 2 : 4;
+        p.group_tiles = row_tiles > 4 ? 4 : l.tiles > 600 ? 2 : 1;
+        const uint64_t groups = over(l.tiles, p.group_tiles) * over(row_tiles, p.group_rows);
+        slices = std::max<uint64_t>(1, std::min<uint64_t>(512 / groups, over(l.blocks, 16)));
     } else {
-        groups = (l.tiles + kManyTiles - 1) / kManyTiles * ((row_tiles + kManyRows - 1) / kManyRows);
-        slices = std::max<uint64_t>(1, std::min<uint64_t>(512 / groups, (l.blocks + 15) / 16));
+        // A CU has one workgroup of the larger tile, or two of the smaller, and those two together do half as much: the
+        // larger where it takes fewer rounds. 1,536 rows of 4,096 -> 4,096 took 52 us with the larger and 46 with the
+        // smaller, 1,024 of 8,192 -> 8,192 89 and 87, 2,048 117 with the larger. A few of them share the inputs: 256
+        // rows of 8,192 -> 8,192 took 48 us in one slice, 41 in two, 45 in four.
+        const uint64_t large = over(l.tiles, 16) * over(row_tiles, 16), small = over(l.tiles, 8) * over(row_tiles, 8);
+        p.tiles = over(small, 512) > over(large, 256) ? 16 : 8;
+        slices = p.tiles == 16 ? 1 : std::max<uint64_t>(1, std::min<uint64_t>(256 / small, l.blocks / 16));
     }
-    slices = std::max(slices, (l.blocks + kMostSliceBlocks - 1) / kMostSliceBlocks);
-    p.slice_blocks = static_cast<uint32_t>((l.blocks + slices - 1) / slices);
-    p.slices = static_cast<uint32_t>((l.blocks + p.slice_blocks - 1) / p.slice_blocks);
+    slices = std::max<uint64_t>(slices, over(l.blocks, kMostSliceBlocks));
+    p.slice_blocks = static_cast<uint32_t>(over(l.blocks, slices));
+    p.slices = static_cast<uint32_t>(over(l.blocks, p.slice_blocks));
     if (p.few ? rows * s.inputs > 16384 : s.inputs > kHeldInputs) {
         const uint64_t want = std::max<uint64_t>(4096, (s.inputs + kMostParts - 1) / kMostParts);
         p.part_inputs = static_cast<uint32_t>((want + 15) / 16 * 16);
@@ -631,18 +652,25 @@ void launch_few(const Plan& p, const ProductArgs& a, hipStream_t stream) {
     launch(kKernels[p.group_tiles - 1], grid, dim3(kFewThreads), lds, stream, a);
 }
 
+template <int kN, int kM, int kWavesN, int kWavesM>
+void launch_tiles(const ProductArgs& a, hipStream_t stream) {
+    using Shape = TileShape<kN, kM, kWavesN, kWavesM>;
+    const uint32_t across = (a.tiles + Shape::kOutputs - 1) / Shape::kOutputs, down = (a.row_tiles + Shape::kRows - 1) / Shape::kRows;
+    launch(leo_q8_tiles<kN, kM, kWavesN, kWavesM>, dim3(across * down, a.slices), dim3(64 * Shape::kWaves), kSlots * Shape::kSlotBytes, stream, a, across);
+}
+
 template <class X>
 void launch_product(const Plan& p, const ProductArgs& a, uint32_t* largest, hipStream_t stream) {
     if (a.parts) launch(leo_q8_largest<X>, dim3(a.rows, a.parts), dim3(256), 0, stream, a, largest);
     if (p.few) return launch_few<X>(p, a, stream);
     if (a.parts) launch(leo_q8_quantize_part<X>, dim3(a.rows, a.parts), dim3(256), 0, stream, a);
     else launch(leo_q8_quantize_row<X>, dim3((a.row_tiles + 7) / 8 * 8 * kTile), dim3((a.inputs + 1023) / 1024 * 64), 0, stream, a);
-    if (p.tiles) {
-        using Shape = TileShape<4, 8, 4, 2>;
-        const uint32_t across = (a.tiles + Shape::kOutputs - 1) / Shape::kOutputs, down = (a.row_tiles + Shape::kRows - 1) / Shape::kRows;
-        return launch(leo_q8_tiles<4, 8, 4, 2>, dim3(across * down, a.slices), dim3(64 * Shape::kWaves), kSlots * Shape::kSlotBytes, stream, a, across, down);
-    }
-    launch(leo_q8_many, dim3((a.tiles + kManyTiles - 1) / kManyTiles, (a.row_tiles + kManyRows - 1) / kManyRows, a.slices), dim3(kFewThreads), 0, stream, a);
+    if (p.tiles == 16) return launch_tiles<4, 8, 4, 2>(a, stream);
+    if (p.tiles == 8) return launch_tiles<4, 4, 2, 2>(a, stream);
+    static constexpr void (*kKernels[2][3])(ProductArgs) = {{leo_q8_many<2, 1>, leo_q8_many<2, 2>, leo_q8_many<2, 4>},
+                                                            {leo_q8_many<4, 1>, leo_q8_many<4, 2>, leo_q8_many<4, 4>}};
+    const auto many = kKernels[p.group_rows / 4][p.group_tiles / 2];
+    launch(many, dim3((a.tiles + p.group_tiles - 1) / p.group_tiles, (a.row_tiles + p.group_rows - 1) / p.group_rows, a.slices), dim3(kFewThreads), 0, stream, a);
 }
 
 }  // namespace
@@ -706,7 +734,7 @@ int32_t leo_q8_matmul(const LeoQ8Product* product, void* stream) {
         require(reinterpret_cast<uintptr_t>(p.layout) % 256 == 0, "leo_q8_matmul: layout must be 256-byte aligned");
         const Q8Layout l = layout_of(p.shape);
         require(p.layout_bytes >= l.bytes, "leo_q8_matmul: layout is too small for its shape");
-        require((p.shape.outputs + 31) / 32 * p.rows <= 0x7fffffffu, "leo_q8_matmul: the result is too large");
+        require((p.shape.outputs + 7) / 8 * p.rows <= 0x7fffffffu, "leo_q8_matmul: the result is too large");
         const Plan plan = plan_of(p.shape, p.rows);
         require(plan.workspace == 0 || (p.workspace && reinterpret_cast<uintptr_t>(p.workspace) % 256 == 0 &&
                                         p.workspace_bytes >= plan.workspace),
@@ -740,9 +768,10 @@ int32_t leo_q8_matmul(const LeoQ8Product* product, void* stream) {
         else if (p.x_type == LEO_TYPE_F16) launch_product<F16>(plan, a, largest, at);
         else launch_product<BF16>(plan, a, largest, at);
         if (plan.slices == 1) return;
-        const bool share = plan.slices >= 16;
-        const uint64_t count = (p.shape.outputs + (share ? 31 : 255)) / (share ? 32 : 256) * p.rows;
-        launch(share ? leo_q8_join<8> : leo_q8_join<1>, dim3(static_cast<uint32_t>(count)), dim3(256), 0, at, a);
+        // 340 slices took 1.5 us less with 32 threads an output than with 8, 128 0.4 less with 16
+        const uint32_t share = plan.slices >= 256 ? 32 : plan.slices >= 16 ? 16 : 1;
+        const uint64_t count = (p.shape.outputs + 256 / share - 1) / (256 / share) * p.rows;
+        launch(share == 32 ? leo_q8_join<32> : share == 16 ? leo_q8_join<16> : leo_q8_join<1>, dim3(static_cast<uint32_t>(count)), dim3(256), 0, at, a);
     });
 }
 
