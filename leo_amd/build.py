@@ -77,7 +77,7 @@ def build_binding() -> pathlib.Path:
     _run([os.environ.get("CXX", "g++"), *CXX_FLAGS, "-shared",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
           *(f"-isystem{path}" for path in (*include_paths(), sysconfig.get_paths()["include"])),
-          CSRC / "decode_binding.cpp", "-o", tmp, f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10",
+          CSRC / "decode_binding.cpp", "-o", tmp, f"-L{lib}", "-ltorch_python", "-ltorch_hip", "-ltorch_cpu", "-lc10",
           f"-L{LIB_DIR}", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"])
     os.replace(tmp, BINDING)
     return BINDING

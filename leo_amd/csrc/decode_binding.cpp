@@ -8,7 +8,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -104,8 +104,13 @@ void* stream_of(int index) {
     return p;
 }
 
+// A new dense tensor, without the dispatch that torch.empty goes through first.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+    return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
+
 at::Tensor workspace(uint64_t bytes, const at::Tensor& like) {  // free again in the stream's order
-    return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+    return fresh({static_cast<int64_t>(bytes)}, at::kByte, like);
 }
 
 template <class F>
@@ -165,7 +170,7 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t n) {
             static constexpr at::ScalarType kTypes[] = {at::kFloat, at::kHalf, at::kBFloat16};
             const long type = PyLong_AsLong(args[4]);
             if (type < -1 || type > 2) refuse("the result must be float32, float16 or bfloat16");
-            out = at::empty({x.rows, outputs}, type < 0 ? input.options() : input.options().dtype(kTypes[type]));
+            out = fresh({x.rows, outputs}, type < 0 ? input.scalar_type() : kTypes[type], input);
         } else {
             out = tensor(args[4], "out");
         }
@@ -202,7 +207,7 @@ PyObject* control_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const at::Tensor& logits = tensor(args[0], "logits");
         const int index = logits.get_device();
         const Matrix z = matrix(logits, "logits", index, kFloating);
-        at::Tensor out = args[11] == Py_None ? at::empty({z.rows, z.width}, logits.options()) : tensor(args[11], "out");
+        at::Tensor out = args[11] == Py_None ? fresh({z.rows, z.width}, logits.scalar_type(), logits) : tensor(args[11], "out");
         const Matrix to = matrix(out, "out", index, static_cast<int>(logits.scalar_type()));
         if (to.rows != z.rows || to.width != z.width)
             refuse("out must be (" + std::to_string(z.rows) + ", " + std::to_string(z.width) + ")");
@@ -274,8 +279,8 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t n) {
         s.top_p = vector<float>(args[4], "top_p", at::kFloat, index, z.rows);
         s.min_p = vector<float>(args[5], "min_p", at::kFloat, index, z.rows);
         const c10::DeviceGuard guard(logits.device());
-        at::Tensor drawn = at::empty({z.rows}, logits.options().dtype(at::kInt));
-        at::Tensor logprobs = at::empty({z.rows}, logits.options().dtype(at::kFloat));
+        at::Tensor drawn = fresh({z.rows}, at::kInt, logits);
+        at::Tensor logprobs = fresh({z.rows}, at::kFloat, logits);
         s.out_symbols = static_cast<int32_t*>(drawn.data_ptr());
         s.out_logprobs = static_cast<float*>(logprobs.data_ptr());
         check(leo_sample_workspace_bytes(s.rows, s.symbols, &s.workspace_bytes));
@@ -348,7 +353,7 @@ PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
         check(leo_beam_workspace_bytes(b.groups, b.beams, b.kept, b.symbols, &b.workspace_bytes));
         at::Tensor outs[5];
         const auto out = [&](int i, at::ScalarType type) {
-            outs[i] = at::empty({groups, kept}, logits.options().dtype(type));
+            outs[i] = fresh({groups, kept}, type, logits);
             return outs[i].data_ptr();
         };
         b.out_symbols = static_cast<int32_t*>(out(0, at::kInt));
@@ -434,7 +439,7 @@ PyObject* reorder_states(PyObject*, PyObject* const* args, Py_ssize_t n) {
             std::vector<int64_t> sizes(t.sizes().begin(), t.sizes().end());
             sizes[0] = groups * kept;
             if (args[2] == Py_None) {
-                outs.push_back(at::empty(sizes, t.options()));
+                outs.push_back(fresh(sizes, t.scalar_type(), t));
             } else {
                 const at::Tensor& out = tensor(PyTuple_GET_ITEM(args[2], i), "out");
                 same_device(out, "out", index);
