@@ -547,9 +547,11 @@ void launch_beams(const BeamPlan& p, const LeoBeams& b, hipStream_t stream) {
 
 // --- reordering ------------------------------------------------------------------------------------------------------
 
-// One workgroup 16 bytes a thread of one place of a row, for all of a search's
-// targets: in place a thread holds what it moves in a column of LDS that is its
-// own, so nothing waits for other threads.
+// A thread takes 16 bytes of a place of its search's rows, for all of their targets, so a
+// row that several hypotheses continue comes from memory once. Memory bounds it. Stores
+// start at multiples of 16, loads at multiples of 4: the bytes that a row's place lies off
+// those are shifted in registers. In place a thread writes nothing but the columns that it
+// alone reads, the same in every row, and holds what it moves in LDS that is its own.
 constexpr uint32_t kArrays = 32;
 
 struct ReorderArgs {
@@ -560,44 +562,85 @@ struct ReorderArgs {
     const int32_t* parents;
 };
 
+// 16 bytes from any address, by way of the five words that hold them.
+__device__ __forceinline__ uint4v load_shifted(const char* p) {
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 3u;
+    const char* words = p - off;
+    uint4v v = load_16(__builtin_assume_aligned(words, 4));
+    if (__any(off != 0)) {
+        // where off is 0, the last word again: the next one may be another's
+        const uint32_t next = *reinterpret_cast<const uint32_t*>(words + (off ? 16 : 12));
+        v = uint4v{__builtin_amdgcn_alignbyte(v[1], v[0], off), __builtin_amdgcn_alignbyte(v[2], v[1], off),
+                   __builtin_amdgcn_alignbyte(v[3], v[2], off), __builtin_amdgcn_alignbyte(next, v[3], off)};
+    }
+    return v;
+}
+
+// Columns of 16 bytes that a place of `width` bytes may touch, whatever it starts at.
+__host__ __device__ inline uint64_t columns_of(uint64_t width, bool in_place) { return (width + (in_place ? 15 : 30)) / 16; }
+
 template <bool kInPlace>
 __global__ __launch_bounds__(256) void leo_reorder(ReorderArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint4v held[];
     uint32_t which = 0;
     while (which + 1 < a.count && blockIdx.x >= a.before[which + 1]) ++which;
     const LeoStateArray& s = a.arrays[which];
-    const uint64_t unit = blockIdx.x - a.before[which], wide = blockDim.x * 16, pieces = (s.width + wide - 1) / wide;
-    const uint64_t piece = unit % pieces, outer = unit / pieces % s.outer, group = unit / pieces / s.outer;
-    const uint64_t at = piece * wide + threadIdx.x * 16;
-    if (at >= s.width) return;
-    const uint32_t bytes = static_cast<uint32_t>(min<uint64_t>(16, s.width - at));
-    const char* source = static_cast<const char*>(s.source) + outer * s.source_outer + at;
-    char* target = static_cast<char*>(s.target) + outer * s.target_outer + at;
+    const uint64_t columns = columns_of(s.width, kInPlace), all = columns * s.outer, units = (all + blockDim.x - 1) / blockDim.x;
+    const uint64_t unit = blockIdx.x - a.before[which], group = unit / units, column = unit % units * blockDim.x + threadIdx.x;
+    if (column >= all) return;
+    uint64_t outer = 0;
+    if (s.outer > 1) outer = all >> 32 ? column / columns : static_cast<uint32_t>(column) / static_cast<uint32_t>(columns);
+    const int64_t place = static_cast<int64_t>(column - outer * columns) * 16, width = static_cast<int64_t>(s.width);
+    const char* source = static_cast<const char*>(s.source) + outer * s.source_outer;
+    char* target = static_cast<char*>(s.target) + outer * s.target_outer;
     const int32_t* parents = a.parents + group * a.kept;
+    const auto row_of = [&](uint32_t k) { return target + static_cast<int64_t>(group * a.kept + k) * s.target_row; };
+    const auto start = [&](uint32_t k) {
+        return kInPlace ? place : place - static_cast<int64_t>(reinterpret_cast<uintptr_t>(row_of(k)) & 15u);
+    };
     const auto read = [&](uint32_t k) {
         const int32_t parent = parents[k];
+        const int64_t at = start(k);
         uint4v v = {0, 0, 0, 0};
         if (parent < 0 || parent >= static_cast<int32_t>(a.beams)) return v;
         const char* from = source + static_cast<int64_t>(group * a.beams + parent) * s.source_row;
-        if (bytes == 16) return load_16(from);
-        for (uint32_t i = 0; i < bytes; ++i) v[i / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(from[i])) << (8 * (i % 4));
+        if (at >= 0 && at + 16 <= width) {
+            v = load_shifted(from + at);
+        } else {
+            for (int32_t i = 0; i < 16; ++i)
+                if (at + i >= 0 && at + i < width) v[i / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(from[at + i])) << (8 * (i % 4));
+        }
         return v;
     };
     const auto write = [&](uint32_t k, const uint4v& v) {
-        char* to = target + static_cast<int64_t>(group * a.kept + k) * s.target_row;
-        if (bytes == 16) {
-            __builtin_memcpy(to, &v, 16);
-            return;
+        const int64_t at = start(k);
+        char* to = row_of(k);
+        if (at >= 0 && at + 16 <= width) {
+            // past the caches, which keep what is read: 64 rows of 8 x 511 x 64 16-bit values took 107 us without and 66 so
+            if constexpr (kInPlace) __builtin_memcpy(to + at, &v, 16);
+            else __builtin_nontemporal_store(v, reinterpret_cast<uint4v*>(to + at));
+        } else {
+            for (int32_t i = 0; i < 16; ++i)
+                if (at + i >= 0 && at + i < width) to[at + i] = static_cast<char>(v[i / 4] >> (8 * (i % 4)));
         }
-        for (uint32_t i = 0; i < bytes; ++i) to[i] = static_cast<char>(v[i / 4] >> (8 * (i % 4)));
     };
+    const auto moves = [&](uint32_t k) { return k < a.kept && (!kInPlace || parents[k] != static_cast<int32_t>(k)); };
+    constexpr uint32_t kTogether = 4;  // loads on their way; eight took registers, and 89 us for 80 of 8 planes of 8 rows of 4 MB
+    for (uint32_t k = 0; k < a.kept; k += kTogether) {
+        uint4v v[kTogether];
+#pragma unroll
+        for (uint32_t j = 0; j < kTogether; ++j)
+            if (moves(k + j)) v[j] = read(k + j);
+#pragma unroll
+        for (uint32_t j = 0; j < kTogether; ++j) {
+            if (!moves(k + j)) continue;
+            if (kInPlace) held[(k + j) * blockDim.x + threadIdx.x] = v[j];
+            else write(k + j, v[j]);
+        }
+    }
     if constexpr (kInPlace) {
         for (uint32_t k = 0; k < a.kept; ++k)
-            if (parents[k] != static_cast<int32_t>(k)) held[k * blockDim.x + threadIdx.x] = read(k);
-        for (uint32_t k = 0; k < a.kept; ++k)
-            if (parents[k] != static_cast<int32_t>(k)) write(k, held[k * blockDim.x + threadIdx.x]);
-    } else {
-        for (uint32_t k = 0; k < a.kept; ++k) write(k, read(k));
+            if (moves(k)) write(k, held[k * blockDim.x + threadIdx.x]);
     }
 }
 
@@ -745,8 +788,8 @@ int32_t leo_reorder_states(const LeoReorder* reorder, void* stream) {
             extents.push_back({to, to + span(to_rows, s.target_row, s.target_outer), i, true});
         }
         check_apart(r, extents);
-        // in place, the rows of a piece are held in LDS: 64 KB
-        const uint32_t threads = r.kept <= 16 ? 256 : 64;
+        // in place, the rows of a column are held in LDS: 64 KB
+        const uint32_t threads = r.kept <= 16 ? 256 : r.kept <= 32 ? 128 : 64;
         ReorderArgs a{};
         a.groups = static_cast<uint32_t>(r.groups);
         a.beams = static_cast<uint32_t>(r.beams);
@@ -758,7 +801,7 @@ int32_t leo_reorder_states(const LeoReorder* reorder, void* stream) {
                 a.count = 0;
                 for (; from < order[in_place].size() && a.count < kArrays; ++from) {
                     const LeoStateArray& s = r.arrays[order[in_place][from]];
-                    const unsigned __int128 mine = static_cast<unsigned __int128>((s.width + threads * 16 - 1) / (threads * 16)) * s.outer * r.groups;
+                    const unsigned __int128 mine = (static_cast<unsigned __int128>(columns_of(s.width, in_place)) * s.outer + threads - 1) / threads * r.groups;
                     require(mine <= 0x7fffffffu, "leo_reorder_states: an array is too large");
                     if (units + static_cast<uint64_t>(mine) > 0x7fffffffu) break;
                     a.arrays[a.count] = s;
