@@ -320,15 +320,15 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const S
     if (thread == 0) shared.count = 0;
     __syncthreads();
     const auto score_of = [&](const Hypothesis& h, uint64_t key) {
-        if (h.kind == 1) return h.score;
         const float z = logit_of(key);
-        return h.score + ((z == h.top ? 0.0 : static_cast<double>(z) - h.top) - h.log_mass);
+        const double below = static_cast<double>(z) - h.top, grown = h.score + ((z == h.top ? 0.0 : below) - h.log_mass);
+        return h.kind == 1 ? h.score : grown;
     };
     // rank 0 is none
     const auto ranked = [&](uint32_t list, uint32_t place, uint64_t key) -> Ranked {
         const uint32_t beam = list / lists;
         const Hypothesis& h = shared.hypotheses[beam];
-        if (h.kind == 1) key = place == 0 && list % lists == 0 ? 1 : 0;
+        key = h.kind != 1 ? key : place == 0 && list == beam * lists ? 1 : 0;
         const double score = score_of(h, key);
         const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(score * h.inverse + 0.0));
         const bool none = h.kind == 0 || key == 0 || !(score > -__builtin_inf());

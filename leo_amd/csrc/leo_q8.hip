@@ -267,7 +267,11 @@ __global__ __launch_bounds__(kFewThreads, 4) void leo_q8_few(ProductArgs a) {
                 to[u][t] = reinterpret_cast<const int4v*>(weights[t] + static_cast<uint64_t>(min(block + u, end - 1)) * kBlockBytes)[lane];
     };
     int4v even[kAhead][kTiles], odd[kAhead][kTiles];
-    fetch(even, begin);  // on their way while x is prepared
+    const uint32_t each_row = count * 4, sixteens = a.rows * each_row;
+    const auto load_staged = [&](uint32_t i) { return load_sixteen<X>(a, i / each_row, (first * 4 + i % each_row) * 16); };
+    Sixteen ahead;
+    if (threadIdx.x < sixteens) ahead = load_staged(threadIdx.x);
+    fetch(even, begin);  // on their way while x is prepared, and behind it
     for (uint32_t i = threadIdx.x; i < kTiles * 256; i += kFewThreads) sums[i] = 0;
 
     if (a.parts) {
@@ -290,9 +294,9 @@ __global__ __launch_bounds__(kFewThreads, 4) void leo_q8_few(ProductArgs a) {
         }
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < a.rows * count * 4; i += kFewThreads) {
-        const uint32_t row = i / (count * 4), sixteen = i % (count * 4);
-        staged[sixteen * a.rows + row] = codes_of(load_sixteen<X>(a, row, (first * 4 + sixteen) * 16), scales[row]);
+    for (uint32_t i = threadIdx.x; i < sixteens; i += kFewThreads) {
+        const uint32_t row = i / each_row, sixteen = i % each_row;
+        staged[sixteen * a.rows + row] = codes_of(i == threadIdx.x ? ahead : load_staged(i), scales[row]);
     }
     if (a.slices > 1 && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < a.rows) a.x_scales[threadIdx.x] = scales[threadIdx.x];
     __syncthreads();
@@ -597,7 +601,11 @@ Plan plan_of(const LeoQ8Shape& s, uint64_t rows) {
     const Q8Layout l = layout_of(s);
     const uint64_t row_tiles = (rows + kTile - 1) / kTile;
     Plan p{};
-    p.few = rows <= kTile;
+    const bool whole = l.tiles >= 128 || l.blocks <= 32;
+    // Where every workgroup would bring whole rows to 8 bits by itself, only as long as those are short: 2, 4 and 8 rows of
+    // 8,192 -> 8,192 took 15.4, 20.2 and 30.7 us so and 16.2 to 16.3 with rows brought to 8 bits before, 4 and 8 rows of
+    // 4,096 -> 2,048 7.7 and 11.3 against 9.0 and 9.1.
+    p.few = rows <= kTile && (!whole || rows * s.inputs <= 24576);
     uint64_t slices = 1;
     const auto over = [](uint64_t v, uint64_t by) { return (v + by - 1) / by; };
     if (p.few) {
@@ -605,7 +613,6 @@ Plan plan_of(const LeoQ8Shape& s, uint64_t rows) {
         // short: 8,192 -> 8,192 took 12.9 us with a tile each and 15.0 to 16.7 with more or in slices, 1,024 -> 257 3.3
         // and 5.3. Else slices of 16 blocks, two a wave, and more where they would be over 512, for all tiles in groups
         // that differ little: 8 rows of 131,072 -> 257 in 128 slices took 14.9 us, in 170 16.0, in 85 16.6.
-        const bool whole = l.tiles >= 128 || l.blocks <= 32;
         p.group_tiles = static_cast<uint32_t>(whole ? std::min<uint64_t>(8, over(l.tiles, 512)) : over(l.tiles, over(l.tiles, 8)));
         if (!whole) {
             const uint64_t most = std::max<uint64_t>(1, 1024 / over(l.tiles, p.group_tiles));
@@ -615,10 +622,10 @@ Plan plan_of(const LeoQ8Shape& s, uint64_t rows) {
     } else if (row_tiles <= 8 || l.tiles < 8) {
         // 64 rows of 8,192 -> 8,192 took 20.6 us with 512 workgroups of one tile and 23.0 with 256 of two, of 5,001 ->
         // 11,007 20.3 with 688 and 18.9 with 344; 128 rows, each tile read twice, 24 with four tiles and 29 with two.
-        p.group_rows = row_tiles <= 2 ? 2 : 4;
+        p.group_rows = row_tiles <= 2 ? static_cast<uint32_t>(row_tiles) : 4;
         p.group_tiles = row_tiles > 4 ? 4 : l.tiles > 600 ? 2 : 1;
         const uint64_t groups = over(l.tiles, p.group_tiles) * over(row_tiles, p.group_rows);
-        slices = std::max<uint64_t>(1, std::min<uint64_t>(512 / groups, over(l.blocks, 16)));
+        slices = l.blocks <= 64 ? 1 : std::max<uint64_t>(1, std::min<uint64_t>(512 / groups, over(l.blocks, 16)));
     } else {
         // A CU has one workgroup of the larger tile, or two of the smaller, and those two together do half as much: the
         // larger where it takes fewer rounds. 1,536 rows of 4,096 -> 4,096 took 52 us with the larger and 46 with the
@@ -667,9 +674,10 @@ void launch_product(const Plan& p, const ProductArgs& a, uint32_t* largest, hipS
     else launch(leo_q8_quantize_row<X>, dim3((a.row_tiles + 7) / 8 * 8 * kTile), dim3((a.inputs + 1023) / 1024 * 64), 0, stream, a);
     if (p.tiles == 16) return launch_tiles<4, 8, 4, 2>(a, stream);
     if (p.tiles == 8) return launch_tiles<4, 4, 2, 2>(a, stream);
-    static constexpr void (*kKernels[2][3])(ProductArgs) = {{leo_q8_many<2, 1>, leo_q8_many<2, 2>, leo_q8_many<2, 4>},
+    static constexpr void (*kKernels[3][3])(ProductArgs) = {{leo_q8_many<1, 1>, leo_q8_many<1, 2>, leo_q8_many<1, 4>},
+                                                            {leo_q8_many<2, 1>, leo_q8_many<2, 2>, leo_q8_many<2, 4>},
                                                             {leo_q8_many<4, 1>, leo_q8_many<4, 2>, leo_q8_many<4, 4>}};
-    const auto many = kKernels[p.group_rows / 4][p.group_tiles / 2];
+    const auto many = kKernels[p.group_rows / 2][p.group_tiles / 2];
     launch(many, dim3((a.tiles + p.group_tiles - 1) / p.group_tiles, (a.row_tiles + p.group_rows - 1) / p.group_rows, a.slices), dim3(kFewThreads), 0, stream, a);
 }
 

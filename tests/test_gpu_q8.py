@@ -62,7 +62,7 @@ def make(seed, rows, inputs, outputs, dtype, scale_dtype, spread=1.0):
 
 SIZES = [(1, 1, 1), (1, 15, 16), (2, 16, 17), (15, 17, 15), (16, 63, 257), (17, 64, 31), (1, 1024, 257), (31, 65, 33),
          (33, 127, 100), (64, 129, 257), (65, 257, 48), (130, 500, 257), (4, 5001, 1030), (300, 1000, 130), (257, 2049, 513),
-         (8, 20_001, 257), (1, 40_000, 3), (512, 640, 768), (1, 8192, 2048), (48, 4097, 700)]
+         (8, 20_001, 257), (1, 40_000, 3), (2, 9000, 2050), (7, 4097, 2100), (16, 3000, 9700), (16, 2048, 257), (140, 300, 20), (200, 1025, 400), (512, 640, 768), (1, 8192, 2048), (48, 4097, 700)]
 
 
 @pytest.mark.parametrize("rows, inputs, outputs", SIZES)
