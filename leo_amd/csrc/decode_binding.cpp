@@ -7,15 +7,16 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/core/DimVector.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/util/SmallVector.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
 #include <string>
-#include <vector>
 
 #include "leo_decode.h"
 #include "leo_hip.h"
@@ -423,8 +424,8 @@ PyObject* reorder_states(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int64_t groups = order.size(0), kept = order.size(1);
         if (kept < 1 || kept > 64) refuse("parents have 1 to 64 places a row, not " + std::to_string(kept));
         const c10::DeviceGuard guard(order.device());
-        std::vector<at::Tensor> outs;
-        std::vector<LeoStateArray> arrays;
+        c10::SmallVector<at::Tensor, 16> outs;
+        c10::SmallVector<LeoStateArray, 16> arrays;
         int64_t beams = 0;
         for (Py_ssize_t i = 0; i < count; ++i) {
             const at::Tensor& t = tensor(PyTuple_GET_ITEM(args[0], i), "a state");
@@ -436,7 +437,7 @@ PyObject* reorder_states(PyObject*, PyObject* const* args, Py_ssize_t n) {
                        (i ? " of " + std::to_string(beams) + " beams" : ""));
             if (groups == 0 && t.size(0)) refuse("a state has rows, the parents none");
             beams = groups ? t.size(0) / groups : 1;
-            std::vector<int64_t> sizes(t.sizes().begin(), t.sizes().end());
+            at::DimVector sizes(t.sizes());
             sizes[0] = groups * kept;
             if (args[2] == Py_None) {
                 outs.push_back(fresh(sizes, t.scalar_type(), t));

@@ -281,24 +281,34 @@ struct MergeShared {
 // its way before anything is needed; the lists of finished hypotheses and of those with no
 // score hold anything, and count for nothing.
 constexpr uint32_t kAhead = 4;
-__device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const SpanRecord* records, const uint64_t* candidates,
-                                      uint32_t lists, MergeShared& shared) {
+struct Given {
+    float score;
+    bool finished;
+    int32_t length;
+};
+__device__ __forceinline__ Given given_of(const LeoBeams& a, uint64_t row) {
+    return {a.scores[row], is_finished(a, row), a.lengths ? a.lengths[row] : 0};
+}
+// `mine_given` is what is given for the hypothesis of this thread's wave.
+__device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const Given& mine_given, const SpanRecord* records,
+                                      const uint64_t* candidates, uint32_t lists, MergeShared& shared) {
     const uint64_t first = group * a.beams;
     const uint32_t thread = threadIdx.x, threads = blockDim.x, lane = thread % 64, wave = thread / 64, waves = threads / 64,
                    beams = static_cast<uint32_t>(a.beams), kept = static_cast<uint32_t>(a.kept), all = beams * lists;
-    uint64_t ahead[kAhead];  // of this thread's first list
+    // A thread's first list, so that neighbouring lists fall to different groups of the bar's: where a search begins, one
+    // hypothesis has all that counts.
+    const uint32_t own = thread % waves * 64 + thread / waves;
+    uint64_t ahead[kAhead];
 #pragma unroll
-    for (uint32_t p = 0; p < kAhead; ++p) ahead[p] = thread < all && p < kept ? candidates[static_cast<uint64_t>(thread) * kept + p] : 0;
+    for (uint32_t p = 0; p < kAhead; ++p) ahead[p] = own < all && p < kept ? candidates[static_cast<uint64_t>(own) * kept + p] : 0;
     for (uint32_t b = wave; b < beams; b += waves) {
         const uint64_t row = first + b;
         const SpanRecord none = {negative_infinity(), 0, 0.0};
         const SpanRecord mine = lane < lists ? records[b * lists + lane] : none;
-        const float score = a.scores[row];
-        const bool finished = is_finished(a, row);
-        const int32_t length = a.lengths ? a.lengths[row] : 0;
+        const Given given = b == wave ? mine_given : given_of(a, row);
         Hypothesis h{};
-        h.score = score;
-        h.kind = !(score > negative_infinity()) ? 0 : finished ? 1 : 2;
+        h.score = given.score;
+        h.kind = !(given.score > negative_infinity()) ? 0 : given.finished ? 1 : 2;
         if (h.kind == 2) {
             float top = mine.top;
 #pragma unroll 4
@@ -312,7 +322,7 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const S
         }
         h.inverse = 1.0;
         if (a.length_penalty != 0.0) {
-            const int64_t grown = static_cast<int64_t>(length) + (h.kind == 1 ? 0 : 1);
+            const int64_t grown = static_cast<int64_t>(given.length) + (h.kind == 1 ? 0 : 1);
             h.inverse = 1.0 / pow(static_cast<double>(grown < 1 ? 1 : grown), a.length_penalty);
         }
         if (lane == 0) shared.hypotheses[b] = h;
@@ -359,12 +369,12 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const S
     uint32_t largest = 0;
     if (all >= kept) {
         // the lists' best bound what can be kept, and each list is followed down to the bar
-        for (uint32_t list = thread; list < all; list += threads)
-            largest = max(largest, static_cast<uint32_t>((list == thread ? ranked(list, 0, ahead[0]) : load_ranked(list, 0)).rank >> 32));
+        for (uint32_t list = own; list < all; list += threads)
+            largest = max(largest, static_cast<uint32_t>((list == own ? ranked(list, 0, ahead[0]) : load_ranked(list, 0)).rank >> 32));
         const uint32_t bar = max(bar_of<false>(largest, kept, shared.maxima), 1u);
         for (uint32_t from = 0; from < all; from += threads) {
             if (!__any(largest >= bar)) break;
-            const uint32_t list = from + thread;
+            const uint32_t list = from + own;
             bool more = true;
             if (from == 0) {  // one addition for what the lists' first places hold, which is mostly all
                 Ranked r[kAhead];
@@ -451,6 +461,7 @@ __global__ __launch_bounds__(kMostWaves * 64) void leo_beam_whole(LeoBeams a, ui
     __shared__ uint32_t counters[kMostWaves][2];
     const uint32_t wave = threadIdx.x / 64, beam = wave / spans, base = wave % spans * kSpan, kept = static_cast<uint32_t>(a.kept);
     const uint64_t row = blockIdx.x * a.beams + beam;
+    const Given given = given_of(a, blockIdx.x * a.beams + min(static_cast<uint64_t>(wave), a.beams - 1));
     if (beam < a.beams) {
         Span<T> s;
         s.load(a, row, base);  // also where nothing comes of it: sooner than after asking
@@ -460,7 +471,7 @@ __global__ __launch_bounds__(kMostWaves * 64) void leo_beam_whole(LeoBeams a, ui
         pick<T, true>(s, base, lane_top, kept, shared.pools[wave], kWavePool, counters[wave], nullptr, &candidates[0][0] + wave * kept);
     }
     __syncthreads();
-    merge(a, blockIdx.x, records, &candidates[0][0], spans, shared.merge);
+    merge(a, blockIdx.x, given, records, &candidates[0][0], spans, shared.merge);
 }
 
 // Longer rows: a workgroup a run of spans, a wave each, which leaves its record and its
@@ -492,7 +503,8 @@ __global__ __launch_bounds__(kMostWaves * 64) void leo_beam_groups(LeoBeams a, u
                                                                   const uint64_t* candidates) {
     __shared__ MergeShared shared;
     const uint64_t first = blockIdx.x * a.beams;
-    merge(a, blockIdx.x, records + first * lists, candidates + first * lists * a.kept, lists, shared);
+    const Given given = given_of(a, first + min(static_cast<uint64_t>(threadIdx.x / 64), a.beams - 1));
+    merge(a, blockIdx.x, given, records + first * lists, candidates + first * lists * a.kept, lists, shared);
 }
 
 struct BeamPlan {
@@ -556,7 +568,9 @@ constexpr uint32_t kArrays = 32;
 
 struct ReorderArgs {
     LeoStateArray arrays[kArrays];
-    uint64_t before[kArrays];  // workgroups of the arrays before
+    uint32_t columns[kArrays];  // of 16 bytes, of a place
+    uint32_t units[kArrays];    // workgroups of a search
+    uint32_t before[kArrays];   // workgroups of the arrays before
     uint32_t count;
     uint32_t groups, beams, kept;
     const int32_t* parents;
@@ -576,20 +590,17 @@ __device__ __forceinline__ uint4v load_shifted(const char* p) {
     return v;
 }
 
-// Columns of 16 bytes that a place of `width` bytes may touch, whatever it starts at.
-__host__ __device__ inline uint64_t columns_of(uint64_t width, bool in_place) { return (width + (in_place ? 15 : 30)) / 16; }
-
 template <bool kInPlace>
 __global__ __launch_bounds__(256) void leo_reorder(ReorderArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint4v held[];
     uint32_t which = 0;
     while (which + 1 < a.count && blockIdx.x >= a.before[which + 1]) ++which;
     const LeoStateArray& s = a.arrays[which];
-    const uint64_t columns = columns_of(s.width, kInPlace), all = columns * s.outer, units = (all + blockDim.x - 1) / blockDim.x;
-    const uint64_t unit = blockIdx.x - a.before[which], group = unit / units, column = unit % units * blockDim.x + threadIdx.x;
+    const uint32_t columns = a.columns[which], units = a.units[which], unit = blockIdx.x - a.before[which];
+    const uint64_t group = unit / units, all = columns * s.outer, column = static_cast<uint64_t>(unit % units) * blockDim.x + threadIdx.x;
     if (column >= all) return;
     uint64_t outer = 0;
-    if (s.outer > 1) outer = all >> 32 ? column / columns : static_cast<uint32_t>(column) / static_cast<uint32_t>(columns);
+    if (s.outer > 1) outer = all >> 32 ? column / columns : static_cast<uint32_t>(column) / columns;
     const int64_t place = static_cast<int64_t>(column - outer * columns) * 16, width = static_cast<int64_t>(s.width);
     const char* source = static_cast<const char*>(s.source) + outer * s.source_outer;
     char* target = static_cast<char*>(s.target) + outer * s.target_outer;
@@ -607,8 +618,12 @@ __global__ __launch_bounds__(256) void leo_reorder(ReorderArgs a) {
         if (at >= 0 && at + 16 <= width) {
             v = load_shifted(from + at);
         } else {
-            for (int32_t i = 0; i < 16; ++i)
-                if (at + i >= 0 && at + i < width) v[i / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(from[at + i])) << (8 * (i % 4));
+            // the bytes beyond an end are its own again, so that all are on their way at once
+            uint8_t bytes[16];
+#pragma unroll
+            for (int32_t i = 0; i < 16; ++i) bytes[i] = static_cast<uint8_t>(from[at + i < 0 ? 0 : at + i < width ? at + i : width - 1]);
+#pragma unroll
+            for (int32_t i = 0; i < 16; ++i) v[i / 4] |= static_cast<uint32_t>(bytes[i]) << (8 * (i % 4));
         }
         return v;
     };
@@ -620,6 +635,7 @@ __global__ __launch_bounds__(256) void leo_reorder(ReorderArgs a) {
             if constexpr (kInPlace) __builtin_memcpy(to + at, &v, 16);
             else __builtin_nontemporal_store(v, reinterpret_cast<uint4v*>(to + at));
         } else {
+#pragma unroll
             for (int32_t i = 0; i < 16; ++i)
                 if (at + i >= 0 && at + i < width) to[at + i] = static_cast<char>(v[i / 4] >> (8 * (i % 4)));
         }
@@ -767,7 +783,7 @@ int32_t leo_reorder_states(const LeoReorder* reorder, void* stream) {
             const LeoStateArray& s = r.arrays[i];
             if (s.outer == 0 || s.width == 0) continue;
             require(s.source && s.target, "leo_reorder_states: null array");
-            require(s.outer <= 0x7fffffffu && s.width <= kMost, "leo_reorder_states: an array is too large");
+            require(s.outer <= 0x7fffffffu && s.width <= 1ull << 32, "leo_reorder_states: an array is too large");
             for (int64_t stride : {s.source_row, s.source_outer, s.target_row, s.target_outer})
                 require(stride >= 0 && static_cast<uint64_t>(stride) <= kMost, "leo_reorder_states: strides must be 0 .. 2^46");
             const auto span = [&](uint64_t rows, int64_t row, int64_t outer) {
@@ -801,12 +817,16 @@ int32_t leo_reorder_states(const LeoReorder* reorder, void* stream) {
                 a.count = 0;
                 for (; from < order[in_place].size() && a.count < kArrays; ++from) {
                     const LeoStateArray& s = r.arrays[order[in_place][from]];
-                    const unsigned __int128 mine = (static_cast<unsigned __int128>(columns_of(s.width, in_place)) * s.outer + threads - 1) / threads * r.groups;
-                    require(mine <= 0x7fffffffu, "leo_reorder_states: an array is too large");
-                    if (units + static_cast<uint64_t>(mine) > 0x7fffffffu) break;
+                    // a place that starts anywhere may touch one column more
+                    const bool aligned = (reinterpret_cast<uintptr_t>(s.target) | s.target_row | s.target_outer) % 16 == 0;
+                    const uint64_t columns = (s.width + (in_place || aligned ? 15 : 30)) / 16, mine = (columns * s.outer + threads - 1) / threads;
+                    require(mine * r.groups <= 0x7fffffffu, "leo_reorder_states: an array is too large");
+                    if (units + mine * r.groups > 0x7fffffffu) break;
                     a.arrays[a.count] = s;
-                    a.before[a.count++] = units;
-                    units += static_cast<uint64_t>(mine);
+                    a.columns[a.count] = static_cast<uint32_t>(columns);
+                    a.units[a.count] = static_cast<uint32_t>(mine);
+                    a.before[a.count++] = static_cast<uint32_t>(units);
+                    units += mine * r.groups;
                 }
                 const auto at = static_cast<hipStream_t>(stream);
                 const dim3 grid(static_cast<uint32_t>(units)), block(threads);

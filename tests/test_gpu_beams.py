@@ -254,6 +254,35 @@ def test_streams_and_graphs(require_gpu):
         compare(*cases[0], 8, end=1)
 
 
+def test_two_streams_at_once(require_gpu):
+    cases = [make(7, 2, 4, 257, torch.float32)[:2], make(8, 1, 8, 50_001, torch.bfloat16)[:2], make(9, 3, 2, 9000, torch.float16)[:2]]
+    want = [decode.beam_select(z, s, 8) for z, s in cases]
+    torch.cuda.synchronize()
+    streams, found = [torch.cuda.Stream() for _ in range(3)], []
+    for turn in range(6):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                which = (turn + i) % 3
+                found.append((decode.beam_select(*cases[which], 8), want[which]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for a, b in found for x, y in zip(a[:3], b[:3]))
+
+
+def test_results_and_workspaces_are_freed(require_gpu):
+    z, scores, _ = make(6, 2, 8, 20_001, torch.bfloat16)
+    parents = torch.zeros(2, 8, dtype=torch.int32, device=DEVICE)
+    before = torch.cuda.memory_allocated()
+    for _ in range(10):
+        found = decode.beam_select(z, scores, 16, end=1)
+        decode.reorder_states([z, scores.view(16, 1)], found.parents)
+        del found
+        for call in (lambda: decode.beam_select(z, scores[:1]), lambda: decode.reorder_states([z, scores], parents),
+                     lambda: decode.reorder_states([z], parents, out=[scores])):
+            with pytest.raises(native.LeoError):
+                call()
+    assert torch.cuda.memory_allocated() == before
+
+
 def test_refusals(require_gpu):
     z, scores, _ = make(9, 2, 3, 50, torch.float32)
     flags, lengths = torch.zeros(2, 3, dtype=torch.bool, device=DEVICE), torch.ones(2, 3, dtype=torch.int32, device=DEVICE)

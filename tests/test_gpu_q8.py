@@ -77,7 +77,7 @@ def test_sizes_and_types(require_gpu, rows, inputs, outputs, dtype):
         check(decode.q8_matmul(x[:1], weight, bias, out_dtype=to), x[:1], codes, scales, bias)
 
 
-@pytest.mark.parametrize("rows", [1, 3, 20, 100])
+@pytest.mark.parametrize("rows", [1, 3, 20, 100, 150])
 @pytest.mark.parametrize("inputs, outputs", [(300, 70), (4100, 257)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_strides_and_alignment(require_gpu, rows, inputs, outputs, dtype):
@@ -147,6 +147,47 @@ def test_codes_next_to_a_half(require_gpu, scale):
     check(got, rows, codes, unit, None)
     q, units = quantized(rows.double())
     assert torch.equal((got[:, 0].double() / units).round(), q[:, 1])
+
+
+@pytest.mark.parametrize("rows, inputs, outputs", [(2048, 300, 8300), (130, 131_200, 130), (700, 64, 2500), (129, 1, 128)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_tiles(require_gpu, rows, inputs, outputs, dtype):
+    x, codes, scales, bias = make(rows, rows, inputs, outputs, TYPES[dtype], torch.float32)
+    buffer = torch.full((rows, outputs + 5), 7.0, device=DEVICE, dtype=TYPES[dtype])
+    got = decode.q8_matmul(x, decode.Q8Weight(codes, scales), bias, out=buffer[:, 3:3 + outputs])
+    check(got, x, codes, scales, bias)
+    assert bool((buffer[:, :3] == 7).all()) and bool((buffer[:, 3 + outputs:] == 7).all())
+
+
+def test_two_streams_at_once(require_gpu):
+    cases = []
+    for rows, inputs, outputs in ((1, 200_000, 257), (40, 9000, 900), (600, 1500, 700), (8, 70_000, 257)):
+        x, codes, scales, bias = make(rows, rows, inputs, outputs, torch.bfloat16, torch.float32)
+        weight = decode.Q8Weight(codes, scales)
+        cases.append((x, weight, bias, decode.q8_matmul(x, weight, bias, out_dtype=torch.float32)))
+    torch.cuda.synchronize()
+    streams, found = [torch.cuda.Stream() for _ in range(3)], []
+    for turn in range(6):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                x, weight, bias, want = cases[(turn + i) % len(cases)]
+                found.append((decode.q8_matmul(x, weight, bias, out_dtype=torch.float32), want))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in found)
+
+
+def test_results_and_workspaces_are_freed(require_gpu):
+    weight = decode.Q8Weight.quantize(torch.randn(257, 70_000, device=DEVICE))
+    few, many = torch.randn(5, 70_000, device=DEVICE), torch.randn(40, 70_000, device=DEVICE)
+    wrong = torch.zeros(3, 5, device=DEVICE)
+    before = torch.cuda.memory_allocated()
+    for _ in range(10):
+        decode.q8_matmul(few, weight)
+        decode.q8_matmul(many, weight)
+        for call in (lambda: decode.q8_matmul(wrong, weight), lambda: decode.q8_matmul(few, weight, out=wrong)):
+            with pytest.raises(native.LeoError):
+                call()
+    assert torch.cuda.memory_allocated() == before
 
 
 def test_cancelling_sums_are_exact(require_gpu):
