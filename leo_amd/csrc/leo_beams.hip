@@ -276,6 +276,10 @@ struct MergeShared {
     uint32_t count;
 };
 
+// Where lists are four times as many as what is kept, the best of each say enough. With 16
+// of 16 the least of them would be the bar, and a step of 16 beams of 1,000 took 18.5 us.
+__host__ __device__ inline bool follows_lists(uint32_t all, uint32_t kept) { return all >= 4 * kept; }
+
 // A search's answer from its hypotheses' records and candidates, [beams][lists] and
 // [beams][lists][kept], by a whole workgroup of 2^n waves. What it reads is on
 // its way before anything is needed; the lists of finished hypotheses and of those with no
@@ -367,7 +371,7 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
     };
     const Ranked nothing = {0, 0};
     uint32_t largest = 0;
-    if (all >= kept) {
+    if (follows_lists(all, kept)) {
         // the lists' best bound what can be kept, and each list is followed down to the bar
         for (uint32_t list = own; list < all; list += threads)
             largest = max(largest, static_cast<uint32_t>((list == own ? ranked(list, 0, ahead[0]) : load_ranked(list, 0)).rank >> 32));
@@ -399,12 +403,17 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
             for (uint32_t p = from == 0 ? kAhead : 0; more && p < kept; ++p) more = gather(list < all ? load_ranked(list, p) : nothing, bar);
         }
     } else {
-        // few lists: all their candidates, fewer than 64 * 64
+        // few lists: all their candidates
         const uint32_t items = all * kept;
         const auto item = [&](uint32_t i) { return i < items ? load_ranked(i % all, i / all) : nothing; };
-        for (uint32_t i = thread; i < items; i += threads) largest = max(largest, static_cast<uint32_t>(item(i).rank >> 32));
+        const Ranked one = item(own);
+        largest = static_cast<uint32_t>(one.rank >> 32);
+        for (uint32_t i = own + threads; i < items; i += threads) largest = max(largest, static_cast<uint32_t>(item(i).rank >> 32));
         const uint32_t bar = max(bar_of<false>(largest, kept, shared.maxima), 1u);
-        for (uint32_t from = 0; from < items; from += threads) gather(item(from + thread), bar);
+        for (uint32_t from = 0; from < items; from += threads) {
+            if (!__any(largest >= bar)) break;
+            gather(from == 0 ? one : item(from + own), bar);
+        }
     }
     __syncthreads();
     const uint32_t count = shared.count;
@@ -448,7 +457,7 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
 
 // Searches whose rows make up to 16 spans take one workgroup each: a wave a span,
 // which picks from its registers, then the search's answer.
-constexpr uint32_t kMostWaves = 16, kWavePool = 192;
+constexpr uint32_t kMostWaves = 16, kWavePool = 320;
 template <class T>
 __global__ __launch_bounds__(kMostWaves * 64) void leo_beam_whole(LeoBeams a, uint32_t spans) {
     union Shared {
@@ -522,14 +531,17 @@ BeamPlan beam_plan(uint64_t groups, uint64_t beams, uint64_t kept, uint64_t symb
         return v;
     };
     p.spans = static_cast<uint32_t>((symbols + kSpan - 1) / kSpan);
-    p.whole = beams * p.spans <= kMostWaves;
+    // One launch took 6.4 us for the two's 8.1 for 4 beams of 257, 9.7 for 11.4 for 256 searches of 8 beams of 2,000, but
+    // 8.7 for 8.1 for 4 beams of 4,000, whose rows one workgroup each answers with fewer lists.
+    p.whole = beams * p.spans <= kMostWaves && p.spans <= 2;
     if (p.whole) {
         p.waves = power(beams * p.spans);
         return p;
     }
     p.waves = std::min(power(p.spans), 4u);
     p.lists = (p.spans + p.waves - 1) / p.waves;
-    p.merge_waves = power(std::max(beams, (beams * p.lists + 63) / 64));
+    const uint64_t all = beams * p.lists;
+    p.merge_waves = power(std::max(beams, ((follows_lists(static_cast<uint32_t>(all), static_cast<uint32_t>(kept)) ? all : all * kept) + 63) / 64));
     p.candidates = (rows * p.lists * sizeof(SpanRecord) + 255) / 256 * 256;
     p.workspace = p.candidates + rows * p.lists * kept * sizeof(uint64_t);
     return p;
