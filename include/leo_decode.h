@@ -218,7 +218,7 @@ int32_t leo_q8_matmul(const LeoQ8Product* product, void* stream);
  * hypothesis, scores [groups, beams] the sums of log probabilities so far, -inf where
  * there is none (NaN counts as -inf). Candidates:
  *     symbol v after hypothesis b:  score + z[v] - log sum exp z  (those above -inf)
- *     a finished hypothesis itself:  its score; its logits are not read
+ *     a finished hypothesis itself:  its score; its logits do not count
  * and the `kept` (at most 64, as are the beams) with the largest score / length^length_penalty
  * are taken, largest first; of equals the lower hypothesis, the larger logit, the
  * lower symbol. length counts the symbol that comes in: lengths[b] + 1, lengths[b]
@@ -230,7 +230,8 @@ int32_t leo_q8_matmul(const LeoQ8Product* product, void* stream);
  * finished (bytes, 0 or not) may be NULL: none is. out_finished (may be NULL) is 1
  * for finished ones and where the symbol is `end` (-1: no symbol ends), else 0;
  * out_lengths (may be NULL, needs lengths) the lengths, hypothesis 0's at places that
- * no candidate takes. Outputs have [groups, kept] entries. `workspace` as in leo_q4_matvec. */
+ * no candidate takes. Outputs have [groups, kept] entries and share no memory with
+ * inputs or each other. `workspace` as in leo_q4_matvec. */
 typedef struct LeoBeams {
     uint64_t groups;
     uint64_t beams;
@@ -260,8 +261,9 @@ int32_t leo_beam_select(const LeoBeams* beams, void* stream);
  * becomes row g * beams + parents[g, k] of the source, zeros where the parent is
  * outside 0 .. beams-1. A row is `outer` pieces of `width` bytes; strides are
  * bytes, not negative. An array may be its own target (same address and strides,
- * kept = beams); otherwise no target shares memory with any source or other target,
- * which arrays that interleave have to show by common divisors of their strides.
+ * kept = beams); otherwise no target shares memory with the parents, any source or
+ * other target, which arrays that interleave have to show by common divisors of their
+ * strides.
  * `arrays` is host memory, read during the call. */
 typedef struct LeoStateArray {
     const void* source;

@@ -98,6 +98,20 @@ __device__ __forceinline__ uint32_t wave_min(uint32_t v) {
     return wave_reduce(v, 0xffffffffu, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
 }
 
+// The same for all of a wave's lanes, so what follows from it is scalar.
+__device__ __forceinline__ uint32_t wave_of_workgroup() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64); }
+
+__device__ __forceinline__ float negative_infinity() { return -__builtin_inff(); }
+
+// A float's bits in the order of its value.
+__device__ __forceinline__ uint32_t order_key(float v) {
+    const uint32_t b = __float_as_uint(v);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float from_order_key(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
 // 16 bytes from any address: rows need no alignment.
 __device__ __forceinline__ uint4v load_16(const void* p) {
     uint4v v;

@@ -6,8 +6,6 @@
 namespace leo {
 namespace {
 
-__device__ __forceinline__ float negative_infinity() { return -__builtin_inff(); }
-
 // Entries [begin, end) of a ragged list's row, held inside the list whatever
 // the offsets say.
 struct Run {
@@ -137,15 +135,6 @@ __global__ __launch_bounds__(kControlThreads, 8) void leo_control_rows(LeoLogitC
             T::store(out, from + i, bits_of(from + i) & 1u ? z : negative_infinity());
         }
     }
-}
-
-// A float's bits in the order of its value.
-__device__ __forceinline__ uint32_t order_key(float v) {
-    const uint32_t b = __float_as_uint(v);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float from_order_key(uint32_t k) {
-    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
 // --- the draw ---------------------------------------------------------------

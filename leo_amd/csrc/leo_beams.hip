@@ -11,17 +11,6 @@ namespace {
 
 constexpr uint32_t kMostBeams = 64;
 
-__device__ __forceinline__ float negative_infinity() { return -__builtin_inff(); }
-
-// Floats in the order of whole numbers, -inf above 0.
-__device__ __forceinline__ uint32_t order_key(float z) {
-    const uint32_t b = __float_as_uint(z);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float from_order_key(uint32_t k) {
-    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
-}
-
 // A symbol of a row as one number: the larger logit first, of equals the lower
 // symbol. 0 is none.
 __device__ __forceinline__ uint64_t candidate(float z, uint32_t at) {
@@ -772,6 +761,21 @@ int32_t leo_beam_select(const LeoBeams* beams, void* stream) {
         require(std::isfinite(b.length_penalty), "leo_beam_select: length_penalty must be finite");
         require(b.lengths || (b.length_penalty == 0.0 && !b.out_lengths), "leo_beam_select: length_penalty or out_lengths without lengths");
         require(b.end >= -1 && b.end < static_cast<int64_t>(b.symbols), "leo_beam_select: end must be a symbol, or -1");
+        struct Range {
+            uintptr_t begin, end;
+        };
+        const auto range = [](const void* at, uint64_t bytes) {
+            const uintptr_t begin = reinterpret_cast<uintptr_t>(at);
+            return Range{begin, at ? begin + bytes : begin};
+        };
+        const uint64_t rows = b.groups * b.beams, places = b.groups * b.kept;
+        const Range logits = range(b.logits, ((rows - 1) * static_cast<uint64_t>(b.logits_stride) + b.symbols) * type_bytes(b.type));
+        const Range all[] = {range(b.out_symbols, places * 4), range(b.out_parents, places * 4), range(b.out_scores, places * 4),
+                             range(b.out_finished, places), range(b.out_lengths, places * 4), logits, range(b.scores, rows * 4),
+                             range(b.finished, rows), range(b.lengths, rows * 4)};
+        for (int out = 0; out < 5; ++out)
+            for (int other = out + 1; other < 9; ++other)
+                require(all[out].end <= all[other].begin || all[other].end <= all[out].begin, "leo_beam_select: outputs overlap inputs or each other");
         const BeamPlan p = beam_plan(b.groups, b.beams, b.kept, b.symbols);
         require(p.workspace == 0 || (b.workspace && reinterpret_cast<uintptr_t>(b.workspace) % 256 == 0 && b.workspace_bytes >= p.workspace),
                 "leo_beam_select: workspace is missing, too small or not 256-byte aligned");
@@ -817,6 +821,9 @@ int32_t leo_reorder_states(const LeoReorder* reorder, void* stream) {
                         "leo_reorder_states: an array that is its own target needs the same strides and as many kept as beams");
             order[same].push_back(i);
             const uintptr_t from = reinterpret_cast<uintptr_t>(s.source), to = reinterpret_cast<uintptr_t>(s.target);
+            const uintptr_t listed = reinterpret_cast<uintptr_t>(r.parents);
+            require(listed >= to + span(to_rows, s.target_row, s.target_outer) || listed + to_rows * sizeof(int32_t) <= to,
+                    "leo_reorder_states: a target overlaps the parents");
             if (!same) extents.push_back({from, from + span(from_rows, s.source_row, s.source_outer), i, false});
             extents.push_back({to, to + span(to_rows, s.target_row, s.target_outer), i, true});
         }

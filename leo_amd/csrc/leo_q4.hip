@@ -115,9 +115,6 @@ typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 
-// The same for all of a wave's lanes, so what follows from it is scalar.
-__device__ __forceinline__ uint32_t wave_of_workgroup() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64); }
-
 struct TileArgs {
     const char* codes;
     const char* scales;

@@ -92,7 +92,6 @@ struct ProductArgs {
     int32_t* partials;            // [slice][row][16 tiles]
 };
 
-__device__ __forceinline__ uint32_t wave_of_workgroup() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64); }
 __device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
     return wave_reduce(v, 0u, [](uint32_t p, uint32_t q) { return p > q ? p : q; });
 }

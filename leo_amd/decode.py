@@ -323,7 +323,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, kept: Optional[int] 
     at most.
 
     A hypothesis continues with symbol v at scores + z[v] - log sum exp z, a finished
-    one stays as it is and its logits are not read. The order is that of score /
+    one stays as it is and its logits do not count. The order is that of score /
     length^length_penalty, with the length that the hypothesis then has; of equals
     the lower hypothesis comes first, then the larger logit, then the lower symbol.
     Ranks have 64 bits. Logits of -inf or NaN are no way on, nor are hypotheses whose
@@ -351,7 +351,8 @@ def reorder_states(states: Union[torch.Tensor, Sequence[torch.Tensor]], parents:
              dense: a cache's filled part of each head, cache[:, :, :length], does
     out      tensors for the results. The states themselves, where kept is beams: then
              only rows that move are read and written. Otherwise they share no memory
-             with the states or each other; tensors that interleave have common strides
+             with the parents, the states or each other; tensors that interleave have common
+             strides
     """
     one = isinstance(states, torch.Tensor)
     if one:

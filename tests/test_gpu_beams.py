@@ -213,6 +213,38 @@ def test_special_values(require_gpu, symbols):
         compare(z, scores, kept, finished, torch.full((10, 2), 7, device=DEVICE, dtype=torch.int32), 1.0, 2)
 
 
+@pytest.mark.parametrize("dtype, bits, quiet, signalling", [(torch.float32, torch.int32, 0x7fc00000, 0x7f800001),
+                                                            (torch.bfloat16, torch.int16, 0x7fc0, 0x7f81),
+                                                            (torch.float16, torch.int16, 0x7e00, 0x7c01)])
+@pytest.mark.parametrize("symbols", [100, 5000])
+def test_every_nan_is_no_way_on(require_gpu, dtype, bits, quiet, signalling, symbols):
+    z, scores, _ = make(11, 1, 3, symbols, dtype)
+    z = z.contiguous()
+    raw = z.view(bits)
+    raw[0, ::3] = quiet
+    raw[1, ::2] = signalling
+    raw[2, 1::5] = signalling
+    raw[2, 2::5] = quiet - (1 << 15) if bits is torch.int16 else quiet - (1 << 31)      # with the sign set
+    compare(z, scores, 8)
+
+
+@pytest.mark.parametrize("beams, symbols, kept", [(1, 5_000_003, 7), (2, 8_400_000, 64)])
+def test_very_long_rows(require_gpu, beams, symbols, kept):
+    gen = torch.Generator(DEVICE).manual_seed(symbols)
+    z = torch.randn(beams, symbols, generator=gen, device=DEVICE).clamp_(max=5)
+    at = torch.randint(0, symbols, (beams, kept), generator=gen, device=DEVICE)
+    top = 20 - 0.125 * torch.arange(beams * kept, device=DEVICE).view(kept, beams).t()      # hypotheses in turn
+    z.scatter_(1, at, top)
+    assert all(len(set(row)) == kept for row in at.tolist())
+    lse = torch.logsumexp(z.double(), dim=1)
+    scores = lse.float()[None]      # ranks are the logits, as far as floats go
+    got = decode.beam_select(z, scores, kept)
+    ranks = (z.double().gather(1, at) - lse[:, None] + scores.double().t()).t().reshape(-1)
+    assert got.parents[0].tolist() == [k % beams for k in range(kept)]
+    assert got.symbols[0].tolist() == at.t().reshape(-1)[:kept].tolist()
+    assert float((got.scores[0].double() - ranks[:kept]).abs().max()) <= 25 * 2.0 ** -24 + 2.0 ** -21
+
+
 def test_lengths(require_gpu):
     z, scores, _ = make(4, 3, 4, 100, torch.float32)
     lengths = torch.tensor([[0, 1, 2, 3], [-5, 2**31 - 2, 0, 10], [2**31 - 2, 1, 1, 1]], device=DEVICE, dtype=torch.int32)

@@ -73,15 +73,20 @@ def test_bad_products_are_refused():
 
 
 def test_bad_selections_are_refused():
-    good = dict(groups=2, beams=3, kept=3, symbols=40_000, logits=256, logits_stride=40_000, type=native.TYPE_F32, scores=256,
-                out_symbols=256, out_parents=256, out_scores=256, end=-1, workspace=1 << 20, workspace_bytes=1 << 20)
+    good = dict(groups=2, beams=3, kept=3, symbols=40_000, logits=1 << 24, logits_stride=40_000, type=native.TYPE_F32,
+                scores=256, out_symbols=512, out_parents=768, out_scores=1024, end=-1, workspace=1 << 20,
+                workspace_bytes=1 << 20)
     for change in (dict(beams=0), dict(beams=65), dict(kept=0), dict(kept=65), dict(symbols=0), dict(symbols=(1 << 26) + 1),
                    dict(groups=1 << 20), dict(type=4), dict(logits=None), dict(scores=None), dict(out_symbols=None),
                    dict(out_parents=None), dict(out_scores=None), dict(logits_stride=-1), dict(length_penalty=0.5),
-                   dict(lengths=256, length_penalty=float("nan")), dict(lengths=256, length_penalty=float("inf")),
+                   dict(lengths=2048, length_penalty=float("nan")), dict(lengths=2048, length_penalty=float("inf")),
                    dict(out_lengths=256), dict(end=40_000), dict(end=-2), dict(workspace=None), dict(workspace_bytes=8),
                    dict(workspace=(1 << 20) + 128)):
         _refused("leo_beam_select", ctypes.byref(native.LeoBeams(**{**good, **change})), None)
+    for change in (dict(out_scores=256), dict(out_scores=256 + 20), dict(out_parents=512), dict(out_symbols=(1 << 24) + 8),
+                   dict(finished=1024 + 23), dict(lengths=2048, out_lengths=2048), dict(out_finished=256 - 5),
+                   dict(out_symbols=(1 << 24) + 4 * (5 * 40_000 + 39_999))):
+        assert "overlap" in _refused("leo_beam_select", ctypes.byref(native.LeoBeams(**{**good, **change})), None)
     size = ctypes.c_uint64()
     for sizes in ((1, 65, 1, 5), (1, 1, 65, 5), (1 << 17, 1, 1, 5), (1, 1, 1, 0)):
         _refused("leo_beam_workspace_bytes", *sizes, ctypes.byref(size))
@@ -134,6 +139,11 @@ def test_targets_that_overlap_are_refused():
                    _array(at + 64, at + 64, row=1024, outer=8, piece=128, width=64)])
     # what wraps round the common divisor
     assert _meets([_array(at + 100, at + 100, row=128, width=40), _array(at + 128, at + 128, row=128, width=40)])
+
+
+def test_targets_over_the_parents_are_refused():
+    args, _ = _reorder([_array(1 << 20, 256 + 31)])
+    assert "parents" in _refused("leo_reorder_states", ctypes.byref(args), None)
 
 
 def test_nothing_to_reorder_is_no_error():
