@@ -297,19 +297,19 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
     for (uint32_t b = wave; b < beams; b += waves) {
         const uint64_t row = first + b;
         const SpanRecord none = {negative_infinity(), 0, 0.0};
-        const SpanRecord mine = lane < lists ? records[b * lists + lane] : none;
+        const SpanRecord mine = lane < lists ? records[b * lists + lane] : none, next = lane + 64 < lists ? records[b * lists + lane + 64] : none;
         const Given given = b == wave ? mine_given : given_of(a, row);
         Hypothesis h{};
         h.score = given.score;
         h.kind = !(given.score > negative_infinity()) ? 0 : given.finished ? 1 : 2;
         if (h.kind == 2) {
-            float top = mine.top;
+            float top = fmaxf(mine.top, next.top);
 #pragma unroll 4
-            for (uint32_t i = lane + 64; i < lists; i += 64) top = fmaxf(top, records[b * lists + i].top);
+            for (uint32_t i = lane + 128; i < lists; i += 64) top = fmaxf(top, records[b * lists + i].top);
             top = wave_max(top);
-            double mass = against(mine, top);
+            double mass = against(mine, top) + against(next, top);
 #pragma unroll 4
-            for (uint32_t i = lane + 64; i < lists; i += 64) mass += against(records[b * lists + i], top);
+            for (uint32_t i = lane + 128; i < lists; i += 64) mass += against(records[b * lists + i], top);
             h.log_mass = log(wave_sum(mass));
             h.top = top;
         }
