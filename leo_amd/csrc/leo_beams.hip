@@ -273,7 +273,7 @@ __host__ __device__ inline bool follows_lists(uint32_t all, uint32_t kept) { ret
 // [beams][lists][kept], by a whole workgroup of 2^n waves. What it reads is on
 // its way before anything is needed; the lists of finished hypotheses and of those with no
 // score hold anything, and count for nothing.
-constexpr uint32_t kAhead = 4;
+constexpr uint32_t kAhead = 2;
 struct Given {
     float score;
     bool finished;
@@ -302,6 +302,11 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
         Hypothesis h{};
         h.score = given.score;
         h.kind = !(given.score > negative_infinity()) ? 0 : given.finished ? 1 : 2;
+        h.inverse = 1.0;
+        if (a.length_penalty != 0.0) {  // while the records are on their way
+            const int64_t grown = static_cast<int64_t>(given.length) + (h.kind == 1 ? 0 : 1);
+            h.inverse = 1.0 / pow(static_cast<double>(grown < 1 ? 1 : grown), a.length_penalty);
+        }
         if (h.kind == 2) {
             float top = fmaxf(mine.top, next.top);
 #pragma unroll 4
@@ -312,11 +317,6 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
             for (uint32_t i = lane + 128; i < lists; i += 64) mass += against(records[b * lists + i], top);
             h.log_mass = log(wave_sum(mass));
             h.top = top;
-        }
-        h.inverse = 1.0;
-        if (a.length_penalty != 0.0) {
-            const int64_t grown = static_cast<int64_t>(given.length) + (h.kind == 1 ? 0 : 1);
-            h.inverse = 1.0 / pow(static_cast<double>(grown < 1 ? 1 : grown), a.length_penalty);
         }
         if (lane == 0) shared.hypotheses[b] = h;
     }
