@@ -72,17 +72,34 @@ __device__ __forceinline__ uint32_t kth_of_wave(uint32_t v, uint32_t kept) {
 
 // The same over a workgroup of 1, 2, 4, 8 or 16 waves, whose lanes make 64 groups: so
 // many different groups hold something as large that the value bounds the kept-th
-// largest of all. `maxima`: 64 words of LDS, not used where kWave.
+// largest of all. Where much is kept, every thread is a group: the least of 64 groups'
+// largest lets through five times what is kept, and 32 x 8 beams of 131,075 to 64 took
+// 1.2 ms. `maxima`: a word of LDS for each thread, none where kWave.
+constexpr uint32_t kFewKept = 16, kMostWaves = 16;
 template <bool kWave>
 __device__ __forceinline__ uint32_t bar_of(uint32_t largest, uint32_t kept, uint32_t* maxima) {
     const uint32_t lane = threadIdx.x % 64, waves = kWave ? 1 : blockDim.x / 64;
-    if (waves > 1) {
+    if (waves == 1) return kth_of_wave(largest, kept);
+    if (kept <= kFewKept) {
         const uint32_t m = group_max(largest, waves);
         if (lane % waves == 0) maxima[(threadIdx.x / 64 * 64 + lane) / waves] = m;
         __syncthreads();
-        largest = maxima[lane];
+        return kth_of_wave(maxima[lane], kept);
     }
-    return kth_of_wave(largest, kept);
+    maxima[threadIdx.x] = largest;
+    __syncthreads();
+    uint32_t all[kMostWaves], t = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kMostWaves; ++w) all[w] = w < waves ? maxima[w * 64 + lane] : 0;
+    for (int bit = 31; bit >= 12; --bit) {
+        const uint32_t higher = t | 1u << bit;
+        uint32_t count = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kMostWaves; ++w)
+            if (w < waves) count += static_cast<uint32_t>(__popcll(__ballot(all[w] >= higher)));
+        if (count >= kept) t = higher;
+    }
+    return t;
 }
 
 // Orders what one wave (kWave) or a workgroup wrote to LDS.
@@ -172,7 +189,19 @@ __device__ __forceinline__ void pick(const Span<T>& s, uint32_t base, float lane
     const uint32_t thread = kWave ? threadIdx.x % 64 : threadIdx.x, threads = kWave ? 64 : blockDim.x;
     if (thread == 0) counters[0] = counters[1] = 0;
     const uint32_t largest = lane_top > negative_infinity() ? order_key(lane_top + 0.0f) : 0;
-    const float bar = from_order_key(max(bar_of<kWave>(largest, kept, maxima), 0x00800000u));  // the lowest finite value or more
+    uint32_t key = 0;
+    if (kWave && kept > kFewKept) {  // the kept-th largest of the wave's symbols themselves
+        for (int bit = 31; bit >= 12; --bit) {
+            const float higher = from_order_key(key | 1u << bit);
+            uint32_t above = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; ++i) above += static_cast<uint32_t>(__popcll(__ballot(s.z[i] >= higher)));
+            if (above >= kept) key |= 1u << bit;
+        }
+    } else {
+        key = bar_of<kWave>(largest, kept, maxima);
+    }
+    const float bar = from_order_key(max(key, 0x00800000u));  // the lowest finite value or more
     settle_lds<kWave>();
     const auto gather = [&](auto&& stays) {
         if (!__any(lane_top >= bar)) return;
@@ -261,7 +290,7 @@ struct MergeShared {
     Hypothesis hypotheses[kMostBeams];
     Ranked pool[kPool];
     Ranked best[16];
-    uint32_t maxima[64];
+    uint32_t maxima[kMostWaves * 64];
     uint32_t count;
 };
 
@@ -447,7 +476,7 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
 // Searches whose rows make up to 16 spans take one workgroup each: a wave a span,
 // which picks from its registers, then the search's answer. A chain of reductions bounds
 // it: 7.0 us for 4 beams of 257, of which a launch is some 3.
-constexpr uint32_t kMostWaves = 16, kWavePool = 320;
+constexpr uint32_t kWavePool = 320;
 template <class T>
 __global__ __launch_bounds__(kMostWaves * 64) void leo_beam_whole(LeoBeams a, uint32_t spans) {
     union Shared {
@@ -481,7 +510,7 @@ constexpr uint32_t kRowPool = 1024;
 template <class T>
 __global__ __launch_bounds__(256) void leo_beam_rows(LeoBeams a, uint32_t lists, SpanRecord* records, uint64_t* candidates) {
     __shared__ uint64_t pool[kRowPool];
-    __shared__ uint32_t maxima[64], counters[2];
+    __shared__ uint32_t maxima[256], counters[2];
     __shared__ SpanRecord parts[4];
     const uint64_t row = blockIdx.y;
     if (!is_open(a, row)) return;
