@@ -366,7 +366,13 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
         const bool none = h.kind == 0 || key == 0 || !(score > -__builtin_inf());
         return {none ? 0 : bits >> 63 ? ~bits : bits | 1ull << 63, Ranked::second_of(beam, key)};
     };
-    const auto load_ranked = [&](uint32_t list, uint32_t place) { return ranked(list, place, candidates[static_cast<uint64_t>(list) * kept + place]); };
+    const Ranked nothing = {0, 0};
+    const auto load_ranked = [&](uint32_t list, uint32_t place) {
+        if (shared.hypotheses[list / lists].kind == 0) return nothing;
+        return ranked(list, place, candidates[static_cast<uint64_t>(list) * kept + place]);
+    };
+    const uint32_t items = all * kept;
+    const auto item = [&](uint32_t i) { return i < items ? load_ranked(i % all, i / all) : nothing; };
     const auto answer = [&](uint32_t k, const Ranked& r) {
         const bool found = r.rank != 0;
         const uint32_t beam = found ? r.beam() : 0;
@@ -387,9 +393,10 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
         if (taken && at < kPool) shared.pool[at] = r;
         return true;
     };
-    const Ranked nothing = {0, 0};
+    const uint32_t kind = lane < beams ? shared.hypotheses[lane].kind : 0;
+    const uint32_t live = static_cast<uint32_t>(__popcll(__ballot(kind == 2))) * lists + static_cast<uint32_t>(__popcll(__ballot(kind == 1)));
     uint32_t largest = 0;
-    if (follows_lists(all, kept)) {
+    if (follows_lists(live, kept)) {
         // the lists' best bound what can be kept, and each list is followed down to the bar
         for (uint32_t list = own; list < all; list += threads)
             largest = max(largest, static_cast<uint32_t>((list == own ? ranked(list, 0, ahead[0]) : load_ranked(list, 0)).rank >> 32));
@@ -422,10 +429,9 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
         }
     } else {
         // few lists: all their candidates
-        const uint32_t items = all * kept;
-        const auto item = [&](uint32_t i) { return i < items ? load_ranked(i % all, i / all) : nothing; };
         const Ranked one = item(own);
         largest = static_cast<uint32_t>(one.rank >> 32);
+#pragma unroll 4
         for (uint32_t i = own + threads; i < items; i += threads) largest = max(largest, static_cast<uint32_t>(item(i).rank >> 32));
         const uint32_t bar = max(bar_of<false>(largest, kept, shared.maxima), 1u);
         for (uint32_t from = 0; from < items; from += threads) {
@@ -434,7 +440,30 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
         }
     }
     __syncthreads();
-    const uint32_t count = shared.count;
+    uint32_t count = shared.count;
+    if (count > kPool) {
+        // the bar let through too much, as with rows in falling order: the kept-th rank's upper half, bit by bit
+        uint32_t bar = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t higher = bar | 1u << bit;
+            uint32_t mine = 0;
+#pragma unroll 4
+            for (uint32_t i = thread; i < items; i += threads) mine += item(i).rank >> 32 >= higher;
+            mine = wave_sum(mine);
+            __syncthreads();
+            if (thread == 0) shared.count = 0;
+            __syncthreads();
+            if (lane == 0) atomicAdd(&shared.count, mine);
+            __syncthreads();
+            if (shared.count >= kept) bar = higher;
+        }
+        __syncthreads();
+        if (thread == 0) shared.count = 0;
+        __syncthreads();
+        for (uint32_t from = 0; from < items; from += threads) gather(item(from + thread), max(bar, 1u));
+        __syncthreads();
+        count = shared.count;
+    }
     if (count <= kPool) {
         for (uint32_t i = thread; i < count; i += threads) {
             const Ranked mine = shared.pool[i];
@@ -450,8 +479,9 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
     Ranked last = {~0ull, ~0ull};
     for (uint32_t k = 0; k < kept; ++k) {
         Ranked best = nothing;
-        for (uint32_t i = thread; i < all * kept; i += threads) {
-            const Ranked r = load_ranked(i % all, i / all);
+#pragma unroll 4
+        for (uint32_t i = thread; i < items; i += threads) {
+            const Ranked r = item(i);
             if (r.rank && before(last, r) && (!best.rank || before(r, best))) best = r;
         }
         const auto meet = [&](const Ranked& other) {

@@ -187,6 +187,22 @@ def test_order_of_rows(require_gpu, symbols, kept):
     compare(z, scores.view(2, -1), kept)
 
 
+@pytest.mark.parametrize("beams, symbols, kept", [(8, 131_075, 64), (3, 100_000, 40), (64, 9000, 64), (16, 2000, 17)])
+def test_more_than_the_pool_holds(require_gpu, beams, symbols, kept):
+    """Rows in falling order, whose first lists hold all; ties; one hypothesis of many."""
+    gen = torch.Generator(DEVICE).manual_seed(symbols)
+    z = torch.randn(beams, symbols, generator=gen, device=DEVICE).sort(dim=1, descending=True).values
+    scores = -5 - torch.rand(1, beams, generator=gen, device=DEVICE)
+    compare(z, scores, kept)
+    compare(z.bfloat16(), scores, kept)
+    compare(torch.zeros_like(z), torch.full_like(scores, -1.0), kept, exact=True)
+    for alive in (0, beams - 1):
+        one = torch.full_like(scores, -torch.inf)
+        one[0, alive] = -2.0
+        compare(z, one, kept, exact=True)
+        compare(z, one, kept, torch.arange(beams, device=DEVICE)[None] == alive, exact=True)
+
+
 @pytest.mark.parametrize("symbols", [40, 300, 17_000])
 def test_special_values(require_gpu, symbols):
     z, scores, _ = make(3, 10, 2, symbols, torch.float32)
