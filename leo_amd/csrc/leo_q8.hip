@@ -633,7 +633,7 @@ Plan plan_of(const LeoQ8Shape& s, uint64_t rows) {
         // 64 rows of 8,192 -> 8,192 took 20.6 us with 512 workgroups of one tile and 23.0 with 256 of two, of 5,001 ->
         // 11,007 20.3 with 688 and 18.9 with 344; 128 rows, each tile read twice, 24 with four tiles and 29 with two.
         p.group_rows = row_tiles <= 2 ? static_cast<uint32_t>(row_tiles) : 4;
-        p.group_tiles = row_tiles > 4 ? 4 : l.tiles > 600 ? 2 : 1;
+        p.group_tiles = row_tiles > 4 ? (l.tiles > 2 ? 4 : static_cast<uint32_t>(l.tiles)) : l.tiles > 600 ? 2 : 1;
         const uint64_t groups = over(l.tiles, p.group_tiles) * over(row_tiles, p.group_rows);
         slices = l.blocks <= 64 ? 1 : std::max<uint64_t>(1, std::min<uint64_t>(512 / groups, over(l.blocks, 16)));
     } else {
@@ -687,10 +687,10 @@ void launch_product(const Plan& p, const ProductArgs& a, uint32_t* largest, hipS
     else launch(leo_q8_quantize_row<X>, dim3((a.row_tiles + 7) / 8 * 8 * kTile), dim3((a.inputs + 1023) / 1024 * 64), 0, stream, a);
     if (p.tiles == 16) return launch_tiles<4, 8, 4, 2>(a, stream);
     if (p.tiles == 8) return launch_tiles<4, 4, 2, 2>(a, stream);
-    static constexpr void (*kKernels[3][3])(ProductArgs) = {{leo_q8_many<1, 1>, leo_q8_many<1, 2>, leo_q8_many<1, 4>},
-                                                            {leo_q8_many<2, 1>, leo_q8_many<2, 2>, leo_q8_many<2, 4>},
-                                                            {leo_q8_many<4, 1>, leo_q8_many<4, 2>, leo_q8_many<4, 4>}};
-    const auto many = kKernels[p.group_rows / 2][p.group_tiles / 2];
+    const bool one = p.group_tiles == 1;
+    const auto many = p.group_rows == 1 ? (one ? leo_q8_many<1, 1> : leo_q8_many<1, 2>)
+                      : p.group_rows == 2 ? (one ? leo_q8_many<2, 1> : leo_q8_many<2, 2>)
+                      : p.group_tiles == 4 ? leo_q8_many<4, 4> : one ? leo_q8_many<4, 1> : leo_q8_many<4, 2>;
     launch(many, dim3((a.tiles + p.group_tiles - 1) / p.group_tiles, (a.row_tiles + p.group_rows - 1) / p.group_rows, a.slices), dim3(kFewThreads), 0, stream, a);
 }
 

@@ -261,6 +261,15 @@ def test_very_long_rows(require_gpu, beams, symbols, kept):
     assert float((got.scores[0].double() - ranks[:kept]).abs().max()) <= 25 * 2.0 ** -24 + 2.0 ** -21
 
 
+def test_offsets_past_32_bits(require_gpu):
+    wide = torch.empty(5, 1 << 30, dtype=torch.bfloat16, device=DEVICE)
+    z, scores, _ = make(12, 1, 5, 3000, torch.bfloat16)
+    wide[:, 3:3003] = z
+    compare(wide[:, 3:3003], scores, 9)
+    wide[:, 3:260] = z[:, :257]
+    compare(wide[:, 3:260], scores, 9)
+
+
 def test_lengths(require_gpu):
     z, scores, _ = make(4, 3, 4, 100, torch.float32)
     lengths = torch.tensor([[0, 1, 2, 3], [-5, 2**31 - 2, 0, 10], [2**31 - 2, 1, 1, 1]], device=DEVICE, dtype=torch.int32)

@@ -159,6 +159,33 @@ def test_large_tiles(require_gpu, rows, inputs, outputs, dtype):
     assert bool((buffer[:, :3] == 7).all()) and bool((buffer[:, 3 + outputs:] == 7).all())
 
 
+def test_offsets_past_32_bits(require_gpu):
+    # rows of x and of the result 2^30 values apart
+    wide, out = torch.empty(3, 1 << 30, dtype=torch.bfloat16, device=DEVICE), torch.empty(3, 1 << 30, dtype=torch.float16, device=DEVICE)
+    x, codes, scales, bias = make(1, 3, 1100, 300, torch.bfloat16, torch.float32)
+    wide[:, 7:1107] = x
+    got = decode.q8_matmul(wide[:, 7:1107], decode.Q8Weight(codes, scales), bias, out=out[:, 5:305])
+    check(got, x, codes, scales, bias)
+    del wide, out, got
+    # weights past 4 GiB
+    gen = torch.Generator(DEVICE).manual_seed(4)
+    codes = torch.randint(-128, 128, (33_000, 140_000), generator=gen, device=DEVICE, dtype=torch.int8)
+    scales = torch.rand(33_000, generator=gen, device=DEVICE) * 0.01
+    weight = decode.Q8Weight(codes, scales)
+    some = torch.tensor([0, 1, 15_339, 15_340, 16_400, 32_000, 32_990, 32_998, 32_999], device=DEVICE)
+    for rows in (1, 20, 140):
+        x = torch.randn(rows, 140_000, generator=gen, device=DEVICE)
+        check(decode.q8_matmul(x, weight)[:, some].contiguous(), x, codes[some], scales[some], None)
+
+
+@pytest.mark.parametrize("rows", [90, 1000])
+@pytest.mark.parametrize("outputs", [1, 16, 17, 33, 49, 112])
+def test_many_rows_of_few_outputs(require_gpu, rows, outputs):
+    for inputs in (70, 5000):
+        x, codes, scales, bias = make(rows + outputs, rows, inputs, outputs, torch.bfloat16, torch.float32)
+        check(decode.q8_matmul(x, decode.Q8Weight(codes, scales), bias, out_dtype=torch.float32), x, codes, scales, bias)
+
+
 def test_two_streams_at_once(require_gpu):
     cases = []
     for rows, inputs, outputs in ((1, 200_000, 257), (40, 9000, 900), (600, 1500, 700), (8, 70_000, 257)):
