@@ -345,7 +345,7 @@ __global__ __launch_bounds__(kFewThreads, 4) void leo_q8_few(ProductArgs a) {
 
 // More rows: 16 kRows rows and 16 kTiles outputs a workgroup, x and the weights
 // straight from their layouts to registers, the blocks of a slice shared by eight waves, one
-// block ahead (two ahead took the same time). 64 rows of 5,001 -> 11,007, 55 MB, take 15.1 us:
+// block ahead (two ahead, or 4 or 16 waves, took as long or longer). 64 rows of 5,001 -> 11,007, 55 MB, take 15.1 us:
 // 344 workgroups on 256 CUs, and 323 KB of x for each of them from L2.
 template <int kManyRows, int kManyTiles>
 __global__ __launch_bounds__(kFewThreads) void leo_q8_many(ProductArgs a) {
