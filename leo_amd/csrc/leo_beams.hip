@@ -190,7 +190,7 @@ __device__ __forceinline__ void pick(const Span<T>& s, uint32_t base, float lane
     if (thread == 0) counters[0] = counters[1] = 0;
     const uint32_t largest = lane_top > negative_infinity() ? order_key(lane_top + 0.0f) : 0;
     uint32_t key = 0;
-    if (kWave && kept > kFewKept) {  // the kept-th largest of the wave's symbols themselves
+    if ((kWave || blockDim.x == 64) && kept > kFewKept) {  // the kept-th largest of the wave's symbols themselves
         for (int bit = 31; bit >= 12; --bit) {
             const float higher = from_order_key(key | 1u << bit);
             uint32_t above = 0;
