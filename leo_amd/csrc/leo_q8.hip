@@ -132,8 +132,9 @@ __device__ __forceinline__ float scale_of(uint32_t largest) {
 // The whole numbers nearest to the exact quotients x / s, of two the even one. The sum
 // with 1.5 * 2^23 of x and the rounded inverse rounds to a whole number once and has it in
 // its last byte. The inverse is off by 2^-24 of itself, so a quotient of 127 at most by
-// less than 2^-16: only where one lies as near to a half, as in some 3% of waves, the
-// remainder x - n s tells, which needs no rounding near s / 2.
+// less than 2^-16: only where one lies as near to a half, as in some 3% of waves, twice the
+// remainder x - n s tells, held against s: near s / 2 neither it nor its double needs rounding,
+// whereas half of a scale below 2^-125 may.
 __device__ __forceinline__ uint4v codes_of(const Sixteen& s, float scale) {
     constexpr float kMagic = 12582912.0f;
     const float inverse = 1.0f / scale;
@@ -144,13 +145,12 @@ __device__ __forceinline__ uint4v codes_of(const Sixteen& s, float scale) {
         off = fmaxf(off, fabsf(__builtin_fmaf(s.f[i], inverse, kMagic - number[i])));
     }
     if (__any(off > 0.5f - 0x1p-16f)) {
-        const float half = 0.5f * scale;
 #pragma unroll
         for (uint32_t i = 0; i < 16; ++i) {
-            const float n = number[i] - kMagic, rest = __builtin_fmaf(-n, scale, s.f[i]);
+            const float n = number[i] - kMagic, rest = __builtin_fmaf(-n, scale, s.f[i]), twice = rest + rest;
             const bool odd = __float_as_uint(number[i]) & 1u;
-            if (rest > half || (rest == half && odd)) number[i] += 1.0f;
-            if (rest < -half || (rest == -half && odd)) number[i] -= 1.0f;
+            if (twice > scale || (twice == scale && odd)) number[i] += 1.0f;
+            if (twice < -scale || (twice == -scale && odd)) number[i] -= 1.0f;
         }
     }
     uint4v words;
