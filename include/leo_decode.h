@@ -224,7 +224,8 @@ int32_t leo_q8_matmul(const LeoQ8Product* product, void* stream);
  * lower symbol. length counts the symbol that comes in: lengths[b] + 1, lengths[b]
  * of a finished one, at least 1; lengths may be NULL where length_penalty is 0.
  * Logits count as in leo_sample, those of +inf share all probability. Ranks are
- * held in 64 bits.
+ * held in 64 bits; the log of a row's sum is off by up to 2^-21, the same for all of its
+ * symbols.
  * out_parents is the hypothesis within its search; out_symbols is -1 for a finished
  * one. Places that no candidate takes have symbol -1, parent 0 and score -inf.
  * finished (bytes, 0 or not) may be NULL: none is. out_finished (may be NULL) is 1

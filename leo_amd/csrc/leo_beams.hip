@@ -39,13 +39,6 @@ __device__ __forceinline__ double wave_sum(double v) {
     return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(last(static_cast<uint32_t>(bits >> 32))) << 32 | last(static_cast<uint32_t>(bits))));
 }
 
-// exp(d) for d <= 0, to some 2^-23 of itself: the product with log2(e) in two parts.
-__device__ __forceinline__ float exp_of(float d) {
-    const float high = d * 1.44269504f, low = __builtin_fmaf(d, 1.44269504f, -high) + d * 1.92596299e-8f;
-    const float e = __builtin_amdgcn_exp2f(high);
-    return e > 0.0f ? __builtin_fmaf(e, low * 0.693147181f, e) : 0.0f;
-}
-
 // The largest of v in each group of `lanes` neighbouring lanes (a power of two up to 16).
 __device__ __forceinline__ uint32_t group_max(uint32_t v, uint32_t lanes) {
     const auto step = [&](auto ctrl) {
@@ -154,29 +147,54 @@ struct Span {
     }
 };
 
-// What a span, or a run of them, leaves for its row: its largest logit and the sum of
-// exponentials against it. Lanes' sums of 16 are floats, what joins them has 64 bits.
+// What a span, or a run of them, leaves for its row: its largest logit, and the sum of
+// exponentials as mass * 2^power_of(top) * e^base_of(top). A power of two in place of the
+// largest itself, so that no difference of two logits is rounded, and sums of spans meet
+// exactly. From 2^20 on the largest comes off first: floats that size differ by nothing or by
+// 2^-4 at least, and where the difference counts at all it is exact.
+constexpr float kLog2E = 1.44269504f, kLog2ELow = 1.92596299e-8f;  // log2(e) in two parts
+constexpr double kLn2 = 0.69314718055994531;
+__device__ __forceinline__ float base_of(float top) { return fabsf(top) < 0x1p20f ? 0.0f : top; }
+__device__ __forceinline__ float power_of(float top) { return fabsf(top) < 0x1p20f ? ceilf(top * kLog2E) : 0.0f; }
+
 struct SpanRecord {
     float top;
     uint32_t pad0;
     double mass;
 };
 __device__ __forceinline__ double against(const SpanRecord& r, float top) {
-    return r.top == top ? r.mass : r.top > negative_infinity() ? r.mass * exp_of(r.top - top) : 0.0;
+    if (!(r.top > negative_infinity())) return 0.0;
+    const float base = base_of(r.top), to = base_of(top), power = power_of(r.top) - power_of(top);
+    if (base == to) return ldexp(r.mass, static_cast<int>(power));
+    return r.mass * exp(static_cast<double>(base) - to + power * kLn2);
 }
+// z log2(e) - power is a whole number and a fraction of at most a half, which the fused
+// products have to 2^-25; the exponential is off by 2^-23 at most, and sixteen of them are
+// added in four steps of 2^-24 each. Together less than 2^-21 of the sum, however alike its
+// terms are; what follows has 64 bits. What lies 80 below the largest is taken as lying there,
+// which 2^26 of them cannot bring to 2^-64.
 template <class T>
 __device__ __forceinline__ SpanRecord weigh(const Span<T>& s, float lane_top) {
     const float top = wave_max(lane_top);
-    float mass = 0.0f;
     if (top == negative_infinity()) return {top, 0, 0.0};
+    float e[kEach];
     if (top < __builtin_inff()) {
+        const float base = base_of(top), least = top - base - 80.0f, magic = 12582912.0f - power_of(top);  // 1.5 * 2^23
 #pragma unroll
-        for (uint32_t i = 0; i < kEach; ++i) mass += __builtin_amdgcn_exp2f((s.z[i] - top) * 1.44269504f);
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const float z = fmaxf(s.z[i] - base, least), whole = __builtin_fmaf(z, kLog2E, magic);
+            const float rest = __builtin_fmaf(z, kLog2ELow, __builtin_fmaf(z, kLog2E, magic - whole));
+            e[i] = __uint_as_float(__float_as_uint(__builtin_amdgcn_exp2f(rest)) + (__float_as_uint(whole) << 23));
+        }
     } else {
 #pragma unroll
-        for (uint32_t i = 0; i < kEach; ++i) mass += s.z[i] == top ? 1.0f : 0.0f;
+        for (uint32_t i = 0; i < kEach; ++i) e[i] = s.z[i] == top ? 1.0f : 0.0f;
     }
-    return {top, 0, wave_sum(static_cast<double>(mass))};
+#pragma unroll
+    for (uint32_t half = kEach / 2; half; half /= 2)
+#pragma unroll
+        for (uint32_t i = 0; i < half; ++i) e[i] += e[i + half];
+    return {top, 0, wave_sum(static_cast<double>(e[0]))};
 }
 
 // The `kept` best of the spans of a workgroup (or of one wave's span, kWave), in
@@ -265,7 +283,7 @@ __device__ __forceinline__ bool is_open(const LeoBeams& a, uint64_t row) { retur
 
 // What makes a hypothesis' logits comparable with another's.
 struct Hypothesis {
-    double score, log_mass, inverse;  // 1 over the length's power
+    double score, log_mass, inverse;  // log_mass against the top; 1 over the length's power
     float top;
     uint32_t kind;  // 0: none, 1: finished, 2: open
 };
@@ -344,7 +362,7 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
             double mass = against(mine, top) + against(next, top);
 #pragma unroll 4
             for (uint32_t i = lane + 128; i < lists; i += 64) mass += against(records[b * lists + i], top);
-            h.log_mass = log(wave_sum(mass));
+            h.log_mass = log(wave_sum(mass)) + (base_of(top) == top ? 0.0 : power_of(top) * kLn2 - top);
             h.top = top;
         }
         if (lane == 0) shared.hypotheses[b] = h;

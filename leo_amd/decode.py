@@ -326,7 +326,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, kept: Optional[int] 
     one stays as it is and its logits do not count. The order is that of score /
     length^length_penalty, with the length that the hypothesis then has; of equals
     the lower hypothesis comes first, then the larger logit, then the lower symbol.
-    Ranks have 64 bits. Logits of -inf or NaN are no way on, nor are hypotheses whose
+    Ranks have 64 bits, but the log of a row's sum is off by up to 2^-21, the same for all of
+    its symbols. Logits of -inf or NaN are no way on, nor are hypotheses whose
     score is -inf or NaN. Where fewer than `kept` are left, the others have symbol
     -1, parent 0, score -inf, and the length of hypothesis 0.
 
