@@ -281,9 +281,22 @@ __device__ __forceinline__ void pick(const Span<T>& s, uint32_t base, float lane
 __device__ __forceinline__ bool is_finished(const LeoBeams& a, uint64_t row) { return a.finished && a.finished[row]; }
 __device__ __forceinline__ bool is_open(const LeoBeams& a, uint64_t row) { return !is_finished(a, row) && a.scores[row] > negative_infinity(); }
 
+// n^p for p >= 0. Whole and half powers by products and a root, which round nothing where
+// the result is a whole number below 2^53, so that ranks that are equal as quotients tie;
+// pow may be off by a step there, as it is for a p of 1.
+__device__ __forceinline__ double power_of_length(double n, double p) {
+    const double whole = floor(p);
+    if (whole > 64.0 || (p != whole && p != whole + 0.5)) return pow(n, p);
+    double r = p == whole ? 1.0 : sqrt(n), square = n;
+    for (uint32_t left = static_cast<uint32_t>(whole); left; left /= 2, square *= square)
+        if (left % 2) r *= square;
+    return r;
+}
+
 // What makes a hypothesis' logits comparable with another's.
 struct Hypothesis {
-    double score, log_mass, inverse;  // log_mass against the top; 1 over the length's power
+    double score, log_mass;  // log_mass against the top
+    double factor, power;    // what makes a score a rank; the length's power that it is the inverse of
     float top;
     uint32_t kind;  // 0: none, 1: finished, 2: open
 };
@@ -349,10 +362,12 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
         Hypothesis h{};
         h.score = given.score;
         h.kind = !(given.score > negative_infinity()) ? 0 : given.finished ? 1 : 2;
-        h.inverse = 1.0;
+        h.factor = 1.0;
         if (a.length_penalty != 0.0) {  // while the records are on their way
             const int64_t grown = static_cast<int64_t>(given.length) + (h.kind == 1 ? 0 : 1);
-            h.inverse = 1.0 / pow(static_cast<double>(grown < 1 ? 1 : grown), a.length_penalty);
+            const double power = power_of_length(static_cast<double>(grown < 1 ? 1 : grown), fabs(a.length_penalty));
+            h.factor = a.length_penalty < 0.0 ? power : 1.0 / power;
+            h.power = power < __builtin_inf() ? power : 0.0;
         }
         if (h.kind == 2) {
             float top = fmaxf(mine.top, next.top);
@@ -380,7 +395,11 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
         const Hypothesis& h = shared.hypotheses[beam];
         key = h.kind != 1 ? key : place == 0 && list == beam * lists ? 1 : 0;
         const double score = score_of(h, key);
-        const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(score * h.inverse + 0.0));
+        // The remainder of the product with the inverse makes it the quotient, rounded once: -49 over 49 and -3 over 3 are
+        // one rank. A division here took 590 us of a step of 32 x 8 beams of 131,075 to 64 whose pool runs over, this 555, the product alone 520.
+        double value = score * h.factor;
+        if (a.length_penalty > 0.0) value = __builtin_fma(__builtin_fma(-value, h.power, score), h.factor, value);
+        const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(value + 0.0));
         const bool none = h.kind == 0 || key == 0 || !(score > -__builtin_inf());
         return {none ? 0 : bits >> 63 ? ~bits : bits | 1ull << 63, Ranked::second_of(beam, key)};
     };

@@ -51,3 +51,27 @@ def test_spans_far_apart(require_gpu, symbols):
         z[2, symbols // 2:] = low
         z[3, :symbols // 2] = -torch.inf
         compare(z, torch.tensor([[-1.0, -1.5], [-2.0, -1.0]], device=DEVICE), 5)
+
+
+@pytest.mark.parametrize("penalty", [1.0, 2.0, 3.0, 0.5, 1.5, -1.0])
+def test_hypotheses_of_one_rank_come_in_their_order(require_gpu, penalty):
+    """Scores that are whole multiples of their length's power: the quotients tie, whatever the length."""
+    rng = np.random.default_rng(5)
+    for turn in range(6):
+        lengths = rng.permutation(np.arange(1, 65))
+        if penalty in (1.0, 2.0):
+            lengths += 64 * (turn % 3)
+        elif penalty in (0.5, 1.5):
+            lengths = lengths ** 2
+        elif penalty == -1.0:
+            lengths = rng.choice([n for n in range(1, 5041) if 5040 % n == 0], 64)
+        scores = -5040.0 / lengths if penalty < 0 else -3.0 * np.float64(lengths) ** penalty
+        assert (np.float32(scores) == scores).all() and (scores == np.round(scores)).all()
+        for symbols in (70, 5000):
+            z = torch.randn(64, symbols, device=DEVICE)
+            got = decode.beam_select(z, torch.from_numpy(scores.astype(np.float32)).to(DEVICE)[None],
+                                     finished=torch.ones(1, 64, dtype=torch.bool, device=DEVICE),
+                                     lengths=torch.from_numpy(lengths.astype(np.int32)).to(DEVICE)[None],
+                                     length_penalty=penalty)
+            assert got.parents[0].tolist() == list(range(64))
+            assert got.scores[0].tolist() == scores.tolist()
