@@ -421,9 +421,9 @@ constexpr uint32_t kSlots = 4;  // steps in LDS
 
 // 16 bytes a lane from `from` + `offset` to 1,024 bytes of LDS. The instruction writes
 // no register, so nothing can be read before it has come but LDS, whose waits a step
-// makes itself. M0 holds the place in LDS and is used for nothing else here.
+// makes itself. M0 holds the place in LDS.
 __device__ __forceinline__ void load_to_lds(uint32_t lds, const char* from, uint32_t offset) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(from) : "memory", "m0");
 }
 
 template <int kN, int kM, int kWavesN, int kWavesM>
