@@ -641,7 +641,7 @@ void check_beams(const char* who, uint64_t groups, uint64_t beams, uint64_t kept
     };
     need(beams >= 1 && beams <= kMostBeams, "beams must be 1 .. 64");
     need(kept >= 1 && kept <= kMostBeams, "kept must be 1 .. 64");
-    need(groups * beams <= 65535, "too many hypotheses");
+    need(groups <= 65535 / beams, "too many hypotheses");  // a product could wrap
     need(symbols >= 1 && symbols <= 1u << 26, "symbols must be 1 .. 2^26");
 }
 
