@@ -799,7 +799,7 @@ bool may_meet(const LeoReorder& r, const std::vector<Extent>& extents) {
             modulus = std::gcd(modulus, row);
             if (pieces) modulus = std::gcd(modulus, outer);
         }
-        if (modulus == 0) return true;
+        if (modulus == 0) continue;  // single rows, whose pieces may still lie apart
         std::vector<Extent> folded;
         bool fits = true;
         for (const Extent& e : extents) {

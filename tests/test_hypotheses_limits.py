@@ -30,3 +30,22 @@ def test_the_most_hypotheses_have_a_workspace():
     for groups, beams in ((65_535, 1), (1023, 64), (21_845, 3)):
         assert lib.leo_beam_workspace_bytes(groups, beams, 4, 40_000, ctypes.byref(size)) == native.OK
         assert size.value > 0
+
+
+def _array(source, target, **more):
+    return native.LeoStateArray(**{**dict(source=source, target=target, outer=8, width=64, source_row=1024, source_outer=128,
+                                          target_row=1024, target_outer=128), **more})
+
+
+@pytest.mark.parametrize("groups, beams, kept", [(1, 1, 1), (1, 2, 1), (1, 1, 2), (2, 4, 4)])
+def test_pieces_that_meet_are_refused_in_single_rows_too(groups, beams, kept):
+    at, lib = 1 << 20, native.load()
+    for first, second in (((1 << 30, at), (1 << 31, at + 63)),                      # targets, by one byte
+                          ((1 << 30, at), (at + 64 + 127, 1 << 31)),                # a source, by one byte past the end
+                          ((1 << 30, at), (1 << 31, at)), ((1 << 30, at), (at, 1 << 31))):
+        entries = (native.LeoStateArray * 2)(_array(*first), _array(*second))
+        args = native.LeoReorder(arrays=ctypes.addressof(entries), count=2, groups=groups, beams=beams, kept=kept, parents=256)
+        assert "overlaps another array" in _refused("leo_reorder_states", ctypes.byref(args), None)
+    entries = (native.LeoStateArray * 2)(_array(1 << 30, at, outer=1), _array(1 << 31, at + 63, outer=1))
+    args = native.LeoReorder(arrays=ctypes.addressof(entries), count=2, groups=1, beams=1, kept=1, parents=256)
+    assert "overlaps another array" in _refused("leo_reorder_states", ctypes.byref(args), None)
