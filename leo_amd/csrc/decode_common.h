@@ -168,6 +168,12 @@ inline bool overlap(const Rows& a, const Rows& b) {
     return false;
 }
 
+// An axis of a grid has to have fewer than 2^32 threads: workgroups past the first 2^22 go on
+// along the second axis, whose last row may hold some too many.
+constexpr uint32_t kAcross = 1u << 22;
+inline dim3 grid_of(uint32_t count) { return dim3(count < kAcross ? count : kAcross, (count + kAcross - 1) / kAcross); }
+__device__ __forceinline__ uint32_t block_of_grid() { return blockIdx.y * kAcross + blockIdx.x; }
+
 // Launches through the returned status, not the thread's last error, which an
 // earlier call of the program may have left.
 template <class... Args>

@@ -673,6 +673,7 @@ struct ReorderArgs {
     uint32_t columns[kArrays];  // of 16 bytes, of a place
     uint32_t units[kArrays];    // workgroups of a search
     uint32_t before[kArrays];   // workgroups of the arrays before
+    uint32_t all;               // workgroups
     uint32_t count;
     uint32_t groups, beams, kept;
     const int32_t* parents;
@@ -695,10 +696,12 @@ __device__ __forceinline__ uint4v load_shifted(const char* p) {
 template <bool kInPlace>
 __global__ __launch_bounds__(256) void leo_reorder(ReorderArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint4v held[];
+    const uint32_t block = block_of_grid();
+    if (block >= a.all) return;
     uint32_t which = 0;
-    while (which + 1 < a.count && blockIdx.x >= a.before[which + 1]) ++which;
+    while (which + 1 < a.count && block >= a.before[which + 1]) ++which;
     const LeoStateArray& s = a.arrays[which];
-    const uint32_t columns = a.columns[which], units = a.units[which], unit = blockIdx.x - a.before[which];
+    const uint32_t columns = a.columns[which], units = a.units[which], unit = block - a.before[which];
     const uint64_t group = unit / units, all = columns * s.outer, column = static_cast<uint64_t>(unit % units) * blockDim.x + threadIdx.x;
     if (column >= all) return;
     uint64_t outer = 0;
@@ -940,7 +943,7 @@ int32_t leo_reorder_states(const LeoReorder* reorder, void* stream) {
                     // a place that starts anywhere may touch one column more
                     const bool aligned = (reinterpret_cast<uintptr_t>(s.target) | s.target_row | s.target_outer) % 16 == 0;
                     const uint64_t columns = (s.width + (in_place || aligned ? 15 : 30)) / 16, mine = (columns * s.outer + threads - 1) / threads;
-                    require(mine * r.groups <= 0x7fffffffu, "leo_reorder_states: an array is too large");
+                    require(mine <= 0x7fffffffu / r.groups, "leo_reorder_states: an array is too large");
                     if (units + mine * r.groups > 0x7fffffffu) break;
                     a.arrays[a.count] = s;
                     a.columns[a.count] = static_cast<uint32_t>(columns);
@@ -949,7 +952,8 @@ int32_t leo_reorder_states(const LeoReorder* reorder, void* stream) {
                     units += mine * r.groups;
                 }
                 const auto at = static_cast<hipStream_t>(stream);
-                const dim3 grid(static_cast<uint32_t>(units)), block(threads);
+                a.all = static_cast<uint32_t>(units);
+                const dim3 grid = grid_of(a.all), block(threads);
                 if (in_place) launch(leo_reorder<true>, grid, block, a.kept * threads * 16, at, a);
                 else launch(leo_reorder<false>, grid, block, 0, at, a);
             }

@@ -27,3 +27,15 @@ def test_arrays_that_interleave_in_one_row(require_gpu, groups, beams, kept):
     if beams == kept:
         decode.reorder_states(views, parents, out=views)
         assert all(same(v, w) for v, w in zip(views, want))
+
+
+def test_more_than_2_32_threads_reorder(require_gpu):
+    """2^31 - 1 pieces of two bytes, each of which may touch two columns."""
+    pieces = 2 ** 31 - 1
+    source = torch.randint(-2 ** 15, 2 ** 15, (1, pieces, 2), device=DEVICE, dtype=torch.int16)
+    target = torch.zeros(1, pieces, 2, device=DEVICE, dtype=torch.int16)
+    parents = torch.zeros(1, 1, device=DEVICE, dtype=torch.int32)
+    decode.reorder_states(source[:, :, :1], parents, out=target[:, :, :1])
+    for begin in range(0, pieces, 1 << 28):
+        part = slice(begin, begin + (1 << 28))
+        assert torch.equal(target[0, part, 0], source[0, part, 0]) and not bool(target[0, part, 1].any())
