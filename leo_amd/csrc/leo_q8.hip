@@ -581,8 +581,9 @@ template <uint32_t kShare>
 __global__ __launch_bounds__(256) void leo_q8_join(ProductArgs a) {
     constexpr uint32_t kOutputs = 256 / kShare;
     __shared__ int64_t parts[kShare][kOutputs];
-    const uint32_t wide = (a.outputs + kOutputs - 1) / kOutputs, row = blockIdx.x / wide;
-    const uint32_t n = blockIdx.x % wide * kOutputs + threadIdx.x % kOutputs, share = threadIdx.x / kOutputs;
+    const uint32_t wide = (a.outputs + kOutputs - 1) / kOutputs, block = block_of_grid(), row = block / wide;
+    if (row >= a.rows) return;
+    const uint32_t n = block % wide * kOutputs + threadIdx.x % kOutputs, share = threadIdx.x / kOutputs;
     int64_t sum = 0;
     if (n < a.outputs) {
 #pragma unroll 8
@@ -792,7 +793,7 @@ int32_t leo_q8_matmul(const LeoQ8Product* product, void* stream) {
         // 340 slices took 1.5 us less with 32 threads an output than with 8, 128 0.4 less with 16
         const uint32_t share = plan.slices >= 256 ? 32 : plan.slices >= 16 ? 16 : 1;
         const uint64_t count = (p.shape.outputs + 256 / share - 1) / (256 / share) * p.rows;
-        launch(share == 32 ? leo_q8_join<32> : share == 16 ? leo_q8_join<16> : leo_q8_join<1>, dim3(static_cast<uint32_t>(count)), dim3(256), 0, at, a);
+        launch(share == 32 ? leo_q8_join<32> : share == 16 ? leo_q8_join<16> : leo_q8_join<1>, grid_of(static_cast<uint32_t>(count)), dim3(256), 0, at, a);
     });
 }
 

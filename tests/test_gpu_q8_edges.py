@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from leo_amd import decode
+from tests.test_gpu_q8 import check
 
 pytestmark = pytest.mark.gpu
 DEVICE = "cuda:0"
@@ -45,3 +46,21 @@ def test_codes_next_to_a_half_of_odd_scales(require_gpu, seed):
     eye = torch.eye(row.shape[1], device=DEVICE).to(torch.int8)
     got = decode.q8_matmul(row, decode.Q8Weight(eye, torch.ones(row.shape[1], device=DEVICE)))
     assert torch.equal((got[0, 1:].double() / float(scale)).round(), want)
+
+
+def test_more_than_2_32_threads_join(require_gpu):
+    """A result of 2^32 values of two slices."""
+    rows = outputs = 65_536
+    inputs = 131_073
+    gen = torch.Generator(DEVICE).manual_seed(1)
+    codes = torch.randint(-128, 128, (outputs, inputs), generator=gen, device=DEVICE, dtype=torch.int8)
+    scales = torch.rand(outputs, generator=gen, device=DEVICE) * 0.01
+    one = torch.randn(1, inputs, generator=gen, device=DEVICE, dtype=torch.bfloat16)
+    weight = decode.Q8Weight(codes, scales)
+    some = torch.tensor([0, 1, 255, 256, 4097, 30_000, 65_279, 65_280, 65_534, 65_535], device=DEVICE)
+    kept = codes[some]
+    del codes
+    got = decode.q8_matmul(one.expand(rows, inputs), weight)
+    check(got[:1][:, some].contiguous(), one, kept, scales[some], None)
+    for begin in range(0, rows, 4096):
+        assert bool((got[begin:begin + 4096] == got[:1]).all())
