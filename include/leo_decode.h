@@ -192,7 +192,8 @@ int32_t leo_q8_layout(const LeoQ8Source* source, void* stream);
  * x[m, k] / s[m], of two the even one. Sums of codes are exact; rounded to float they
  * are multiplied by scale[n], which has to leave a finite float, then by s[m] with the
  * bias in one fused operation, and rounded to y_type. A row of x with an infinity or
- * NaN gives NaN. bias (float) may be NULL. y and x share no memory. `workspace`: at least
+ * NaN gives NaN. bias (float) may be NULL. y and x share no memory. Results whose launch
+ * would have 2^32 threads, 2^28 outputs or more, may be refused. `workspace`: at least
  * leo_q8_workspace_bytes() bytes (none where that is 0), 256-byte aligned, whatever
  * they hold; free again when the call's work is done. */
 typedef struct LeoQ8Product {

@@ -756,8 +756,10 @@ int32_t leo_q8_matmul(const LeoQ8Product* product, void* stream) {
         require(reinterpret_cast<uintptr_t>(p.layout) % 256 == 0, "leo_q8_matmul: layout must be 256-byte aligned");
         const Q8Layout l = layout_of(p.shape);
         require(p.layout_bytes >= l.bytes, "leo_q8_matmul: layout is too small for its shape");
-        require((p.shape.outputs + 7) / 8 * p.rows <= 0x7fffffffu, "leo_q8_matmul: the result is too large");
         const Plan plan = plan_of(p.shape, p.rows);
+        const uint64_t wide = plan.tiles ? plan.tiles : plan.group_tiles, high = plan.tiles ? plan.tiles * uint64_t{kTile} : p.rows;
+        const uint64_t groups = (l.tiles + wide - 1) / wide * ((p.rows + high - 1) / high);  // on the grid's first axis
+        require((p.shape.outputs + 7) / 8 * p.rows <= 0x7fffffffu && groups * kFewThreads < 1ull << 32, "leo_q8_matmul: the result is too large");
         require(plan.workspace == 0 || (p.workspace && reinterpret_cast<uintptr_t>(p.workspace) % 256 == 0 &&
                                         p.workspace_bytes >= plan.workspace),
                 "leo_q8_matmul: workspace is missing, too small or not 256-byte aligned");

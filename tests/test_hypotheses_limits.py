@@ -49,3 +49,14 @@ def test_pieces_that_meet_are_refused_in_single_rows_too(groups, beams, kept):
     entries = (native.LeoStateArray * 2)(_array(1 << 30, at, outer=1), _array(1 << 31, at + 63, outer=1))
     args = native.LeoReorder(arrays=ctypes.addressof(entries), count=2, groups=1, beams=1, kept=1, parents=256)
     assert "overlaps another array" in _refused("leo_reorder_states", ctypes.byref(args), None)
+
+
+@pytest.mark.parametrize("outputs, inputs, rows", [((1 << 30) + 1, 64, 1), (1 << 31, 1, 16), ((1 << 28) + 1, 64, 17),
+                                                   ((1 << 29) + 1, 2000, 16)])
+def test_results_past_a_launch_are_refused(outputs, inputs, rows):
+    lib, shape, size = native.load(), native.LeoQ8Shape(outputs=outputs, inputs=inputs), ctypes.c_uint64()
+    assert lib.leo_q8_workspace_bytes(ctypes.byref(shape), rows, native.TYPE_F32, ctypes.byref(size)) == native.OK
+    product = native.LeoQ8Product(shape=shape, layout=1 << 44, layout_bytes=1 << 43, rows=rows, x=1 << 20, x_stride=inputs,
+                                  y=1 << 45, y_stride=outputs, x_type=native.TYPE_F32, y_type=native.TYPE_F32,
+                                  workspace=1 << 40, workspace_bytes=1 << 43)
+    assert "too large" in _refused("leo_q8_matmul", ctypes.byref(product), None)
