@@ -66,7 +66,8 @@ int32_t leo_q4_layout(const LeoQ4Source* source, void* stream);
  * 128 inputs: bfloat16 in one part, float in two (22 bits), both to 2^-39 of the
  * largest of those 128. Scales have to stay below 2^100 in magnitude: a group's sum
  * is scaled before that power of two is taken back. bias (float) may be NULL. y and
- * x share no memory. `workspace`: at least leo_q4_workspace_bytes()
+ * x share no memory, nor do y and the bias but where y is one row of floats and the
+ * bias itself. `workspace`: at least leo_q4_workspace_bytes()
  * bytes (none where that is 0), 256-byte aligned, whatever they hold; free again
  * when the call's work is done. */
 typedef struct LeoQ4Product {
@@ -192,7 +193,8 @@ int32_t leo_q8_layout(const LeoQ8Source* source, void* stream);
  * x[m, k] / s[m], of two the even one. Sums of codes are exact; rounded to float they
  * are multiplied by scale[n], which has to leave a finite float, then by s[m] with the
  * bias in one fused operation, and rounded to y_type. A row of x with an infinity or
- * NaN gives NaN. bias (float) may be NULL. y and x share no memory. Results whose launch
+ * NaN gives NaN. bias (float) may be NULL. y and x share no memory, nor do y and the bias
+ * but where y is one row of floats and the bias itself. Results whose launch
  * would have 2^32 threads, 2^28 outputs or more, may be refused. `workspace`: at least
  * leo_q8_workspace_bytes() bytes (none where that is 0), 256-byte aligned, whatever
  * they hold; free again when the call's work is done. */

@@ -168,6 +168,13 @@ inline bool overlap(const Rows& a, const Rows& b) {
     return false;
 }
 
+// Whether a product's result shares memory with its float bias. One row of floats may be the bias itself: each of its
+// values is read by the thread that writes it, and before.
+inline bool meets_bias(const float* bias, const Rows& y, uint64_t outputs, int32_t y_type) {
+    if (!bias || (y.count == 1 && y_type == LEO_TYPE_F32 && y.at == reinterpret_cast<uintptr_t>(bias))) return false;
+    return overlap(rows_of(bias, 1, outputs, 0, LEO_TYPE_F32), y);
+}
+
 // An axis of a grid has to have fewer than 2^32 threads: workgroups past the first 2^22 go on
 // along the second axis, whose last row may hold some too many.
 constexpr uint32_t kAcross = 1u << 22;

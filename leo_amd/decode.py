@@ -175,7 +175,8 @@ def q4_matvec(x: torch.Tensor, weight: Q4Weight, bias: Optional[torch.Tensor] = 
     bfloat16: sums in 32 bits, rounded once to `out_dtype` (x's type by default). A
     float32 x enters with 22 bits of each value, and to 2^-39 of the largest of its
     row's 128 neighbouring inputs, to which a bfloat16 x is held too; scales have to
-    stay below 2^100. bias: float32 [outputs]. `out` and x share no memory."""
+    stay below 2^100. bias: float32 [outputs]. `out` and x share no memory;
+    nor do `out` and the bias, but one float32 row may be the bias itself."""
     if isinstance(x, torch.Tensor) and x.dim() == 1:
         if out is not None:
             _refuse("out needs x with two axes")
@@ -249,7 +250,8 @@ def q8_matmul(x: torch.Tensor, weight: Q8Weight, bias: Optional[torch.Tensor] = 
     float32 (at least 2^-126), its codes the nearest whole numbers to x over that, of
     two the even one. Sums of codes are exact, scales and bias come to them in float32
     before the rounding to `out_dtype` (x's type by default). A row with an infinity or
-    NaN gives NaN. bias: float32 [outputs]. `out` and x share no memory."""
+    NaN gives NaN. bias: float32 [outputs]. `out` and x share no memory;
+    nor do `out` and the bias, but one float32 row may be the bias itself."""
     if isinstance(x, torch.Tensor) and x.dim() == 1:
         if out is not None:
             _refuse("out needs x with two axes")

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from leo_amd import decode
-from tests.test_gpu_q8 import check
+from tests.test_gpu_q8 import check, make
 
 pytestmark = pytest.mark.gpu
 DEVICE = "cuda:0"
@@ -64,3 +64,16 @@ def test_more_than_2_32_threads_join(require_gpu):
     check(got[:1][:, some].contiguous(), one, kept, scales[some], None)
     for begin in range(0, rows, 4096):
         assert bool((got[begin:begin + 4096] == got[:1]).all())
+
+
+def test_one_row_is_added_to_its_bias(require_gpu):
+    """The bias may be the result itself where there is one row: y = y + x W^T."""
+    for inputs, outputs in ((64, 8), (1024, 257), (100_000, 257), (9000, 2100)):
+        x, codes, scales, bias = make(inputs, 1, inputs, outputs, torch.float32, torch.float32)
+        weight, y = decode.Q8Weight(codes, scales), bias[None].clone()
+        decode.q8_matmul(x, weight, y[0], out=y)
+        check(y, x, codes, scales, bias)
+        packed = decode.Q4Weight.quantize(torch.randn(outputs, inputs, device=DEVICE))
+        want, y = decode.q4_matvec(x, packed, bias), bias[None].clone()
+        decode.q4_matvec(x, packed, y[0], out=y)
+        assert torch.equal(y, want)

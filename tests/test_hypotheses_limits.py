@@ -60,3 +60,15 @@ def test_results_past_a_launch_are_refused(outputs, inputs, rows):
                                   y=1 << 45, y_stride=outputs, x_type=native.TYPE_F32, y_type=native.TYPE_F32,
                                   workspace=1 << 40, workspace_bytes=1 << 43)
     assert "too large" in _refused("leo_q8_matmul", ctypes.byref(product), None)
+
+
+@pytest.mark.parametrize("rows, y, y_type", [(2, 8192, native.TYPE_F32), (3, 8192 - 4 * 20, native.TYPE_F32),
+                                             (1, 8192 + 4, native.TYPE_F32), (1, 8192 - 4 * 15, native.TYPE_F32),
+                                             (1, 8192, native.TYPE_F16), (1, 8192 + 62, native.TYPE_BF16)])
+def test_results_over_the_bias_are_refused(rows, y, y_type):
+    good = dict(layout=1 << 20, layout_bytes=1 << 20, rows=rows, x=1 << 28, x_stride=128, bias=8192, y=y, y_stride=20,
+                x_type=native.TYPE_F32, y_type=y_type, workspace=1 << 24, workspace_bytes=1 << 20)
+    eight = native.LeoQ8Product(shape=native.LeoQ8Shape(outputs=16, inputs=128), **good)
+    assert "overlaps the bias" in _refused("leo_q8_matmul", ctypes.byref(eight), None)
+    four = native.LeoQ4Product(shape=native.LeoQ4Shape(outputs=16, inputs=128, group=32, scale_type=native.TYPE_F32), **good)
+    assert "overlaps the bias" in _refused("leo_q4_matvec", ctypes.byref(four), None)
