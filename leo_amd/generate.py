@@ -202,6 +202,7 @@ class Generator:
         if not 1 <= beams <= 64:
             raise native.LeoError(native.ERR_INVALID_ARGUMENT, f"beams must be 1 to 64, not {beams}")
         if count < 1:
+            self._document = None
             return [(b"", 0.0)]
         prefix = self._written
         # what each hypothesis has on the GPU: its bytes, with those before it, and its state of UTF-8
