@@ -147,15 +147,14 @@ struct Span {
     }
 };
 
-// What a span, or a run of them, leaves for its row: its largest logit, and the sum of
-// exponentials as mass * 2^power_of(top) * e^base_of(top). A power of two in place of the
-// largest itself, so that no difference of two logits is rounded, and sums of spans meet
-// exactly. From 2^20 on the largest comes off first: floats that size differ by nothing or by
-// 2^-4 at least, and where the difference counts at all it is exact.
-constexpr float kLog2E = 1.44269504f, kLog2ELow = 1.92596299e-8f;  // log2(e) in two parts
-constexpr double kLn2 = 0.69314718055994531;
-__device__ __forceinline__ float base_of(float top) { return fabsf(top) < 0x1p20f ? 0.0f : top; }
-__device__ __forceinline__ float power_of(float top) { return fabsf(top) < 0x1p20f ? ceilf(top * kLog2E) : 0.0f; }
+// What symbols, a span or a run of spans leave for their row: the largest logit, and the sum
+// of exponentials as mass * 2^power_of(top) * e^base_of(top). A power of two in place of the
+// largest itself, so that no difference of two logits is rounded, and sums meet exactly. From
+// 2^10 on the largest comes off first, which is exact for all that counts beside it.
+constexpr float kLog2E = 1.44269504f;
+constexpr double kLog2ERest = 1.92596299e-8, kLn2 = 0.69314718055994531;  // log2(e) is kLog2E + kLog2ERest
+__device__ __forceinline__ float base_of(float top) { return fabsf(top) < 0x1p10f ? 0.0f : top; }
+__device__ __forceinline__ float power_of(float top) { return fabsf(top) < 0x1p10f ? ceilf(top * kLog2E) : 0.0f; }
 
 struct SpanRecord {
     float top;
@@ -163,38 +162,38 @@ struct SpanRecord {
     double mass;
 };
 __device__ __forceinline__ double against(const SpanRecord& r, float top) {
-    if (!(r.top > negative_infinity())) return 0.0;
+    if (r.top == top) return r.mass;
+    if (!(r.top > top - 800.0f)) return 0.0;
     const float base = base_of(r.top), to = base_of(top), power = power_of(r.top) - power_of(top);
     if (base == to) return ldexp(r.mass, static_cast<int>(power));
     return r.mass * exp(static_cast<double>(base) - to + power * kLn2);
 }
-// z log2(e) - power is a whole number and a fraction of at most a half, which the fused
-// products have to 2^-25; the exponential is off by 2^-23 at most, and sixteen of them are
-// added in four steps of 2^-24 each. Together less than 2^-21 of the sum, however alike its
-// terms are; what follows has 64 bits. What lies 80 below the largest is taken as lying there,
-// which 2^26 of them cannot bring to 2^-64.
+// A lane takes its sixteen against a power of two near their own largest, in floats: the fused
+// product rounds an exponent by half a step, which is 2^-25 for one near that power and grows as
+// the exponential gets smaller: for fifteen beside the largest 1.1e-7 of the sum at most, when
+// they lie four powers of two below. Exponentials are off by a step, 1.2e-7, three additions by
+// 2^-24 each, 1.8e-7, what is left of log2(e) by 0.3e-7 once the lane's largest has it: together
+// 4.4e-7, less than 2^-21, however alike the terms are. All else has 64 bits.
 template <class T>
 __device__ __forceinline__ SpanRecord weigh(const Span<T>& s, float lane_top) {
     const float top = wave_max(lane_top);
     if (top == negative_infinity()) return {top, 0, 0.0};
     float e[kEach];
+    const float base = base_of(top), mine = fmaxf(lane_top - base, -2000.0f), power = ceilf(mine * kLog2E);  // much lower ones come to 0
     if (top < __builtin_inff()) {
-        const float base = base_of(top), least = top - base - 80.0f, magic = 12582912.0f - power_of(top);  // 1.5 * 2^23
 #pragma unroll
-        for (uint32_t i = 0; i < kEach; ++i) {
-            const float z = fmaxf(s.z[i] - base, least), whole = __builtin_fmaf(z, kLog2E, magic);
-            const float rest = __builtin_fmaf(z, kLog2ELow, __builtin_fmaf(z, kLog2E, magic - whole));
-            e[i] = __uint_as_float(__float_as_uint(__builtin_amdgcn_exp2f(rest)) + (__float_as_uint(whole) << 23));
-        }
+        for (uint32_t i = 0; i < kEach; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s.z[i] - base, kLog2E, -power));
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) e[i] = s.z[i] == top ? 1.0f : 0.0f;
     }
 #pragma unroll
-    for (uint32_t half = kEach / 2; half; half /= 2)
+    for (uint32_t half = kEach / 2; half > 1; half /= 2)
 #pragma unroll
         for (uint32_t i = 0; i < half; ++i) e[i] += e[i + half];
-    return {top, 0, wave_sum(static_cast<double>(e[0]))};
+    const double sum = static_cast<double>(e[0]) + e[1], rest = mine * static_cast<float>(kLog2ERest * kLn2);
+    if (top == __builtin_inff()) return {top, 0, wave_sum(sum)};
+    return {top, 0, wave_sum(ldexp(__builtin_fma(sum, rest, sum), static_cast<int>(power - power_of(top))))};
 }
 
 // The `kept` best of the spans of a workgroup (or of one wave's span, kWave), in

@@ -15,7 +15,7 @@ DEVICE = "cuda:0"
 
 
 @pytest.mark.parametrize("symbols", [900, 32_001, 131_075, 262_147, 2_000_003, 1 << 26])
-@pytest.mark.parametrize("top", [0.0, 5.3, -8.7, 1000.1, -70_000.3, 3.0e6])
+@pytest.mark.parametrize("top", [0.0, 5.3, -8.7, 1000.1, 1023.9, -1013.3, -70_000.3, 3.0e6])
 def test_one_large_logit_above_a_flat_tail(require_gpu, symbols, top):
     """The error of one small term is that of all, so nothing averages out. The bound is that of
     the other selections' sums: 2^-21 of the log."""
@@ -45,8 +45,10 @@ def test_one_large_logit_above_a_flat_tail(require_gpu, symbols, top):
 def test_spans_far_apart(require_gpu, symbols):
     """What a row's parts leave is joined exactly, however far apart they lie."""
     rng = np.random.default_rng(symbols)
-    for low, high in ((-30.0, 4.0), (1e5, 1.1e5), (-2e6, 12.5), (12.5, 3e6), (-3e38, 3e38), (2.0e6, 2.0e6 + 2), (1048574.0, 1048578.0)):
+    for low, high in ((-30.0, 4.0), (1e5, 1.1e5), (-2e6, 12.5), (12.5, 3e6), (-3e38, 3e38), (2.0e6, 2.0e6 + 2), (1048574.0, 1048578.0),
+                      (1000.0, 1048.0), (-1048.0, -1000.0), (1020.0, 1026.0), (-1026.0, -1020.0), (-2010.0, -1990.0), (-5000.0, -4990.0)):
         z = torch.from_numpy(rng.uniform(low, high, (4, symbols)).astype(np.float32)).to(DEVICE)
+        z[0, ::3] = -1e9
         z[1] = z[1].sort().values
         z[2, symbols // 2:] = low
         z[3, :symbols // 2] = -torch.inf
