@@ -541,7 +541,7 @@ __device__ __forceinline__ void merge(const LeoBeams& a, uint64_t group, const G
 
 // Searches whose rows make up to 16 spans take one workgroup each: a wave a span,
 // which picks from its registers, then the search's answer. A chain of reductions bounds
-// it: 7.1 us for 4 beams of 257, of which a launch is some 3.
+// it: 7.4 us for 4 beams of 257.
 constexpr uint32_t kWavePool = 320;
 template <class T>
 __global__ __launch_bounds__(kMostWaves * 64) void leo_beam_whole(LeoBeams a, uint32_t spans) {
@@ -569,9 +569,10 @@ __global__ __launch_bounds__(kMostWaves * 64) void leo_beam_whole(LeoBeams a, ui
 }
 
 // Longer rows: a workgroup a run of spans, a wave each, which leaves its record and its
-// best candidates; then a workgroup a search. Memory bounds the first, 111 MB of 32 x 8
-// beams of 131,075 in 20.7 us (5.4 TB/s; with 16 waves a workgroup, which wait for each
-// other longer, a fifth more), latency the second: 7.4 to 7.9 us.
+// best candidates; then a workgroup a search. 32 x 8 beams of 131,075, of which 94 MB count,
+// take the first 21.3 us (4.4 TB/s) and 23.1 where no input is left in the cache beside memory,
+// four fifths of its rate (with 16 waves a workgroup, which wait for each other longer, a fifth
+// more). Latency bounds the second: 7.4 to 8.0 us.
 constexpr uint32_t kRowPool = 1024;
 template <class T>
 __global__ __launch_bounds__(256) void leo_beam_rows(LeoBeams a, uint32_t lists, SpanRecord* records, uint64_t* candidates) {
@@ -663,8 +664,8 @@ void launch_beams(const BeamPlan& p, const LeoBeams& b, hipStream_t stream) {
 // start at multiples of 16, loads at multiples of 4: the bytes that a row's place lies off
 // those are shifted in registers. In place a thread writes nothing but the columns that it
 // alone reads, the same in every row, and holds what it moves in LDS that is its own. 8
-// planes of 8 rows of 4 MB take 75 to 89 us (5.0 to 5.9 TB/s), 8-bit caches with rows off all
-// boundaries, 266 MB, 57 to 64.
+// planes of 8 rows of 4 MB take 75 to 89 us (5.0 to 5.9 TB/s of memory and the cache beside
+// it), 8-bit caches with rows off all boundaries, 266 MB, 57, and 66 from memory alone.
 constexpr uint32_t kArrays = 32;
 
 struct ReorderArgs {

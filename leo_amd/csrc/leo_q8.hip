@@ -241,8 +241,8 @@ __global__ __launch_bounds__(256) void leo_q8_quantize_part(ProductArgs a) {
 // last read it again and are not stored. Whole sums go to LDS by whole-number
 // additions, whose order does not matter. The slice of x is asked for before the weights,
 // which would stand before it in memory's queue: 13.9 us for 14.7 with 8 rows of 131,072
-// -> 257. Memory bounds a long product, 1 row of 1,048,576 -> 257 in 51.6 us (5.2 TB/s), a
-// launch a short one, 1,024 -> 257 in 4.0.
+// -> 257. Memory bounds a long product, 1 row of 1,048,576 -> 257 in 51.5 to 51.9 us for 298 MB (5.7
+// TB/s, also where no input is left in the cache beside memory), a launch a short one, 1,024 -> 257 in 4.0.
 constexpr uint32_t kFewThreads = 512, kFewWaves = kFewThreads / 64;
 constexpr uint32_t kFewStage = 48 << 10;  // bytes of x in LDS
 
@@ -345,8 +345,9 @@ __global__ __launch_bounds__(kFewThreads, 4) void leo_q8_few(ProductArgs a) {
 
 // More rows: 16 kRows rows and 16 kTiles outputs a workgroup, x and the weights
 // straight from their layouts to registers, the blocks of a slice shared by eight waves, one
-// block ahead (two ahead, or 4 or 16 waves, took as long or longer). 64 rows of 5,001 -> 11,007, 55 MB, take 15.1 us:
-// 344 workgroups on 256 CUs, and 323 KB of x for each of them from L2.
+// block ahead (two ahead, or 4 or 16 waves, took as long or longer). 64 rows of 5,001 -> 11,007, 55 MB, take 15.1 us
+// with the weights in the cache beside memory and 23 without: 344 workgroups on 256 CUs, and 323 KB of x for each of
+// them from L2.
 template <int kManyRows, int kManyTiles>
 __global__ __launch_bounds__(kFewThreads) void leo_q8_many(ProductArgs a) {
     __shared__ int32_t sums[kManyRows * kManyTiles * 256];

@@ -248,8 +248,9 @@ def q8_matmul(x: torch.Tensor, weight: Q8Weight, bias: Optional[torch.Tensor] = 
     """bias + x W^T for x [rows, inputs] (or [inputs]) of float32, float16 or
     bfloat16, with x in 8 bits: a row's scale is its largest magnitude times 1 / 127 in
     float32 (at least 2^-126), its codes the nearest whole numbers to x over that, of
-    two the even one. Sums of codes are exact, scales and bias come to them in float32
-    before the rounding to `out_dtype` (x's type by default). A row with an infinity or
+    two the even one. Sums of codes are exact; the output's scale, with which a sum has to
+    stay finite, the row's and the bias come to them in float32 before the rounding to
+    `out_dtype` (x's type by default). A row with an infinity or
     NaN gives NaN. bias: float32 [outputs]. `out` and x share no memory;
     nor do `out` and the bias, but one float32 row may be the bias itself."""
     if isinstance(x, torch.Tensor) and x.dim() == 1:
